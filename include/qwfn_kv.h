@@ -80,7 +80,8 @@ const char * qwfn_last_error(void);
 /* Make `device` current for this thread and create the per-device status word. */
 int          qwfn_init(int device);
 /* Synchronise `stream`, then read and clear the device-side error flags
- * (bit 0: set_rows index out of range; bit 1: get_rows index out of range). */
+ * (bit 0: set_rows index out of range; bit 1: get_rows index out of range;
+ * bit 2: a request without room or a bad length in qwfn_paged.h's tables). */
 int          qwfn_device_status(void * stream, uint32_t * flags);
 
 /* ------------------------------------------------------------ cache append */

@@ -247,6 +247,48 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
                          int32_t n_k_heads, int32_t n_v_heads, int32_t head_dim, float scale, float * state, float * out,
                          float * snap, size_t snap_stride_bytes, int32_t n_snap, void * stream);
 
+/* ------------------------------------------------- linear attention */
+
+/* Linear attention with a decay per head, over a batch of sequences of any
+ * lengths: per value head h (key head h / (n_v_heads / n_k_heads)) and sequence,
+ * state S [dk][dv] (the second index contiguous), token t:
+ *   S = exp(g[t][h]) S + k_t v_t^T;   out[t][h] = scale S^T q_t
+ * the DeltaNet update above without the delta rule's correction; no counterpart
+ * in the reference. Sequence b's tokens are cu[b] .. cu[b + 1] - 1 of the packed
+ * tensors (cu: device I32 [n_seq + 1], cu_new of qwfn_paged_extend), none to
+ * max_len of them:
+ *   q, k  F32, F16 or BF16 [dk, n_k_heads, n_tok]; v, dst [dv, n_v_heads, n_tok] of
+ *         q's type; rows contiguous, any token and head strides that are multiples
+ *         of 16 bytes; dst contiguous
+ *   g     F32 log decays (at most 0 in use; -inf forgets everything), token t's at
+ *         g + t * g_token_stride floats; a stride of 0 gives every token the same
+ *         n_v_heads decays
+ *   state_in, state_out  F32 [n_slots][n_v_heads][dk][dv], 16-byte aligned, equal or
+ *         not overlapping; sequence b reads and writes slot slots[b] (device I32, each
+ *         slot at most once in a call; NULL: slot b). state_in NULL: zero states. A
+ *         slot of -1: a zero state, and none is written; another slot outside
+ *         [0, n_slots): the same, and bit 0 of qwfn_device_status. A sequence of no
+ *         tokens leaves its slot of state_out unwritten. With two buffers, a step
+ *         with rejected drafts is taken back by running the accepted tokens again
+ *         from state_in.
+ * dk and dv multiples of 16, dk <= 256, dv <= 512. States, decays and sums are F32
+ * (sums of decays inside a chunk F64); the 16-bit types' products are exact, what
+ * is rounded on the way to an output is stated at the kernels; outputs are
+ * rounded once. Tokens outside every sequence (cu[0] > 0, past cu[n_seq]) are not
+ * read and their dst rows not written. cu is read as clipped to [0, n_tok] and to
+ * max_len tokens a sequence; a cu that descends or that is clipped sets bit 0 of
+ * qwfn_device_status (a descending pair: no tokens). A sequence's results do not
+ * depend on the rest of the batch beyond rounding. max_len <= 8 runs token by
+ * token; longer ones in chunks, long sequences cut into parts that are joined
+ * through ws.
+ * ws: device memory of at least qwfn_linear_attn_workspace_size bytes, 16-byte
+ * aligned (NULL where that is 0). */
+size_t qwfn_linear_attn_workspace_size(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len);
+int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const float * g,
+                     int64_t g_token_stride, const int32_t * cu, int32_t n_seq, int32_t max_len, const int32_t * slots,
+                     int32_t n_slots, const float * state_in, float * state_out, float scale, const qwfn_tensor * dst,
+                     void * ws, size_t ws_bytes, void * stream);
+
 /* ------------------------------------------------- QSA index producer */
 
 /* The indexer's key geometry and the rope / norm constants of the model

@@ -40,6 +40,7 @@
 //            f16 hi + lo.
 //   merge  : the key groups of a block merge in LDS; key splits merge in a
 //            second kernel (log-sum-exp weights), one block per quarter row.
+#include "fattn_device.h"
 #include "q8_device.h"
 #include "qwfn_common.h"
 
@@ -53,8 +54,6 @@
 namespace qwfn {
 namespace {
 
-typedef int      v4i __attribute__((ext_vector_type(4)));
-typedef float    v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
@@ -210,26 +209,6 @@ __device__ __forceinline__ int bmod(int b, int n) {
     return b < n ? b : b % n;
 }
 
-// The compiler's hazard recognizer does not see the VALU writes inside inline
-// asm, and an MFMA that reads a VGPR needs two wait states after a VALU wrote
-// it. Every asm below whose result can feed an MFMA operand therefore ends
-// with s_nop 1.
-
-// One V block's A operands for the lane's 4 keys: v[j] holds dims 2m, 2m+1 of
-// key j in its low two bytes (one 2-byte LDS read each); a0[q] = f16 pair
-// (dim 2m of keys 2q, 2q+1), a1[q] = f16 pair (dim 2m+1). int8 -> f16 is exact.
-__device__ __forceinline__ void cvt_v_block(const uint32_t v[4], uint32_t a0[2], uint32_t a1[2]) {
-#define QWFN_SDWA(D, S, DSEL, UNUSED, SSEL) "v_cvt_f16_i16_sdwa " D ", sext(" S ") dst_sel:" DSEL " dst_unused:" UNUSED " src0_sel:" SSEL "\n\t"
-#define QWFN_PAIR(D, S0, S1, B) QWFN_SDWA(D, S0, "WORD_0", "UNUSED_PAD", B) QWFN_SDWA(D, S1, "WORD_1", "UNUSED_PRESERVE", B)
-    asm(QWFN_PAIR("%0", "%4", "%5", "BYTE_0") QWFN_PAIR("%1", "%6", "%7", "BYTE_0")
-        QWFN_PAIR("%2", "%4", "%5", "BYTE_1") QWFN_PAIR("%3", "%6", "%7", "BYTE_1")
-        "s_nop 1"
-        : "=&v"(a0[0]), "=&v"(a0[1]), "=&v"(a1[0]), "=&v"(a1[1])
-        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
-#undef QWFN_PAIR
-#undef QWFN_SDWA
-}
-
 // B operands of one V block: for key pairs q (keys 2q, 2q+1), P*d_v as an f16
 // hi pair and an f16 lo pair. hi = f16(P16 * d_v) with P16 = P rounded toward
 // zero to f16 (one packed multiply per pair; p16[q] is computed once per
@@ -247,64 +226,6 @@ __device__ __forceinline__ void pdv_hilo(const float p[4], const uint32_t p16[2]
                  : "=&v"(bh[0]), "=&v"(bh[1]), "=&v"(bl[0]), "=&v"(bl[1])
                  : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p16[0]), "v"(p16[1]), "v"(dv[0]), "v"(dv[1]));
 #undef QWFN_HILO
-}
-
-// x * f16 (low or high half of a packed dword), one v_fma_mix_f32.
-__device__ __forceinline__ float mul_f16lo(float x, uint32_t h) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(h));
-    return r;
-}
-__device__ __forceinline__ float mul_f16hi(float x, uint32_t h) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x), "v"(h));
-    return r;
-}
-// x + f16 * c (f16 in the low or high half of a packed dword), one v_fma_mix_f32.
-__device__ __forceinline__ float fma_f16lo(uint32_t h, float c, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(c), "v"(x));
-    return r;
-}
-__device__ __forceinline__ float fma_f16hi(uint32_t h, float c, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(c), "v"(x));
-    return r;
-}
-__device__ __forceinline__ float xmax(float a, float b) { return a > b ? a : b; }
-// max of two scores (finite or -inf, never NaN) in one v_max_f32: fmaxf on an
-// asm result gets both operands canonicalised first, and the ternary above is
-// a compare plus a select
-__device__ __forceinline__ float vmax(float a, float b) {
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-
-// Reductions over the 4 lanes l, l^16, l^32, l^48 (the four lane groups
-// holding one MFMA column), with gfx950's cross-row swaps instead of LDS
-// permutes: a swap pair holds lanes l and l^16 (or l^32) between its two
-// results. The two results pass through an empty asm: without it the
-// compiler's IR folds the second result into the first (r[0] op r[1] becomes
-// r[0] op r[0]), which silently turns the reduction into x op x.
-template <typename Op>
-__device__ __forceinline__ float reduce_lanes16_32(float x, Op op) {
-    const unsigned u = __builtin_bit_cast(unsigned, x);
-    const auto r16 = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    unsigned a = r16[0], b = r16[1];
-    asm volatile("" : "+v"(a), "+v"(b));
-    x = op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-    const unsigned w = __builtin_bit_cast(unsigned, x);
-    const auto r32 = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    unsigned c = r32[0], d = r32[1];
-    asm volatile("" : "+v"(c), "+v"(d));
-    return op(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
-}
-__device__ __forceinline__ float xmax_lanes16_32(float x) {
-    return reduce_lanes16_32(x, [](float a, float b) { return vmax(a, b); });
-}
-__device__ __forceinline__ float sum_lanes16_32(float x) {
-    return reduce_lanes16_32(x, [](float a, float b) { return a + b; });
 }
 
 // x of the lane 8 away in the row of 16
@@ -400,14 +321,6 @@ __device__ __forceinline__ uint32_t rsrc_bytes(int64_t rem) {
 
 __device__ __forceinline__ uint32_t lds_addr(const void * p) {
     return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) p;
-}
-
-// LDS writes of this wave become visible to its other lanes (LDS operations of
-// one wave complete in order; the fences keep the compiler from moving them).
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // 16-byte store marked non-temporal (p 16-byte aligned).

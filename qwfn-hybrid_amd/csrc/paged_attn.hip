@@ -1,0 +1,709 @@
+// Decode attention over a paged q8_0 cache: many requests of different lengths,
+// T newest tokens each, keys found through block tables.
+//
+//   s_j = c sum_b dq_b dk_jb (qq_b . kq_jb)      q requantised to q8_0, integer dots
+//   out = sum_j 2^(s_j - M) dv_j vq_j / sum_j 2^(s_j - M),   c = scale log2(e)
+//
+// What bounds it: the rows, n_kv * 34 D / 32 bytes of K and of V a KV head, read
+// once (at 8 query heads a KV head 7.5 operations a byte).
+//
+// Work: the requests' keys in tiles of 32, all requests' tiles in one row; each
+// workgroup takes an equal run of it for one KV head and one tile of 16 query
+// rows, whatever the lengths are (they are known on the device only). A run that
+// crosses a request's end is cut there. A request inside one run is finished by its
+// workgroup; the parts of the others go to the workspace as (O, M, l) and
+// k_paged_merge joins them in the order of the runs, so results repeat bit for bit.
+// The KV heads and row tiles of one run are blocks next to each other on one XCD:
+// the cache lines that two heads share come from one L2.
+//
+// Inside a workgroup the 4 waves take every fourth tile of the run, each on its
+// own: a tile's rows are loaded into registers while the tile before is computed,
+// so no barrier and no wave waits for another's data. The rows then pass through
+// the wave's part of the LDS:
+//   S^T = K Q^T   v_mfma_i32_16x16x64_i8 a q8_0 block: A is the 64-byte window of the
+//                 row (from a 16-byte boundary) that holds the block's 32 quants, B
+//                 the query's quants at the same place of a window that is zero
+//                 elsewhere, so whatever else the row's window holds adds nothing.
+//   O^T = V^T P^T v_mfma_f32_16x16x32_f16: the accumulators of S^T are the B operand as
+//                 they lie (the sum over keys takes them in the order of the
+//                 registers). V's int8 are exact in f16; P dv enters as an f16 pair hi
+//                 + lo (22 bits; one f16 alone is 3e-4 off).
+// The reference M of a row is its running maximum, moved up by the exponent of the
+// largest dv of the tile and down by 8: P dv then lies below 2^8 whatever the
+// scales of V are, and 33 bits of range lie below it in f16. It follows a rise
+// of up to 2^6 late (P dv < 2^15), so O is rescaled rarely.
+#include "fattn_device.h"
+#include "q8_device.h"
+#include "qwfn_common.h"
+#include "qwfn_paged.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace qwfn {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_THREADS = PA_WAVES * 64;
+constexpr int PA_TILE = 32;            // keys of a tile
+constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
+constexpr int PA_WGS = 512;            // workgroups of a launch: two a CU
+constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
+constexpr float PA_LOG2E = 1.4426950408889634f;
+constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
+constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M
+
+// x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), is off by at
+// most d <= 2^s, and x (m d - 2^(31 + s)) < 2^(31 + s) keeps the quotient whole.
+struct fast_div { uint32_t d, m, s; };
+fast_div make_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    return {d, (uint32_t) (((1ull << (31 + s)) / d) + 1), s};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t x, fast_div f) { return f.s == 0 ? x : __umulhi(x, f.m) >> (f.s - 1); }
+
+struct pa_args {
+    const char *    q; size_t q_nb1, q_nb2, q_nb3;
+    const char *    k; const char * v;
+    uint32_t        nb1;               // bytes of a cache row
+    size_t          nb2;               // and of a head's offset
+    int64_t         n_pages;
+    const int32_t * table; int64_t t_stride;
+    const int32_t * n_kv;
+    int64_t         max_kv;            // max_pages * page
+    fast_div        page;
+    const char *    gate; char * dst;
+    int32_t         type;              // of q, gate and dst
+    int32_t         n_seq, T, nh, nh_kv, rep, R, RT, x86;
+    int32_t         runs;              // runs the tiles are cut into, at most
+    float           c;                 // scale * log2(e)
+    float *         part_o;            // [run + request][nh_kv][R][D]
+    float2 *        part_ml;           // [run + request][nh_kv][R]
+    int2 *          span;              // [request]: its first and last run
+    uint32_t *      status;
+};
+
+template <int D> struct pa_cfg {
+    static constexpr int NBLK = D / QK;
+    static constexpr int SEG = NBLK * QBLOCK;            // bytes of a head row
+    static constexpr int PB = SEG / 17;                  // bytes a lane loads at once: 17 pieces a row
+    static constexpr int LS = (SEG + 15) / 16 * 16;      // of a row in LDS
+    static constexpr int ROWS = PA_TILE * LS;            // of a tensor's tile in LDS
+    static constexpr int PIECES = PA_TILE * 17;
+    static constexpr int LOADS = (PIECES + 63) / 64;
+    static constexpr int WAVE = 2 * ROWS + 2 * PA_TILE + 2 * NBLK * PA_TILE * 2;   // K, V, each key's largest dv, scales
+    static constexpr int IMG = 16 * NBLK * 64;           // the query windows
+    static_assert(PB == 16 || PB == 8 || PB == 4, "whole loads");
+    static_assert(PA_WAVES * WAVE >= IMG + 16 * NBLK * 4 && WAVE >= 16 * D * 4, "the LDS holds the query image and O");
+    static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
+};
+template <int PB> struct pa_piece;
+template <> struct pa_piece<16> { typedef v4u type; };
+template <> struct pa_piece<8>  { typedef uint2 type; };
+template <> struct pa_piece<4>  { typedef uint32_t type; };
+
+constexpr int pa_win(int b) { return (QBLOCK * b + 2) / 16; }              // first 16 bytes of block b's window
+
+__device__ __forceinline__ void load4(const char * p, int32_t type, float x[4]) {
+    if (type == QWFN_TYPE_F32) {
+        const float4 f = *(const float4 *) p;
+        x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+    } else {
+        const uint2 u = *(const uint2 *) p;
+        const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x[i] = type == QWFN_TYPE_F16 ? dev::f16_bits_to_f32((uint16_t) h[i]) : __builtin_bit_cast(float, h[i] << 16);
+    }
+}
+// bf16 of x, to nearest even; a NaN stays one
+__device__ __forceinline__ uint32_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16) x); }
+__device__ __forceinline__ void store4(char * p, int32_t type, const float x[4]) {
+    if (type == QWFN_TYPE_F32) {
+        *(float4 *) p = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = type == QWFN_TYPE_F16 ? dev::f32_to_f16_bits(x[i]) : bf16_bits(x[i]);
+        *(uint2 *) p = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+}
+__device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[4]) {
+    const size_t es = a.type == QWFN_TYPE_F32 ? 4 : 2;
+    if (a.gate) {
+        float g[4];
+        load4(a.gate + elem * es, a.type, g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = x[i] / (1.f + expf(-g[i]));
+    }
+    store4(a.dst + elem * es, a.type, x);
+}
+
+// The f16 pair of x = p d for the keys of a pair (d packed): hi toward zero, lo = p d - hi from one
+// fused step each.
+__device__ __forceinline__ void hilo(float p0, float p1, uint32_t d, uint32_t & hi, uint32_t & lo) {
+    const float x0 = mul_f16lo(p0, d), x1 = mul_f16hi(p1, d);
+    asm("v_cvt_pkrtz_f16_f32 %0, %4, %5\n\t"
+        "v_fma_mixlo_f16 %1, %2, %6, -%0 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %1, %3, %6, -%0 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "s_nop 1"
+        : "=&v"(hi), "=&v"(lo) : "v"(p0), "v"(p1), "v"(x0), "v"(x1), "v"(d));
+}
+// The same where keys are masked: a key that a row does not see (p = 0) adds nothing, whatever its d is.
+__device__ __forceinline__ void hilo_masked(float p0, float p1, uint32_t d, uint32_t & hi, uint32_t & lo) {
+    const float d0 = dev::f16_bits_to_f32((uint16_t) d), d1 = dev::f16_bits_to_f32((uint16_t) (d >> 16));
+    const float x0 = p0 == 0.f ? 0.f : p0 * d0, x1 = p1 == 0.f ? 0.f : p1 * d1;
+    const _Float16 h0 = (_Float16) x0, h1 = (_Float16) x1;
+    hi = dev::f32_to_f16_bits(x0) | (uint32_t) dev::f32_to_f16_bits(x1) << 16;
+    lo = dev::f32_to_f16_bits(x0 - (float) h0) | (uint32_t) dev::f32_to_f16_bits(x1 - (float) h1) << 16;
+}
+
+// The block's run of the tiles of all requests.
+struct pa_run { int b; int32_t off, left, pos, per; };
+
+// Where run g starts: the request and its tile. Every thread sums the tiles of a few requests.
+__device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * sh) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int c = (a.n_seq + PA_THREADS - 1) / PA_THREADS;
+    int32_t sum = 0;
+    for (int i = 0; i < c; i++) {
+        const int b = tid * c + i;
+        if (b < a.n_seq) {
+            const int64_t n = a.n_kv[b];
+            sum += n <= 0 ? 0 : (int32_t) (((n < a.max_kv ? n : a.max_kv) + PA_TILE - 1) / PA_TILE);
+        }
+    }
+    int32_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int32_t x = __shfl_up(incl, d);
+        if (lane >= d) incl += x;
+    }
+    if (lane == 63) sh[w] = incl;
+    __syncthreads();
+    int32_t before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < PA_WAVES; i++) {
+        const int32_t x = sh[i];
+        if (i < w) before += x;
+        total += x;
+    }
+    incl += before;
+    int32_t per = (total + a.runs - 1) / a.runs;
+    per = (per + PA_WAVES - 1) / PA_WAVES * PA_WAVES;       // a wave's tiles: whole rounds
+    per = per < PA_MIN_TILES ? PA_MIN_TILES : per;
+    const int64_t start = (int64_t) g * per;
+    if (start >= incl - sum && start < incl) {
+        int32_t at = incl - sum;
+        for (int i = 0; i < c; i++) {
+            const int b = tid * c + i;
+            const int64_t n = b < a.n_seq ? a.n_kv[b] : 0;
+            const int32_t t = n <= 0 ? 0 : (int32_t) (((n < a.max_kv ? n : a.max_kv) + PA_TILE - 1) / PA_TILE);
+            if (start >= at && start < at + t) {
+                sh[PA_WAVES] = b;
+                sh[PA_WAVES + 1] = (int32_t) (start - at);
+            }
+            at += t;
+        }
+    }
+    __syncthreads();
+    pa_run r{0, 0, 0, 0, per};
+    if (start < total) {
+        r.b = __builtin_amdgcn_readfirstlane(sh[PA_WAVES]);
+        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
+        r.left = __builtin_amdgcn_readfirstlane(total - start < per ? (int32_t) (total - start) : per);
+        r.pos = (int32_t) start;
+    }
+    return r;
+}
+
+template <int D>
+__global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
+    using C = pa_cfg<D>;
+    using piece = typename pa_piece<C::PB>::type;
+    constexpr int NBLK = C::NBLK;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PA_WAVES * C::WAVE];
+    __shared__ float2 ml[PA_WAVES][16];
+    __shared__ int32_t sh[PA_WAVES + 2];
+    const int tid = threadIdx.x, lane = tid & 63, ln = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    // blocks -> (run, KV head, row tile): those of one run follow each other on one XCD
+    const int inner = a.nh_kv * a.RT;
+    const int j = blockIdx.x >> 3, g = j / inner * 8 + (int) (blockIdx.x & 7), hr = j % inner;
+    const int kvh = hr % a.nh_kv, rt = hr / a.nh_kv;
+    pa_run run = find_run(a, g, sh);
+
+    uint8_t * const my = lds + wave * C::WAVE;                   // K rows, V rows, scales
+    uint16_t * const vmax = (uint16_t *) (my + 2 * C::ROWS);
+    uint16_t * const kscl = vmax + PA_TILE;
+    uint16_t * const vscl = kscl + NBLK * PA_TILE;
+    const char * kh = a.k + (size_t) kvh * a.nb2;
+    const char * vh = a.v + (size_t) kvh * a.nb2;
+    // this lane's query row
+    const int row = 16 * rt + ln, trow = row / a.rep;
+
+    for (; run.left > 0; run.b++, run.off = 0) {
+        const int b = run.b;
+        const int32_t n_in = a.n_kv[b];
+        const int32_t n = n_in <= 0 ? 0 : n_in < a.max_kv ? n_in : (int32_t) a.max_kv;
+        if (n != n_in && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+        const int32_t tiles = (int32_t) (((int64_t) n + PA_TILE - 1) / PA_TILE);
+        if (tiles == 0) continue;
+        const int32_t nt = tiles - run.off < run.left ? tiles - run.off : run.left;   // tiles of this part
+        const bool whole = nt == tiles;
+        if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(run.pos / run.per, (run.pos + tiles - 1) / run.per);
+        const int32_t * table = a.table + (int64_t) b * a.t_stride;
+
+        // the cache row of the lane's key (lanes l and l + 32 the same) of a tile, -1 for none
+        auto slots = [&](int t) -> int32_t {
+            const int32_t key = (run.off + t) * PA_TILE + (lane & 31);
+            const bool in = t < nt && key < n;
+            const uint32_t col = div_by((uint32_t) (in ? key : 0), a.page);
+            const int32_t page = in ? table[col] : -1;
+            if (in && (uint32_t) page >= (uint32_t) a.n_pages) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+            return (uint32_t) page < (uint32_t) a.n_pages ? page * (int32_t) a.page.d + (key - (int32_t) (col * a.page.d)) : -1;
+        };
+        piece kr[C::LOADS], vr[C::LOADS];
+        auto rows = [&](int32_t slot) {
+#pragma unroll
+            for (int i = 0; i < C::LOADS; i++) {
+                const int p = lane + 64 * i, key = (p * 241) >> 12;          // p / 17 for p < 544
+                int32_t s = __shfl(slot, key & 31);
+                s = s < 0 ? 0 : s;
+                const size_t off = (size_t) (uint32_t) s * a.nb1 + (size_t) (p - 17 * key) * C::PB;
+                if (64 * (i + 1) <= C::PIECES || p < C::PIECES) {
+                    kr[i] = *(const piece *) (kh + off);
+                    vr[i] = *(const piece *) (vh + off);
+                }
+            }
+        };
+        int32_t cur = slots(wave), next = slots(wave + PA_WAVES);
+        rows(cur);
+
+        // the query image: rows requantised, each block at its place of its window
+        __syncthreads();                                   // the LDS of the part before is read
+        for (int i = tid; i < C::IMG / 16; i += PA_THREADS) ((v4u *) lds)[i] = v4u{0, 0, 0, 0};
+        __syncthreads();
+        float * dql = (float *) (lds + C::IMG);
+        for (int i = tid >> 3; i < 16 * NBLK; i += PA_THREADS / 8) {
+            const int r = i / NBLK, blk = i % NBLK, rr = 16 * rt + r, sub = tid & 7;
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (rr < a.R) {
+                const int t = rr / a.rep, h = kvh * a.rep + (rr - t * a.rep);
+                load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 +
+                          (size_t) (blk * QK + sub * 4) * (a.type == QWFN_TYPE_F32 ? 4 : 2), a.type, x);
+            }
+            uint16_t d16;
+            float dq;
+            const uint32_t q4 = dev::q8_quantize_lane4(x, a.x86 != 0, &d16, &dq);
+            const int at = QBLOCK * blk + 2 - (QBLOCK * blk + 2) / 16 * 16;
+            uint16_t * qp = (uint16_t *) (lds + (r * NBLK + blk) * 64 + at + sub * 4);
+            qp[0] = (uint16_t) q4;
+            qp[1] = (uint16_t) (q4 >> 16);
+            if (sub == 0) dql[r * NBLK + blk] = dq;
+        }
+        __syncthreads();
+        v4i qw[NBLK];
+        float dq[NBLK];
+#pragma unroll
+        for (int blk = 0; blk < NBLK; blk++) {
+            qw[blk] = *(const v4i *) (lds + (ln * NBLK + blk) * 64 + 16 * lg);
+            dq[blk] = dql[ln * NBLK + blk];
+        }
+        __syncthreads();
+
+        v4f O[NBLK][2] = {};
+        float M = -INFINITY, l = 0.f;
+        const int32_t limit = n - a.T + trow + 1;          // the row sees keys below it
+        for (int t = wave; t < nt; t += PA_WAVES) {
+            const uint32_t live = (uint32_t) __ballot(cur >= 0);   // the tile's keys that exist
+            const int32_t key0 = (run.off + t) * PA_TILE;
+            const bool masked = live != 0xffffffffu || key0 + PA_TILE > n - a.T + 1;
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < C::LOADS; i++) {
+                const int p = lane + 64 * i, key = (p * 241) >> 12, at = key * C::LS + (p - 17 * key) * C::PB;
+                if (64 * (i + 1) <= C::PIECES || p < C::PIECES) {
+                    *(piece *) (my + at) = kr[i];
+                    *(piece *) (my + C::ROWS + at) = vr[i];
+                }
+            }
+            wave_lds_sync();
+            cur = next;
+            rows(cur);
+            next = slots(t + 2 * PA_WAVES);
+            // the scales by block and key; V's largest (finite) of each key and of the tile
+            uint32_t dmax = 0;
+            {
+                const int key = lane & 31, half = lane >> 5;
+                const bool on = live >> key & 1;
+#pragma unroll
+                for (int i = 0; i < NBLK / 2; i++) {
+                    const int blk = half * (NBLK / 2) + i;
+                    const uint16_t dk = *(const uint16_t *) (my + key * C::LS + QBLOCK * blk);
+                    const uint16_t dv = on ? *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk) : (uint16_t) 0;
+                    kscl[blk * PA_TILE + key] = dk;
+                    vscl[blk * PA_TILE + key] = dv;
+                    const uint32_t mag = dv & 0x7fffu;
+                    dmax = max(dmax, mag < 0x7c00u ? mag : 0u);
+                }
+                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
+                if (half == 0) vmax[key] = (uint16_t) dmax;
+            }
+            for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
+            wave_lds_sync();
+
+            // S^T: lane (row ln, keys 16 u + 4 lg + r)
+            float s[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint8_t * kl = my + (16 * u + ln) * C::LS + 16 * lg;
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) {
+                    const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
+                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{0, 0, 0, 0}, 0, 0, 0);
+                    const uint2 dk = *(const uint2 *) (kscl + blk * PA_TILE + 16 * u + 4 * lg);
+                    acc[0] = __fmaf_rn((float) d[0], mul_f16lo(dq[blk], dk.x), acc[0]);
+                    acc[1] = __fmaf_rn((float) d[1], mul_f16hi(dq[blk], dk.x), acc[1]);
+                    acc[2] = __fmaf_rn((float) d[2], mul_f16lo(dq[blk], dk.y), acc[2]);
+                    acc[3] = __fmaf_rn((float) d[3], mul_f16hi(dq[blk], dk.y), acc[3]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[u][r] = acc[r];
+            }
+            if (masked) {
+                dmax = 0;                                  // of the keys that the row sees
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int k = 16 * u + 4 * lg + r;
+                        if (!(live >> k & 1) || key0 + k >= limit) s[u][r] = -INFINITY;
+                        else dmax = max(dmax, (uint32_t) vmax[k]);
+                    }
+                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 16));
+                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    top = fmaxf(top, masked && s[u][r] == -INFINITY ? -INFINITY : s[u][r] * a.c);
+            top = xmax_lanes16_32(top);
+            const int e = (int) (dmax >> 10) < 1 ? 1 : (int) (dmax >> 10);        // d < 2^(e - 14)
+            const float ref = top + (float) (e - 14 - PA_BIAS);
+            if (__ballot(ref > M + PA_SLACK)) {
+                const float to = fmaxf(M, ref);
+                const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - to);
+                M = to;
+                l *= f;
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) { O[blk][0] *= f; O[blk][1] *= f; }
+            }
+            const float m = M == -INFINITY ? 0.f : M;
+            float p[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[u][r] = masked && s[u][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fmaf_rn(s[u][r], a.c, -m));
+                    l += p[u][r];
+                }
+            // O^T: A lane (dims 2 ln + e of the block, keys 4 lg + r of both halves)
+            auto pv = [&](auto fn) {
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) {
+                    const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
+                    uint32_t av[2][4];
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) av[u][r] = *(const uint16_t *) (vl + (16 * u + r) * C::LS);
+                    v4u a0, a1, bh, bl;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t x0[2], x1[2];
+                        cvt_v_block(av[u], x0, x1);
+                        a0[2 * u] = x0[0]; a0[2 * u + 1] = x0[1];
+                        a1[2 * u] = x1[0]; a1[2 * u + 1] = x1[1];
+                        const uint2 dv = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
+                        uint32_t h0, h1, l0, l1;
+                        fn(p[u][0], p[u][1], dv.x, h0, l0);
+                        fn(p[u][2], p[u][3], dv.y, h1, l1);
+                        bh[2 * u] = h0; bh[2 * u + 1] = h1;
+                        bl[2 * u] = l0; bl[2 * u + 1] = l1;
+                    }
+                    const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
+                    const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
+                    O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[blk][0], 0, 0, 0);
+                    O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[blk][1], 0, 0, 0);
+                    O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[blk][0], 0, 0, 0);
+                    O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[blk][1], 0, 0, 0);
+                }
+            };
+            if (masked) pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo_masked(p0, p1, d, h, lo); });
+            else        pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo(p0, p1, d, h, lo); });
+        }
+        l = sum_lanes16_32(l);
+
+        // the waves' parts meet in LDS: O[row][dim] of each
+        __syncthreads();
+        float * ob = (float *) (lds + wave * C::WAVE) + ln * D;
+#pragma unroll
+        for (int blk = 0; blk < NBLK; blk++)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2)
+                *(float4 *) (ob + QK * blk + 8 * lg + 2 * r) = make_float4(O[blk][0][r], O[blk][1][r], O[blk][0][r + 1], O[blk][1][r + 1]);
+        if (lg == 0) ml[wave][ln] = make_float2(M, l);
+        __syncthreads();
+        {
+            const int r = tid >> 4, rr = 16 * rt + r;
+            float2 e[PA_WAVES];
+            float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; w++) { e[w] = ml[w][r]; mm = fmaxf(mm, e[w].x); }
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; w++) {
+                e[w].x = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - mm);
+                ll += e[w].x * e[w].y;
+            }
+            if (rr < a.R) {
+                const int t = rr / a.rep, h = kvh * a.rep + (rr - t * a.rep);
+                const size_t part = ((size_t) (run.pos / run.per + b) * a.nh_kv + kvh) * a.R + rr;
+                const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
+                for (int d0 = 4 * (tid & 15); d0 < D; d0 += 64) {
+                    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < PA_WAVES; w++) {
+                        const float4 x = *(const float4 *) ((const float *) (lds + w * C::WAVE) + r * D + d0);
+                        if (e[w].x != 0.f) {
+                            o[0] += e[w].x * x.x; o[1] += e[w].x * x.y; o[2] += e[w].x * x.z; o[3] += e[w].x * x.w;
+                        }
+                    }
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[i] *= inv;
+                        finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + d0, o);
+                    } else {
+                        *(float4 *) (a.part_o + part * D + d0) = make_float4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+                if (!whole && (tid & 15) == 0) a.part_ml[part] = make_float2(mm, ll);
+            }
+        }
+        run.left -= nt;
+        run.pos += nt;
+    }
+}
+
+// The parts of a request joined: a workgroup per query row and 64 dims, 16 groups of
+// 16 lanes that take every 16th part. Requests of one run are done; those without a
+// key are written here (0).
+constexpr int PM_GROUPS = 16;
+
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
+    __shared__ float4 acc[PM_GROUPS][16];
+    __shared__ float2 gl[PM_GROUPS];
+    const int quarter = blockIdx.x % (D / 64);
+    const int64_t rowi = blockIdx.x / (D / 64);
+    const int r = (int) (rowi % a.R), kvh = (int) (rowi / a.R % a.nh_kv), b = (int) (rowi / a.R / a.nh_kv);
+    const int g = threadIdx.x >> 4, q = threadIdx.x & 15;
+    const int t = r / a.rep, h = kvh * a.rep + (r - t * a.rep);
+    const size_t elem = (((size_t) b * a.T + t) * a.nh + h) * D + 64 * quarter + 4 * q;
+    const int32_t n = a.n_kv[b];
+    if (n <= 0) {
+        if (n < 0 && threadIdx.x == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+        if (g == 0) store4(a.dst + elem * (a.type == QWFN_TYPE_F32 ? 4 : 2), a.type, z);
+        return;
+    }
+    const int2 sp = a.span[b];
+    if (sp.x == sp.y) return;
+    float M = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = sp.x + g; s <= sp.y; s += PM_GROUPS) {
+        const size_t part = ((size_t) (s + b) * a.nh_kv + kvh) * a.R + r;
+        const float2 e = a.part_ml[part];
+        const float4 x = *(const float4 *) (a.part_o + part * D + 64 * quarter + 4 * q);
+        if (e.x == -INFINITY) continue;
+        const float to = fmaxf(M, e.x), f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to),
+                    w = __builtin_amdgcn_exp2f(e.x - to);
+        o.x = o.x * f + w * x.x; o.y = o.y * f + w * x.y; o.z = o.z * f + w * x.z; o.w = o.w * f + w * x.w;
+        l = l * f + w * e.y;
+        M = to;
+    }
+    acc[g][q] = o;
+    if (q == 0) gl[g] = make_float2(M, l);
+    __syncthreads();
+    if (g == 0) {
+        float mm = -INFINITY, ll = 0.f;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < PM_GROUPS; i++) mm = fmaxf(mm, gl[i].x);
+#pragma unroll
+        for (int i = 0; i < PM_GROUPS; i++) {
+            if (gl[i].x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(gl[i].x - mm);
+            const float4 v = acc[i][q];
+            ll += w * gl[i].y;
+            x[0] += w * v.x; x[1] += w * v.y; x[2] += w * v.z; x[3] += w * v.w;
+        }
+        const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] *= inv;
+        finish4(a, elem, x);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+struct pa_plan {
+    int32_t RT, runs;
+    size_t  off_o, off_ml, bytes;
+};
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Runs: as many as fill two workgroups a CU, whole rounds of the 8 XCDs; no more than the longest
+// requests could need.
+pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv) {
+    pa_plan p;
+    const int64_t R = T * (nh / nh_kv);
+    p.RT = (int32_t) ((R + 15) / 16);
+    const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE) + PA_MIN_TILES - 1) / PA_MIN_TILES;
+    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(PA_WGS / (nh_kv * p.RT), most));
+    const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
+    p.off_o = round256((size_t) n_seq * sizeof(int2));
+    p.off_ml = p.off_o + round256(parts * D * sizeof(float));
+    p.bytes = p.off_ml + round256(parts * sizeof(float2));
+    return p;
+}
+
+int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, int32_t max_pages, int32_t page_size,
+                pa_plan * pl) {
+    const char * op = "flash_attn_ext_paged";
+    auto err = [&](int code, const char * what) { return set_error2(code, op, what); };
+    if (!q || !q->data || !k || !k->data || !v || !v->data) return err(QWFN_EINVAL, ": q, k or v is NULL");
+    if (q->type != QWFN_TYPE_F32 && q->type != QWFN_TYPE_F16 && q->type != QWFN_TYPE_BF16)
+        return err(QWFN_EINVAL, ": q must be f32, f16 or bf16");
+    if (k->type != QWFN_TYPE_Q8_0 || v->type != QWFN_TYPE_Q8_0) return err(QWFN_EINVAL, ": k and v must be q8_0");
+    for (int i = 0; i < 4; i++)
+        if (q->ne[i] < 1 || k->ne[i] < 1) return err(QWFN_EINVAL, ": empty tensor");
+    const int64_t D = q->ne[0], T = q->ne[1], nh = q->ne[2], B = q->ne[3], nh_kv = k->ne[2];
+    if (D != 64 && D != 128 && D != 256) return err(QWFN_ENOTSUP, ": head size must be 64, 128 or 256");
+    if (k->ne[0] != D) return err(QWFN_EINVAL, ": q and k head sizes differ");
+    if (k->ne[3] != 1) return err(QWFN_ENOTSUP, ": k and v are one pool (ne[3] == 1)");
+    if (nh % nh_kv) return err(QWFN_EINVAL, ": n_head must be a multiple of n_head_kv");
+    if (T > PA_MAX_ROWS || T * (nh / nh_kv) > PA_MAX_ROWS)
+        return err(QWFN_ENOTSUP, ": at most 64 query rows per KV head (T * n_head / n_head_kv)");
+    if (nh_kv > 128) return err(QWFN_ENOTSUP, ": at most 128 KV heads");
+    if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff - 2 * PA_TILE * PA_WAVES)
+        return err(QWFN_EINVAL, ": page_size and max_pages must be positive, their product below 2^31 - 256");
+    if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1) > 0x7fffffff)
+        return err(QWFN_ENOTSUP, ": at most 65536 requests and 2^31 tiles of 32 keys");
+    if (B * nh * T * (D / 64) > 0x7fffffff) return err(QWFN_ENOTSUP, ": too many query rows");
+    if (k->ne[1] < page_size) return err(QWFN_EINVAL, ": the pool holds no whole page");
+    if (k->ne[1] > 0x7fffffff) return err(QWFN_ENOTSUP, ": a pool of at most 2^31 - 1 rows");
+    *pl = plan_paged(D, T, nh, nh_kv, B, (int64_t) page_size * max_pages);
+    return QWFN_OK;
+}
+
+template <int D>
+int launch_paged(const pa_args & a, hipStream_t s) {
+    const int64_t blocks = (int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * a.RT;
+    hipLaunchKernelGGL(k_paged_attn<D>, dim3((unsigned) blocks), dim3(PA_THREADS), 0, s, a);
+    if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
+    const int64_t rows = (int64_t) a.n_seq * a.nh_kv * a.R;
+    hipLaunchKernelGGL(k_paged_merge<D>, dim3((unsigned) (rows * (D / 64))), dim3(256), 0, s, a);
+    return hip_check(hipGetLastError(), "flash_attn_ext_paged launch");
+}
+
+}  // namespace
+}  // namespace qwfn
+
+using namespace qwfn;
+
+extern "C" size_t qwfn_fattn_workspace_size_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                                  int32_t max_pages, int32_t page_size) {
+    return ::qwfn::abi_value<size_t>("fattn_workspace_size_paged", 0, [&]() -> size_t {
+        pa_plan pl;
+        return check_paged(q, k, v, max_pages, page_size, &pl) ? 0 : pl.bytes;
+    });
+}
+
+extern "C" int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                              const int32_t * table, int64_t table_stride, int32_t max_pages,
+                                              int32_t page_size, const int32_t * n_kv, float scale, const qwfn_tensor * gate,
+                                              const qwfn_tensor * dst, int variant, void * ws, size_t ws_bytes,
+                                              void * stream) {
+    return ::qwfn::abi_call("flash_attn_ext_paged", [&]() -> int {
+        auto err = [&](int code, const char * what) { return set_error2(code, "flash_attn_ext_paged", what); };
+        pa_plan pl;
+        if (int rc = check_paged(q, k, v, max_pages, page_size, &pl)) return rc;
+        if (!table || !n_kv || !dst || !dst->data) return err(QWFN_EINVAL, ": table, n_kv or dst is NULL");
+        if (!std::isfinite(scale)) return err(QWFN_EINVAL, ": scale must be finite");
+        if (variant != QWFN_Q8_REF && variant != QWFN_Q8_X86) return err(QWFN_EINVAL, ": unknown rounding variant");
+        const int64_t D = q->ne[0], T = q->ne[1], nh = q->ne[2], B = q->ne[3], nh_kv = k->ne[2];
+        const size_t es = q->type == QWFN_TYPE_F32 ? 4 : 2, seg = (size_t) D / QK * QBLOCK, al = (size_t) D / 16;
+        for (int i = 0; i < 4; i++)
+            if (v->ne[i] != k->ne[i] || (i < 3 && v->nb[i] != k->nb[i]))
+                return err(QWFN_EINVAL, ": k and v must have the same shape and strides");
+        if (k->nb[0] != QBLOCK) return err(QWFN_EINVAL, ": k and v nb[0] must be 34");
+        if (!is_aligned(k->data, al) || !is_aligned(v->data, al) || k->nb[1] % al || k->nb[2] % al)
+            return err(QWFN_EALIGN, ": k and v rows and strides must be aligned to head size / 16 bytes");
+        if (k->nb[1] > 0xffffffffu) return err(QWFN_ENOTSUP, ": a row stride of 2^32 bytes or more");
+        // heads inside a row, or rows inside a head
+        if (k->nb[1] < (size_t) (nh_kv - 1) * k->nb[2] + seg && k->nb[2] < (size_t) (k->ne[1] - 1) * k->nb[1] + seg)
+            return err(QWFN_EINVAL, ": k and v rows or heads overlap");
+        if (k->nb[1] < seg || (nh_kv > 1 && k->nb[2] < seg)) return err(QWFN_EINVAL, ": k and v rows or heads overlap");
+        if (q->nb[0] != es) return err(QWFN_EINVAL, ": q rows must be contiguous");
+        if (!is_aligned(q->data, 16) || q->nb[1] % 16 || q->nb[2] % 16 || q->nb[3] % 16)
+            return err(QWFN_EALIGN, ": q must be 16-byte aligned");
+        const int64_t ne[4] = {D, nh, T, B};
+        for (int g = 0; g < 2; g++) {
+            const qwfn_tensor * t = g ? gate : dst;
+            if (!t) continue;
+            if (!t->data || t->type != q->type) return err(QWFN_EINVAL, g ? ": gate must have q's type" : ": dst must have q's type");
+            size_t nb = es;
+            for (int i = 0; i < 4; i++) {
+                if (t->ne[i] != ne[i] || t->nb[i] != nb)
+                    return err(QWFN_EINVAL, g ? ": gate must be contiguous [D, n_head, T, n_seq]" : ": dst must be contiguous [D, n_head, T, n_seq]");
+                nb *= (size_t) ne[i];
+            }
+            if (!is_aligned(t->data, 16)) return err(QWFN_EALIGN, g ? ": gate must be 16-byte aligned" : ": dst must be 16-byte aligned");
+        }
+        if (table_stride < max_pages && B > 1) return err(QWFN_EINVAL, ": table rows overlap (table_stride < max_pages)");
+        if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
+        if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
+        if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");
+        if (!ws) {
+            size_t got = 0;
+            if (int rc = library_workspace(pl.bytes, pl.bytes, as_stream(stream), &ws, &got)) return rc;
+        }
+        pa_args a{};
+        if (int rc = status_word(&a.status)) return rc;
+        a.q = (const char *) q->data; a.q_nb1 = q->nb[1]; a.q_nb2 = q->nb[2]; a.q_nb3 = q->nb[3];
+        a.k = (const char *) k->data; a.v = (const char *) v->data; a.nb1 = (uint32_t) k->nb[1]; a.nb2 = k->nb[2];
+        a.n_pages = k->ne[1] / page_size;
+        a.table = table; a.t_stride = table_stride; a.n_kv = n_kv; a.max_kv = (int64_t) max_pages * page_size;
+        a.page = make_div((uint32_t) page_size);
+        a.gate = gate ? (const char *) gate->data : nullptr; a.dst = (char *) dst->data; a.type = q->type;
+        a.n_seq = (int32_t) B; a.T = (int32_t) T; a.nh = (int32_t) nh; a.nh_kv = (int32_t) nh_kv;
+        a.rep = (int32_t) (nh / nh_kv); a.R = a.T * a.rep; a.RT = pl.RT; a.x86 = variant == QWFN_Q8_X86;
+        a.runs = pl.runs; a.c = scale * PA_LOG2E;
+        a.span = (int2 *) ws; a.part_o = (float *) ((char *) ws + pl.off_o); a.part_ml = (float2 *) ((char *) ws + pl.off_ml);
+        switch (D) {
+            case 64:  return launch_paged<64>(a, as_stream(stream));
+            case 128: return launch_paged<128>(a, as_stream(stream));
+            default:  return launch_paged<256>(a, as_stream(stream));
+        }
+    });
+}

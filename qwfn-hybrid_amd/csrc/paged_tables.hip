@@ -1,0 +1,373 @@
+// Page tables of the paged KV cache, built on the GPU from request lengths:
+// qwfn_paged_extend hands out pages and lists the new tokens' cache rows,
+// qwfn_paged_trim takes pages back. With P tokens a page:
+//   have = ceil(past / P), need = ceil((past + new) / P) - have
+//   c = inclusive sum of need over the requests; the i-th page of request b is
+//   free[n_free - 1 - (c_b - need_b + i)]
+//   token t of request b: p = past_b + t, row table[b][p / P] * P + p % P
+// and back: back = ceil(n_kv / P) - ceil(keep / P), to free[n_free + (sum of back
+// before b) + i].
+//
+// A few KB to a MB move, so the calls are bound by launches and the chain load ->
+// scan -> store, not by bytes. k_extend_scan / k_trim_scan are one workgroup: the
+// prefix sums need every request, and one workgroup that has read everything
+// before it writes is what lets the lengths and the stack's size be updated in
+// place. It also writes the lists of a decoding step itself (a thread per request
+// for the first tokens, a wave together for the rest). Where there are more than
+// EXT_FEW tokens a request on average, a second launch writes the lists, a thread
+// per token.
+#include "qwfn_common.h"
+#include "qwfn_paged.h"
+
+#include <algorithm>
+
+namespace qwfn {
+namespace {
+
+constexpr int PT_THREADS = 1024;       // of a scan
+constexpr int PT_WAVES   = PT_THREADS / 64;
+constexpr int EXT_FEW    = 8;          // tokens a request, on average, that the scan's workgroup still writes itself
+constexpr int ROW_THREADS = 256;       // of the second launches
+constexpr int64_t PT_MAX_SEQ = 65536;
+
+// What a scan leaves for the second launch.
+struct pt_req {
+    int32_t past;      // extend: tokens held; trim: first column given back
+    int32_t have;      // extend: pages held; trim: pages given back
+    int32_t at;        // the call's pages of the requests before this one
+    int32_t served;
+};
+struct pt_head {
+    int32_t n_free;    // at the start of the call, clipped
+    int32_t total;     // extend: listed tokens (cu_new[n_seq])
+    int32_t pad[2];
+};
+
+struct ext_args {
+    const int32_t * past; const int32_t * fresh;
+    int32_t *       table; int64_t t_stride;
+    const int32_t * free_pages; int32_t free_cap;
+    const int32_t * n_free; int32_t * n_free_out;
+    int32_t *       n_kv; int32_t * cu; int32_t * slots; int32_t * pos; int32_t * seq;
+    int64_t         n_tok;
+    int32_t         n_seq, page, max_pages, pad_slot;
+    int32_t         lists;             // the scan writes the lists and the table
+    pt_head *       head;
+    pt_req *        req;
+    uint32_t *      status;
+};
+
+__device__ __forceinline__ int64_t shfl_up64(int64_t v, int d) { return __shfl_up((long long) v, d); }
+
+// Inclusive sums of two values over the workgroup's threads, in thread order.
+struct pair64 { int64_t x, y; };
+__device__ __forceinline__ pair64 block_scan(pair64 v, pair64 (*part)[PT_WAVES]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t x = shfl_up64(v.x, d), y = shfl_up64(v.y, d);
+        if (lane >= d) { v.x += x; v.y += y; }
+    }
+    if (lane == 63) (*part)[w] = v;
+    __syncthreads();
+    for (int i = 0; i < w; i++) { v.x += (*part)[i].x; v.y += (*part)[i].y; }
+    return v;
+}
+
+__device__ __forceinline__ int64_t ceil_div(int64_t a, int32_t b) { return (int64_t) (((uint32_t) a + (uint32_t) b - 1u) / (uint32_t) b); }
+
+// Entry i of the lists: token t of request b. The first token of a new page writes its column.
+__device__ __forceinline__ void list_token(const ext_args & a, int64_t i, int32_t b, const pt_req & r, int32_t n_free, int64_t t) {
+    int32_t slot = a.pad_slot, pos = -1;
+    if (r.served) {
+        const uint32_t p = (uint32_t) (r.past + t), c = p / (uint32_t) a.page, at = p - c * (uint32_t) a.page;
+        int32_t * entry = a.table + (int64_t) b * a.t_stride + c;
+        int32_t page;
+        if ((int32_t) c >= r.have) {
+            page = a.free_pages[n_free - 1 - (r.at + ((int32_t) c - r.have))];
+            if (at == 0) *entry = page;
+        } else {
+            page = *entry;
+        }
+        if (page >= 0 && (int64_t) page * a.page + at <= 0x7fffffff) {
+            slot = page * a.page + (int32_t) at;
+            pos = (int32_t) p;
+        } else {
+            atomicOr(a.status, DEVERR_PAGES);
+        }
+    }
+    a.slots[i] = slot;
+    if (a.pos) a.pos[i] = pos;
+    if (a.seq) a.seq[i] = b;
+}
+
+__global__ __launch_bounds__(PT_THREADS) void k_extend_scan(ext_args a) {
+    __shared__ pair64 part[2][PT_WAVES];
+    __shared__ pair64 last;
+    const int tid = threadIdx.x, lane = tid & 63;
+    bool bad = false;
+    const int32_t nf_in = *a.n_free;
+    const int32_t n_free = nf_in < 0 ? 0 : nf_in > a.free_cap ? a.free_cap : nf_in;
+    bad |= n_free != nf_in;
+    const int64_t room = (int64_t) a.max_pages * a.page;
+    pair64 carry{0, 0};
+    int64_t given = 0;                       // pages handed out by this thread's requests
+    for (int64_t b0 = 0, it = 0; b0 < a.n_seq; b0 += blockDim.x, it++) {
+        const int64_t b = b0 + tid;
+        const bool in = b < a.n_seq;
+        const int32_t past_in = in ? a.past[b] : 0, new_in = in ? a.fresh[b] : 0;
+        const int32_t past = past_in < 0 ? 0 : past_in, fresh = new_in < 0 ? 0 : new_in;
+        bad |= past != past_in || fresh != new_in;
+        const int64_t total = (int64_t) past + fresh;
+        const int64_t have = ceil_div(past, a.page);
+        // the lists first: a request's tokens have to lie below n_tok
+        pair64 s = block_scan({fresh, 0}, &part[0]);
+        const int64_t cu1 = carry.x + s.x, cu0 = cu1 - fresh;
+        const bool fits = total <= room && cu1 <= a.n_tok;
+        const int64_t need = in && fits ? ceil_div(total, a.page) - have : 0;
+        const pair64 s2 = block_scan({fresh, need}, &part[1]);
+        const int64_t c = carry.y + s2.y;
+        pt_req r{past, (int32_t) have, (int32_t) (c - need < INT32_MAX ? c - need : INT32_MAX), in && fits && (need == 0 || c <= n_free)};
+        if (in) {
+            bad |= !r.served;
+            if (r.served) given += need;
+            a.n_kv[b] = r.served ? (int32_t) total : past;
+            if (b == 0) a.cu[0] = 0;
+            a.cu[b + 1] = (int32_t) (cu1 < a.n_tok ? cu1 : a.n_tok);
+            a.req[b] = r;
+        }
+        if (a.lists) {
+            // each thread the first tokens of its request, then the waves the rest together
+            const int64_t end = cu1 < a.n_tok ? cu1 : a.n_tok;
+            const int64_t n = in && cu0 < end ? end - cu0 : 0;
+            for (int64_t t = 0; t < n && t < 4; t++) list_token(a, cu0 + t, (int32_t) b, r, n_free, t);
+            uint64_t more = __ballot(n > 4);
+            while (more) {
+                const int src = __builtin_ctzll(more);
+                more &= more - 1;
+                const pt_req q{__shfl(r.past, src), __shfl(r.have, src), __shfl(r.at, src), __shfl(r.served, src)};
+                const int64_t at = __shfl((long long) cu0, src), cnt = __shfl((long long) n, src);
+                const int32_t bs = (int32_t) (b - lane + src);
+                for (int64_t t = 4 + lane; t < cnt; t += 64) list_token(a, at + t, bs, q, n_free, t);
+            }
+        }
+        // the running sums: the last thread's
+        if (tid == (int) blockDim.x - 1) last = {cu1, c};
+        __syncthreads();
+        carry = last;
+        __syncthreads();
+    }
+    const int64_t listed = carry.x < a.n_tok ? carry.x : a.n_tok;
+    if (a.lists)
+        for (int64_t i = listed + tid; i < a.n_tok; i += blockDim.x) {
+            a.slots[i] = a.pad_slot;
+            if (a.pos) a.pos[i] = -1;
+            if (a.seq) a.seq[i] = -1;
+        }
+    const pair64 g = block_scan({given, 0}, &part[0]);
+    if (tid == (int) blockDim.x - 1) {
+        *a.n_free_out = n_free - (int32_t) g.x;
+        *a.head = pt_head{n_free, (int32_t) listed, {0, 0}};
+    }
+    if (__ballot(bad) && lane == 0) atomicOr(a.status, DEVERR_PAGES);
+}
+
+// A thread per token: its request by bisection of cu_new.
+__global__ __launch_bounds__(ROW_THREADS) void k_extend_lists(ext_args a) {
+    const int64_t i = (int64_t) blockIdx.x * ROW_THREADS + threadIdx.x;
+    if (i >= a.n_tok) return;
+    const pt_head h = *a.head;
+    if (i >= h.total) {
+        a.slots[i] = a.pad_slot;
+        if (a.pos) a.pos[i] = -1;
+        if (a.seq) a.seq[i] = -1;
+        return;
+    }
+    int32_t lo = 0, hi = a.n_seq - 1;        // the last request whose list starts at or before i
+    while (lo < hi) {
+        const int32_t mid = (lo + hi + 1) >> 1;
+        if (a.cu[mid] <= i) lo = mid;
+        else hi = mid - 1;
+    }
+    list_token(a, i, lo, a.req[lo], h.n_free, i - a.cu[lo]);
+}
+
+struct trim_args {
+    const int32_t * keep; const int32_t * n_kv;
+    const int32_t * table; int64_t t_stride;
+    int32_t *       free_pages; int32_t free_cap;
+    const int32_t * n_free; int32_t * n_free_out; int32_t * n_kv_out;
+    int32_t         n_seq, page, max_pages;
+    pt_head *       head;
+    pt_req *        req;
+    uint32_t *      status;
+};
+
+__global__ __launch_bounds__(PT_THREADS) void k_trim_scan(trim_args a) {
+    __shared__ pair64 part[PT_WAVES];
+    __shared__ int64_t last;
+    const int tid = threadIdx.x, lane = tid & 63;
+    bool bad = false;
+    const int32_t nf_in = *a.n_free;
+    const int32_t n_free = nf_in < 0 ? 0 : nf_in > a.free_cap ? a.free_cap : nf_in;
+    bad |= n_free != nf_in;
+    const int32_t room = a.max_pages * a.page;
+    int64_t carry = 0, given = 0;
+    for (int64_t b0 = 0; b0 < a.n_seq; b0 += blockDim.x) {
+        const int64_t b = b0 + tid;
+        const bool in = b < a.n_seq;
+        const int32_t n_in = in ? a.n_kv[b] : 0, k_in = in ? a.keep[b] : 0;
+        const int32_t n = n_in < 0 ? 0 : n_in > room ? room : n_in;
+        bad |= n != n_in;
+        const int32_t keep = k_in < 0 ? 0 : k_in > n ? n : k_in;
+        const int32_t first = (int32_t) ceil_div(keep, a.page), back = (int32_t) ceil_div(n, a.page) - first;
+        const int64_t c = carry + block_scan({back, 0}, &part).x;
+        const bool served = in && (back == 0 || c <= a.free_cap - n_free);
+        if (in) {
+            bad |= !served;
+            a.n_kv_out[b] = served ? keep : n;
+            if (served) given += back;
+            a.req[b] = pt_req{first, served ? back : 0, (int32_t) (c - back < INT32_MAX ? c - back : INT32_MAX), served};
+            // the first pages here, more than that by the second launch
+            if (served)
+                for (int32_t i = 0; i < back && i < 2; i++)
+                    a.free_pages[n_free + (c - back) + i] = a.table[b * a.t_stride + first + i];
+        }
+        if (tid == (int) blockDim.x - 1) last = c;
+        __syncthreads();
+        carry = last;
+        __syncthreads();
+    }
+    const pair64 g = block_scan({given, 0}, &part);
+    if (tid == (int) blockDim.x - 1) {
+        *a.n_free_out = n_free + (int32_t) g.x;
+        *a.head = pt_head{n_free, 0, {0, 0}};
+    }
+    if (__ballot(bad) && lane == 0) atomicOr(a.status, DEVERR_PAGES);
+}
+
+// Pages 2 .. of the requests that give back more than two: a wave per request.
+__global__ __launch_bounds__(ROW_THREADS) void k_trim_pages(trim_args a) {
+    const int64_t b = (int64_t) blockIdx.x * (ROW_THREADS / 64) + (threadIdx.x >> 6);
+    if (b >= a.n_seq) return;
+    const pt_req r = a.req[b];
+    const int32_t * src = a.table + b * a.t_stride + r.past;
+    int32_t * dst = a.free_pages + a.head->n_free + (int64_t) r.at;
+    for (int32_t i = 2 + (threadIdx.x & 63); i < r.have; i += 64) dst[i] = src[i];
+}
+
+int scan_threads(int32_t n_seq) { return std::min(PT_THREADS, (n_seq + 63) / 64 * 64); }
+
+bool overlaps(const void * a, size_t an, const void * b, size_t bn) {
+    const uintptr_t x = (uintptr_t) a, y = (uintptr_t) b;
+    return a && b && an && bn && x < y + bn && y < x + an;
+}
+
+struct span { const void * p; size_t n; const char * name; };
+
+int check_tables(const char * op, int32_t n_seq, int32_t page_size, const int32_t * table, int64_t table_stride,
+                 int32_t max_pages, int32_t free_cap, const void * ws, size_t ws_bytes) {
+    const std::string o(op);
+    if (n_seq < 1 || n_seq > PT_MAX_SEQ) return set_error(QWFN_EINVAL, o + ": n_seq must lie in [1, 65536]");
+    if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff)
+        return set_error(QWFN_EINVAL, o + ": page_size and max_pages must be positive, their product below 2^31");
+    if (table_stride < max_pages) return set_error(QWFN_EINVAL, o + ": table rows overlap (table_stride < max_pages)");
+    if (free_cap < 0) return set_error(QWFN_EINVAL, o + ": free_cap must not be negative");
+    if (!ws || ws_bytes < qwfn_paged_workspace_size(n_seq))
+        return set_error(QWFN_ENOMEM, o + ": ws must hold qwfn_paged_workspace_size bytes");
+    if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, o + ": ws must be 16-byte aligned");
+    (void) table;
+    return QWFN_OK;
+}
+
+// Every span 4-byte aligned and present, and no `out` over another span; in-place pairs are passed once.
+int check_spans(const char * op, const span * in, int n_in, const span * out, int n_out) {
+    for (int i = 0; i < n_in + n_out; i++) {
+        const span & s = i < n_in ? in[i] : out[i - n_in];
+        if (!is_aligned(s.p, 4)) return set_error(QWFN_EALIGN, std::string(op) + ": " + s.name + " must be 4-byte aligned");
+    }
+    for (int i = 0; i < n_out; i++) {
+        for (int j = 0; j < n_in; j++)
+            if (overlaps(out[i].p, out[i].n, in[j].p, in[j].n))
+                return set_error(QWFN_EINVAL, std::string(op) + ": " + out[i].name + " overlaps " + in[j].name);
+        for (int j = 0; j < i; j++)
+            if (overlaps(out[i].p, out[i].n, out[j].p, out[j].n))
+                return set_error(QWFN_EINVAL, std::string(op) + ": " + out[i].name + " overlaps " + out[j].name);
+    }
+    return QWFN_OK;
+}
+
+}  // namespace
+}  // namespace qwfn
+
+using namespace qwfn;
+
+extern "C" size_t qwfn_paged_workspace_size(int32_t n_seq) {
+    return n_seq < 1 || n_seq > PT_MAX_SEQ ? 0 : sizeof(pt_head) + (size_t) n_seq * sizeof(pt_req);
+}
+
+extern "C" int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size,
+                                 int32_t * table, int64_t table_stride, int32_t max_pages, const int32_t * free_pages,
+                                 int32_t free_cap, const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv,
+                                 int32_t * cu_new, int32_t * slots, int32_t * pos, int32_t * seq, int64_t n_tok,
+                                 int32_t pad_slot, void * ws, size_t ws_bytes, void * stream) {
+    return ::qwfn::abi_call("paged_extend", [&]() -> int {
+        if (!n_past || !n_new || !table || !free_pages || !n_free || !n_free_out || !n_kv || !cu_new || (!slots && n_tok))
+            return set_error(QWFN_EINVAL, "paged_extend: NULL pointer");
+        if (int rc = check_tables("paged_extend", n_seq, page_size, table, table_stride, max_pages, free_cap, ws, ws_bytes))
+            return rc;
+        if (n_tok < 0 || n_tok > 0x7fffffff) return set_error(QWFN_EINVAL, "paged_extend: n_tok must lie in [0, 2^31)");
+        const size_t per = (size_t) n_seq * 4, tok = (size_t) n_tok * 4;
+        const size_t tab = ((size_t) (n_seq - 1) * table_stride + max_pages) * 4;
+        const span in[] = {{n_kv == n_past ? nullptr : n_past, per, "n_past"}, {n_new, per, "n_new"},
+                           {free_pages, (size_t) free_cap * 4, "free_pages"},
+                           {n_free_out == n_free ? nullptr : n_free, 4, "n_free"}};
+        const span out[] = {{table, tab, "table"}, {n_free_out, 4, "n_free_out"}, {n_kv, per, "n_kv"},
+                            {cu_new, per + 4, "cu_new"}, {slots, tok, "slots"}, {pos, tok, "pos"}, {seq, tok, "seq"},
+                            {ws, qwfn_paged_workspace_size(n_seq), "ws"}};
+        if (int rc = check_spans("paged_extend", in, 4, out, 8)) return rc;
+        ext_args a{};
+        if (int rc = status_word(&a.status)) return rc;
+        a.past = n_past; a.fresh = n_new; a.table = table; a.t_stride = table_stride;
+        a.free_pages = free_pages; a.free_cap = free_cap; a.n_free = n_free; a.n_free_out = n_free_out;
+        a.n_kv = n_kv; a.cu = cu_new; a.slots = slots; a.pos = pos; a.seq = seq; a.n_tok = n_tok;
+        a.n_seq = n_seq; a.page = page_size; a.max_pages = max_pages; a.pad_slot = pad_slot;
+        a.head = (pt_head *) ws; a.req = (pt_req *) ((char *) ws + sizeof(pt_head));
+        a.lists = n_tok <= (int64_t) EXT_FEW * n_seq;
+        hipLaunchKernelGGL(k_extend_scan, dim3(1), dim3(scan_threads(n_seq)), 0, as_stream(stream), a);
+        if (int rc = hip_check(hipGetLastError(), "paged_extend launch")) return rc;
+        if (a.lists) return QWFN_OK;
+        hipLaunchKernelGGL(k_extend_lists, dim3((unsigned) ((n_tok + ROW_THREADS - 1) / ROW_THREADS)), dim3(ROW_THREADS), 0,
+                           as_stream(stream), a);
+        return hip_check(hipGetLastError(), "paged_extend launch");
+    });
+}
+
+extern "C" int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq, int32_t page_size,
+                               const int32_t * table, int64_t table_stride, int32_t max_pages, int32_t * free_pages,
+                               int32_t free_cap, const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv_out,
+                               void * ws, size_t ws_bytes, void * stream) {
+    return ::qwfn::abi_call("paged_trim", [&]() -> int {
+        if (!n_keep || !n_kv || !table || !free_pages || !n_free || !n_free_out || !n_kv_out)
+            return set_error(QWFN_EINVAL, "paged_trim: NULL pointer");
+        if (int rc = check_tables("paged_trim", n_seq, page_size, table, table_stride, max_pages, free_cap, ws, ws_bytes))
+            return rc;
+        const size_t per = (size_t) n_seq * 4, tab = ((size_t) (n_seq - 1) * table_stride + max_pages) * 4;
+        const span in[] = {{n_keep, per, "n_keep"}, {n_kv_out == n_kv ? nullptr : n_kv, per, "n_kv"}, {table, tab, "table"},
+                           {n_free_out == n_free ? nullptr : n_free, 4, "n_free"}};
+        const span out[] = {{free_pages, (size_t) free_cap * 4, "free_pages"}, {n_free_out, 4, "n_free_out"},
+                            {n_kv_out, per, "n_kv_out"}, {ws, qwfn_paged_workspace_size(n_seq), "ws"}};
+        if (int rc = check_spans("paged_trim", in, 4, out, 4)) return rc;
+        trim_args a{};
+        if (int rc = status_word(&a.status)) return rc;
+        a.keep = n_keep; a.n_kv = n_kv; a.table = table; a.t_stride = table_stride;
+        a.free_pages = free_pages; a.free_cap = free_cap; a.n_free = n_free; a.n_free_out = n_free_out; a.n_kv_out = n_kv_out;
+        a.n_seq = n_seq; a.page = page_size; a.max_pages = max_pages;
+        a.head = (pt_head *) ws; a.req = (pt_req *) ((char *) ws + sizeof(pt_head));
+        hipLaunchKernelGGL(k_trim_scan, dim3(1), dim3(scan_threads(n_seq)), 0, as_stream(stream), a);
+        if (int rc = hip_check(hipGetLastError(), "paged_trim launch")) return rc;
+        hipLaunchKernelGGL(k_trim_pages, dim3((unsigned) ((n_seq + ROW_THREADS / 64 - 1) / (ROW_THREADS / 64))),
+                           dim3(ROW_THREADS), 0, as_stream(stream), a);
+        return hip_check(hipGetLastError(), "paged_trim launch");
+    });
+}

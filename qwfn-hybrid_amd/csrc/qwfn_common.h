@@ -19,6 +19,7 @@ constexpr int QBLOCK  = 34;
 // Device-side error flag bits (qwfn_device_status).
 constexpr uint32_t DEVERR_SET_ROWS_INDEX = 1u << 0;
 constexpr uint32_t DEVERR_GET_ROWS_INDEX = 1u << 1;
+constexpr uint32_t DEVERR_PAGES          = 1u << 2;
 
 // x / d through m = ceil(2^32 / d): floor(x * m / 2^32) = floor(x / d) while
 // x * d < 2^32 (the host checks the ranges of a call); d = 1 needs no m.

@@ -28,6 +28,7 @@ OK, EINVAL, ERANGE, EALIGN, ENOTSUP, EDEVICE, ENOMEM, ESIZE = 0, -1, -2, -3, -4,
 
 DEVERR_SET_ROWS_INDEX = 1
 DEVERR_GET_ROWS_INDEX = 2
+DEVERR_PAGES = 4
 
 # attention kernel families (qwfn_fattn_force_kernel)
 FA_KERNEL_AUTO, FA_KERNEL_VD, FA_KERNEL_DEC, FA_KERNEL_GENERAL, FA_KERNEL_PRE, FA_KERNEL_VS = 0, 1, 2, 3, 4, 5
@@ -156,7 +157,10 @@ EXPORTS = [
     "qwfn_snap_pool_split", "qwfn_snap_pool_restore_or_reset",
     "qwfn_qsa_select_workspace_size", "qwfn_qsa_select_cells",
     "qwfn_qsa_pool_cfg_default", "qwfn_set_rows_f16", "qwfn_qsa_pool_decode", "qwfn_qsa_pool_rebuild",
-    "qwfn_gated_delta_net",
+    "qwfn_gated_delta_net", "qwfn_linear_attn_workspace_size", "qwfn_linear_attn",
+    # include/qwfn_paged.h
+    "qwfn_paged_workspace_size", "qwfn_paged_extend", "qwfn_paged_trim", "qwfn_fattn_workspace_size_paged",
+    "qwfn_flash_attn_ext_q8_0_paged",
 ]
 
 _lib = None
@@ -281,6 +285,18 @@ def load(path: str = LIB_PATH):
     L.qwfn_qsa_pool_rebuild.argtypes = [vp, i64, i64, i32, vp, vp, i64, ctypes.POINTER(QsaPoolCfg), vp]
     L.qwfn_gated_delta_net.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, ctypes.c_float, vp, vp,
                                        vp, sz, i32, vp]
+    L.qwfn_linear_attn_workspace_size.argtypes = [T, T, i32, i32]
+    L.qwfn_linear_attn_workspace_size.restype = sz
+    L.qwfn_linear_attn.argtypes = [T, T, T, vp, i64, vp, i32, i32, vp, i32, vp, vp, ctypes.c_float, T, vp, sz, vp]
+    # include/qwfn_paged.h
+    L.qwfn_paged_workspace_size.argtypes = [i32]
+    L.qwfn_paged_workspace_size.restype = sz
+    L.qwfn_paged_extend.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp, sz, vp]
+    L.qwfn_paged_trim.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp, sz, vp]
+    L.qwfn_fattn_workspace_size_paged.argtypes = [T, T, T, i32, i32]
+    L.qwfn_fattn_workspace_size_paged.restype = sz
+    L.qwfn_flash_attn_ext_q8_0_paged.argtypes = [T, T, T, vp, i64, i32, i32, vp, ctypes.c_float, T, T, ctypes.c_int, vp,
+                                                 sz, vp]
     L.qwfn_qsa_select_workspace_size.argtypes = [i64, i32]
     L.qwfn_qsa_select_workspace_size.restype = sz
     L.qwfn_qsa_select_cells.argtypes = [vp, sz, i64, vp, i32, sz, vp, sz, i32, i32, vp, i32, vp, vp, vp, sz, vp]
@@ -356,14 +372,23 @@ def f32_view(t) -> Tensor:
     return tensor(t.data_ptr(), TYPE_F32, dims, strides)
 
 
+def float_type(t) -> int:
+    """TYPE_F32, TYPE_F16 or TYPE_BF16 of a torch tensor."""
+    import torch
+    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if t.dtype not in types:
+        raise ValueError(f"a float32, float16 or bfloat16 tensor is needed, got {t.dtype}")
+    return types[t.dtype]
+
+
 def q_view(q) -> Tensor:
     """Q in the projection's natural order, torch [B, T, n_head, hd] (or [T, n_head, hd]),
     as the graph's permuted view [hd, T, n_head, B] (qwfn_graph.cpp:466, :697)."""
     if q.dim() == 3:
         q = q.unsqueeze(0)
     B, T, nh, hd = q.shape
-    s = q.stride()
-    return tensor(q.data_ptr(), TYPE_F32, (hd, T, nh, B), (4, s[1] * 4, s[2] * 4, s[0] * 4))
+    s, e = q.stride(), q.element_size()
+    return tensor(q.data_ptr(), float_type(q), (hd, T, nh, B), (s[3] * e, s[1] * e, s[2] * e, s[0] * e))
 
 
 def mask_view(mask) -> Tensor:
@@ -376,11 +401,19 @@ def mask_view(mask) -> Tensor:
 
 
 def out_view(out) -> Tensor:
-    """Output torch [B, T, n_head, hd] float32 contiguous = ggml [hd, n_head, T, B]."""
+    """Output torch [B, T, n_head, hd], contiguous (float32 but for the paged attention) = ggml [hd, n_head, T, B]."""
     if out.dim() == 3:
         out = out.unsqueeze(0)
     B, T, nh, hd = out.shape
-    return tensor(out.data_ptr(), TYPE_F32, (hd, nh, T, B), (4, hd * 4, hd * nh * 4, hd * nh * T * 4))
+    e = out.element_size()
+    return tensor(out.data_ptr(), float_type(out), (hd, nh, T, B), (e, hd * e, hd * nh * e, hd * nh * T * e))
+
+
+def heads_view(x) -> Tensor:
+    """Packed tokens torch [n_tok, n_heads, d] (contiguous rows) = ggml [d, n_heads, n_tok]."""
+    n, h, d = x.shape
+    s, e = x.stride(), x.element_size()
+    return tensor(x.data_ptr(), float_type(x), (d, h, n, 1), (s[2] * e, s[1] * e, s[0] * e, max(1, n) * s[0] * e))
 
 
 # --------------------------------------------------------------------- ops
@@ -711,3 +744,123 @@ def gated_delta_net(q, k, v, g, beta, state, out, n_k: int, snap=None, n_snap: i
                                              state.data_ptr(), out.data_ptr(),
                                              snap.data_ptr() if snap is not None else None,
                                              snap.stride(0) * 4 if snap is not None else 0, n_snap, _stream(stream)))
+
+
+# --------------------------------------------------------------------- paged cache
+
+def _dev_i32(op, **tensors):
+    """Device int32 tensors, contiguous (a table: contiguous rows), all on one GPU."""
+    where = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if str(t.dtype) != "torch.int32" or not t.is_cuda:
+            raise ValueError(f"{op}: {name} must be a device int32 tensor")
+        if (t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1) or (t.dim() < 2 and not t.is_contiguous()):
+            raise ValueError(f"{op}: {name} must have contiguous rows")
+        if where is not None and t.device != where:
+            raise ValueError(f"{op}: {name} must be on {where}")
+        where = t.device
+
+
+def _lengths(op, n, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (t.dim() != 1 or t.shape[0] < n):
+            raise ValueError(f"{op}: {name} must be [{n}]")
+
+
+def _ws(ws):
+    return (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (None, 0)
+
+
+def paged_workspace_size(n_seq: int) -> int:
+    return int(load().qwfn_paged_workspace_size(n_seq))
+
+
+def paged_extend(n_past, n_new, page_size: int, table, free_pages, n_free, n_free_out, n_kv, cu_new, slots, pos=None,
+                 seq=None, pad_slot: int = -1, ws=None, stream=None):
+    """Pages and cache rows for n_new[b] more tokens of each request: device int32 n_past, n_new, n_kv [n_seq] (n_kv may
+    be n_past), table [n_seq, max_pages], free_pages [free_cap], n_free, n_free_out [1] (may be one tensor), cu_new
+    [n_seq + 1], slots, pos, seq [n_tok]."""
+    n_seq = n_past.shape[0]
+    _dev_i32("paged_extend", n_past=n_past, n_new=n_new, table=table, free_pages=free_pages, n_free=n_free,
+             n_free_out=n_free_out, n_kv=n_kv, cu_new=cu_new, slots=slots, pos=pos, seq=seq)
+    if table.dim() != 2 or table.shape[0] < n_seq:
+        raise ValueError(f"paged_extend: table must be [{n_seq}, max_pages]")
+    _lengths("paged_extend", n_seq, n_new=n_new, n_kv=n_kv)
+    _lengths("paged_extend", n_seq + 1, cu_new=cu_new)
+    _lengths("paged_extend", slots.shape[0], pos=pos, seq=seq)
+    _lengths("paged_extend", 1, n_free=n_free, n_free_out=n_free_out)
+    p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    return check(load().qwfn_paged_extend(p(n_past), p(n_new), n_seq, page_size, p(table), table.stride(0), table.shape[1],
+                                          p(free_pages), free_pages.shape[0], p(n_free), p(n_free_out), p(n_kv), p(cu_new),
+                                          p(slots), p(pos), p(seq), slots.shape[0], pad_slot, *_ws(ws), _stream(stream)))
+
+
+def paged_trim(n_keep, n_kv, page_size: int, table, free_pages, n_free, n_free_out, n_kv_out, ws=None, stream=None):
+    """Request b keeps its first n_keep[b] of n_kv[b] tokens; the pages behind them go onto the free stack. Tensors as
+    in paged_extend; n_kv_out may be n_kv, n_free_out n_free."""
+    n_seq = n_kv.shape[0]
+    _dev_i32("paged_trim", n_keep=n_keep, n_kv=n_kv, table=table, free_pages=free_pages, n_free=n_free,
+             n_free_out=n_free_out, n_kv_out=n_kv_out)
+    if table.dim() != 2 or table.shape[0] < n_seq:
+        raise ValueError(f"paged_trim: table must be [{n_seq}, max_pages]")
+    _lengths("paged_trim", n_seq, n_keep=n_keep, n_kv_out=n_kv_out)
+    _lengths("paged_trim", 1, n_free=n_free, n_free_out=n_free_out)
+    return check(load().qwfn_paged_trim(n_keep.data_ptr(), n_kv.data_ptr(), n_seq, page_size, table.data_ptr(),
+                                        table.stride(0), table.shape[1], free_pages.data_ptr(), free_pages.shape[0],
+                                        n_free.data_ptr(), n_free_out.data_ptr(), n_kv_out.data_ptr(), *_ws(ws),
+                                        _stream(stream)))
+
+
+def fattn_workspace_size_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int) -> int:
+    return int(load().qwfn_fattn_workspace_size_paged(ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.shape[1],
+                                                      page_size))
+
+
+def flash_attn_ext_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int, n_kv, scale: float, ov: Tensor,
+                         gate=None, variant: int = Q8_X86, ws=None, stream=None):
+    """Attention of each request's last T tokens over its pages: qv of torch [n_seq, T, n_head, hd] (q_view), kv and vv
+    views of the pool's caches (cache_attn_view over all rows), table device int32 [n_seq, max_pages], n_kv device
+    int32 [n_seq]; times sigmoid(gate) when gate (laid out as the output) is given."""
+    n_seq = qv.ne[3]
+    _dev_i32("flash_attn_ext_paged", table=table, n_kv=n_kv)
+    if table.dim() != 2 or table.shape[0] < n_seq:
+        raise ValueError(f"flash_attn_ext_paged: table must be [{n_seq}, max_pages]")
+    _lengths("flash_attn_ext_paged", n_seq, n_kv=n_kv)
+    gv = out_view(gate) if gate is not None else None
+    return check(load().qwfn_flash_attn_ext_q8_0_paged(
+        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.shape[1], page_size,
+        n_kv.data_ptr(), scale, ctypes.byref(gv) if gv is not None else None, ctypes.byref(ov), variant, *_ws(ws),
+        _stream(stream)))
+
+
+# --------------------------------------------------------------------- linear attention
+
+def linear_attn_workspace_size(q, v, n_seq: int, max_len: int) -> int:
+    return int(load().qwfn_linear_attn_workspace_size(ctypes.byref(heads_view(q)), ctypes.byref(heads_view(v)), n_seq,
+                                                      max_len))
+
+
+def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=None, scale: float | None = None, ws=None,
+                stream=None):
+    """Linear attention with a decay per head over packed sequences: q, k torch [n_tok, n_k, dk], v, out [n_tok, n_v, dv]
+    (float32, float16 or bfloat16, one type); g float32 [n_tok, n_v], or [n_v] for constant decays; cu device int32
+    [n_seq + 1]; state_in (or None), state_out float32 [n_slots, n_v, dk, dv]; slots device int32 [n_seq] or None."""
+    n_seq, n_tok, dk = cu.shape[0] - 1, q.shape[0], q.shape[2]
+    _dev_i32("linear_attn", cu=cu, slots=slots)
+    _lengths("linear_attn", n_seq, slots=slots)
+    want = (state_out.shape[0], v.shape[1], dk, v.shape[2])
+    for name, t in (("state_in", state_in), ("state_out", state_out)):
+        if t is not None and (str(t.dtype) != "torch.float32" or tuple(t.shape) != want or not t.is_contiguous()):
+            raise ValueError(f"linear_attn: {name} must be contiguous float32 {list(want)}")
+    if str(g.dtype) != "torch.float32" or g.shape[-1] != v.shape[1] or (g.stride(-1) != 1 and g.shape[-1] > 1) \
+            or g.dim() not in (1, 2) or (g.dim() == 2 and g.shape[0] < n_tok):
+        raise ValueError("linear_attn: g must be float32 [n_tok, n_v] or [n_v]")
+    scale = dk ** -0.5 if scale is None else scale
+    qv, kv, vv, ov = (heads_view(x) for x in (q, k, v, out))
+    return check(load().qwfn_linear_attn(
+        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0,
+        cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.shape[0],
+        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, ctypes.byref(ov), *_ws(ws),
+        _stream(stream)))

@@ -1,0 +1,152 @@
+"""Refusals of the paged-cache and linear-attention entry points, before anything is launched."""
+import ctypes
+
+import pytest
+
+import qwfn_kv as K
+
+FAKE = 0x7F0000000000          # never dereferenced: validation fails first
+GB = 1 << 30
+
+
+def refused(rc, code, needle):
+    assert rc == code, (rc, K.load().qwfn_last_error())
+    assert needle in K.load().qwfn_last_error().decode(), K.load().qwfn_last_error()
+
+
+def extend(**kw):
+    a = dict(past=FAKE, new=FAKE + GB, n_seq=4, page=16, table=FAKE + 2 * GB, stride=8, cols=8, free=FAKE + 3 * GB, cap=10,
+             n_free=FAKE + 4 * GB, n_free_out=FAKE + 5 * GB, n_kv=FAKE + 6 * GB, cu=FAKE + 7 * GB, slots=FAKE + 8 * GB,
+             pos=None, seq=None, n_tok=9, pad=-1, ws=FAKE + 9 * GB, ws_bytes=1 << 20)
+    a.update(kw)
+    return K.load().qwfn_paged_extend(*a.values(), None)
+
+
+def trim(**kw):
+    a = dict(keep=FAKE, n_kv=FAKE + GB, n_seq=4, page=16, table=FAKE + 2 * GB, stride=8, cols=8, free=FAKE + 3 * GB, cap=10,
+             n_free=FAKE + 4 * GB, n_free_out=FAKE + 5 * GB, n_kv_out=FAKE + 6 * GB, ws=FAKE + 9 * GB, ws_bytes=1 << 20)
+    a.update(kw)
+    return K.load().qwfn_paged_trim(*a.values(), None)
+
+
+@pytest.mark.parametrize("call", [extend, trim])
+def test_tables_refusals(call):
+    refused(call(n_free=None), K.EINVAL, "NULL")
+    refused(call(table=None), K.EINVAL, "NULL")
+    refused(call(n_seq=0), K.EINVAL, "n_seq")
+    refused(call(n_seq=65537), K.EINVAL, "n_seq")
+    refused(call(page=0), K.EINVAL, "page_size")
+    refused(call(cols=0), K.EINVAL, "max_pages")
+    refused(call(page=1 << 20, cols=1 << 11, stride=1 << 11), K.EINVAL, "2^31")
+    refused(call(stride=7), K.EINVAL, "overlap")
+    refused(call(cap=-1), K.EINVAL, "free_cap")
+    refused(call(ws=None), K.ENOMEM, "ws")
+    refused(call(ws_bytes=16), K.ENOMEM, "ws")
+    refused(call(ws=FAKE + 9 * GB + 4), K.EALIGN, "16-byte")
+    refused(call(table=FAKE + 2 * GB + 2), K.EALIGN, "table")
+    refused(call(free=FAKE + 2 * GB + 4), K.EINVAL, "overlaps")
+    refused(call(n_free=FAKE + 5 * GB + 4, n_free_out=FAKE + 5 * GB + 2), K.EALIGN, "n_free_out")
+    assert K.paged_workspace_size(0) == 0 and K.paged_workspace_size(65537) == 0 and K.paged_workspace_size(5) > 0
+
+
+def test_extend_refusals():
+    refused(extend(n_tok=-1), K.EINVAL, "n_tok")
+    refused(extend(n_tok=1 << 31), K.EINVAL, "n_tok")
+    refused(extend(slots=None), K.EINVAL, "NULL")
+    refused(extend(n_kv=FAKE + 4), K.EINVAL, "n_kv overlaps n_past")
+    refused(extend(n_kv=FAKE + GB), K.EINVAL, "n_kv overlaps n_new")
+    refused(extend(pos=FAKE + 8 * GB + 32), K.EINVAL, "pos overlaps slots")
+    refused(extend(cu=FAKE + 9 * GB + 64), K.EINVAL, "ws overlaps cu_new")
+    refused(trim(n_kv_out=FAKE + GB + 8), K.EINVAL, "n_kv_out overlaps n_kv")
+
+
+def paged_views(D=256, T=1, nh=16, B=4, kvh=2, rows=640, qtype=K.TYPE_F32, nb1=None, nb2=None):
+    es = 4 if qtype == K.TYPE_F32 else 2
+    seg = D // 32 * 34
+    q = K.tensor(FAKE, qtype, (D, T, nh, B), (es, nh * D * es, D * es, T * nh * D * es))
+    k = K.tensor(FAKE + GB, K.TYPE_Q8_0, (D, rows, kvh, 1), (34, nb1 or kvh * seg, nb2 or seg, rows * kvh * seg))
+    o = K.tensor(FAKE + 2 * GB, qtype, (D, nh, T, B), (es, D * es, nh * D * es, T * nh * D * es))
+    return q, k, o
+
+
+def paged(q, k, o, v=None, table=FAKE, stride=40, cols=40, page=16, n_kv=FAKE, scale=0.0625, gate=None, variant=1,
+          ws=FAKE + 3 * GB, ws_bytes=1 << 30):
+    r = ctypes.byref
+    return K.load().qwfn_flash_attn_ext_q8_0_paged(r(q), r(k), r(v or k), table, stride, cols, page, n_kv, scale,
+                                                   r(gate) if gate else None, r(o), variant, ws, ws_bytes, None)
+
+
+def test_paged_attention_refusals():
+    q, k, o = paged_views()
+    assert K.load().qwfn_fattn_workspace_size_paged(ctypes.byref(q), ctypes.byref(k), ctypes.byref(k), 40, 16) > 0
+    for D in (32, 96, 512):
+        refused(paged(*paged_views(D=D)), K.ENOTSUP, "head size")
+    refused(paged(*paged_views(qtype=K.TYPE_I32)), K.EINVAL, "f32, f16 or bf16")
+    refused(paged(*paged_views(nh=15)), K.EINVAL, "multiple of n_head_kv")
+    refused(paged(*paged_views(T=9)), K.ENOTSUP, "64 query rows")
+    refused(paged(*paged_views(rows=15)), K.EINVAL, "no whole page")
+    refused(paged(*paged_views(nb1=544 + 8)), K.EALIGN, "aligned")
+    refused(paged(*paged_views(nb1=528)), K.EINVAL, "overlap")
+    refused(paged(*paged_views(nb2=256)), K.EINVAL, "overlap")
+    refused(paged(q, k, o, table=None), K.EINVAL, "NULL")
+    refused(paged(q, k, o, n_kv=None), K.EINVAL, "NULL")
+    refused(paged(q, k, o, page=0), K.EINVAL, "page_size")
+    refused(paged(q, k, o, cols=1 << 27, stride=1 << 27), K.EINVAL, "2^31")
+    refused(paged(q, k, o, stride=39), K.EINVAL, "overlap")
+    refused(paged(q, k, o, scale=float("inf")), K.EINVAL, "finite")
+    refused(paged(q, k, o, variant=3), K.EINVAL, "variant")
+    refused(paged(q, k, o, ws_bytes=64), K.ENOMEM, "ws")
+    refused(paged(q, k, o, ws=FAKE + 8), K.EALIGN, "ws")
+    refused(paged(q, k, o, n_kv=FAKE + 2), K.EALIGN, "n_kv")
+    refused(paged(q, k, o, v=paged_views(rows=641)[1]), K.EINVAL, "same shape")
+    half = paged_views(qtype=K.TYPE_BF16)[2]
+    refused(paged(q, k, half), K.EINVAL, "dst must have q's type")
+    refused(paged(q, k, o, gate=half), K.EINVAL, "gate must have q's type")
+    wrong = paged_views(B=3)[2]
+    refused(paged(q, k, wrong), K.EINVAL, "dst must be contiguous")
+    refused(paged(q, k, o, gate=wrong), K.EINVAL, "gate must be contiguous")
+    q.data = FAKE + 4
+    refused(paged(q, k, o), K.EALIGN, "q must be")
+    q.data = None
+    refused(paged(q, k, o), K.EINVAL, "NULL")
+
+
+def heads(d, h, n, typ=K.TYPE_BF16, at=FAKE, stride=None):
+    es = 4 if typ == K.TYPE_F32 else 2
+    return K.tensor(at, typ, (d, h, n, 1), (es, d * es, stride or d * h * es, (n or 1) * d * h * es))
+
+
+def linear(q=None, k=None, v=None, g=FAKE, g_ts=6, cu=FAKE, n_seq=3, max_len=50, slots=None, n_slots=4, s_in=FAKE,
+           s_out=FAKE + GB, scale=1.0, dst=None, ws=FAKE, ws_bytes=1 << 30):
+    r = ctypes.byref
+    q, k = q or heads(128, 2, 100), k or heads(128, 2, 100)
+    v, dst = v or heads(128, 6, 100), dst or heads(128, 6, 100)
+    return K.load().qwfn_linear_attn(r(q), r(k), r(v), g, g_ts, cu, n_seq, max_len, slots, n_slots, s_in, s_out, scale, r(dst),
+                                     ws, ws_bytes, None)
+
+
+def test_linear_attention_refusals():
+    refused(linear(g=None), K.EINVAL, "NULL")
+    refused(linear(cu=None), K.EINVAL, "NULL")
+    refused(linear(s_out=None), K.EINVAL, "NULL")
+    refused(linear(q=heads(128, 2, 100, K.TYPE_I32)), K.EINVAL, "f32, f16 or bf16")
+    refused(linear(k=heads(128, 2, 100, K.TYPE_F16)), K.EINVAL, "one type")
+    refused(linear(dst=heads(128, 6, 100, K.TYPE_F32)), K.EINVAL, "one type")
+    refused(linear(q=heads(120, 2, 100), k=heads(120, 2, 100)), K.ENOTSUP, "multiples of 16")
+    refused(linear(q=heads(272, 2, 100), k=heads(272, 2, 100)), K.ENOTSUP, "at most 256")
+    refused(linear(v=heads(528, 6, 100), dst=heads(528, 6, 100)), K.ENOTSUP, "dv at most 512")
+    refused(linear(v=heads(128, 5, 100), dst=heads(128, 5, 100)), K.EINVAL, "multiple of n_k_heads")
+    refused(linear(v=heads(128, 6, 99)), K.EINVAL, "same tokens")
+    refused(linear(k=heads(128, 2, 99)), K.EINVAL, "same shape")
+    refused(linear(dst=heads(128, 6, 99)), K.EINVAL, "v's shape")
+    refused(linear(dst=heads(128, 6, 100, stride=128 * 6 * 2 + 16)), K.EINVAL, "contiguous")
+    refused(linear(q=heads(128, 2, 100, at=FAKE + 8)), K.EALIGN, "16-byte")
+    refused(linear(q=heads(128, 2, 100, stride=520)), K.EALIGN, "16-byte")
+    refused(linear(n_seq=0), K.EINVAL, "n_seq")
+    refused(linear(max_len=0), K.EINVAL, "max_len")
+    refused(linear(g_ts=5), K.EINVAL, "g_token_stride")
+    refused(linear(n_slots=2), K.EINVAL, "slots")
+    refused(linear(scale=float("nan")), K.EINVAL, "scale")
+    refused(linear(s_in=FAKE + 4), K.EALIGN, "16-byte")
+    refused(linear(s_in=FAKE + GB + 4096), K.EINVAL, "overlap")
+    assert linear(q=heads(128, 2, 0), k=heads(128, 2, 0), v=heads(128, 6, 0), dst=heads(128, 6, 0)) == K.OK   # no tokens
