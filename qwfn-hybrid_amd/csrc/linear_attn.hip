@@ -7,7 +7,8 @@
 // rows rg + 16 i; the state stays in registers for the sequence's tokens and is
 // read and written once. The output's sum over rows is finished across the lanes
 // (permlane swaps) and the waves (LDS), in a fixed order, one barrier a token.
-// What bounds it: the state, 8 dk dv bytes a head and sequence.
+// What bounds it: the state, 8 dk dv bytes a head and sequence. Longer sequences run
+// in chunks (below).
 #include "fattn_device.h"
 #include "qwfn_common.h"
 #include "qwfn_state.h"
@@ -144,6 +145,519 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
     }
 }
 
+// ---------------------------------------------------------------- in chunks
+//
+// Chunks of C tokens as matrix products, G the sum of g from the chunk's start
+// (inclusive), S the state before it:
+//   o_i = scale (e^{G_i} S^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j)
+//   S'  = e^{G_C} S + sum_j k_j (e^{G_C - G_j} v_j)^T
+// on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16), F32 accumulators. A value
+// enters as NT bf16 terms, each the rounded rest of the ones before: bf16 is one
+// term, f16 two (its 11 bits exactly), f32 three (24 bits exactly); a product keeps
+// the pairs of terms that reach NT terms' accuracy. The state's update always
+// takes three terms of e^{G_C - G_j} v_j, so the state stays an F32 sum whatever the
+// type; on the way to an output the state and the weighted scores are rounded to NT
+// terms (bf16: once to bf16 each, as the output itself is).
+// G and its differences are F64: a chunk's strong decays leave the weak ones exact.
+// A decay below e^-1000 counts as e^-1000, which is 0 in F32, so -inf is exact.
+//
+// A workgroup takes 32 columns a wave, its state in the waves' accumulators: lane m
+// of wave w, tile u holds column 32 w + 8 (m >> 2) + 4 u + (m & 3), rows 4 (l >> 4) + r
+// of each 16-row tile. As the state lies it is the A operand of S^T q (rows of a
+// 32-row block in the order of the registers; q and k lie in LDS in that order), and
+// O^T has 8 consecutive columns of a token in a lane: no data moves between the
+// products but the scores, which the waves share through LDS. q, k (rows), k^T and v^T
+// lie in LDS, a 16-byte unit at the place of an exclusive or with its row, so that
+// neither the row reads nor the transposed writes meet a bank often. The next chunk
+// is loaded into registers meanwhile. Three barriers a chunk.
+//
+// A non-finite v_j must not reach tokens before j: a chunk that holds one takes its
+// scores times v by plain sums over j <= i.
+//
+// A long sequence is cut into parts that run at once: k_linear_chunks<.., true> leaves
+// each part's own contribution U to the state and its decay in the workspace, and the
+// second launch starts a part from S0 and the U of the parts before it.
+typedef __bf16   v8b __attribute__((ext_vector_type(8)));
+typedef uint32_t v4w __attribute__((ext_vector_type(4)));
+typedef uint32_t v2w __attribute__((ext_vector_type(2)));
+
+constexpr int LC_WCOLS = 32;           // columns of a wave
+constexpr int LC_STEP_MAX = 8;         // up to this length token by token
+constexpr double LC_LOG2E = 1.4426950408889634;
+constexpr float LC_FLOOR = -1000.f;
+
+struct lc_args {
+    la_args   a;
+    int32_t   L;                       // tokens of a part, a multiple of the chunk; 0: sequences are whole
+    float *   U;                       // [part][n_v][dk][dv]
+    double *  G;                       // [part][n_v]: log2 of the part's decay
+};
+
+template <int NT, int DK, int NW> struct lc_cfg {
+    static constexpr int C = NT == 1 ? 64 : 32;          // tokens of a chunk
+    static constexpr int IT = C / 16;                    // 16-token tiles
+    static constexpr int JB = C / 32;                    // 32-token blocks of a sum
+    static constexpr int KT = DK / 16, KB = DK / 32;
+    static constexpr int COLS = LC_WCOLS * NW, THREADS = 64 * NW;
+    static constexpr int ES = NT == 3 ? 4 : 2;           // bytes of a value
+    static constexpr int LPU = NT == 3 ? 2 : 1;          // 16-byte loads of 8 values
+    // a staged unit: 8 values of two tokens
+    static constexpr int KN = C / 2 * (DK / 8), VN = C / 2 * (COLS / 8);
+    static constexpr int KU = (KN + THREADS - 1) / THREADS, VU = VN / THREADS;
+    static constexpr int QK = C * DK * 2, T = DK * C * 2, V = COLS * C * 2, P = C * C * 2;   // bytes of a term
+    static constexpr int OQ = 0, OK = OQ + NT * QK, OKT = OK + NT * QK, OV = OKT + NT * T, OP = OV + NT * V,
+                         LDS = OP + NT * P;
+    static constexpr int WAVES_EU = NT == 1 && DK <= 128 && NW == 4 ? 2 : 1;
+    static_assert((KN % THREADS == 0 || KU == 1) && VN % THREADS == 0, "whole units a thread, or one for some");
+    static_assert(LDS + 2048 <= 160 * 1024, "LDS of a CU");
+};
+
+// Byte of a 16-byte unit in the rows of q and k ([token][dk]) and in k^T and v^T ([row][token]).
+template <int DK> __device__ __forceinline__ int lc_row(int row, int unit) { return row * (DK * 2) + ((unit ^ (row & 7)) * 16); }
+template <int C> __device__ __forceinline__ int lc_col(int row, int unit) {
+    return row * (C * 2) + ((unit ^ ((row ^ (row >> 3)) & (C / 8 - 1))) * 16);
+}
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, v2b{(__bf16) x, (__bf16) y});
+}
+// x and y as NT bf16 terms, packed by term
+template <int NT> __device__ __forceinline__ void bf16_terms(float x, float y, uint32_t (&t)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        t[i] = bf16_pair(x, y);
+        if (i + 1 < NT) {
+            x -= __builtin_bit_cast(float, t[i] << 16);
+            y -= __builtin_bit_cast(float, t[i] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __builtin_bit_cast(float, u & 0xffff0000u); }
+__device__ __forceinline__ v4f mfma_bf16(v4w x, v4w y, v4f z) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), z, 0, 0, 0);
+}
+// sum over the pairs of terms whose product reaches NT terms' accuracy, the small ones first
+template <int NX, int NY, int NT> __device__ __forceinline__ v4f mfma_terms(const v4w (&x)[NX], const v4w (&y)[NY], v4f z) {
+#pragma unroll
+    for (int s = NT - 1; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NX; i++)
+            if (s - i >= 0 && s - i < NY) z = mfma_bf16(x[i], y[s - i], z);
+    return z;
+}
+
+// A part of a sequence: its first token and length, how many parts of the sequence come before and after,
+// its place in the workspace, and the state's slot.
+struct lc_part { int32_t b, t0, len, before, after, index, slot; };
+
+// Part `want` of the batch, parts in order of the sequences.
+__device__ lc_part find_part(const lc_args & x, int want, bool report, int threads, int32_t * sh) {
+    const la_args & a = x.a;
+    lc_part p{want, 0, 0, 0, 0, want, -1};
+    if (x.L > 0) {
+        // every thread counts the parts of a few sequences
+        const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = (a.n_seq + threads - 1) / threads;
+        int32_t sum = 0;
+        for (int i = 0; i < c; i++) {
+            const int b = tid * c + i;
+            if (b < a.n_seq) sum += (la_sequence(a, b, report).len + x.L - 1) / x.L;
+        }
+        int32_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t y = __shfl_up(incl, d);
+            if (lane >= d) incl += y;
+        }
+        if (lane == 63) sh[w] = incl;
+        if (tid == 0) sh[8] = -1;
+        __syncthreads();
+        for (int i = 0; i < w; i++) incl += sh[i];
+        if (want >= incl - sum && want < incl) {
+            int32_t at = incl - sum;
+            for (int i = 0; i < c; i++) {
+                const int b = tid * c + i;
+                const int32_t n = b < a.n_seq ? (la_sequence(a, b, false).len + x.L - 1) / x.L : 0;
+                if (want >= at && want < at + n) { sh[8] = b; sh[9] = want - at; sh[10] = n; }
+                at += n;
+            }
+        }
+        __syncthreads();
+        p.b = __builtin_amdgcn_readfirstlane(sh[8]);
+        if (p.b < 0) return p;
+        p.before = __builtin_amdgcn_readfirstlane(sh[9]);
+        p.after = __builtin_amdgcn_readfirstlane(sh[10]) - p.before - 1;
+    }
+    const la_seq s = la_sequence(a, p.b, report && x.L == 0 && threadIdx.x == 0);
+    p.t0 = s.t0 + p.before * x.L;
+    p.len = p.after > 0 ? x.L : s.len - p.before * x.L;
+    p.slot = s.slot;
+    return p;
+}
+
+// STATES: only what the part adds to the state, to the workspace.
+template <int NT, int DK, int NW, bool STATES>
+__global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_linear_chunks(lc_args x) {
+    using F = lc_cfg<NT, DK, NW>;
+    constexpr int C = F::C;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[F::LDS];
+    __shared__ double G[C];                    // log2 of the decay from the chunk's start
+    __shared__ float eG[C], wG[C];             // 2^G, 2^(G_end - G)
+    __shared__ int32_t sh[12];
+    __shared__ int32_t odd_v[2];               // a chunk, by parity, holds a non-finite v
+    const la_args & a = x.a;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // consecutive blocks (the heads of a key head) on one XCD
+    int blk = blockIdx.x;
+    if (gridDim.x % 8 == 0) blk = (blk % 8) * (int) (gridDim.x / 8) + blk / 8;
+    const int cb = blk % a.ct, h = blk / a.ct % a.n_v;
+    const lc_part part = find_part(x, blk / a.ct / a.n_v, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
+    if (part.b < 0) return;
+    if (part.len <= 0 || (STATES && part.after == 0)) return;
+
+    const int hk = h / a.rep, c0 = cb * F::COLS;
+    const char * qh = a.q + (int64_t) hk * a.q_nb1, * kh = a.k + (int64_t) hk * a.k_nb1;
+    const char * vh = a.v + (int64_t) h * a.v_nb1;
+    // the next chunk on its way: unit i of the thread: 8 values from 8 eu of tokens 2 ta and 2 ta + 1
+    v4w rq[F::KU][2][F::LPU], rk[F::KU][2][F::LPU], rv[F::VU][2][F::LPU];
+    float rg = 0.f;
+    auto load_unit = [&](v4w (&r)[2][F::LPU], const char * base, int64_t nb2, int t, int e8, int d) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < F::LPU; j++) {
+                const int tt = t + i < part.len ? t + i : part.len - 1, e = e8 + j * (8 / F::LPU);
+                r[i][j] = v4w{0, 0, 0, 0};
+                if (e < d) r[i][j] = *(const v4w *) (base + (int64_t) (part.t0 + tt) * nb2 + e * F::ES);
+            }
+    };
+    auto load = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < F::KU; i++) {
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = t0 + 2 * (u / (DK / 8));
+            if (F::KN < F::THREADS && u >= F::KN) break;
+            if (!STATES) load_unit(rq[i], qh, a.q_nb2, t, e8, a.dk);
+            load_unit(rk[i], kh, a.k_nb2, t, e8, a.dk);
+        }
+#pragma unroll
+        for (int i = 0; i < F::VU; i++) {
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), t = t0 + 2 * (u / (F::COLS / 8));
+            load_unit(rv[i], vh, a.v_nb2, t, c0 + e8, a.dv);
+        }
+        const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
+        if (w == 0) rg = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
+    };
+    // 8 values of a staged token as NT terms of 4 packed pairs; zeros past the part
+    auto terms = [&](const v4w (&r)[F::LPU], bool on, uint32_t (&o)[NT][4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t t[NT];
+            if constexpr (NT == 1) {
+                t[0] = r[0][i];
+            } else if constexpr (NT == 2) {
+                typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+                const uint32_t y = r[0][i];        // (a bit cast of a vector's element itself takes element 0)
+                const v2h f = __builtin_bit_cast(v2h, y);
+                bf16_terms<NT>((float) f[0], (float) f[1], t);
+            } else {
+                const uint32_t y0 = r[i >> 1][2 * (i & 1)], y1 = r[i >> 1][2 * (i & 1) + 1];
+                bf16_terms<NT>(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1), t);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) o[n][i] = on ? t[n] : 0u;
+        }
+    };
+    auto rows = [&](int at, int token, int e8, const uint32_t (&o)[NT][4]) {      // q, k: two groups of 4 values
+        const int kb = e8 >> 5, uu = (e8 & 31) >> 3;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *(v2w *) (lds + at + n * F::QK + lc_row<DK>(token, 4 * kb + (2 * uu & 3) + i) + 8 * (uu >> 1)) = v2w{o[n][2 * i], o[n][2 * i + 1]};
+    };
+    auto columns = [&](int at, int size, int pair, int e8, const uint32_t (&o0)[NT][4], const uint32_t (&o1)[NT][4]) {   // k^T, v^T
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = __builtin_amdgcn_perm(o1[n][i], o0[n][i], 0x05040100u), hi = __builtin_amdgcn_perm(o1[n][i], o0[n][i], 0x07060302u);
+                *(uint32_t *) (lds + at + n * size + lc_col<C>(e8 + 2 * i, pair >> 2) + 4 * (pair & 3)) = lo;
+                *(uint32_t *) (lds + at + n * size + lc_col<C>(e8 + 2 * i + 1, pair >> 2) + 4 * (pair & 3)) = hi;
+            }
+    };
+    auto stage = [&](int t0) {
+        uint32_t odd = 0;                     // a non-finite v
+#pragma unroll
+        for (int i = 0; i < F::KU; i++) {
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), pair = u / (DK / 8), t = t0 + 2 * pair;
+            if (F::KN < F::THREADS && u >= F::KN) break;
+            uint32_t o0[NT][4], o1[NT][4];
+            if (!STATES) {
+                terms(rq[i][0], t < part.len, o0);
+                terms(rq[i][1], t + 1 < part.len, o1);
+                rows(F::OQ, 2 * pair, e8, o0);
+                rows(F::OQ, 2 * pair + 1, e8, o1);
+            }
+            terms(rk[i][0], t < part.len, o0);
+            terms(rk[i][1], t + 1 < part.len, o1);
+            if (!STATES) {
+                rows(F::OK, 2 * pair, e8, o0);
+                rows(F::OK, 2 * pair + 1, e8, o1);
+            }
+            columns(F::OKT, F::T, pair, e8, o0, o1);
+        }
+#pragma unroll
+        for (int i = 0; i < F::VU; i++) {
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), pair = u / (F::COLS / 8), t = t0 + 2 * pair;
+            uint32_t o0[NT][4], o1[NT][4];
+            terms(rv[i][0], t < part.len, o0);
+            terms(rv[i][1], t + 1 < part.len, o1);
+            columns(F::OV, F::V, pair, e8, o0, o1);
+#pragma unroll
+            for (int j = 0; j < 4; j++)          // an exponent of all ones carries into the sign's place
+                odd |= ((o0[0][j] & 0x7f807f80u) + 0x00800080u) | ((o1[0][j] & 0x7f807f80u) + 0x00800080u);
+        }
+        if (!STATES && __ballot(odd & 0x80008000u) && lane == 0) odd_v[t0 / C & 1] = 1;
+        if (w == 0) {
+            float gt = t0 + lane < part.len && lane < C ? rg : 0.f;
+            gt = gt < LC_FLOOR ? LC_FLOOR : gt;
+            double s = (double) gt * LC_LOG2E;
+#pragma unroll
+            for (int d = 1; d < C; d <<= 1) {
+                const double y = __shfl_up(s, d);
+                if (lane >= d) s += y;
+            }
+            const double end = __shfl(s, C - 1);
+            if (lane < C) {
+                G[lane] = s;
+                eG[lane] = __builtin_amdgcn_exp2f((float) s);
+                wG[lane] = __builtin_amdgcn_exp2f((float) (end - s));
+            }
+        }
+    };
+    load(0);
+
+    // the state of the lane: [row tile][column tile] of rows 16 t + 4 g + r
+    v4f S[F::KT][2];
+    const size_t hs = (size_t) a.dk * a.dv, per = (size_t) a.n_v * hs;
+    int col[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) col[u] = c0 + LC_WCOLS * w + 8 * (m >> 2) + 4 * u + (m & 3);
+    const bool live = c0 + LC_WCOLS * w < a.dv;            // the wave has columns
+    auto each = [&](auto fn) {                             // fn(value, element of a head's state)
+#pragma unroll
+        for (int t = 0; t < F::KT; t++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = 16 * t + 4 * g + r;
+                    if (row < a.dk && col[u] < a.dv) fn(S[t][u], r, (size_t) row * a.dv + col[u]);
+                }
+    };
+#pragma unroll
+    for (int t = 0; t < F::KT; t++) S[t][0] = S[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (!STATES) {
+        if (part.slot >= 0 && a.s_in) {
+            const float * s0 = a.s_in + part.slot * per + h * hs;
+            each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
+        }
+        for (int p = 0; p < part.before; p++) {
+            const size_t at = (size_t) (part.index - part.before + p) * a.n_v + h;
+            const float f = __builtin_amdgcn_exp2f((float) x.G[at]);
+            const float * up = x.U + at * hs;
+            each([&](v4f & s, int r, size_t e) { s[r] = __fmaf_rn(s[r], f, up[e]); });
+        }
+        // the scores of tokens behind a 32-token block's last one stay 0
+        for (int i = tid; i < NT * F::P / 16; i += F::THREADS) *(v4w *) (lds + F::OP + 16 * i) = v4w{0, 0, 0, 0};
+        if (tid < 2) odd_v[tid] = 0;
+    }
+    double total = 0.;
+    __syncthreads();
+
+    for (int t0 = 0; t0 < part.len; t0 += C) {
+        stage(t0);
+        __syncthreads();
+        if (t0 + C < part.len) load(t0 + C);
+        const float cend = eG[C - 1];
+        if (STATES) total += G[C - 1];
+        if constexpr (!STATES) {
+            const bool odd = odd_v[t0 / C & 1] != 0;
+            if (tid == 0) odd_v[~(t0 / C) & 1] = 0;            // read in the chunk before, written in the next
+            // the scores, a 16 x 16 tile of tokens (j rows, i columns) at a time
+            for (int n = w; n < F::IT * (F::IT + 1) / 2; n += NW) {
+                int it = 0, jt = n;
+                while (jt > it) jt -= ++it;
+                v4f p{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kb = 0; kb < F::KB; kb++) {
+                    v4w kx[NT], qx[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        kx[t] = *(const v4w *) (lds + F::OK + t * F::QK + lc_row<DK>(16 * jt + m, 4 * kb + g));
+                        qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * it + m, 4 * kb + g));
+                    }
+                    p = mfma_terms<NT, NT, NT>(kx, qx, p);
+                }
+                const int i = 16 * it + m;
+                const double gi = G[i];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = 16 * jt + 4 * g + r;
+                    p[r] = j <= i ? p[r] * __builtin_amdgcn_exp2f((float) (gi - G[j])) : 0.f;
+                }
+                uint32_t lo[NT], hi[NT];
+                bf16_terms<NT>(p[0], p[1], lo);
+                bf16_terms<NT>(p[2], p[3], hi);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    *(v2w *) (lds + F::OP + t * F::P + lc_col<C>(i, 2 * jt + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
+            }
+            // S^T q
+            v4f o[F::IT][2];
+#pragma unroll
+            for (int i = 0; i < F::IT; i++) o[i][0] = o[i][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (live) {
+#pragma unroll
+                for (int kb = 0; kb < F::KB; kb++) {
+                    v4w sx[2][NT];
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const v4f & s = S[2 * kb + (i >> 1)][u];
+                            uint32_t t[NT];
+                            bf16_terms<NT>(s[2 * (i & 1)], s[2 * (i & 1) + 1], t);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) sx[u][n][i] = t[n];
+                        }
+#pragma unroll
+                    for (int i = 0; i < F::IT; i++) {
+                        v4w qx[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; t++) qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * i + m, 4 * kb + g));
+                        o[i][0] = mfma_terms<NT, NT, NT>(sx[0], qx, o[i][0]);
+                        o[i][1] = mfma_terms<NT, NT, NT>(sx[1], qx, o[i][1]);
+                    }
+                }
+            }
+            __syncthreads();                   // the scores
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < F::IT; i++) {
+                    const float e = eG[16 * i + m];
+                    o[i][0] *= e;
+                    o[i][1] *= e;
+                }
+                if (!odd) {
+#pragma unroll
+                    for (int jb = 0; jb < F::JB; jb++) {
+                        v4w vx[2][NT];
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int t = 0; t < NT; t++) vx[u][t] = *(const v4w *) (lds + F::OV + t * F::V + lc_col<C>(col[u] - c0, 4 * jb + g));
+#pragma unroll
+                        for (int i = 2 * jb; i < F::IT; i++) {
+                            v4w px[NT];
+#pragma unroll
+                            for (int t = 0; t < NT; t++) px[t] = *(const v4w *) (lds + F::OP + t * F::P + lc_col<C>(16 * i + m, 4 * jb + g));
+                            o[i][0] = mfma_terms<NT, NT, NT>(vx[0], px, o[i][0]);
+                            o[i][1] = mfma_terms<NT, NT, NT>(vx[1], px, o[i][1]);
+                        }
+                    }
+                } else {
+                    auto value = [&](int at, int size, int row, int t) {
+                        float f = 0.f;
+                        for (int n = 0; n < NT; n++)
+                            f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size + lc_col<C>(row, t >> 3) + 2 * (t & 7)) << 16);
+                        return f;
+                    };
+                    for (int i = 0; i < F::IT; i++)
+                        for (int j = 0; j <= 16 * i + m; j++) {
+                            const float p = value(F::OP, F::P, 16 * i + m, j);
+                            for (int u = 0; u < 2; u++)
+                                for (int r = 0; r < 4; r++) {
+                                    const float v = value(F::OV, F::V, LC_WCOLS * w + 8 * g + 4 * u + r, j);
+                                    // (the index is not a constant: written out for each of the tiles)
+#pragma unroll
+                                    for (int ii = 0; ii < F::IT; ii++)
+                                        if (ii == i) o[ii][u][r] = __fmaf_rn(p, v, o[ii][u][r]);
+                                }
+                        }
+                }
+                // 8 columns of a token
+#pragma unroll
+                for (int i = 0; i < F::IT; i++) {
+                    const int t = t0 + 16 * i + m, c = c0 + LC_WCOLS * w + 8 * g;
+                    if (t < part.len && c < a.dv) {
+                        char * p = a.out + ((int64_t) (part.t0 + t) * a.n_v * a.dv + (int64_t) h * a.dv + c) * F::ES;
+                        const v4f y0 = o[i][0] * a.scale, y1 = o[i][1] * a.scale;
+                        if constexpr (NT == 3) {
+                            *(v4f *) p = y0;
+                            *(v4f *) (p + 16) = y1;
+                        } else {
+                            const int type = NT == 1 ? QWFN_TYPE_BF16 : QWFN_TYPE_F16;
+                            *(v4w *) p = v4w{la_pack2(y0[0], y0[1], type), la_pack2(y0[2], y0[3], type),
+                                             la_pack2(y1[0], y1[1], type), la_pack2(y1[2], y1[3], type)};
+                        }
+                    }
+                }
+            }
+        }
+        // the state at the chunk's end
+        if (live) {
+            v4w vx[F::JB][2][3];
+#pragma unroll
+            for (int jb = 0; jb < F::JB; jb++) {
+                float wt[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) wt[i] = wG[32 * jb + 8 * g + i];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    v4w vt[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) vt[t] = *(const v4w *) (lds + F::OV + t * F::V + lc_col<C>(col[u] - c0, 4 * jb + g));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float lo = 0.f, hi = 0.f;
+#pragma unroll
+                        for (int t = NT - 1; t >= 0; t--) { lo += bf16_lo(vt[t][i]); hi += bf16_hi(vt[t][i]); }
+                        uint32_t t3[3];
+                        bf16_terms<3>(lo * wt[2 * i], hi * wt[2 * i + 1], t3);
+#pragma unroll
+                        for (int t = 0; t < 3; t++) vx[jb][u][t][i] = t3[t];
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < F::KT; t++) {
+                S[t][0] *= cend;
+                S[t][1] *= cend;
+#pragma unroll
+                for (int jb = 0; jb < F::JB; jb++) {
+                    v4w kx[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) kx[n] = *(const v4w *) (lds + F::OKT + n * F::T + lc_col<C>(16 * t + m, 4 * jb + g));
+                    S[t][0] = mfma_terms<NT, 3, 3>(kx, vx[jb][0], S[t][0]);
+                    S[t][1] = mfma_terms<NT, 3, 3>(kx, vx[jb][1], S[t][1]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if constexpr (STATES) {
+        const size_t at = (size_t) part.index * a.n_v + h;
+        float * up = x.U + at * hs;
+        each([&](v4f & s, int r, size_t e) { up[e] = s[r]; });
+        if (tid == 0 && cb == 0) x.G[at] = total;
+    } else if (part.after == 0 && part.slot >= 0) {
+        float * so = a.s_out + part.slot * per + h * hs;
+        each([&](v4f & s, int r, size_t e) { so[e] = s[r]; });
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 int check_heads(const qwfn_tensor * t, int32_t type, const char * name, bool packed) {
@@ -176,6 +690,58 @@ int check_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, in
     return QWFN_OK;
 }
 
+struct lc_plan {
+    bool    step;                      // token by token
+    int32_t NT, DK, NW, ct, L;
+    int64_t parts;                     // blocks along the tokens, at most
+    size_t  off_g, bytes;
+};
+
+// Parts of a sequence: as many as fill the CUs once, but no shorter than LC_MIN_PART tokens (a part costs its
+// state's way through the workspace and a second pass over its k and v).
+constexpr int64_t LC_TARGET = 256, LC_MIN_PART = 256;
+
+lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
+    lc_plan p{};
+    const int64_t dk = q->ne[0], dv = v->ne[0], n_v = v->ne[1], n_tok = q->ne[2];
+    p.NT = q->type == QWFN_TYPE_BF16 ? 1 : q->type == QWFN_TYPE_F16 ? 2 : 3;
+    p.DK = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
+    // three terms of 256 rows of q, k and k^T are more than the LDS of a CU
+    p.step = max_len <= LC_STEP_MAX || (p.NT == 3 && p.DK == 256);
+    if (p.step) return p;
+    p.NW = dv <= 2 * LC_WCOLS ? 2 : 4;
+    p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
+    const int64_t longest = std::min<int64_t>(max_len, n_tok), C = p.NT == 1 ? 64 : 32;
+    int64_t L = std::max<int64_t>(LC_MIN_PART, (n_tok * n_v * p.ct + LC_TARGET - 1) / LC_TARGET);
+    L = (L + C - 1) / C * C;
+    p.parts = n_seq;
+    if (L < longest) {
+        p.L = (int32_t) L;
+        p.parts = n_seq + n_tok / L;
+        p.off_g = ((size_t) p.parts * n_v * dk * dv * sizeof(float) + 255) / 256 * 256;
+        p.bytes = p.off_g + (size_t) p.parts * n_v * sizeof(double);
+    }
+    return p;
+}
+
+template <int NT, int DK, int NW>
+int launch_chunks(const lc_args & x, const lc_plan & p, hipStream_t s) {
+    const dim3 grid((unsigned) (p.parts * x.a.n_v * p.ct)), blk(64 * NW);
+    if (p.L > 0) {
+        hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, true>), grid, blk, 0, s, x);
+        if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
+    }
+    hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, false>), grid, blk, 0, s, x);
+    return hip_check(hipGetLastError(), "linear_attn launch");
+}
+template <int NT>
+int launch_type(const lc_args & x, const lc_plan & p, hipStream_t s) {
+    if (p.DK == 64)  return p.NW == 2 ? launch_chunks<NT, 64, 2>(x, p, s) : launch_chunks<NT, 64, 4>(x, p, s);
+    if (p.DK == 128) return p.NW == 2 ? launch_chunks<NT, 128, 2>(x, p, s) : launch_chunks<NT, 128, 4>(x, p, s);
+    if constexpr (NT < 3) return p.NW == 2 ? launch_chunks<NT, 256, 2>(x, p, s) : launch_chunks<NT, 256, 4>(x, p, s);
+    return QWFN_ENOTSUP;
+}
+
 }  // namespace
 }  // namespace qwfn
 
@@ -183,8 +749,7 @@ using namespace qwfn;
 
 extern "C" size_t qwfn_linear_attn_workspace_size(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
     return ::qwfn::abi_value<size_t>("linear_attn_workspace_size", 0, [&]() -> size_t {
-        if (check_linear(q, v, n_seq, max_len)) return 0;
-        return 0;
+        return check_linear(q, v, n_seq, max_len) ? 0 : plan_linear(q, v, n_seq, max_len).bytes;
     });
 }
 
@@ -212,6 +777,10 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             (uintptr_t) state_out < (uintptr_t) state_in + states)
             return set_error(QWFN_EINVAL, "linear_attn: state_in and state_out must be equal or not overlap");
         if (n_tok == 0) return QWFN_OK;
+        const lc_plan pl = plan_linear(q, v, n_seq, max_len);
+        if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
+            return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");
+        if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, "linear_attn: ws must be 16-byte aligned");
         la_args a{};
         if (int rc = status_word(&a.status)) return rc;
         a.q = (const char *) q->data; a.k = (const char *) k->data; a.v = (const char *) v->data; a.out = (char *) dst->data;
@@ -220,6 +789,13 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         a.g = g; a.g_ts = g_token_stride; a.cu = cu; a.slots = slots; a.s_in = state_in; a.s_out = state_out; a.scale = scale;
         a.type = q->type; a.n_seq = n_seq; a.max_len = max_len; a.n_slots = n_slots; a.n_tok = (int32_t) n_tok;
         a.n_k = (int32_t) q->ne[1]; a.n_v = (int32_t) n_v; a.rep = a.n_v / a.n_k; a.dk = (int32_t) dk; a.dv = (int32_t) dv;
+        if (!pl.step) {
+            if (pl.parts * n_v * pl.ct > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
+            a.ct = pl.ct;
+            const lc_args x{a, pl.L, (float *) ws, (double *) ((char *) ws + pl.off_g)};
+            return pl.NT == 1 ? launch_type<1>(x, pl, as_stream(stream)) : pl.NT == 2 ? launch_type<2>(x, pl, as_stream(stream))
+                                                                                      : launch_type<3>(x, pl, as_stream(stream));
+        }
         a.ct = (int32_t) ((dv + LA_COLS - 1) / LA_COLS);
         const int64_t blocks = (int64_t) n_seq * n_v * a.ct;
         if (blocks > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
