@@ -17,9 +17,12 @@
 // the cache lines that two heads share come from one L2.
 //
 // Inside a workgroup the 4 waves take every fourth tile of the run, each on its
-// own: a tile's rows are loaded into registers while the tile before is computed,
-// so no barrier and no wave waits for another's data. The rows then pass through
-// the wave's part of the LDS:
+// own: no barrier, and no wave waits for another's data. A tile's rows come by LDS
+// DMA into the wave's part of the LDS, one buffer for K and one for V: K of the
+// next tile is sent for when the scores are done, V when the products are. The table
+// entries go the same way, two tiles ahead, so that every vector-memory operation of the
+// loop is one whose place in the order is known, and a wait leaves just the later
+// ones in flight.
 //   S^T = K Q^T   v_mfma_i32_16x16x64_i8 a q8_0 block: A is the 64-byte window of the
 //                 row (from a 16-byte boundary) that holds the block's 32 quants, B
 //                 the query's quants at the same place of a window that is zero
@@ -90,23 +93,36 @@ struct pa_args {
 template <int D> struct pa_cfg {
     static constexpr int NBLK = D / QK;
     static constexpr int SEG = NBLK * QBLOCK;            // bytes of a head row
-    static constexpr int PB = SEG / 17;                  // bytes a lane loads at once: 17 pieces a row
-    static constexpr int LS = (SEG + 15) / 16 * 16;      // of a row in LDS
+    // a row goes to LDS in units of a DMA lane, 16 bytes where a head row is whole ones; UPR of them a row
+    // (rows from 16-byte boundaries), the last UPR - UV only fill
+    static constexpr int UB = SEG % 16 == 0 ? 16 : 4, UV = SEG / UB;
+    static constexpr int LS = (SEG + 15) / 16 * 16, UPR = LS / UB;        // bytes of a row in LDS
+    static constexpr int UNITS = PA_TILE * UPR, DMAS = (UNITS + 63) / 64;
+    static constexpr int UMUL = 65536 / UPR + 1;         // i / UPR = i UMUL >> 16 for i < UNITS
     static constexpr int ROWS = PA_TILE * LS;            // of a tensor's tile in LDS
-    static constexpr int PIECES = PA_TILE * 17;
-    static constexpr int LOADS = (PIECES + 63) / 64;
-    static constexpr int WAVE = 2 * ROWS + 2 * PA_TILE + 2 * NBLK * PA_TILE * 2;   // K, V, each key's largest dv, scales
-    static constexpr int IMG = 16 * NBLK * 64;           // the query windows
-    static_assert(PB == 16 || PB == 8 || PB == 4, "whole loads");
-    static_assert(PA_WAVES * WAVE >= IMG + 16 * NBLK * 4 && WAVE >= 16 * D * 4, "the LDS holds the query image and O");
+    // of a wave: K, V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
+    static constexpr int OA = 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
+    static constexpr int WAVE = OS + 2 * NBLK * PA_TILE * 2;
+    static constexpr int IMG = 16 * NBLK * 64;           // the query windows, in the first wave's V
+    static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * D * 4 && WAVE % 16 == 0, "V holds the query image, a wave's part its O");
+    static_assert((UNITS - 1) * (UMUL * UPR - 65536) < 65536, "the division is exact");
     static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
 };
-template <int PB> struct pa_piece;
-template <> struct pa_piece<16> { typedef v4u type; };
-template <> struct pa_piece<8>  { typedef uint2 type; };
-template <> struct pa_piece<4>  { typedef uint32_t type; };
-
 constexpr int pa_win(int b) { return (QBLOCK * b + 2) / 16; }              // first 16 bytes of block b's window
+
+// One wave-wide LDS DMA: lane i copies its UB bytes to LDS[at + UB i]. Inline asm, so that the compiler neither
+// moves memory operations across it nor waits for it: the kernel's own counts do. (m0 is read one wait state after
+// its write at the earliest; the compiler keeps nothing in it here.)
+template <int UB> __device__ __forceinline__ void pa_dma(uint64_t from, uint32_t at) {
+    if constexpr (UB == 16)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(at) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(from), "s"(at) : "memory");
+}
+// Waits until at most N vector-memory operations are in flight, or for this wave's LDS operations.
+template <int N> __device__ __forceinline__ void pa_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void pa_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t pa_lds(const void * p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) p; }
 
 __device__ __forceinline__ void load4(const char * p, int32_t type, float x[4]) {
     if (type == QWFN_TYPE_F32) {
@@ -224,12 +240,12 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
 template <int D>
 __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     using C = pa_cfg<D>;
-    using piece = typename pa_piece<C::PB>::type;
-    constexpr int NBLK = C::NBLK;
+    constexpr int NBLK = C::NBLK, ND = C::DMAS;
     __shared__ __attribute__((aligned(16))) uint8_t lds[PA_WAVES * C::WAVE];
     __shared__ float2 ml[PA_WAVES][16];
     __shared__ int32_t sh[PA_WAVES + 2];
-    const int tid = threadIdx.x, lane = tid & 63, ln = lane & 15, lg = lane >> 4;
+    const int tid = threadIdx.x;
+    int lane = tid & 63, ln = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     // blocks -> (run, KV head, row tile): those of one run follow each other on one XCD
@@ -238,10 +254,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     const int kvh = hr % a.nh_kv, rt = hr / a.nh_kv;
     pa_run run = find_run(a, g, sh);
 
-    uint8_t * const my = lds + wave * C::WAVE;                   // K rows, V rows, scales
-    uint16_t * const vmax = (uint16_t *) (my + 2 * C::ROWS);
-    uint16_t * const kscl = vmax + PA_TILE;
+    uint8_t * const my = lds + wave * C::WAVE;
+    uint64_t * const addr = (uint64_t *) (my + C::OA);
+    const int32_t * const entry = (const int32_t *) (my + C::OE);
+    uint16_t * const vmax = (uint16_t *) (my + C::OM);
+    uint16_t * const kscl = (uint16_t *) (my + C::OS);
     uint16_t * const vscl = kscl + NBLK * PA_TILE;
+    const uint32_t at_k = pa_lds(my), at_v = at_k + C::ROWS, at_e = at_k + C::OE;
     const char * kh = a.k + (size_t) kvh * a.nb2;
     const char * vh = a.v + (size_t) kvh * a.nb2;
     // this lane's query row
@@ -259,37 +278,47 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
         if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(run.pos / run.per, (run.pos + tiles - 1) / run.per);
         const int32_t * table = a.table + (int64_t) b * a.t_stride;
 
-        // the cache row of the lane's key (lanes l and l + 32 the same) of a tile, -1 for none
-        auto slots = [&](int t) -> int32_t {
-            const int32_t key = (run.off + t) * PA_TILE + (lane & 31);
-            const bool in = t < nt && key < n;
-            const uint32_t col = div_by((uint32_t) (in ? key : 0), a.page);
-            const int32_t page = in ? table[col] : -1;
-            if (in && (uint32_t) page >= (uint32_t) a.n_pages) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
-            return (uint32_t) page < (uint32_t) a.n_pages ? page * (int32_t) a.page.d + (key - (int32_t) (col * a.page.d)) : -1;
+        // the table entries of a tile's keys (lanes l and l + 32 the same), clipped to the part's last key
+        const int32_t end = (run.off + nt) * PA_TILE < n ? (run.off + nt) * PA_TILE : n;
+        auto entries = [&](int t) {
+            int32_t key = (run.off + t) * PA_TILE + (lane & 31);
+            key = key < end ? key : end - 1;
+            pa_dma<4>((uint64_t) (uintptr_t) (table + div_by((uint32_t) key, a.page)), at_e);
         };
-        piece kr[C::LOADS], vr[C::LOADS];
-        auto rows = [&](int32_t slot) {
+        // the addresses of the tile's rows of K, and which of its keys exist
+        auto rows_of = [&](int t) -> uint32_t {
+            const int32_t key = (run.off + t) * PA_TILE + (lane & 31), page = entry[lane];
+            const bool in = t < nt && key < end, ok = in && (uint32_t) page < (uint32_t) a.n_pages;
+            if (in && !ok) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+            const uint32_t slot = ok ? (uint32_t) page * a.page.d + ((uint32_t) key - div_by((uint32_t) key, a.page) * a.page.d) : 0u;
+            if (lane < PA_TILE) addr[lane] = (uint64_t) (uintptr_t) kh + (uint64_t) slot * a.nb1;
+            return (uint32_t) __ballot(ok);
+        };
+        const uint64_t v_k = (uint64_t) (vh - kh);
+        auto send = [&](uint32_t at, uint64_t delta) {
 #pragma unroll
-            for (int i = 0; i < C::LOADS; i++) {
-                const int p = lane + 64 * i, key = (p * 241) >> 12;          // p / 17 for p < 544
-                int32_t s = __shfl(slot, key & 31);
-                s = s < 0 ? 0 : s;
-                const size_t off = (size_t) (uint32_t) s * a.nb1 + (size_t) (p - 17 * key) * C::PB;
-                if (64 * (i + 1) <= C::PIECES || p < C::PIECES) {
-                    kr[i] = *(const piece *) (kh + off);
-                    vr[i] = *(const piece *) (vh + off);
-                }
+            for (int i = 0; i < ND; i++) {
+                const int x = lane + 64 * i, key = (x * C::UMUL) >> 16, u = x - key * C::UPR;
+                if (64 * (i + 1) <= C::UNITS || x < C::UNITS)
+                    pa_dma<C::UB>(addr[key] + delta + (uint64_t) (uint32_t) ((u < C::UV ? u : C::UV - 1) * C::UB), at + 64 * C::UB * i);
             }
         };
-        int32_t cur = slots(wave), next = slots(wave + PA_WAVES);
-        rows(cur);
+        __syncthreads();                                   // the LDS of the part before is read
+        uint32_t live = 0, live_next = 0;                  // the tile's keys that exist
+        if (wave < nt) {
+            entries(wave);
+            pa_wait<0>();
+            live = rows_of(wave);
+            wave_lds_sync();
+            send(at_k, 0);
+            entries(wave + PA_WAVES);
+        }
 
         // the query image: rows requantised, each block at its place of its window
-        __syncthreads();                                   // the LDS of the part before is read
-        for (int i = tid; i < C::IMG / 16; i += PA_THREADS) ((v4u *) lds)[i] = v4u{0, 0, 0, 0};
+        uint8_t * const img = lds + C::ROWS;
+        for (int i = tid; i < C::IMG / 16; i += PA_THREADS) ((v4u *) img)[i] = v4u{0, 0, 0, 0};
         __syncthreads();
-        float * dql = (float *) (lds + C::IMG);
+        float * dql = (float *) (img + C::IMG);
         for (int i = tid >> 3; i < 16 * NBLK; i += PA_THREADS / 8) {
             const int r = i / NBLK, blk = i % NBLK, rr = 16 * rt + r, sub = tid & 7;
             float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -302,7 +331,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             float dq;
             const uint32_t q4 = dev::q8_quantize_lane4(x, a.x86 != 0, &d16, &dq);
             const int at = QBLOCK * blk + 2 - (QBLOCK * blk + 2) / 16 * 16;
-            uint16_t * qp = (uint16_t *) (lds + (r * NBLK + blk) * 64 + at + sub * 4);
+            uint16_t * qp = (uint16_t *) (img + (r * NBLK + blk) * 64 + at + sub * 4);
             qp[0] = (uint16_t) q4;
             qp[1] = (uint16_t) (q4 >> 16);
             if (sub == 0) dql[r * NBLK + blk] = dq;
@@ -312,7 +341,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
         float dq[NBLK];
 #pragma unroll
         for (int blk = 0; blk < NBLK; blk++) {
-            qw[blk] = *(const v4i *) (lds + (ln * NBLK + blk) * 64 + 16 * lg);
+            qw[blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
             dq[blk] = dql[ln * NBLK + blk];
         }
         __syncthreads();
@@ -320,42 +349,25 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
         v4f O[NBLK][2] = {};
         float M = -INFINITY, l = 0.f;
         const int32_t limit = n - a.T + trow + 1;          // the row sees keys below it
+        if (wave < nt) {
+            pa_wait_lds();
+            send(at_v, v_k);
+        }
+        // in flight at the top, in this order: K of the tile, the entries of the next, V of the tile
         for (int t = wave; t < nt; t += PA_WAVES) {
-            const uint32_t live = (uint32_t) __ballot(cur >= 0);   // the tile's keys that exist
+            // the lane's places are computed anew in every tile: kept over the loop they cost 40 registers, spilled
+            asm volatile("" : "+v"(lane), "+v"(ln), "+v"(lg));
             const int32_t key0 = (run.off + t) * PA_TILE;
             const bool masked = live != 0xffffffffu || key0 + PA_TILE > n - a.T + 1;
-            wave_lds_sync();
-#pragma unroll
-            for (int i = 0; i < C::LOADS; i++) {
-                const int p = lane + 64 * i, key = (p * 241) >> 12, at = key * C::LS + (p - 17 * key) * C::PB;
-                if (64 * (i + 1) <= C::PIECES || p < C::PIECES) {
-                    *(piece *) (my + at) = kr[i];
-                    *(piece *) (my + C::ROWS + at) = vr[i];
-                }
-            }
-            wave_lds_sync();
-            cur = next;
-            rows(cur);
-            next = slots(t + 2 * PA_WAVES);
-            // the scales by block and key; V's largest (finite) of each key and of the tile
-            uint32_t dmax = 0;
-            {
+            pa_wait<ND + 1>();
+            {   // K's scales by block and key
                 const int key = lane & 31, half = lane >> 5;
-                const bool on = live >> key & 1;
 #pragma unroll
                 for (int i = 0; i < NBLK / 2; i++) {
                     const int blk = half * (NBLK / 2) + i;
-                    const uint16_t dk = *(const uint16_t *) (my + key * C::LS + QBLOCK * blk);
-                    const uint16_t dv = on ? *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk) : (uint16_t) 0;
-                    kscl[blk * PA_TILE + key] = dk;
-                    vscl[blk * PA_TILE + key] = dv;
-                    const uint32_t mag = dv & 0x7fffu;
-                    dmax = max(dmax, mag < 0x7c00u ? mag : 0u);
+                    kscl[blk * PA_TILE + key] = *(const uint16_t *) (my + key * C::LS + QBLOCK * blk);
                 }
-                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
-                if (half == 0) vmax[key] = (uint16_t) dmax;
             }
-            for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
             wave_lds_sync();
 
             // S^T: lane (row ln, keys 16 u + 4 lg + r)
@@ -366,6 +378,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int blk = 0; blk < NBLK; blk++) {
+                    if (blk % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
                     const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{0, 0, 0, 0}, 0, 0, 0);
                     const uint2 dk = *(const uint2 *) (kscl + blk * PA_TILE + 16 * u + 4 * lg);
@@ -377,6 +390,32 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[u][r] = acc[r];
             }
+            // the next tile's K
+            pa_wait<ND>();
+            live_next = rows_of(t + PA_WAVES);
+            wave_lds_sync();
+            pa_wait_lds();
+            send(at_k, 0);
+            entries(t + 2 * PA_WAVES);
+            // V's scales; its largest (finite) of each key and of the tile
+            pa_wait<ND + 1>();
+            uint32_t dmax = 0;
+            {
+                const int key = lane & 31, half = lane >> 5;
+                const bool on = live >> key & 1;
+#pragma unroll
+                for (int i = 0; i < NBLK / 2; i++) {
+                    const int blk = half * (NBLK / 2) + i;
+                    const uint16_t dv = on ? *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk) : (uint16_t) 0;
+                    vscl[blk * PA_TILE + key] = dv;
+                    const uint32_t mag = dv & 0x7fffu;
+                    dmax = max(dmax, mag < 0x7c00u ? mag : 0u);
+                }
+                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
+                if (half == 0) vmax[key] = (uint16_t) dmax;
+            }
+            for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
+            wave_lds_sync();
             if (masked) {
                 dmax = 0;                                  // of the keys that the row sees
 #pragma unroll
@@ -420,6 +459,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             auto pv = [&](auto fn) {
 #pragma unroll
                 for (int blk = 0; blk < NBLK; blk++) {
+                    if (blk % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
                     uint32_t av[2][4];
 #pragma unroll
@@ -450,7 +490,11 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             };
             if (masked) pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo_masked(p0, p1, d, h, lo); });
             else        pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo(p0, p1, d, h, lo); });
+            pa_wait_lds();
+            send(at_v, v_k);
+            live = live_next;
         }
+        pa_wait<0>();
         l = sum_lanes16_32(l);
 
         // the waves' parts meet in LDS: O[row][dim] of each
