@@ -58,6 +58,8 @@ constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
 constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M
+constexpr float PA_IBIAS = 12582912.f; // 1.5 2^23: an integer below 2^22 added to its bits is added to its value
+constexpr int PA_IBITS = 0x4b400000;   // (a block's dot is at most 32 128 128 = 2^19)
 
 // x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), is off by at
 // most d <= 2^s, and x (m d - 2^(31 + s)) < 2^(31 + s) keeps the quotient whole.
@@ -83,7 +85,7 @@ struct pa_args {
     int32_t         type;              // of q, gate and dst
     int32_t         n_seq, T, nh, nh_kv, rep, R, RT, x86;
     int32_t         runs;              // runs the tiles are cut into, at most
-    float           c;                 // scale * log2(e)
+    float           c;                 // scale * log2(e): scores are in log2 units
     float *         part_o;            // [run + request][nh_kv][R][D]
     float2 *        part_ml;           // [run + request][nh_kv][R]
     int2 *          span;              // [request]: its first and last run
@@ -169,15 +171,6 @@ __device__ __forceinline__ void hilo(float p0, float p1, uint32_t d, uint32_t & 
         "s_nop 1"
         : "=&v"(hi), "=&v"(lo) : "v"(p0), "v"(p1), "v"(x0), "v"(x1), "v"(d));
 }
-// The same where keys are masked: a key that a row does not see (p = 0) adds nothing, whatever its d is.
-__device__ __forceinline__ void hilo_masked(float p0, float p1, uint32_t d, uint32_t & hi, uint32_t & lo) {
-    const float d0 = dev::f16_bits_to_f32((uint16_t) d), d1 = dev::f16_bits_to_f32((uint16_t) (d >> 16));
-    const float x0 = p0 == 0.f ? 0.f : p0 * d0, x1 = p1 == 0.f ? 0.f : p1 * d1;
-    const _Float16 h0 = (_Float16) x0, h1 = (_Float16) x1;
-    hi = dev::f32_to_f16_bits(x0) | (uint32_t) dev::f32_to_f16_bits(x1) << 16;
-    lo = dev::f32_to_f16_bits(x0 - (float) h0) | (uint32_t) dev::f32_to_f16_bits(x1 - (float) h1) << 16;
-}
-
 // The block's run of the tiles of all requests.
 struct pa_run { int b; int32_t off, left, pos, per; };
 
@@ -257,7 +250,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     uint8_t * const my = lds + wave * C::WAVE;
     uint64_t * const addr = (uint64_t *) (my + C::OA);
     const int32_t * const entry = (const int32_t *) (my + C::OE);
-    uint16_t * const vmax = (uint16_t *) (my + C::OM);
+    uint16_t * const vtop = (uint16_t *) (my + C::OM);
     uint16_t * const kscl = (uint16_t *) (my + C::OS);
     uint16_t * const vscl = kscl + NBLK * PA_TILE;
     const uint32_t at_k = pa_lds(my), at_v = at_k + C::ROWS, at_e = at_k + C::OE;
@@ -338,11 +331,12 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
         }
         __syncthreads();
         v4i qw[NBLK];
-        float dq[NBLK];
+        float dq[NBLK];                                    // dq c to 22 bits: PA_IBIAS dq is exact
 #pragma unroll
         for (int blk = 0; blk < NBLK; blk++) {
             qw[blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
-            dq[blk] = dql[ln * NBLK + blk];
+            const uint32_t x = __builtin_bit_cast(uint32_t, dql[ln * NBLK + blk] * a.c);
+            dq[blk] = __builtin_bit_cast(float, (x + 2u) & ~3u);
         }
         __syncthreads();
 
@@ -370,7 +364,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             }
             wave_lds_sync();
 
-            // S^T: lane (row ln, keys 16 u + 4 lg + r)
+            // S^T: lane (row ln, keys 16 u + 4 lg + r). An integer dot comes out of the MFMA on top of the bits of
+            // PA_IBIAS, so it is PA_IBIAS + dot as a float, and one fused step makes dot dq of it.
             float s[2][4];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -378,14 +373,15 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int blk = 0; blk < NBLK; blk++) {
-                    if (blk % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
-                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{0, 0, 0, 0}, 0, 0, 0);
+                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{PA_IBITS, PA_IBITS, PA_IBITS, PA_IBITS}, 0, 0, 0);
                     const uint2 dk = *(const uint2 *) (kscl + blk * PA_TILE + 16 * u + 4 * lg);
-                    acc[0] = __fmaf_rn((float) d[0], mul_f16lo(dq[blk], dk.x), acc[0]);
-                    acc[1] = __fmaf_rn((float) d[1], mul_f16hi(dq[blk], dk.x), acc[1]);
-                    acc[2] = __fmaf_rn((float) d[2], mul_f16lo(dq[blk], dk.y), acc[2]);
-                    acc[3] = __fmaf_rn((float) d[3], mul_f16hi(dq[blk], dk.y), acc[3]);
+                    const int d0 = d[0], d1 = d[1], d2 = d[2], d3 = d[3];
+                    const float nb = -PA_IBIAS * dq[blk];
+                    acc[0] = fma_f16lo(dk.x, __fmaf_rn(__builtin_bit_cast(float, d0), dq[blk], nb), acc[0]);
+                    acc[1] = fma_f16hi(dk.x, __fmaf_rn(__builtin_bit_cast(float, d1), dq[blk], nb), acc[1]);
+                    acc[2] = fma_f16lo(dk.y, __fmaf_rn(__builtin_bit_cast(float, d2), dq[blk], nb), acc[2]);
+                    acc[3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), dq[blk], nb), acc[3]);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[u][r] = acc[r];
@@ -397,22 +393,25 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             pa_wait_lds();
             send(at_k, 0);
             entries(t + 2 * PA_WAVES);
-            // V's scales; its largest (finite) of each key and of the tile
+            // V's scales; its largest of each key and of the tile. One that is not finite counts as 0 here and in
+            // the products, and is added by itself below.
             pa_wait<ND + 1>();
             uint32_t dmax = 0;
+            bool odd = false;
             {
                 const int key = lane & 31, half = lane >> 5;
                 const bool on = live >> key & 1;
 #pragma unroll
                 for (int i = 0; i < NBLK / 2; i++) {
                     const int blk = half * (NBLK / 2) + i;
-                    const uint16_t dv = on ? *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk) : (uint16_t) 0;
-                    vscl[blk * PA_TILE + key] = dv;
-                    const uint32_t mag = dv & 0x7fffu;
-                    dmax = max(dmax, mag < 0x7c00u ? mag : 0u);
+                    const uint32_t dv = *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk), mag = dv & 0x7fffu;
+                    const bool fine = on && mag < 0x7c00u;
+                    vscl[blk * PA_TILE + key] = (uint16_t) (fine ? dv : 0u);
+                    dmax = max(dmax, fine ? mag : 0u);
+                    odd |= on && mag >= 0x7c00u;
                 }
                 dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
-                if (half == 0) vmax[key] = (uint16_t) dmax;
+                if (half == 0) vtop[key] = (uint16_t) dmax;
             }
             for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
             wave_lds_sync();
@@ -424,17 +423,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                     for (int r = 0; r < 4; r++) {
                         const int k = 16 * u + 4 * lg + r;
                         if (!(live >> k & 1) || key0 + k >= limit) s[u][r] = -INFINITY;
-                        else dmax = max(dmax, (uint32_t) vmax[k]);
+                        else dmax = max(dmax, (uint32_t) vtop[k]);
                     }
                 dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 16));
                 dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    top = fmaxf(top, masked && s[u][r] == -INFINITY ? -INFINITY : s[u][r] * a.c);
+            float top = vmax(vmax(s[0][0], s[0][1]), vmax(s[0][2], s[0][3]));
+            top = vmax(top, vmax(vmax(s[1][0], s[1][1]), vmax(s[1][2], s[1][3])));
             top = xmax_lanes16_32(top);
             const int e = (int) (dmax >> 10) < 1 ? 1 : (int) (dmax >> 10);        // d < 2^(e - 14)
             const float ref = top + (float) (e - 14 - PA_BIAS);
@@ -452,44 +447,65 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    p[u][r] = masked && s[u][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fmaf_rn(s[u][r], a.c, -m));
+                    p[u][r] = __builtin_amdgcn_exp2f(s[u][r] - m);       // 2^-inf = 0
                     l += p[u][r];
                 }
             // O^T: A lane (dims 2 ln + e of the block, keys 4 lg + r of both halves)
-            auto pv = [&](auto fn) {
 #pragma unroll
-                for (int blk = 0; blk < NBLK; blk++) {
-                    if (blk % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-                    const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
-                    uint32_t av[2][4];
+            for (int blk = 0; blk < NBLK; blk++) {
+                const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
+                uint32_t av[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) av[u][r] = *(const uint16_t *) (vl + (16 * u + r) * C::LS);
+                v4u a0, a1, bh, bl;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    uint32_t x0[2], x1[2];
+                    cvt_v_block(av[u], x0, x1);
+                    a0[2 * u] = x0[0]; a0[2 * u + 1] = x0[1];
+                    a1[2 * u] = x1[0]; a1[2 * u + 1] = x1[1];
+                    const uint2 dv = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
+                    uint32_t h0, h1, l0, l1;
+                    hilo(p[u][0], p[u][1], dv.x, h0, l0);
+                    hilo(p[u][2], p[u][3], dv.y, h1, l1);
+                    bh[2 * u] = h0; bh[2 * u + 1] = h1;
+                    bl[2 * u] = l0; bl[2 * u + 1] = l1;
+                }
+                const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
+                const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
+                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[blk][0], 0, 0, 0);
+                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[blk][1], 0, 0, 0);
+                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[blk][0], 0, 0, 0);
+                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[blk][1], 0, 0, 0);
+            }
+            if (__builtin_expect(__ballot(odd) != 0, 0)) {
+                // blocks of V whose scale is not finite, for the rows that see their key
+                for (int k = 0; k < PA_TILE; k++) {
+                    const int from = (k >> 2 & 3) * 16 + ln;
+                    float pk = 0.f;
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) av[u][r] = *(const uint16_t *) (vl + (16 * u + r) * C::LS);
-                    v4u a0, a1, bh, bl;
+                        for (int r = 0; r < 4; r++) {
+                            const float y = __shfl(p[u][r], from);
+                            if (k == 16 * u + (k & 12) + r) pk = y;
+                        }
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        uint32_t x0[2], x1[2];
-                        cvt_v_block(av[u], x0, x1);
-                        a0[2 * u] = x0[0]; a0[2 * u + 1] = x0[1];
-                        a1[2 * u] = x1[0]; a1[2 * u + 1] = x1[1];
-                        const uint2 dv = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
-                        uint32_t h0, h1, l0, l1;
-                        fn(p[u][0], p[u][1], dv.x, h0, l0);
-                        fn(p[u][2], p[u][3], dv.y, h1, l1);
-                        bh[2 * u] = h0; bh[2 * u + 1] = h1;
-                        bl[2 * u] = l0; bl[2 * u + 1] = l1;
+                    for (int blk = 0; blk < NBLK; blk++) {
+                        const uint8_t * vb = my + C::ROWS + k * C::LS + QBLOCK * blk;
+                        const uint16_t dv = *(const uint16_t *) vb;
+                        if ((dv & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
+#pragma unroll
+                        for (int e2 = 0; e2 < 2; e2++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (pk != 0.f)
+                                    O[blk][e2][r] += pk * dev::f16_bits_to_f32(dv) * (float) *(const int8_t *) (vb + 2 + 2 * (4 * lg + r) + e2);
                     }
-                    const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
-                    const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
-                    O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[blk][0], 0, 0, 0);
-                    O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[blk][1], 0, 0, 0);
-                    O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[blk][0], 0, 0, 0);
-                    O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[blk][1], 0, 0, 0);
                 }
-            };
-            if (masked) pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo_masked(p0, p1, d, h, lo); });
-            else        pv([](float p0, float p1, uint32_t d, uint32_t & h, uint32_t & lo) { hilo(p0, p1, d, h, lo); });
+            }
             pa_wait_lds();
             send(at_v, v_k);
             live = live_next;
