@@ -13,7 +13,7 @@
 // crosses a request's end is cut there. A request inside one run is finished by its
 // workgroup; the parts of the others go to the workspace as (O, M, l) and
 // k_paged_merge joins them in the order of the runs, so results repeat bit for bit.
-// The KV heads and row tiles of one run are blocks next to each other on one XCD:
+// The KV heads and row groups of one run are blocks next to each other on one XCD:
 // the cache lines that two heads share come from one L2.
 //
 // Inside a workgroup the 4 waves take every fourth tile of the run, each on its
@@ -53,7 +53,7 @@ constexpr int PA_WAVES = 4;
 constexpr int PA_THREADS = PA_WAVES * 64;
 constexpr int PA_TILE = 32;            // keys of a tile
 constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
-constexpr int PA_WGS = 512;            // workgroups of a launch: two a CU
+constexpr int PA_CUS = 256;            // two workgroups a CU of one row tile, one of two (registers)
 constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
@@ -83,8 +83,9 @@ struct pa_args {
     fast_div        page;
     const char *    gate; char * dst;
     int32_t         type;              // of q, gate and dst
-    int32_t         n_seq, T, nh, nh_kv, rep, R, RT, x86;
+    int32_t         n_seq, T, nh, nh_kv, rep, R, x86;
     int32_t         runs;              // runs the tiles are cut into, at most
+    fast_div        f_runs, f_inner, f_kv, f_rep;      // runs, blocks of a run, KV heads, rep
     float           c;                 // scale * log2(e): scores are in log2 units
     float *         part_o;            // [run + request][nh_kv][R][D]
     float2 *        part_ml;           // [run + request][nh_kv][R]
@@ -102,11 +103,13 @@ template <int D> struct pa_cfg {
     static constexpr int UNITS = PA_TILE * UPR, DMAS = (UNITS + 63) / 64;
     static constexpr int UMUL = 65536 / UPR + 1;         // i / UPR = i UMUL >> 16 for i < UNITS
     static constexpr int ROWS = PA_TILE * LS;            // of a tensor's tile in LDS
+    static constexpr int OROW = D + 4;                   // floats of a row of O in LDS: rows from other banks
     // of a wave: K, V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
     static constexpr int OA = 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
     static constexpr int WAVE = OS + 2 * NBLK * PA_TILE * 2;
-    static constexpr int IMG = 16 * NBLK * 64;           // the query windows, in the first wave's V
-    static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * D * 4 && WAVE % 16 == 0, "V holds the query image, a wave's part its O");
+    static constexpr int IMG = 16 * NBLK * 64;           // the query windows of a row tile, in a wave's V
+    static constexpr int QI = NBLK / 2;                  // 4-value groups a thread quantises, a row tile
+    static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * OROW * 4 && WAVE % 16 == 0, "V holds the query image, a wave's part its O");
     static_assert((UNITS - 1) * (UMUL * UPR - 65536) < 65536, "the division is exact");
     static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
 };
@@ -171,20 +174,47 @@ __device__ __forceinline__ void hilo(float p0, float p1, uint32_t d, uint32_t & 
         "s_nop 1"
         : "=&v"(hi), "=&v"(lo) : "v"(p0), "v"(p1), "v"(x0), "v"(x1), "v"(d));
 }
-// The block's run of the tiles of all requests.
-struct pa_run { int b; int32_t off, left, pos, per; };
+// A block's run of the tiles of all requests: the request it starts in and its length, the tile there, the
+// tiles left, how many tiles a run has.
+struct pa_run { int32_t b, n, off, left, pos, per; };
 
-// Where run g starts: the request and its tile. Every thread sums the tiles of a few requests.
+__device__ __forceinline__ int32_t clip_len(const pa_args & a, int32_t n) { return n <= 0 ? 0 : n < a.max_kv ? n : (int32_t) a.max_kv; }
+__device__ __forceinline__ int32_t tiles_of(int32_t n) { return (int32_t) (((uint32_t) n + PA_TILE - 1) / PA_TILE); }
+__device__ __forceinline__ int32_t run_len(const pa_args & a, int32_t total) {
+    const int32_t per = ((int32_t) div_by((uint32_t) (total + a.runs - 1), a.f_runs) + PA_WAVES - 1) / PA_WAVES * PA_WAVES;
+    return per < PA_MIN_TILES ? PA_MIN_TILES : per;         // whole rounds of the waves
+}
+
+// Where run g starts. Up to 64 requests: a lane each, every wave on its own. More: every thread sums the tiles of
+// a few requests.
 __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * sh) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    pa_run r{0, 0, 0, 0, 0, 0};
+    if (a.n_seq <= 64) {
+        const int32_t n = lane < a.n_seq ? clip_len(a, a.n_kv[lane]) : 0, t = tiles_of(n);
+        int32_t incl = t;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t x = __shfl_up(incl, d);
+            if (lane >= d) incl += x;
+        }
+        const int32_t total = __builtin_amdgcn_readlane(incl, 63);
+        r.per = run_len(a, total);
+        const int64_t start = (int64_t) g * r.per;
+        if (start < total) {
+            r.b = __builtin_popcountll(__ballot(incl <= (int32_t) start));
+            r.n = __builtin_amdgcn_readlane(n, r.b);
+            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b);
+            r.left = total - (int32_t) start < r.per ? total - (int32_t) start : r.per;
+            r.pos = (int32_t) start;
+        }
+        return r;
+    }
     const int c = (a.n_seq + PA_THREADS - 1) / PA_THREADS;
     int32_t sum = 0;
     for (int i = 0; i < c; i++) {
         const int b = tid * c + i;
-        if (b < a.n_seq) {
-            const int64_t n = a.n_kv[b];
-            sum += n <= 0 ? 0 : (int32_t) (((n < a.max_kv ? n : a.max_kv) + PA_TILE - 1) / PA_TILE);
-        }
+        if (b < a.n_seq) sum += tiles_of(clip_len(a, a.n_kv[b]));
     }
     int32_t incl = sum;
 #pragma unroll
@@ -202,49 +232,46 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
         total += x;
     }
     incl += before;
-    int32_t per = (total + a.runs - 1) / a.runs;
-    per = (per + PA_WAVES - 1) / PA_WAVES * PA_WAVES;       // a wave's tiles: whole rounds
-    per = per < PA_MIN_TILES ? PA_MIN_TILES : per;
-    const int64_t start = (int64_t) g * per;
+    r.per = run_len(a, total);
+    const int64_t start = (int64_t) g * r.per;
     if (start >= incl - sum && start < incl) {
         int32_t at = incl - sum;
         for (int i = 0; i < c; i++) {
             const int b = tid * c + i;
-            const int64_t n = b < a.n_seq ? a.n_kv[b] : 0;
-            const int32_t t = n <= 0 ? 0 : (int32_t) (((n < a.max_kv ? n : a.max_kv) + PA_TILE - 1) / PA_TILE);
+            const int32_t n = b < a.n_seq ? clip_len(a, a.n_kv[b]) : 0, t = tiles_of(n);
             if (start >= at && start < at + t) {
                 sh[PA_WAVES] = b;
-                sh[PA_WAVES + 1] = (int32_t) (start - at);
+                sh[PA_WAVES + 1] = n;
+                sh[PA_WAVES + 2] = (int32_t) (start - at);
             }
             at += t;
         }
     }
     __syncthreads();
-    pa_run r{0, 0, 0, 0, per};
     if (start < total) {
         r.b = __builtin_amdgcn_readfirstlane(sh[PA_WAVES]);
-        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
-        r.left = __builtin_amdgcn_readfirstlane(total - start < per ? (int32_t) (total - start) : per);
+        r.n = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
+        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 2]);
+        r.left = __builtin_amdgcn_readfirstlane(total - start < r.per ? (int32_t) (total - start) : r.per);
         r.pos = (int32_t) start;
     }
     return r;
 }
 
-template <int D>
-__global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
+template <int D, int RT>
+__global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
     using C = pa_cfg<D>;
-    constexpr int NBLK = C::NBLK, ND = C::DMAS;
+    constexpr int NBLK = C::NBLK, ND = C::DMAS, ROWS = 16 * RT;
     __shared__ __attribute__((aligned(16))) uint8_t lds[PA_WAVES * C::WAVE];
-    __shared__ float2 ml[PA_WAVES][16];
-    __shared__ int32_t sh[PA_WAVES + 2];
+    __shared__ float2 ml[PA_WAVES][ROWS];
+    __shared__ int32_t sh[PA_WAVES + 3];
     const int tid = threadIdx.x;
     int lane = tid & 63, ln = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // blocks -> (run, KV head, row tile): those of one run follow each other on one XCD
-    const int inner = a.nh_kv * a.RT;
-    const int j = blockIdx.x >> 3, g = j / inner * 8 + (int) (blockIdx.x & 7), hr = j % inner;
-    const int kvh = hr % a.nh_kv, rt = hr / a.nh_kv;
+    // blocks -> (run, KV head, row group): those of one run follow each other on one XCD
+    const uint32_t j = blockIdx.x >> 3, jq = div_by(j, a.f_inner), hr = j - jq * a.f_inner.d;
+    const int g = (int) jq * 8 + (int) (blockIdx.x & 7), rg = (int) div_by(hr, a.f_kv), kvh = (int) hr - rg * a.nh_kv;
     pa_run run = find_run(a, g, sh);
 
     uint8_t * const my = lds + wave * C::WAVE;
@@ -256,19 +283,19 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     const uint32_t at_k = pa_lds(my), at_v = at_k + C::ROWS, at_e = at_k + C::OE;
     const char * kh = a.k + (size_t) kvh * a.nb2;
     const char * vh = a.v + (size_t) kvh * a.nb2;
-    // this lane's query row
-    const int row = 16 * rt + ln, trow = row / a.rep;
+    const uint64_t v_k = (uint64_t) (vh - kh);
+    const size_t es = a.type == QWFN_TYPE_F32 ? 4 : 2;
+    // element of dst (and gate) of row r's first value
+    auto element = [&](int b, int r) {
+        const uint32_t t = div_by((uint32_t) r, a.f_rep), h = (uint32_t) (kvh * a.rep + r) - t * (uint32_t) a.rep;
+        return (((size_t) b * a.T + t) * a.nh + h) * D;
+    };
 
-    for (; run.left > 0; run.b++, run.off = 0) {
+    while (run.left > 0) {
         const int b = run.b;
-        const int32_t n_in = a.n_kv[b];
-        const int32_t n = n_in <= 0 ? 0 : n_in < a.max_kv ? n_in : (int32_t) a.max_kv;
-        if (n != n_in && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
-        const int32_t tiles = (int32_t) (((int64_t) n + PA_TILE - 1) / PA_TILE);
-        if (tiles == 0) continue;
+        const int32_t n = run.n, tiles = tiles_of(n);
         const int32_t nt = tiles - run.off < run.left ? tiles - run.off : run.left;   // tiles of this part
         const bool whole = nt == tiles;
-        if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(run.pos / run.per, (run.pos + tiles - 1) / run.per);
         const int32_t * table = a.table + (int64_t) b * a.t_stride;
 
         // the table entries of a tile's keys (lanes l and l + 32 the same), clipped to the part's last key
@@ -287,7 +314,6 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             if (lane < PA_TILE) addr[lane] = (uint64_t) (uintptr_t) kh + (uint64_t) slot * a.nb1;
             return (uint32_t) __ballot(ok);
         };
-        const uint64_t v_k = (uint64_t) (vh - kh);
         auto send = [&](uint32_t at, uint64_t delta) {
 #pragma unroll
             for (int i = 0; i < ND; i++) {
@@ -297,52 +323,86 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             }
         };
         __syncthreads();                                   // the LDS of the part before is read
+        // query values on their way: 8 lanes a q8_0 block
+        float qx[RT][C::QI][4];
+        const int sub = tid & 7;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int i = 0; i < C::QI; i++) {
+                const int x = (tid >> 3) + 32 * i, r = x / NBLK, blk = x % NBLK;
+                int rr = ROWS * rg + 16 * rt + r;
+                rr = rr < a.R ? rr : a.R - 1;
+                const uint32_t t = div_by((uint32_t) rr, a.f_rep), h = (uint32_t) (kvh * a.rep + rr) - t * (uint32_t) a.rep;
+                load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 + (size_t) (blk * QK + sub * 4) * es,
+                      a.type, qx[rt][i]);
+            }
         uint32_t live = 0, live_next = 0;                  // the tile's keys that exist
         if (wave < nt) {
             entries(wave);
             pa_wait<0>();
             live = rows_of(wave);
+        }
+        // (they have come with the entries: a wait for them behind the rows' DMA would wait for the rows too)
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int i = 0; i < C::QI; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) asm volatile("" : "+v"(qx[rt][i][k]));
+        if (wave < nt) {
             wave_lds_sync();
             send(at_k, 0);
             entries(wave + PA_WAVES);
         }
-
-        // the query image: rows requantised, each block at its place of its window
-        uint8_t * const img = lds + C::ROWS;
-        for (int i = tid; i < C::IMG / 16; i += PA_THREADS) ((v4u *) img)[i] = v4u{0, 0, 0, 0};
-        __syncthreads();
-        float * dql = (float *) (img + C::IMG);
-        for (int i = tid >> 3; i < 16 * NBLK; i += PA_THREADS / 8) {
-            const int r = i / NBLK, blk = i % NBLK, rr = 16 * rt + r, sub = tid & 7;
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (rr < a.R) {
-                const int t = rr / a.rep, h = kvh * a.rep + (rr - t * a.rep);
-                load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 +
-                          (size_t) (blk * QK + sub * 4) * (a.type == QWFN_TYPE_F32 ? 4 : 2), a.type, x);
-            }
-            uint16_t d16;
-            float dq;
-            const uint32_t q4 = dev::q8_quantize_lane4(x, a.x86 != 0, &d16, &dq);
-            const int at = QBLOCK * blk + 2 - (QBLOCK * blk + 2) / 16 * 16;
-            uint16_t * qp = (uint16_t *) (img + (r * NBLK + blk) * 64 + at + sub * 4);
-            qp[0] = (uint16_t) q4;
-            qp[1] = (uint16_t) (q4 >> 16);
-            if (sub == 0) dql[r * NBLK + blk] = dq;
-        }
-        __syncthreads();
-        v4i qw[NBLK];
-        float dq[NBLK];                                    // dq c to 22 bits: PA_IBIAS dq is exact
+        // the query image: rows requantised, each block at its place of a window that is zero elsewhere; row tile rt
+        // in wave rt's V
 #pragma unroll
-        for (int blk = 0; blk < NBLK; blk++) {
-            qw[blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
-            const uint32_t x = __builtin_bit_cast(uint32_t, dql[ln * NBLK + blk] * a.c);
-            dq[blk] = __builtin_bit_cast(float, (x + 2u) & ~3u);
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int i = 0; i < C::QI; i++)
+                *(uint2 *) (lds + rt * C::WAVE + C::ROWS + ((tid >> 3) + 32 * i) * 64 + sub * 8) = make_uint2(0u, 0u);
+        wave_lds_sync();                                   // a block's 8 lanes zero its window, then write into it
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            uint8_t * const img = lds + rt * C::WAVE + C::ROWS;
+            float * dql = (float *) (img + C::IMG);
+#pragma unroll
+            for (int i = 0; i < C::QI; i++) {
+                const int x = (tid >> 3) + 32 * i, blk = x % NBLK;
+                uint16_t d16;
+                float dq;
+                const uint32_t q4 = dev::q8_quantize_lane4(qx[rt][i], a.x86 != 0, &d16, &dq);
+                uint16_t * qp = (uint16_t *) (img + x * 64 + (QBLOCK * blk + 2) % 16 + sub * 4);
+                qp[0] = (uint16_t) q4;
+                qp[1] = (uint16_t) (q4 >> 16);
+                if (sub == 0) dql[x] = dq;
+            }
+        }
+        __syncthreads();
+        v4i qw[RT][NBLK];
+        float dq[RT][NBLK];                                // dq c to 22 bits: PA_IBIAS dq is exact
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const uint8_t * img = lds + rt * C::WAVE + C::ROWS;
+#pragma unroll
+            for (int blk = 0; blk < NBLK; blk++) {
+                qw[rt][blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
+                const uint32_t x = __builtin_bit_cast(uint32_t, ((const float *) (img + C::IMG))[ln * NBLK + blk] * a.c);
+                dq[rt][blk] = __builtin_bit_cast(float, (x + 2u) & ~3u);
+            }
         }
         __syncthreads();
 
-        v4f O[NBLK][2] = {};
-        float M = -INFINITY, l = 0.f;
-        const int32_t limit = n - a.T + trow + 1;          // the row sees keys below it
+        v4f O[RT][NBLK][2] = {};
+        float M[RT], l[RT];
+        int32_t limit[RT];                                 // the lane's row sees keys below it
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            M[rt] = -INFINITY;
+            l[rt] = 0.f;
+            limit[rt] = n - a.T + (int32_t) div_by((uint32_t) (ROWS * rg + 16 * rt + ln), a.f_rep) + 1;
+        }
         if (wave < nt) {
             pa_wait_lds();
             send(at_v, v_k);
@@ -366,25 +426,25 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
 
             // S^T: lane (row ln, keys 16 u + 4 lg + r). An integer dot comes out of the MFMA on top of the bits of
             // PA_IBIAS, so it is PA_IBIAS + dot as a float, and one fused step makes dot dq of it.
-            float s[2][4];
+            float s[RT][2][4] = {};
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const uint8_t * kl = my + (16 * u + ln) * C::LS + 16 * lg;
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int blk = 0; blk < NBLK; blk++) {
                     const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
-                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{PA_IBITS, PA_IBITS, PA_IBITS, PA_IBITS}, 0, 0, 0);
                     const uint2 dk = *(const uint2 *) (kscl + blk * PA_TILE + 16 * u + 4 * lg);
-                    const int d0 = d[0], d1 = d[1], d2 = d[2], d3 = d[3];
-                    const float nb = -PA_IBIAS * dq[blk];
-                    acc[0] = fma_f16lo(dk.x, __fmaf_rn(__builtin_bit_cast(float, d0), dq[blk], nb), acc[0]);
-                    acc[1] = fma_f16hi(dk.x, __fmaf_rn(__builtin_bit_cast(float, d1), dq[blk], nb), acc[1]);
-                    acc[2] = fma_f16lo(dk.y, __fmaf_rn(__builtin_bit_cast(float, d2), dq[blk], nb), acc[2]);
-                    acc[3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), dq[blk], nb), acc[3]);
-                }
 #pragma unroll
-                for (int r = 0; r < 4; r++) s[u][r] = acc[r];
+                    for (int rt = 0; rt < RT; rt++) {
+                        const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[rt][blk], v4i{PA_IBITS, PA_IBITS, PA_IBITS, PA_IBITS}, 0, 0, 0);
+                        const int d0 = d[0], d1 = d[1], d2 = d[2], d3 = d[3];
+                        const float f = dq[rt][blk], nb = -PA_IBIAS * f;
+                        s[rt][u][0] = fma_f16lo(dk.x, __fmaf_rn(__builtin_bit_cast(float, d0), f, nb), s[rt][u][0]);
+                        s[rt][u][1] = fma_f16hi(dk.x, __fmaf_rn(__builtin_bit_cast(float, d1), f, nb), s[rt][u][1]);
+                        s[rt][u][2] = fma_f16lo(dk.y, __fmaf_rn(__builtin_bit_cast(float, d2), f, nb), s[rt][u][2]);
+                        s[rt][u][3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), f, nb), s[rt][u][3]);
+                    }
+                }
             }
             // the next tile's K
             pa_wait<ND>();
@@ -415,116 +475,133 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             }
             for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
             wave_lds_sync();
-            if (masked) {
-                dmax = 0;                                  // of the keys that the row sees
+            float p[RT][2][4];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                uint32_t top_d = dmax;
+                if (masked) {
+                    top_d = 0;                             // of the keys that the row sees
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int k = 16 * u + 4 * lg + r;
+                            if (!(live >> k & 1) || key0 + k >= limit[rt]) s[rt][u][r] = -INFINITY;
+                            else top_d = max(top_d, (uint32_t) vtop[k]);
+                        }
+                    top_d = max(top_d, (uint32_t) __shfl_xor((int) top_d, 16));
+                    top_d = max(top_d, (uint32_t) __shfl_xor((int) top_d, 32));
+                }
+                float top = vmax(vmax(s[rt][0][0], s[rt][0][1]), vmax(s[rt][0][2], s[rt][0][3]));
+                top = vmax(top, vmax(vmax(s[rt][1][0], s[rt][1][1]), vmax(s[rt][1][2], s[rt][1][3])));
+                top = xmax_lanes16_32(top);
+                const int e = (int) (top_d >> 10) < 1 ? 1 : (int) (top_d >> 10);      // d < 2^(e - 14)
+                const float ref = top + (float) (e - 14 - PA_BIAS);
+                if (__ballot(ref > M[rt] + PA_SLACK)) {
+                    const float to = fmaxf(M[rt], ref);
+                    const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M[rt] - to);
+                    M[rt] = to;
+                    l[rt] *= f;
+#pragma unroll
+                    for (int blk = 0; blk < NBLK; blk++) { O[rt][blk][0] *= f; O[rt][blk][1] *= f; }
+                }
+                const float m = M[rt] == -INFINITY ? 0.f : M[rt];
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int k = 16 * u + 4 * lg + r;
-                        if (!(live >> k & 1) || key0 + k >= limit) s[u][r] = -INFINITY;
-                        else dmax = max(dmax, (uint32_t) vtop[k]);
+                        p[rt][u][r] = __builtin_amdgcn_exp2f(s[rt][u][r] - m);       // 2^-inf = 0
+                        l[rt] += p[rt][u][r];
                     }
-                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 16));
-                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
             }
-            float top = vmax(vmax(s[0][0], s[0][1]), vmax(s[0][2], s[0][3]));
-            top = vmax(top, vmax(vmax(s[1][0], s[1][1]), vmax(s[1][2], s[1][3])));
-            top = xmax_lanes16_32(top);
-            const int e = (int) (dmax >> 10) < 1 ? 1 : (int) (dmax >> 10);        // d < 2^(e - 14)
-            const float ref = top + (float) (e - 14 - PA_BIAS);
-            if (__ballot(ref > M + PA_SLACK)) {
-                const float to = fmaxf(M, ref);
-                const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - to);
-                M = to;
-                l *= f;
-#pragma unroll
-                for (int blk = 0; blk < NBLK; blk++) { O[blk][0] *= f; O[blk][1] *= f; }
-            }
-            const float m = M == -INFINITY ? 0.f : M;
-            float p[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    p[u][r] = __builtin_amdgcn_exp2f(s[u][r] - m);       // 2^-inf = 0
-                    l += p[u][r];
-                }
             // O^T: A lane (dims 2 ln + e of the block, keys 4 lg + r of both halves)
 #pragma unroll
             for (int blk = 0; blk < NBLK; blk++) {
                 const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
                 uint32_t av[2][4];
+                uint2 dv[2];
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) av[u][r] = *(const uint16_t *) (vl + (16 * u + r) * C::LS);
-                v4u a0, a1, bh, bl;
+                    dv[u] = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
+                }
+                v4u a0, a1;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     uint32_t x0[2], x1[2];
                     cvt_v_block(av[u], x0, x1);
                     a0[2 * u] = x0[0]; a0[2 * u + 1] = x0[1];
                     a1[2 * u] = x1[0]; a1[2 * u + 1] = x1[1];
-                    const uint2 dv = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
-                    uint32_t h0, h1, l0, l1;
-                    hilo(p[u][0], p[u][1], dv.x, h0, l0);
-                    hilo(p[u][2], p[u][3], dv.y, h1, l1);
-                    bh[2 * u] = h0; bh[2 * u + 1] = h1;
-                    bl[2 * u] = l0; bl[2 * u + 1] = l1;
                 }
                 const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
-                const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
-                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[blk][0], 0, 0, 0);
-                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[blk][1], 0, 0, 0);
-                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[blk][0], 0, 0, 0);
-                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[blk][1], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    v4u bh, bl;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t h0, h1, l0, l1;
+                        hilo(p[rt][u][0], p[rt][u][1], dv[u].x, h0, l0);
+                        hilo(p[rt][u][2], p[rt][u][3], dv[u].y, h1, l1);
+                        bh[2 * u] = h0; bh[2 * u + 1] = h1;
+                        bl[2 * u] = l0; bl[2 * u + 1] = l1;
+                    }
+                    const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
+                    O[rt][blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[rt][blk][0], 0, 0, 0);
+                    O[rt][blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[rt][blk][1], 0, 0, 0);
+                    O[rt][blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[rt][blk][0], 0, 0, 0);
+                    O[rt][blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[rt][blk][1], 0, 0, 0);
+                }
             }
             if (__builtin_expect(__ballot(odd) != 0, 0)) {
                 // blocks of V whose scale is not finite, for the rows that see their key
-                for (int k = 0; k < PA_TILE; k++) {
-                    const int from = (k >> 2 & 3) * 16 + ln;
-                    float pk = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                for (int rt = 0; rt < RT; rt++)
+                    for (int k = 0; k < PA_TILE; k++) {
+                        const int from = (k >> 2 & 3) * 16 + ln;
+                        float pk = 0.f;
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const float y = __shfl(p[u][r], from);
-                            if (k == 16 * u + (k & 12) + r) pk = y;
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const float y = __shfl(p[rt][u][r], from);
+                                if (k == 16 * u + (k & 12) + r) pk = y;
+                            }
+#pragma unroll
+                        for (int blk = 0; blk < NBLK; blk++) {
+                            const uint8_t * vb = my + C::ROWS + k * C::LS + QBLOCK * blk;
+                            const uint16_t d = *(const uint16_t *) vb;
+                            if ((d & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
+#pragma unroll
+                            for (int e2 = 0; e2 < 2; e2++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++)
+                                    if (pk != 0.f)
+                                        O[rt][blk][e2][r] += pk * dev::f16_bits_to_f32(d) * (float) *(const int8_t *) (vb + 2 + 2 * (4 * lg + r) + e2);
                         }
-#pragma unroll
-                    for (int blk = 0; blk < NBLK; blk++) {
-                        const uint8_t * vb = my + C::ROWS + k * C::LS + QBLOCK * blk;
-                        const uint16_t dv = *(const uint16_t *) vb;
-                        if ((dv & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
-#pragma unroll
-                        for (int e2 = 0; e2 < 2; e2++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++)
-                                if (pk != 0.f)
-                                    O[blk][e2][r] += pk * dev::f16_bits_to_f32(dv) * (float) *(const int8_t *) (vb + 2 + 2 * (4 * lg + r) + e2);
                     }
-                }
             }
             pa_wait_lds();
             send(at_v, v_k);
             live = live_next;
         }
         pa_wait<0>();
-        l = sum_lanes16_32(l);
 
-        // the waves' parts meet in LDS: O[row][dim] of each
-        __syncthreads();
-        float * ob = (float *) (lds + wave * C::WAVE) + ln * D;
+        // the waves' parts meet in LDS, a row tile at a time: O[row][dim] of each
 #pragma unroll
-        for (int blk = 0; blk < NBLK; blk++)
+        for (int rt = 0; rt < RT; rt++) {
+            const float ls = sum_lanes16_32(l[rt]);
+            __syncthreads();
+            float * ob = (float *) (lds + wave * C::WAVE) + ln * C::OROW;
 #pragma unroll
-            for (int r = 0; r < 4; r += 2)
-                *(float4 *) (ob + QK * blk + 8 * lg + 2 * r) = make_float4(O[blk][0][r], O[blk][1][r], O[blk][0][r + 1], O[blk][1][r + 1]);
-        if (lg == 0) ml[wave][ln] = make_float2(M, l);
-        __syncthreads();
-        {
-            const int r = tid >> 4, rr = 16 * rt + r;
+            for (int blk = 0; blk < NBLK; blk++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                    *(float4 *) (ob + QK * blk + 8 * lg + 2 * r) =
+                        make_float4(O[rt][blk][0][r], O[rt][blk][1][r], O[rt][blk][0][r + 1], O[rt][blk][1][r + 1]);
+            if (lg == 0) ml[wave][ln] = make_float2(M[rt], ls);
+            __syncthreads();
+            const int r = tid >> 4, rr = ROWS * rg + 16 * rt + r;
             float2 e[PA_WAVES];
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -532,25 +609,26 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
 #pragma unroll
             for (int w = 0; w < PA_WAVES; w++) {
                 e[w].x = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - mm);
-                ll += e[w].x * e[w].y;
+                ll += e[w].x * e[w].y;                     // a NaN stays one
             }
             if (rr < a.R) {
-                const int t = rr / a.rep, h = kvh * a.rep + (rr - t * a.rep);
-                const size_t part = ((size_t) (run.pos / run.per + b) * a.nh_kv + kvh) * a.R + rr;
+                const size_t elem = element(b, rr), part = ((size_t) (g + b) * a.nh_kv + kvh) * a.R + rr;
                 const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
-                for (int d0 = 4 * (tid & 15); d0 < D; d0 += 64) {
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) {
+                    const int d0 = 4 * (tid & 15) + 64 * i;
                     float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int w = 0; w < PA_WAVES; w++) {
-                        const float4 x = *(const float4 *) ((const float *) (lds + w * C::WAVE) + r * D + d0);
+                        const float4 x = *(const float4 *) ((const float *) (lds + w * C::WAVE) + r * C::OROW + d0);
                         if (e[w].x != 0.f) {
                             o[0] += e[w].x * x.x; o[1] += e[w].x * x.y; o[2] += e[w].x * x.z; o[3] += e[w].x * x.w;
                         }
                     }
                     if (whole) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[i] *= inv;
-                        finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + d0, o);
+                        for (int k = 0; k < 4; k++) o[k] *= inv;
+                        finish4(a, elem + d0, o);
                     } else {
                         *(float4 *) (a.part_o + part * D + d0) = make_float4(o[0], o[1], o[2], o[3]);
                     }
@@ -558,88 +636,122 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                 if (!whole && (tid & 15) == 0) a.part_ml[part] = make_float2(mm, ll);
             }
         }
+        if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(g, (run.pos + tiles - 1) / run.per);
         run.left -= nt;
         run.pos += nt;
+        run.off = 0;
+        if (run.left > 0)
+            do run.n = clip_len(a, a.n_kv[++run.b]);
+            while (run.n == 0);
+    }
+    // requests without a key, and lengths that were clipped
+    for (int b = g; b < a.n_seq; b += (int) (gridDim.x / a.f_inner.d)) {
+        const int32_t n = a.n_kv[b];
+        if (n != clip_len(a, n) && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+        if (n > 0) continue;
+        const float z[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r = tid >> 4; r < ROWS; r += PA_THREADS / 16)
+            if (ROWS * rg + r < a.R)
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) store4(a.dst + (element(b, ROWS * rg + r) + 4 * (tid & 15) + 64 * i) * es, a.type, z);
+        if (hr == 0 && tid == 0) a.span[b] = make_int2(0, 0);
     }
 }
 
-// The parts of a request joined: a workgroup per query row and 64 dims, 16 groups of
-// 16 lanes that take every 16th part. Requests of one run are done; those without a
-// key are written here (0).
-constexpr int PM_GROUPS = 16;
+// The parts of a request joined, log-sum-exp weights: GROUPS groups of 16 lanes a query row and 64 of its dims,
+// each taking every GROUPS-th part, PM_BATCH of them in flight. A wave (4 groups) where a request has a few parts, a
+// workgroup (16) where it has many. Requests of one part are done.
+constexpr int PM_BATCH = 8;
 
-template <int D>
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
-    __shared__ float4 acc[PM_GROUPS][16];
-    __shared__ float2 gl[PM_GROUPS];
-    const int quarter = blockIdx.x % (D / 64);
-    const int64_t rowi = blockIdx.x / (D / 64);
-    const int r = (int) (rowi % a.R), kvh = (int) (rowi / a.R % a.nh_kv), b = (int) (rowi / a.R / a.nh_kv);
-    const int g = threadIdx.x >> 4, q = threadIdx.x & 15;
-    const int t = r / a.rep, h = kvh * a.rep + (r - t * a.rep);
-    const size_t elem = (((size_t) b * a.T + t) * a.nh + h) * D + 64 * quarter + 4 * q;
-    const int32_t n = a.n_kv[b];
-    if (n <= 0) {
-        if (n < 0 && threadIdx.x == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
-        if (g == 0) store4(a.dst + elem * (a.type == QWFN_TYPE_F32 ? 4 : 2), a.type, z);
-        return;
-    }
-    const int2 sp = a.span[b];
-    if (sp.x == sp.y) return;
+    __shared__ float4 acc[16][16];
+    __shared__ float2 gl[16];
+    const int sub = GROUPS == 16 ? 0 : (int) threadIdx.x >> 6;
+    const int64_t unit = GROUPS == 16 ? (int64_t) blockIdx.x : (int64_t) blockIdx.x * 4 + sub;
+    const int quarter = (int) (unit % (D / 64));
+    const uint32_t row = (uint32_t) (unit / (D / 64)), bk = row / (uint32_t) a.R, r = row - bk * (uint32_t) a.R;
+    const uint32_t b = div_by(bk, a.f_kv), kvh = bk - b * (uint32_t) a.nh_kv;
+    const bool on = b < (uint32_t) a.n_seq;
+    const int2 sp = on ? a.span[b] : make_int2(0, 0);
+    if (GROUPS == 16 && sp.x == sp.y) return;
+    const int g = (int) (threadIdx.x >> 4) % GROUPS, q = threadIdx.x & 15;
     float M = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = sp.x + g; s <= sp.y; s += PM_GROUPS) {
-        const size_t part = ((size_t) (s + b) * a.nh_kv + kvh) * a.R + r;
-        const float2 e = a.part_ml[part];
-        const float4 x = *(const float4 *) (a.part_o + part * D + 64 * quarter + 4 * q);
-        if (e.x == -INFINITY) continue;
-        const float to = fmaxf(M, e.x), f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to),
-                    w = __builtin_amdgcn_exp2f(e.x - to);
-        o.x = o.x * f + w * x.x; o.y = o.y * f + w * x.y; o.z = o.z * f + w * x.z; o.w = o.w * f + w * x.w;
-        l = l * f + w * e.y;
-        M = to;
+    if (sp.x != sp.y) {
+        const size_t step = (size_t) a.nh_kv * a.R;
+        const size_t p0 = ((size_t) (sp.x + (int) b) * a.nh_kv + kvh) * a.R + r;
+        const float * po = a.part_o + p0 * D + 64 * quarter + 4 * q;
+        const int n = sp.y - sp.x + 1;
+        for (int s0 = g; s0 < n; s0 += GROUPS * PM_BATCH) {
+            float2 e[PM_BATCH];
+            float4 x[PM_BATCH];
+            float to = M;
+#pragma unroll
+            for (int i = 0; i < PM_BATCH; i++) {
+                const int s = s0 + i * GROUPS < n ? s0 + i * GROUPS : s0;
+                e[i] = a.part_ml[p0 + s * step];
+                x[i] = *(const float4 *) (po + s * step * D);
+            }
+#pragma unroll
+            for (int i = 0; i < PM_BATCH; i++) {
+                if (s0 + i * GROUPS >= n) e[i] = make_float2(-INFINITY, 0.f);
+                to = fmaxf(to, e[i].x);
+            }
+            const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to);
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < PM_BATCH; i++) {
+                const float w = e[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[i].x - to);
+                l += w * e[i].y;                           // a NaN stays one
+                if (w != 0.f) { o.x += w * x[i].x; o.y += w * x[i].y; o.z += w * x[i].z; o.w += w * x[i].w; }
+            }
+            M = to;
+        }
     }
-    acc[g][q] = o;
-    if (q == 0) gl[g] = make_float2(M, l);
+    const int slot = sub * GROUPS % 16 + g;
+    acc[slot][q] = o;
+    if (q == 0) gl[slot] = make_float2(M, l);
     __syncthreads();
-    if (g == 0) {
+    if (g == 0 && sp.x != sp.y) {
         float mm = -INFINITY, ll = 0.f;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < PM_GROUPS; i++) mm = fmaxf(mm, gl[i].x);
+        for (int i = 0; i < GROUPS; i++) mm = fmaxf(mm, gl[slot + i].x);
 #pragma unroll
-        for (int i = 0; i < PM_GROUPS; i++) {
-            if (gl[i].x == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(gl[i].x - mm);
-            const float4 v = acc[i][q];
-            ll += w * gl[i].y;
-            x[0] += w * v.x; x[1] += w * v.y; x[2] += w * v.z; x[3] += w * v.w;
+        for (int i = 0; i < GROUPS; i++) {
+            const float w = gl[slot + i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(gl[slot + i].x - mm);
+            const float4 v = acc[slot + i][q];
+            ll += w * gl[slot + i].y;
+            if (w != 0.f) { x[0] += w * v.x; x[1] += w * v.y; x[2] += w * v.z; x[3] += w * v.w; }
         }
         const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] *= inv;
-        finish4(a, elem, x);
+        const uint32_t t = div_by(r, a.f_rep), h = kvh * (uint32_t) a.rep + r - t * (uint32_t) a.rep;
+        finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 64 * quarter + 4 * q, x);
     }
 }
 
 // ---------------------------------------------------------------- host
 
 struct pa_plan {
-    int32_t RT, runs;
+    int32_t RT, groups, runs;          // row tiles of a workgroup, row groups
     size_t  off_o, off_ml, bytes;
 };
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Runs: as many as fill two workgroups a CU, whole rounds of the 8 XCDs; no more than the longest
-// requests could need.
+// Runs: as many as fill the CUs (two workgroups each, or one of two row tiles), whole rounds of the 8 XCDs; no
+// more than the longest requests could need.
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    p.RT = (int32_t) ((R + 15) / 16);
+    p.RT = R > 16 ? 2 : 1;
+    p.groups = (int32_t) ((R + 16 * p.RT - 1) / (16 * p.RT));
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE) + PA_MIN_TILES - 1) / PA_MIN_TILES;
-    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(PA_WGS / (nh_kv * p.RT), most));
+    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(PA_CUS * (3 - p.RT) / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
     p.off_o = round256((size_t) n_seq * sizeof(int2));
     p.off_ml = p.off_o + round256(parts * D * sizeof(float));
@@ -667,9 +779,9 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
     if (nh_kv > 128) return err(QWFN_ENOTSUP, ": at most 128 KV heads");
     if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff - 2 * PA_TILE * PA_WAVES)
         return err(QWFN_EINVAL, ": page_size and max_pages must be positive, their product below 2^31 - 256");
-    if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1) > 0x7fffffff)
+    if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1) > 0x7ffff000)
         return err(QWFN_ENOTSUP, ": at most 65536 requests and 2^31 tiles of 32 keys");
-    if (B * nh * T * (D / 64) > 0x7fffffff) return err(QWFN_ENOTSUP, ": too many query rows");
+    if (B * nh * T * (D / 64) > 0x7ffff000) return err(QWFN_ENOTSUP, ": too many query rows");
     if (k->ne[1] < page_size) return err(QWFN_EINVAL, ": the pool holds no whole page");
     if (k->ne[1] > 0x7fffffff) return err(QWFN_ENOTSUP, ": a pool of at most 2^31 - 1 rows");
     *pl = plan_paged(D, T, nh, nh_kv, B, (int64_t) page_size * max_pages);
@@ -677,12 +789,17 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
 }
 
 template <int D>
-int launch_paged(const pa_args & a, hipStream_t s) {
-    const int64_t blocks = (int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * a.RT;
-    hipLaunchKernelGGL(k_paged_attn<D>, dim3((unsigned) blocks), dim3(PA_THREADS), 0, s, a);
+int launch_paged(const pa_args & a, const pa_plan & p, hipStream_t s) {
+    const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * p.groups));
+    if (p.RT == 1) hipLaunchKernelGGL((k_paged_attn<D, 1>), grid, dim3(PA_THREADS), 0, s, a);
+    else           hipLaunchKernelGGL((k_paged_attn<D, 2>), grid, dim3(PA_THREADS), 0, s, a);
     if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
-    const int64_t rows = (int64_t) a.n_seq * a.nh_kv * a.R;
-    hipLaunchKernelGGL(k_paged_merge<D>, dim3((unsigned) (rows * (D / 64))), dim3(256), 0, s, a);
+    // the requests' parts: on average runs / n_seq each, with long requests among short ones more
+    const int64_t units = (int64_t) a.n_seq * a.nh_kv * a.R * (D / 64);
+    if (a.runs > 16 * (int64_t) a.n_seq)
+        hipLaunchKernelGGL((k_paged_merge<D, 16>), dim3((unsigned) units), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_paged_merge<D, 4>), dim3((unsigned) ((units + 3) / 4)), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "flash_attn_ext_paged launch");
 }
 
@@ -757,13 +874,15 @@ extern "C" int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_
         a.page = make_div((uint32_t) page_size);
         a.gate = gate ? (const char *) gate->data : nullptr; a.dst = (char *) dst->data; a.type = q->type;
         a.n_seq = (int32_t) B; a.T = (int32_t) T; a.nh = (int32_t) nh; a.nh_kv = (int32_t) nh_kv;
-        a.rep = (int32_t) (nh / nh_kv); a.R = a.T * a.rep; a.RT = pl.RT; a.x86 = variant == QWFN_Q8_X86;
+        a.rep = (int32_t) (nh / nh_kv); a.R = a.T * a.rep; a.x86 = variant == QWFN_Q8_X86;
+        a.f_runs = make_div((uint32_t) pl.runs); a.f_inner = make_div((uint32_t) (nh_kv * pl.groups));
+        a.f_kv = make_div((uint32_t) nh_kv); a.f_rep = make_div((uint32_t) a.rep);
         a.runs = pl.runs; a.c = scale * PA_LOG2E;
         a.span = (int2 *) ws; a.part_o = (float *) ((char *) ws + pl.off_o); a.part_ml = (float2 *) ((char *) ws + pl.off_ml);
         switch (D) {
-            case 64:  return launch_paged<64>(a, as_stream(stream));
-            case 128: return launch_paged<128>(a, as_stream(stream));
-            default:  return launch_paged<256>(a, as_stream(stream));
+            case 64:  return launch_paged<64>(a, pl, as_stream(stream));
+            case 128: return launch_paged<128>(a, pl, as_stream(stream));
+            default:  return launch_paged<256>(a, pl, as_stream(stream));
         }
     });
 }
