@@ -53,6 +53,7 @@ constexpr int PA_WAVES = 4;
 constexpr int PA_THREADS = PA_WAVES * 64;
 constexpr int PA_TILE = 32;            // keys of a tile
 constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
+constexpr int PA_LEAD = 8;             // tiles that a request counts more than it has
 constexpr int PA_CUS = 256;            // two workgroups a CU of one row tile, one of two (registers)
 constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
 constexpr float PA_LOG2E = 1.4426950408889634f;
@@ -93,7 +94,7 @@ struct pa_args {
     uint32_t *      status;
 };
 
-template <int D> struct pa_cfg {
+template <int D, int NS> struct pa_cfg {
     static constexpr int NBLK = D / QK;
     static constexpr int SEG = NBLK * QBLOCK;            // bytes of a head row
     // a row goes to LDS in units of a DMA lane, 16 bytes where a head row is whole ones; UPR of them a row
@@ -104,12 +105,12 @@ template <int D> struct pa_cfg {
     static constexpr int UMUL = 65536 / UPR + 1;         // i / UPR = i UMUL >> 16 for i < UNITS
     static constexpr int ROWS = PA_TILE * LS;            // of a tensor's tile in LDS
     static constexpr int OROW = D + 4;                   // floats of a row of O in LDS: rows from other banks
-    // of a wave: K, V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
-    static constexpr int OA = 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
+    // of a wave: NS stages of K and V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
+    static constexpr int OA = NS * 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
     static constexpr int WAVE = OS + 2 * NBLK * PA_TILE * 2;
-    static constexpr int IMG = 16 * NBLK * 64;           // the query windows of a row tile, in a wave's V
+    static constexpr int IMG = 16 * NBLK * 64;           // the query windows of a row tile
     static constexpr int QI = NBLK / 2;                  // 4-value groups a thread quantises, a row tile
-    static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * OROW * 4 && WAVE % 16 == 0, "V holds the query image, a wave's part its O");
+    static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * OROW * 4 && WAVE % 16 == 0, "the query images fit, and a wave's O in its part");
     static_assert((UNITS - 1) * (UMUL * UPR - 65536) < 65536, "the division is exact");
     static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
 };
@@ -175,11 +176,14 @@ __device__ __forceinline__ void hilo(float p0, float p1, uint32_t d, uint32_t & 
         : "=&v"(hi), "=&v"(lo) : "v"(p0), "v"(p1), "v"(x0), "v"(x1), "v"(d));
 }
 // A block's run of the tiles of all requests: the request it starts in and its length, the tile there, the
-// tiles left, how many tiles a run has.
+// tiles left, its place, how many tiles a run has. A request counts PA_LEAD tiles more than it has, in front of
+// its own (off starts at -PA_LEAD): what its queries and its output cost the workgroup that begins it. 48 ragged
+// requests without that: 102 us, the workgroups with two requests last.
 struct pa_run { int32_t b, n, off, left, pos, per; };
 
 __device__ __forceinline__ int32_t clip_len(const pa_args & a, int32_t n) { return n <= 0 ? 0 : n < a.max_kv ? n : (int32_t) a.max_kv; }
 __device__ __forceinline__ int32_t tiles_of(int32_t n) { return (int32_t) (((uint32_t) n + PA_TILE - 1) / PA_TILE); }
+__device__ __forceinline__ int32_t cost_of(int32_t n) { return n > 0 ? tiles_of(n) + PA_LEAD : 0; }
 __device__ __forceinline__ int32_t run_len(const pa_args & a, int32_t total) {
     const int32_t per = ((int32_t) div_by((uint32_t) (total + a.runs - 1), a.f_runs) + PA_WAVES - 1) / PA_WAVES * PA_WAVES;
     return per < PA_MIN_TILES ? PA_MIN_TILES : per;         // whole rounds of the waves
@@ -191,7 +195,7 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     pa_run r{0, 0, 0, 0, 0, 0};
     if (a.n_seq <= 64) {
-        const int32_t n = lane < a.n_seq ? clip_len(a, a.n_kv[lane]) : 0, t = tiles_of(n);
+        const int32_t n = lane < a.n_seq ? clip_len(a, a.n_kv[lane]) : 0, t = cost_of(n);
         int32_t incl = t;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -204,7 +208,7 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
         if (start < total) {
             r.b = __builtin_popcountll(__ballot(incl <= (int32_t) start));
             r.n = __builtin_amdgcn_readlane(n, r.b);
-            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b);
+            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b) - PA_LEAD;
             r.left = total - (int32_t) start < r.per ? total - (int32_t) start : r.per;
             r.pos = (int32_t) start;
         }
@@ -214,7 +218,7 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
     int32_t sum = 0;
     for (int i = 0; i < c; i++) {
         const int b = tid * c + i;
-        if (b < a.n_seq) sum += tiles_of(clip_len(a, a.n_kv[b]));
+        if (b < a.n_seq) sum += cost_of(clip_len(a, a.n_kv[b]));
     }
     int32_t incl = sum;
 #pragma unroll
@@ -238,7 +242,7 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
         int32_t at = incl - sum;
         for (int i = 0; i < c; i++) {
             const int b = tid * c + i;
-            const int32_t n = b < a.n_seq ? clip_len(a, a.n_kv[b]) : 0, t = tiles_of(n);
+            const int32_t n = b < a.n_seq ? clip_len(a, a.n_kv[b]) : 0, t = cost_of(n);
             if (start >= at && start < at + t) {
                 sh[PA_WAVES] = b;
                 sh[PA_WAVES + 1] = n;
@@ -251,7 +255,7 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
     if (start < total) {
         r.b = __builtin_amdgcn_readfirstlane(sh[PA_WAVES]);
         r.n = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
-        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 2]);
+        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 2]) - PA_LEAD;
         r.left = __builtin_amdgcn_readfirstlane(total - start < r.per ? (int32_t) (total - start) : r.per);
         r.pos = (int32_t) start;
     }
@@ -260,7 +264,10 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
 
 template <int D, int RT>
 __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
-    using C = pa_cfg<D>;
+    // one row tile: one stage a wave, two waves a SIMD; two: one wave a SIMD, and two stages (head size 128 would
+    // have more DMAs in flight than the counter of a wave holds)
+    constexpr int NS = RT == 2 && 4 * pa_cfg<D, 1>::DMAS + 1 < 63 ? 2 : 1;
+    using C = pa_cfg<D, NS>;
     constexpr int NBLK = C::NBLK, ND = C::DMAS, ROWS = 16 * RT;
     __shared__ __attribute__((aligned(16))) uint8_t lds[PA_WAVES * C::WAVE];
     __shared__ float2 ml[PA_WAVES][ROWS];
@@ -281,6 +288,10 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
     uint16_t * const kscl = (uint16_t *) (my + C::OS);
     uint16_t * const vscl = kscl + NBLK * PA_TILE;
     const uint32_t at_k = pa_lds(my), at_v = at_k + C::ROWS, at_e = at_k + C::OE;
+    // the query image of row tile rt, at image + rt IMG_STEP: with one stage in wave rt's V (sent for when the image is
+    // read), with two in the first wave's second stage (K's part, V's part)
+    constexpr int IMG_STEP = NS == 1 ? C::WAVE : C::ROWS;
+    uint8_t * const image = lds + (NS == 1 ? C::ROWS : 2 * C::ROWS);
     const char * kh = a.k + (size_t) kvh * a.nb2;
     const char * vh = a.v + (size_t) kvh * a.nb2;
     const uint64_t v_k = (uint64_t) (vh - kh);
@@ -294,6 +305,13 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
     while (run.left > 0) {
         const int b = run.b;
         const int32_t n = run.n, tiles = tiles_of(n);
+        if (run.off < 0) {                                 // the tiles in front count, no more
+            const int32_t lead = -run.off < run.left ? -run.off : run.left;
+            run.off += lead;
+            run.left -= lead;
+            run.pos += lead;
+            if (run.left == 0) break;
+        }
         const int32_t nt = tiles - run.off < run.left ? tiles - run.off : run.left;   // tiles of this part
         const bool whole = nt == tiles;
         const int32_t * table = a.table + (int64_t) b * a.t_stride;
@@ -352,20 +370,25 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                 for (int k = 0; k < 4; k++) asm volatile("" : "+v"(qx[rt][i][k]));
         if (wave < nt) {
             wave_lds_sync();
-            send(at_k, 0);
-            entries(wave + PA_WAVES);
+            if constexpr (NS == 1) {
+                send(at_k, 0);
+                entries(wave + PA_WAVES);
+            } else {
+                entries(wave + PA_WAVES);
+                send(at_k, 0);
+                send(at_v, v_k);
+            }
         }
-        // the query image: rows requantised, each block at its place of a window that is zero elsewhere; row tile rt
-        // in wave rt's V
+        // the query image: rows requantised, each block at its place of a window that is zero elsewhere
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int i = 0; i < C::QI; i++)
-                *(uint2 *) (lds + rt * C::WAVE + C::ROWS + ((tid >> 3) + 32 * i) * 64 + sub * 8) = make_uint2(0u, 0u);
+                *(uint2 *) (image + rt * IMG_STEP + ((tid >> 3) + 32 * i) * 64 + sub * 8) = make_uint2(0u, 0u);
         wave_lds_sync();                                   // a block's 8 lanes zero its window, then write into it
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            uint8_t * const img = lds + rt * C::WAVE + C::ROWS;
+            uint8_t * const img = image + rt * IMG_STEP;
             float * dql = (float *) (img + C::IMG);
 #pragma unroll
             for (int i = 0; i < C::QI; i++) {
@@ -384,7 +407,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         float dq[RT][NBLK];                                // dq c to 22 bits: PA_IBIAS dq is exact
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const uint8_t * img = lds + rt * C::WAVE + C::ROWS;
+            const uint8_t * img = image + rt * IMG_STEP;
 #pragma unroll
             for (int blk = 0; blk < NBLK; blk++) {
                 qw[rt][blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
@@ -403,23 +426,37 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             l[rt] = 0.f;
             limit[rt] = n - a.T + (int32_t) div_by((uint32_t) (ROWS * rg + 16 * rt + ln), a.f_rep) + 1;
         }
-        if (wave < nt) {
+        if (NS == 1 && wave < nt) {
             pa_wait_lds();
             send(at_v, v_k);
         }
-        // in flight at the top, in this order: K of the tile, the entries of the next, V of the tile
+        // in flight at the top, in this order: with one stage K of the tile, the entries of the next, V of the tile;
+        // with two the entries of the next tile, K and V of this one
+        int stage = 0;                                     // bytes
         for (int t = wave; t < nt; t += PA_WAVES) {
             // the lane's places are computed anew in every tile: kept over the loop they cost 40 registers, spilled
             asm volatile("" : "+v"(lane), "+v"(ln), "+v"(lg));
             const int32_t key0 = (run.off + t) * PA_TILE;
             const bool masked = live != 0xffffffffu || key0 + PA_TILE > n - a.T + 1;
-            pa_wait<ND + 1>();
+            if constexpr (NS == 1) {
+                pa_wait<ND + 1>();
+            } else {
+                pa_wait<2 * ND>();
+                live_next = rows_of(t + PA_WAVES);
+                wave_lds_sync();
+                pa_wait_lds();
+                entries(t + 2 * PA_WAVES);
+                send(at_k + (2 * C::ROWS - stage), 0);
+                send(at_v + (2 * C::ROWS - stage), v_k);
+                pa_wait<3 * ND + 1>();
+            }
+            const uint8_t * const kt = my + stage, * const vt = kt + C::ROWS;
             {   // K's scales by block and key
                 const int key = lane & 31, half = lane >> 5;
 #pragma unroll
                 for (int i = 0; i < NBLK / 2; i++) {
                     const int blk = half * (NBLK / 2) + i;
-                    kscl[blk * PA_TILE + key] = *(const uint16_t *) (my + key * C::LS + QBLOCK * blk);
+                    kscl[blk * PA_TILE + key] = *(const uint16_t *) (kt + key * C::LS + QBLOCK * blk);
                 }
             }
             wave_lds_sync();
@@ -429,7 +466,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             float s[RT][2][4] = {};
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint8_t * kl = my + (16 * u + ln) * C::LS + 16 * lg;
+                const uint8_t * kl = kt + (16 * u + ln) * C::LS + 16 * lg;
 #pragma unroll
                 for (int blk = 0; blk < NBLK; blk++) {
                     const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
@@ -446,16 +483,17 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                     }
                 }
             }
-            // the next tile's K
-            pa_wait<ND>();
-            live_next = rows_of(t + PA_WAVES);
-            wave_lds_sync();
-            pa_wait_lds();
-            send(at_k, 0);
-            entries(t + 2 * PA_WAVES);
+            if constexpr (NS == 1) {                       // the next tile's K
+                pa_wait<ND>();
+                live_next = rows_of(t + PA_WAVES);
+                wave_lds_sync();
+                pa_wait_lds();
+                send(at_k, 0);
+                entries(t + 2 * PA_WAVES);
+            }
             // V's scales; its largest of each key and of the tile. One that is not finite counts as 0 here and in
             // the products, and is added by itself below.
-            pa_wait<ND + 1>();
+            pa_wait<(2 * NS - 1) * ND + 1>();
             uint32_t dmax = 0;
             bool odd = false;
             {
@@ -464,7 +502,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
 #pragma unroll
                 for (int i = 0; i < NBLK / 2; i++) {
                     const int blk = half * (NBLK / 2) + i;
-                    const uint32_t dv = *(const uint16_t *) (my + C::ROWS + key * C::LS + QBLOCK * blk), mag = dv & 0x7fffu;
+                    const uint32_t dv = *(const uint16_t *) (vt + key * C::LS + QBLOCK * blk), mag = dv & 0x7fffu;
                     const bool fine = on && mag < 0x7c00u;
                     vscl[blk * PA_TILE + key] = (uint16_t) (fine ? dv : 0u);
                     dmax = max(dmax, fine ? mag : 0u);
@@ -517,7 +555,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             // O^T: A lane (dims 2 ln + e of the block, keys 4 lg + r of both halves)
 #pragma unroll
             for (int blk = 0; blk < NBLK; blk++) {
-                const uint8_t * vl = my + C::ROWS + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
+                const uint8_t * vl = vt + 4 * lg * C::LS + QBLOCK * blk + 2 + 2 * ln;
                 uint32_t av[2][4];
                 uint2 dv[2];
 #pragma unroll
@@ -569,7 +607,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                             }
 #pragma unroll
                         for (int blk = 0; blk < NBLK; blk++) {
-                            const uint8_t * vb = my + C::ROWS + k * C::LS + QBLOCK * blk;
+                            const uint8_t * vb = vt + k * C::LS + QBLOCK * blk;
                             const uint16_t d = *(const uint16_t *) vb;
                             if ((d & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
 #pragma unroll
@@ -581,8 +619,12 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                         }
                     }
             }
-            pa_wait_lds();
-            send(at_v, v_k);
+            if constexpr (NS == 1) {
+                pa_wait_lds();
+                send(at_v, v_k);
+            } else {
+                stage = 2 * C::ROWS - stage;
+            }
             live = live_next;
         }
         pa_wait<0>();
@@ -639,7 +681,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(g, (run.pos + tiles - 1) / run.per);
         run.left -= nt;
         run.pos += nt;
-        run.off = 0;
+        run.off = -PA_LEAD;
         if (run.left > 0)
             do run.n = clip_len(a, a.n_kv[++run.b]);
             while (run.n == 0);
@@ -750,7 +792,7 @@ pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_se
     const int64_t R = T * (nh / nh_kv);
     p.RT = R > 16 ? 2 : 1;
     p.groups = (int32_t) ((R + 16 * p.RT - 1) / (16 * p.RT));
-    const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE) + PA_MIN_TILES - 1) / PA_MIN_TILES;
+    const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
     p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(PA_CUS * (3 - p.RT) / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
     p.off_o = round256((size_t) n_seq * sizeof(int2));
@@ -779,7 +821,7 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
     if (nh_kv > 128) return err(QWFN_ENOTSUP, ": at most 128 KV heads");
     if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff - 2 * PA_TILE * PA_WAVES)
         return err(QWFN_EINVAL, ": page_size and max_pages must be positive, their product below 2^31 - 256");
-    if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1) > 0x7ffff000)
+    if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1 + PA_LEAD) > 0x7ffff000)
         return err(QWFN_ENOTSUP, ": at most 65536 requests and 2^31 tiles of 32 keys");
     if (B * nh * T * (D / 64) > 0x7ffff000) return err(QWFN_ENOTSUP, ": too many query rows");
     if (k->ne[1] < page_size) return err(QWFN_EINVAL, ": the pool holds no whole page");
