@@ -125,6 +125,16 @@ template <int UB> __device__ __forceinline__ void pa_dma(uint64_t from, uint32_t
     else
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(from), "s"(at) : "memory");
 }
+// The same from `from` + delta (delta the same for all lanes); the sum stands in m0's wait state.
+template <int UB> __device__ __forceinline__ void pa_dma_plus(uint64_t from, uint64_t delta, uint32_t at) {
+    uint64_t sum;
+    if constexpr (UB == 16)
+        asm volatile("s_mov_b32 m0, %3\n\tv_lshl_add_u64 %0, %1, 0, %2\n\tglobal_load_lds_dwordx4 %0, off"
+                     : "=&v"(sum) : "v"(from), "s"(delta), "s"(at) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %3\n\tv_lshl_add_u64 %0, %1, 0, %2\n\tglobal_load_lds_dword %0, off"
+                     : "=&v"(sum) : "v"(from), "s"(delta), "s"(at) : "memory");
+}
 // Waits until at most N vector-memory operations are in flight, or for this wave's LDS operations.
 template <int N> __device__ __forceinline__ void pa_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void pa_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -165,16 +175,67 @@ __device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[
     store4(a.dst + elem * es, a.type, x);
 }
 
-// The f16 pair of x = p d for the keys of a pair (d packed): hi toward zero, lo = p d - hi from one
-// fused step each.
-__device__ __forceinline__ void hilo(float p0, float p1, uint32_t d, uint32_t & hi, uint32_t & lo) {
-    const float x0 = mul_f16lo(p0, d), x1 = mul_f16hi(p1, d);
-    asm("v_cvt_pkrtz_f16_f32 %0, %4, %5\n\t"
-        "v_fma_mixlo_f16 %1, %2, %6, -%0 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
-        "v_fma_mixhi_f16 %1, %3, %6, -%0 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+// B operands of a V block: x = p d of the lane's 8 keys (p[u], d[u] packed) as f16 pairs, hi toward zero, lo = p d - hi from
+// one fused step each. One asm: a single pair of wait states before the MFMA (fattn_device.h) for all of it.
+__device__ __forceinline__ void hilo(const float (&p)[2][4], const uint2 (&d)[2], v4u & hi, v4u & lo) {
+    uint32_t h0, h1, h2, h3, l0, l1, l2, l3;
+    float x, y;
+#define QWFN_HILO(H, L, P0, P1, DV)                                                        \
+    "v_fma_mix_f32 %8, " P0 ", " DV ", 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"             \
+    "v_fma_mix_f32 %9, " P1 ", " DV ", 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"             \
+    "v_cvt_pkrtz_f16_f32 " H ", %8, %9\n\t"                                               \
+    "v_fma_mixlo_f16 " L ", " P0 ", " DV ", -" H " op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"   \
+    "v_fma_mixhi_f16 " L ", " P1 ", " DV ", -" H " op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+    asm(QWFN_HILO("%0", "%4", "%10", "%11", "%18") QWFN_HILO("%1", "%5", "%12", "%13", "%19")
+        QWFN_HILO("%2", "%6", "%14", "%15", "%20") QWFN_HILO("%3", "%7", "%16", "%17", "%21")
         "s_nop 1"
-        : "=&v"(hi), "=&v"(lo) : "v"(p0), "v"(p1), "v"(x0), "v"(x1), "v"(d));
+        : "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "=&v"(x), "=&v"(y)
+        : "v"(p[0][0]), "v"(p[0][1]), "v"(p[0][2]), "v"(p[0][3]), "v"(p[1][0]), "v"(p[1][1]), "v"(p[1][2]), "v"(p[1][3]),
+          "v"(d[0].x), "v"(d[0].y), "v"(d[1].x), "v"(d[1].y));
+#undef QWFN_HILO
+    hi = v4u{h0, h1, h2, h3};
+    lo = v4u{l0, l1, l2, l3};
 }
+// A operands: dims 2m (a0) and 2m + 1 (a1) of 8 keys from the bytes of v, int8 to f16 (exact).
+__device__ __forceinline__ void cvt_v8(const uint32_t (&v)[2][4], v4u & a0, v4u & a1) {
+    uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+#define QWFN_SDWA(D, S, DSEL, UNUSED, SSEL) "v_cvt_f16_i16_sdwa " D ", sext(" S ") dst_sel:" DSEL " dst_unused:" UNUSED " src0_sel:" SSEL "\n\t"
+#define QWFN_LOW(D, S, B) QWFN_SDWA(D, S, "WORD_0", "UNUSED_PAD", B)
+#define QWFN_HIGH(D, S, B) QWFN_SDWA(D, S, "WORD_1", "UNUSED_PRESERVE", B)
+    asm(QWFN_LOW("%0", "%8", "BYTE_0") QWFN_LOW("%1", "%10", "BYTE_0") QWFN_LOW("%2", "%12", "BYTE_0") QWFN_LOW("%3", "%14", "BYTE_0")
+        QWFN_HIGH("%0", "%9", "BYTE_0") QWFN_HIGH("%1", "%11", "BYTE_0") QWFN_HIGH("%2", "%13", "BYTE_0") QWFN_HIGH("%3", "%15", "BYTE_0")
+        QWFN_LOW("%4", "%8", "BYTE_1") QWFN_LOW("%5", "%10", "BYTE_1") QWFN_LOW("%6", "%12", "BYTE_1") QWFN_LOW("%7", "%14", "BYTE_1")
+        QWFN_HIGH("%4", "%9", "BYTE_1") QWFN_HIGH("%5", "%11", "BYTE_1") QWFN_HIGH("%6", "%13", "BYTE_1") QWFN_HIGH("%7", "%15", "BYTE_1")
+        "s_nop 1"
+        : "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3), "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3)
+        : "v"(v[0][0]), "v"(v[0][1]), "v"(v[0][2]), "v"(v[0][3]), "v"(v[1][0]), "v"(v[1][1]), "v"(v[1][2]), "v"(v[1][3]));
+#undef QWFN_LOW
+#undef QWFN_HIGH
+#undef QWFN_SDWA
+    a0 = v4u{x0, x1, x2, x3};
+    a1 = v4u{y0, y1, y2, y3};
+}
+
+// Largest over lanes l and l ^ 32, l and l ^ 16, a row of 16, without LDS.
+__device__ __forceinline__ uint32_t umax_halves(uint32_t x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    unsigned p = r[0], q = r[1];
+    asm volatile("" : "+v"(p), "+v"(q));
+    return max(p, q);
+}
+__device__ __forceinline__ uint32_t umax_rows(uint32_t x) {           // lanes l and l ^ 16
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    unsigned p = r[0], q = r[1];
+    asm volatile("" : "+v"(p), "+v"(q));
+    return max(p, q);
+}
+__device__ __forceinline__ uint32_t umax_row(uint32_t x) {            // the 16 lanes of a row
+    x = max(x, dev::dpp_u32<dev::DPP_QUAD_1032>(x));
+    x = max(x, dev::dpp_u32<dev::DPP_QUAD_2301>(x));
+    x = max(x, dev::dpp_u32<dev::DPP_HALF_MIRROR>(x));
+    return max(x, dev::dpp_u32<0x140>(x));                            // row_mirror
+}
+
 // A block's run of the tiles of all requests: the request it starts in and its length, the tile there, the
 // tiles left, its place, how many tiles a run has. A request counts PA_LEAD tiles more than it has, in front of
 // its own (off starts at -PA_LEAD): what its queries and its output cost the workgroup that begins it. 48 ragged
@@ -332,14 +393,23 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             if (lane < PA_TILE) addr[lane] = (uint64_t) (uintptr_t) kh + (uint64_t) slot * a.nb1;
             return (uint32_t) __ballot(ok);
         };
-        auto send = [&](uint32_t at, uint64_t delta) {
+        // a lane's units of the tile's rows: K's addresses, V's are v_k further
+        uint64_t from[ND];
+        auto units = [&](auto fn) {
 #pragma unroll
             for (int i = 0; i < ND; i++) {
-                const int x = lane + 64 * i, key = (x * C::UMUL) >> 16, u = x - key * C::UPR;
-                if (64 * (i + 1) <= C::UNITS || x < C::UNITS)
-                    pa_dma<C::UB>(addr[key] + delta + (uint64_t) (uint32_t) ((u < C::UV ? u : C::UV - 1) * C::UB), at + 64 * C::UB * i);
+                const int x = lane + 64 * i;
+                if (64 * (i + 1) <= C::UNITS || x < C::UNITS) fn(i, x);
             }
         };
+        auto send_k = [&](uint32_t at) {
+            units([&](int i, int x) {
+                const int key = (x * C::UMUL) >> 16, u = x - key * C::UPR;
+                from[i] = addr[key] + (uint64_t) (uint32_t) ((u < C::UV ? u : C::UV - 1) * C::UB);
+            });
+            units([&](int i, int) { pa_dma<C::UB>(from[i], at + 64 * C::UB * i); });
+        };
+        auto send_v = [&](uint32_t at) { units([&](int i, int) { pa_dma_plus<C::UB>(from[i], v_k, at + 64 * C::UB * i); }); };
         __syncthreads();                                   // the LDS of the part before is read
         // query values on their way: 8 lanes a q8_0 block
         float qx[RT][C::QI][4];
@@ -371,12 +441,12 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         if (wave < nt) {
             wave_lds_sync();
             if constexpr (NS == 1) {
-                send(at_k, 0);
+                send_k(at_k);
                 entries(wave + PA_WAVES);
             } else {
                 entries(wave + PA_WAVES);
-                send(at_k, 0);
-                send(at_v, v_k);
+                send_k(at_k);
+                send_v(at_v);
             }
         }
         // the query image: rows requantised, each block at its place of a window that is zero elsewhere
@@ -428,7 +498,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         }
         if (NS == 1 && wave < nt) {
             pa_wait_lds();
-            send(at_v, v_k);
+            send_v(at_v);
         }
         // in flight at the top, in this order: with one stage K of the tile, the entries of the next, V of the tile;
         // with two the entries of the next tile, K and V of this one
@@ -446,8 +516,8 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                 wave_lds_sync();
                 pa_wait_lds();
                 entries(t + 2 * PA_WAVES);
-                send(at_k + (2 * C::ROWS - stage), 0);
-                send(at_v + (2 * C::ROWS - stage), v_k);
+                send_k(at_k + (2 * C::ROWS - stage));
+                send_v(at_v + (2 * C::ROWS - stage));
                 pa_wait<3 * ND + 1>();
             }
             const uint8_t * const kt = my + stage, * const vt = kt + C::ROWS;
@@ -488,7 +558,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                 live_next = rows_of(t + PA_WAVES);
                 wave_lds_sync();
                 pa_wait_lds();
-                send(at_k, 0);
+                send_k(at_k);
                 entries(t + 2 * PA_WAVES);
             }
             // V's scales; its largest of each key and of the tile. One that is not finite counts as 0 here and in
@@ -508,10 +578,10 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                     dmax = max(dmax, fine ? mag : 0u);
                     odd |= on && mag >= 0x7c00u;
                 }
-                dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, 32));
+                dmax = umax_halves(dmax);
                 if (half == 0) vtop[key] = (uint16_t) dmax;
             }
-            for (int o = 1; o < 32; o <<= 1) dmax = max(dmax, (uint32_t) __shfl_xor((int) dmax, o));
+            dmax = umax_rows(umax_row(dmax));
             wave_lds_sync();
             float p[RT][2][4];
 #pragma unroll
@@ -527,8 +597,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                             if (!(live >> k & 1) || key0 + k >= limit[rt]) s[rt][u][r] = -INFINITY;
                             else top_d = max(top_d, (uint32_t) vtop[k]);
                         }
-                    top_d = max(top_d, (uint32_t) __shfl_xor((int) top_d, 16));
-                    top_d = max(top_d, (uint32_t) __shfl_xor((int) top_d, 32));
+                    top_d = umax_halves(umax_rows(top_d));
                 }
                 float top = vmax(vmax(s[rt][0][0], s[rt][0][1]), vmax(s[rt][0][2], s[rt][0][3]));
                 top = vmax(top, vmax(vmax(s[rt][1][0], s[rt][1][1]), vmax(s[rt][1][2], s[rt][1][3])));
@@ -565,25 +634,12 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                     dv[u] = *(const uint2 *) (vscl + blk * PA_TILE + 16 * u + 4 * lg);
                 }
                 v4u a0, a1;
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    uint32_t x0[2], x1[2];
-                    cvt_v_block(av[u], x0, x1);
-                    a0[2 * u] = x0[0]; a0[2 * u + 1] = x0[1];
-                    a1[2 * u] = x1[0]; a1[2 * u + 1] = x1[1];
-                }
+                cvt_v8(av, a0, a1);
                 const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     v4u bh, bl;
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        uint32_t h0, h1, l0, l1;
-                        hilo(p[rt][u][0], p[rt][u][1], dv[u].x, h0, l0);
-                        hilo(p[rt][u][2], p[rt][u][3], dv[u].y, h1, l1);
-                        bh[2 * u] = h0; bh[2 * u + 1] = h1;
-                        bl[2 * u] = l0; bl[2 * u + 1] = l1;
-                    }
+                    hilo(p[rt], dv, bh, bl);
                     const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
                     O[rt][blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[rt][blk][0], 0, 0, 0);
                     O[rt][blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[rt][blk][1], 0, 0, 0);
@@ -621,7 +677,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             }
             if constexpr (NS == 1) {
                 pa_wait_lds();
-                send(at_v, v_k);
+                send_v(at_v);
             } else {
                 stage = 2 * C::ROWS - stage;
             }
