@@ -175,8 +175,9 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // scores times v by plain sums over j <= i.
 //
 // A long sequence is cut into parts that run at once: k_linear_chunks<.., true> leaves
-// each part's own contribution U to the state and its decay in the workspace, and the
-// second launch starts a part from S0 and the U of the parts before it.
+// each part's own contribution U to the state and its decay in the workspace,
+// k_linear_join makes the state before each part of them, and the third launch runs
+// the parts from there.
 typedef __bf16   v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
@@ -207,7 +208,9 @@ template <int NT, int DK, int NW> struct lc_cfg {
     static constexpr int QK = C * DK * 2, T = DK * C * 2, V = COLS * C * 2, P = C * C * 2;   // bytes of a term
     static constexpr int OQ = 0, OK = OQ + NT * QK, OKT = OK + NT * QK, OV = OKT + NT * T, OP = OV + NT * V,
                          LDS = OP + NT * P;
-    static constexpr int WAVES_EU = NT == 1 && DK <= 128 && NW == 4 ? 2 : 1;
+    // workgroups of a CU: by LDS, and 8 waves (two a SIMD, 256 registers each)
+    static constexpr int PER_CU = 160 * 1024 / (LDS + 1280) < 8 / NW ? 160 * 1024 / (LDS + 1280) : 8 / NW;
+    static constexpr int WAVES_EU = (PER_CU * NW + 3) / 4;
     static_assert((KN % THREADS == 0 || KU == 1) && VN % THREADS == 0, "whole units a thread, or one for some");
     static_assert(LDS + 2048 <= 160 * 1024, "LDS of a CU");
 };
@@ -306,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     __shared__ int32_t sh[12];
     __shared__ int32_t odd_v[2];               // a chunk, by parity, holds a non-finite v
     const la_args & a = x.a;
-    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // consecutive blocks (the heads of a key head) on one XCD
     int blk = blockIdx.x;
@@ -322,28 +325,45 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     // the next chunk on its way: unit i of the thread: 8 values from 8 eu of tokens 2 ta and 2 ta + 1
     v4w rq[F::KU][2][F::LPU], rk[F::KU][2][F::LPU], rv[F::VU][2][F::LPU];
     float rg = 0.f;
-    auto load_unit = [&](v4w (&r)[2][F::LPU], const char * base, int64_t nb2, int t, int e8, int d) {
+    const char * pq[F::KU], * pk[F::KU], * pv[F::VU];      // the units' places in the first chunk
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+    for (int i = 0; i < F::KU; i++) {
+        const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8));
+        const int64_t t = part.t0 + 2 * (u / (DK / 8));
+        pq[i] = qh + t * a.q_nb2 + e8 * F::ES;
+        pk[i] = kh + t * a.k_nb2 + e8 * F::ES;
+    }
 #pragma unroll
-            for (int j = 0; j < F::LPU; j++) {
-                const int tt = t + i < part.len ? t + i : part.len - 1, e = e8 + j * (8 / F::LPU);
-                r[i][j] = v4w{0, 0, 0, 0};
-                if (e < d) r[i][j] = *(const v4w *) (base + (int64_t) (part.t0 + tt) * nb2 + e * F::ES);
+    for (int i = 0; i < F::VU; i++) {
+        const int u = tid + F::THREADS * i;
+        pv[i] = vh + (int64_t) (part.t0 + 2 * (u / (F::COLS / 8))) * a.v_nb2 + (c0 + 8 * (u % (F::COLS / 8))) * F::ES;
+    }
+    // token t of the unit and the one behind it; past the part the last token is read (and not used)
+    auto load_unit = [&](v4w (&r)[2][F::LPU], const char * p, int64_t nb2, int t, int e8, int d) {
+        const int64_t back = t < part.len ? 0 : (int64_t) (part.len - 1 - t) * nb2;
+        const char * p0 = p + back, * p1 = t + 1 < part.len ? p0 + nb2 : p0;
+#pragma unroll
+        for (int j = 0; j < F::LPU; j++) {
+            r[0][j] = r[1][j] = v4w{0, 0, 0, 0};
+            if (e8 + j * (8 / F::LPU) < d) {
+                r[0][j] = *(const v4w *) (p0 + 16 * j);
+                r[1][j] = *(const v4w *) (p1 + 16 * j);
             }
+        }
     };
     auto load = [&](int t0) {
+        const int64_t dq = t0 * a.q_nb2, dk = t0 * a.k_nb2, dv = t0 * a.v_nb2;
 #pragma unroll
         for (int i = 0; i < F::KU; i++) {
             const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = t0 + 2 * (u / (DK / 8));
             if (F::KN < F::THREADS && u >= F::KN) break;
-            if (!STATES) load_unit(rq[i], qh, a.q_nb2, t, e8, a.dk);
-            load_unit(rk[i], kh, a.k_nb2, t, e8, a.dk);
+            if (!STATES) load_unit(rq[i], pq[i] + dq, a.q_nb2, t, e8, a.dk);
+            load_unit(rk[i], pk[i] + dk, a.k_nb2, t, e8, a.dk);
         }
 #pragma unroll
         for (int i = 0; i < F::VU; i++) {
             const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), t = t0 + 2 * (u / (F::COLS / 8));
-            load_unit(rv[i], vh, a.v_nb2, t, c0 + e8, a.dv);
+            load_unit(rv[i], pv[i] + dv, a.v_nb2, t, c0 + e8, a.dv);
         }
         const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
         if (w == 0) rg = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
@@ -459,16 +479,9 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
     for (int t = 0; t < F::KT; t++) S[t][0] = S[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
     if (!STATES) {
-        if (part.slot >= 0 && a.s_in) {
-            const float * s0 = a.s_in + part.slot * per + h * hs;
-            each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
-        }
-        for (int p = 0; p < part.before; p++) {
-            const size_t at = (size_t) (part.index - part.before + p) * a.n_v + h;
-            const float f = __builtin_amdgcn_exp2f((float) x.G[at]);
-            const float * up = x.U + at * hs;
-            each([&](v4f & s, int r, size_t e) { s[r] = __fmaf_rn(s[r], f, up[e]); });
-        }
+        const float * s0 = part.before > 0 ? x.U + ((size_t) (part.index - 1) * a.n_v + h) * hs
+                           : part.slot >= 0 && a.s_in ? a.s_in + part.slot * per + h * hs : nullptr;
+        if (s0) each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
         // the scores of tokens behind a 32-token block's last one stay 0
         for (int i = tid; i < NT * F::P / 16; i += F::THREADS) *(v4w *) (lds + F::OP + 16 * i) = v4w{0, 0, 0, 0};
         if (tid < 2) odd_v[tid] = 0;
@@ -477,6 +490,8 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     __syncthreads();
 
     for (int t0 = 0; t0 < part.len; t0 += C) {
+        // the thread's places are computed anew in every chunk: kept over the loop they cost registers, spilled
+        asm volatile("" : "+v"(tid), "+v"(lane), "+v"(m), "+v"(g));
         stage(t0);
         __syncthreads();
         if (t0 + C < part.len) load(t0 + C);
@@ -485,34 +500,48 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         if constexpr (!STATES) {
             const bool odd = odd_v[t0 / C & 1] != 0;
             if (tid == 0) odd_v[~(t0 / C) & 1] = 0;            // read in the chunk before, written in the next
-            // the scores, a 16 x 16 tile of tokens (j rows, i columns) at a time
-            for (int n = w; n < F::IT * (F::IT + 1) / 2; n += NW) {
-                int it = 0, jt = n;
-                while (jt > it) jt -= ++it;
-                v4f p{0.f, 0.f, 0.f, 0.f};
+            // the scores, 16 x 16 tiles of tokens (j rows, i columns) with j <= i, PT a wave (the last tile by more than
+            // one wave where they do not come out even)
+            constexpr int TILES = F::IT * (F::IT + 1) / 2, PT = (TILES + NW - 1) / NW;
+            v4f p[PT];
+            int it[PT], jt[PT];
 #pragma unroll
-                for (int kb = 0; kb < F::KB; kb++) {
+            for (int x = 0; x < PT; x++) {
+                const int n = w + NW * x < TILES ? w + NW * x : TILES - 1;
+                it[x] = (n >= 1) + (n >= 3) + (n >= 6);
+                jt[x] = n - it[x] * (it[x] + 1) / 2;
+                p[x] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int kb = 0; kb < F::KB; kb++)
+#pragma unroll
+                for (int x = 0; x < PT; x++) {
                     v4w kx[NT], qx[NT];
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        kx[t] = *(const v4w *) (lds + F::OK + t * F::QK + lc_row<DK>(16 * jt + m, 4 * kb + g));
-                        qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * it + m, 4 * kb + g));
+                        kx[t] = *(const v4w *) (lds + F::OK + t * F::QK + lc_row<DK>(16 * jt[x] + m, 4 * kb + g));
+                        qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * it[x] + m, 4 * kb + g));
                     }
-                    p = mfma_terms<NT, NT, NT>(kx, qx, p);
+                    p[x] = mfma_terms<NT, NT, NT>(kx, qx, p[x]);
                 }
-                const int i = 16 * it + m;
+#pragma unroll
+            for (int x = 0; x < PT; x++) {
+                const int i = 16 * it[x] + m;
                 const double gi = G[i];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int j = 16 * jt + 4 * g + r;
-                    p[r] = j <= i ? p[r] * __builtin_amdgcn_exp2f((float) (gi - G[j])) : 0.f;
+                    const int j = 16 * jt[x] + 4 * g + r;
+                    p[x][r] = j <= i ? p[x][r] * __builtin_amdgcn_exp2f((float) (gi - G[j])) : 0.f;
                 }
+            }
+#pragma unroll
+            for (int x = 0; x < PT; x++) {
                 uint32_t lo[NT], hi[NT];
-                bf16_terms<NT>(p[0], p[1], lo);
-                bf16_terms<NT>(p[2], p[3], hi);
+                bf16_terms<NT>(p[x][0], p[x][1], lo);
+                bf16_terms<NT>(p[x][2], p[x][3], hi);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
-                    *(v2w *) (lds + F::OP + t * F::P + lc_col<C>(i, 2 * jt + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
+                    *(v2w *) (lds + F::OP + t * F::P + lc_col<C>(16 * it[x] + m, 2 * jt[x] + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
             }
             // S^T q
             v4f o[F::IT][2];
@@ -631,17 +660,28 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     }
                 }
             }
+            // (TG row tiles at a time: a sum's products are 2 TG MFMAs apart)
+            constexpr int TG = 4;
 #pragma unroll
-            for (int t = 0; t < F::KT; t++) {
-                S[t][0] *= cend;
-                S[t][1] *= cend;
+            for (int t0g = 0; t0g < F::KT; t0g += TG) {
+#pragma unroll
+                for (int t = t0g; t < t0g + TG; t++) { S[t][0] *= cend; S[t][1] *= cend; }
 #pragma unroll
                 for (int jb = 0; jb < F::JB; jb++) {
-                    v4w kx[NT];
+                    v4w kx[TG][NT];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) kx[n] = *(const v4w *) (lds + F::OKT + n * F::T + lc_col<C>(16 * t + m, 4 * jb + g));
-                    S[t][0] = mfma_terms<NT, 3, 3>(kx, vx[jb][0], S[t][0]);
-                    S[t][1] = mfma_terms<NT, 3, 3>(kx, vx[jb][1], S[t][1]);
+                    for (int t = 0; t < TG; t++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+                            kx[t][n] = *(const v4w *) (lds + F::OKT + n * F::T + lc_col<C>(16 * (t0g + t) + m, 4 * jb + g));
+#pragma unroll
+                    for (int d = 2; d >= 0; d--)
+#pragma unroll
+                        for (int n = 0; n < NT && n <= d; n++)
+#pragma unroll
+                            for (int t = 0; t < TG; t++)
+#pragma unroll
+                                for (int u = 0; u < 2; u++) S[t0g + t][u] = mfma_bf16(kx[t][n], vx[jb][u][d - n], S[t0g + t][u]);
                 }
             }
         }
@@ -655,6 +695,42 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     } else if (part.after == 0 && part.slot >= 0) {
         float * so = a.s_out + part.slot * per + h * hs;
         each([&](v4f & s, int r, size_t e) { so[e] = s[r]; });
+    }
+}
+
+// The states behind the parts of a sequence (but the last), in the place of their U: S = 2^G_p S + U_p. A thread per 4
+// elements of a head's state; the parts' values are loaded LJ_AHEAD at a time.
+constexpr int LJ_AHEAD = 4;
+
+__global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
+    __shared__ int32_t sh[12];
+    const la_args & a = x.a;
+    const int64_t hs = (int64_t) a.dk * a.dv, per = hs * a.n_v;
+    const int blocks = (int) ((hs / 4 + LA_THREADS - 1) / LA_THREADS);
+    const int eb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.n_v;
+    const lc_part part = find_part(x, blockIdx.x / blocks / a.n_v, false, LA_THREADS, sh);
+    if (part.b < 0 || part.before > 0 || part.after == 0) return;
+    const int64_t e = 4 * ((int64_t) eb * LA_THREADS + threadIdx.x);
+    if (e >= hs) return;
+    v4f s{0.f, 0.f, 0.f, 0.f};
+    if (part.slot >= 0 && a.s_in) s = *(const v4f *) (a.s_in + part.slot * per + h * hs + e);
+    float * up = x.U + ((int64_t) part.index * a.n_v + h) * hs + e;
+    const double * gp = x.G + (int64_t) part.index * a.n_v + h;
+    for (int p0 = 0; p0 < part.after; p0 += LJ_AHEAD) {
+        v4f u[LJ_AHEAD];
+        float f[LJ_AHEAD];
+#pragma unroll
+        for (int i = 0; i < LJ_AHEAD; i++) {
+            const int p = p0 + i < part.after ? p0 + i : part.after - 1;
+            u[i] = *(const v4f *) (up + p * per);
+            f[i] = __builtin_amdgcn_exp2f((float) gp[(int64_t) p * a.n_v]);
+        }
+#pragma unroll
+        for (int i = 0; i < LJ_AHEAD; i++) {
+            if (p0 + i >= part.after) break;
+            s = s * f[i] + u[i];
+            *(v4f *) (up + (p0 + i) * per) = s;
+        }
     }
 }
 
@@ -697,9 +773,17 @@ struct lc_plan {
     size_t  off_g, bytes;
 };
 
-// Parts of a sequence: as many as fill the CUs once, but no shorter than LC_MIN_PART tokens (a part costs its
-// state's way through the workspace and a second pass over its k and v).
-constexpr int64_t LC_TARGET = 256, LC_MIN_PART = 256;
+template <int NT> int per_cu(int DK, int NW) {
+    if (DK == 64) return NW == 2 ? lc_cfg<NT, 64, 2>::PER_CU : lc_cfg<NT, 64, 4>::PER_CU;
+    if (DK == 128) return NW == 2 ? lc_cfg<NT, 128, 2>::PER_CU : lc_cfg<NT, 128, 4>::PER_CU;
+    if constexpr (NT < 3) return NW == 2 ? lc_cfg<NT, 256, 2>::PER_CU : lc_cfg<NT, 256, 4>::PER_CU;
+    return 1;
+}
+
+// Parts of a sequence: as many as fill the CUs once, so that no workgroup waits for another (4096 tokens of 48 heads
+// in 6 parts, 288 workgroups: 189 us where 5 parts take 100), but no shorter than LC_MIN_PART tokens: a part costs its
+// state's way through the workspace and a second pass over its k and v.
+constexpr int64_t LC_CUS = 256, LC_MIN_PART = 256;
 
 lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
     lc_plan p{};
@@ -712,8 +796,11 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     p.NW = dv <= 2 * LC_WCOLS ? 2 : 4;
     p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
     const int64_t longest = std::min<int64_t>(max_len, n_tok), C = p.NT == 1 ? 64 : 32;
-    int64_t L = std::max<int64_t>(LC_MIN_PART, (n_tok * n_v * p.ct + LC_TARGET - 1) / LC_TARGET);
-    L = (L + C - 1) / C * C;
+    const int64_t room = LC_CUS * (p.NT == 1 ? per_cu<1>(p.DK, p.NW) : p.NT == 2 ? per_cu<2>(p.DK, p.NW) : per_cu<3>(p.DK, p.NW)) /
+                         (n_v * p.ct);
+    // a sequence's last part is half of one on average
+    const int64_t whole = std::max<int64_t>(1, room - n_seq / 2);
+    const int64_t L = (std::max<int64_t>(LC_MIN_PART, (n_tok + whole - 1) / whole) + C - 1) / C * C;
     p.parts = n_seq;
     if (L < longest) {
         p.L = (int32_t) L;
@@ -729,6 +816,9 @@ int launch_chunks(const lc_args & x, const lc_plan & p, hipStream_t s) {
     const dim3 grid((unsigned) (p.parts * x.a.n_v * p.ct)), blk(64 * NW);
     if (p.L > 0) {
         hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, true>), grid, blk, 0, s, x);
+        if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
+        const int64_t blocks = ((int64_t) x.a.dk * x.a.dv / 4 + LA_THREADS - 1) / LA_THREADS;
+        hipLaunchKernelGGL(k_linear_join, dim3((unsigned) (p.parts * x.a.n_v * blocks)), dim3(LA_THREADS), 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
     }
     hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, false>), grid, blk, 0, s, x);
@@ -790,7 +880,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         a.type = q->type; a.n_seq = n_seq; a.max_len = max_len; a.n_slots = n_slots; a.n_tok = (int32_t) n_tok;
         a.n_k = (int32_t) q->ne[1]; a.n_v = (int32_t) n_v; a.rep = a.n_v / a.n_k; a.dk = (int32_t) dk; a.dv = (int32_t) dv;
         if (!pl.step) {
-            if (pl.parts * n_v * pl.ct > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
+            if (pl.parts * n_v * std::max<int64_t>(pl.ct, dk * dv / (4 * LA_THREADS) + 1) > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
             a.ct = pl.ct;
             const lc_args x{a, pl.L, (float *) ws, (double *) ((char *) ws + pl.off_g)};
             return pl.NT == 1 ? launch_type<1>(x, pl, as_stream(stream)) : pl.NT == 2 ? launch_type<2>(x, pl, as_stream(stream))
