@@ -465,16 +465,22 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
     for (int u = 0; u < 2; u++) col[u] = c0 + LC_WCOLS * w + 8 * (m >> 2) + 4 * u + (m & 3);
     const bool live = c0 + LC_WCOLS * w < a.dv;            // the wave has columns
-    auto each = [&](auto fn) {                             // fn(value, element of a head's state)
+    const bool whole = a.dk == DK && c0 + LC_WCOLS * (w + 1) <= a.dv;      // no row or column past the head's
+    auto each = [&](auto fn) {                             // fn(value, its element, element of a head's state)
+        auto all = [&](auto inside) {
 #pragma unroll
-        for (int t = 0; t < F::KT; t++)
+            for (int t = 0; t < F::KT; t++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = 16 * t + 4 * g + r;
-                    if (row < a.dk && col[u] < a.dv) fn(S[t][u], r, (size_t) row * a.dv + col[u]);
-                }
+                    for (int r = 0; r < 4; r++) {
+                        const int row = 16 * t + 4 * g + r;
+                        if (inside(row, col[u])) fn(S[t][u], r, (size_t) row * a.dv + col[u]);
+                    }
+        };
+        // (without a condition the loads are all in flight at once)
+        if (whole) all([](int, int) { return true; });
+        else       all([&](int row, int c) { return row < a.dk && c < a.dv; });
     };
 #pragma unroll
     for (int t = 0; t < F::KT; t++) S[t][0] = S[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
