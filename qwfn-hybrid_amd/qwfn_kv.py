@@ -342,6 +342,34 @@ def _stream(stream) -> int | None:
     return int(stream) if not hasattr(stream, "cuda_stream") else stream.cuda_stream
 
 
+_NE, _NB = ctypes.c_int64 * 4, ctypes.c_size_t * 4
+
+
+def _tensor4(ptr: int, typ: int, ne, nb) -> Tensor:
+    """tensor() of four sizes and strides that are ints already (a call of it is a good part of a small op's host time)."""
+    return Tensor(ptr, typ, 0, _NE(*ne), _NB(*nb))
+
+
+class _Torch:
+    """torch, what the wrappers ask of it at every call, and its types by code; filled at the first use."""
+    mod = None
+
+    def __new__(cls):
+        if cls.mod is None:
+            import torch
+            cls.int32, cls.float32 = torch.int32, torch.float32
+            cls.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+            cls.device, cls.mod = staticmethod(torch.cuda.current_device), torch
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            cls.stream = staticmethod(raw or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+        return cls
+
+
+def _stream_on(stream, dev: int) -> int | None:
+    """The current stream of device `dev` (the current one), or the given stream."""
+    return _Torch.stream(dev) if stream is None else _stream(stream)
+
+
 # --------------------------------------------------------------------- views
 
 def row_bytes(kv_dim: int) -> int:
@@ -374,11 +402,10 @@ def f32_view(t) -> Tensor:
 
 def float_type(t) -> int:
     """TYPE_F32, TYPE_F16 or TYPE_BF16 of a torch tensor."""
-    import torch
-    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-    if t.dtype not in types:
+    typ = _Torch().types.get(t.dtype)
+    if typ is None:
         raise ValueError(f"a float32, float16 or bfloat16 tensor is needed, got {t.dtype}")
-    return types[t.dtype]
+    return typ
 
 
 def q_view(q) -> Tensor:
@@ -388,7 +415,7 @@ def q_view(q) -> Tensor:
         q = q.unsqueeze(0)
     B, T, nh, hd = q.shape
     s, e = q.stride(), q.element_size()
-    return tensor(q.data_ptr(), float_type(q), (hd, T, nh, B), (s[3] * e, s[1] * e, s[2] * e, s[0] * e))
+    return _tensor4(q.data_ptr(), float_type(q), (hd, T, nh, B), (s[3] * e, s[1] * e, s[2] * e, s[0] * e))
 
 
 def mask_view(mask) -> Tensor:
@@ -406,14 +433,14 @@ def out_view(out) -> Tensor:
         out = out.unsqueeze(0)
     B, T, nh, hd = out.shape
     e = out.element_size()
-    return tensor(out.data_ptr(), float_type(out), (hd, nh, T, B), (e, hd * e, hd * nh * e, hd * nh * T * e))
+    return _tensor4(out.data_ptr(), float_type(out), (hd, nh, T, B), (e, hd * e, hd * nh * e, hd * nh * T * e))
 
 
 def heads_view(x) -> Tensor:
     """Packed tokens torch [n_tok, n_heads, d] (contiguous rows) = ggml [d, n_heads, n_tok]."""
     n, h, d = x.shape
     s, e = x.stride(), x.element_size()
-    return tensor(x.data_ptr(), float_type(x), (d, h, n, 1), (s[2] * e, s[1] * e, s[0] * e, max(1, n) * s[0] * e))
+    return _tensor4(x.data_ptr(), float_type(x), (d, h, n, 1), (s[2] * e, s[1] * e, s[0] * e, (n or 1) * s[0] * e))
 
 
 # --------------------------------------------------------------------- ops
@@ -748,25 +775,22 @@ def gated_delta_net(q, k, v, g, beta, state, out, n_k: int, snap=None, n_snap: i
 
 # --------------------------------------------------------------------- paged cache
 
-def _dev_i32(op, **tensors):
-    """Device int32 tensors, contiguous (a table: contiguous rows), all on one GPU."""
-    where = None
-    for name, t in tensors.items():
+def _check_i32(op, dev, vectors, table=None, rows=0):
+    """Contiguous int32 vectors {name: (tensor or None, least length)} on the current device, and a [rows, max_pages] table
+    with contiguous rows."""
+    i32 = _Torch.int32
+    for name, (t, n) in vectors.items():
         if t is None:
             continue
-        if str(t.dtype) != "torch.int32" or not t.is_cuda:
-            raise ValueError(f"{op}: {name} must be a device int32 tensor")
-        if (t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1) or (t.dim() < 2 and not t.is_contiguous()):
-            raise ValueError(f"{op}: {name} must have contiguous rows")
-        if where is not None and t.device != where:
-            raise ValueError(f"{op}: {name} must be on {where}")
-        where = t.device
-
-
-def _lengths(op, n, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (t.dim() != 1 or t.shape[0] < n):
-            raise ValueError(f"{op}: {name} must be [{n}]")
+        if t.dtype is not i32 or t.get_device() != dev:
+            raise ValueError(f"{op}: {name} must be an int32 tensor on the current device ({dev})")
+        if t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous [{n}]")
+    if table is not None:
+        if table.dtype is not i32 or table.get_device() != dev:
+            raise ValueError(f"{op}: table must be an int32 tensor on the current device ({dev})")
+        if table.dim() != 2 or table.size(0) < rows or (table.stride(1) != 1 and table.size(1) > 1):
+            raise ValueError(f"{op}: table must be [{rows}, max_pages] with contiguous rows")
 
 
 def _ws(ws):
@@ -782,35 +806,29 @@ def paged_extend(n_past, n_new, page_size: int, table, free_pages, n_free, n_fre
     """Pages and cache rows for n_new[b] more tokens of each request: device int32 n_past, n_new, n_kv [n_seq] (n_kv may
     be n_past), table [n_seq, max_pages], free_pages [free_cap], n_free, n_free_out [1] (may be one tensor), cu_new
     [n_seq + 1], slots, pos, seq [n_tok]."""
-    n_seq = n_past.shape[0]
-    _dev_i32("paged_extend", n_past=n_past, n_new=n_new, table=table, free_pages=free_pages, n_free=n_free,
-             n_free_out=n_free_out, n_kv=n_kv, cu_new=cu_new, slots=slots, pos=pos, seq=seq)
-    if table.dim() != 2 or table.shape[0] < n_seq:
-        raise ValueError(f"paged_extend: table must be [{n_seq}, max_pages]")
-    _lengths("paged_extend", n_seq, n_new=n_new, n_kv=n_kv)
-    _lengths("paged_extend", n_seq + 1, cu_new=cu_new)
-    _lengths("paged_extend", slots.shape[0], pos=pos, seq=seq)
-    _lengths("paged_extend", 1, n_free=n_free, n_free_out=n_free_out)
-    p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    return check(load().qwfn_paged_extend(p(n_past), p(n_new), n_seq, page_size, p(table), table.stride(0), table.shape[1],
-                                          p(free_pages), free_pages.shape[0], p(n_free), p(n_free_out), p(n_kv), p(cu_new),
-                                          p(slots), p(pos), p(seq), slots.shape[0], pad_slot, *_ws(ws), _stream(stream)))
+    n_seq, n_tok, dev = n_past.numel(), slots.numel(), _Torch().device()
+    _check_i32("paged_extend", dev, dict(
+        n_past=(n_past, n_seq), n_new=(n_new, n_seq), free_pages=(free_pages, 0), n_free=(n_free, 1),
+        n_free_out=(n_free_out, 1), n_kv=(n_kv, n_seq), cu_new=(cu_new, n_seq + 1), slots=(slots, n_tok), pos=(pos, n_tok),
+        seq=(seq, n_tok)), table, n_seq)
+    return check(load().qwfn_paged_extend(
+        n_past.data_ptr(), n_new.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1),
+        free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(), n_kv.data_ptr(),
+        cu_new.data_ptr(), slots.data_ptr(), pos.data_ptr() if pos is not None else None,
+        seq.data_ptr() if seq is not None else None, n_tok, pad_slot, *_ws(ws), _stream_on(stream, dev)))
 
 
 def paged_trim(n_keep, n_kv, page_size: int, table, free_pages, n_free, n_free_out, n_kv_out, ws=None, stream=None):
     """Request b keeps its first n_keep[b] of n_kv[b] tokens; the pages behind them go onto the free stack. Tensors as
     in paged_extend; n_kv_out may be n_kv, n_free_out n_free."""
-    n_seq = n_kv.shape[0]
-    _dev_i32("paged_trim", n_keep=n_keep, n_kv=n_kv, table=table, free_pages=free_pages, n_free=n_free,
-             n_free_out=n_free_out, n_kv_out=n_kv_out)
-    if table.dim() != 2 or table.shape[0] < n_seq:
-        raise ValueError(f"paged_trim: table must be [{n_seq}, max_pages]")
-    _lengths("paged_trim", n_seq, n_keep=n_keep, n_kv_out=n_kv_out)
-    _lengths("paged_trim", 1, n_free=n_free, n_free_out=n_free_out)
+    n_seq, dev = n_kv.numel(), _Torch().device()
+    _check_i32("paged_trim", dev, dict(
+        n_keep=(n_keep, n_seq), n_kv=(n_kv, n_seq), free_pages=(free_pages, 0), n_free=(n_free, 1),
+        n_free_out=(n_free_out, 1), n_kv_out=(n_kv_out, n_seq)), table, n_seq)
     return check(load().qwfn_paged_trim(n_keep.data_ptr(), n_kv.data_ptr(), n_seq, page_size, table.data_ptr(),
-                                        table.stride(0), table.shape[1], free_pages.data_ptr(), free_pages.shape[0],
+                                        table.stride(0), table.size(1), free_pages.data_ptr(), free_pages.numel(),
                                         n_free.data_ptr(), n_free_out.data_ptr(), n_kv_out.data_ptr(), *_ws(ws),
-                                        _stream(stream)))
+                                        _stream_on(stream, dev)))
 
 
 def fattn_workspace_size_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int) -> int:
@@ -823,16 +841,15 @@ def flash_attn_ext_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: i
     """Attention of each request's last T tokens over its pages: qv of torch [n_seq, T, n_head, hd] (q_view), kv and vv
     views of the pool's caches (cache_attn_view over all rows), table device int32 [n_seq, max_pages], n_kv device
     int32 [n_seq]; times sigmoid(gate) when gate (laid out as the output) is given."""
-    n_seq = qv.ne[3]
-    _dev_i32("flash_attn_ext_paged", table=table, n_kv=n_kv)
-    if table.dim() != 2 or table.shape[0] < n_seq:
-        raise ValueError(f"flash_attn_ext_paged: table must be [{n_seq}, max_pages]")
-    _lengths("flash_attn_ext_paged", n_seq, n_kv=n_kv)
+    n_seq, dev = qv.ne[3], _Torch().device()
+    _check_i32("flash_attn_ext_paged", dev, dict(n_kv=(n_kv, n_seq)), table, n_seq)
+    if gate is not None and not gate.is_contiguous():
+        raise ValueError("flash_attn_ext_paged: gate must be contiguous")
     gv = out_view(gate) if gate is not None else None
     return check(load().qwfn_flash_attn_ext_q8_0_paged(
-        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.shape[1], page_size,
+        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.size(1), page_size,
         n_kv.data_ptr(), scale, ctypes.byref(gv) if gv is not None else None, ctypes.byref(ov), variant, *_ws(ws),
-        _stream(stream)))
+        _stream_on(stream, dev)))
 
 
 # --------------------------------------------------------------------- linear attention
@@ -847,20 +864,23 @@ def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=No
     """Linear attention with a decay per head over packed sequences: q, k torch [n_tok, n_k, dk], v, out [n_tok, n_v, dv]
     (float32, float16 or bfloat16, one type); g float32 [n_tok, n_v], or [n_v] for constant decays; cu device int32
     [n_seq + 1]; state_in (or None), state_out float32 [n_slots, n_v, dk, dv]; slots device int32 [n_seq] or None."""
-    n_seq, n_tok, dk = cu.shape[0] - 1, q.shape[0], q.shape[2]
-    _dev_i32("linear_attn", cu=cu, slots=slots)
-    _lengths("linear_attn", n_seq, slots=slots)
-    want = (state_out.shape[0], v.shape[1], dk, v.shape[2])
+    n_seq, n_tok, dk, n_v, dv, dev = cu.numel() - 1, q.size(0), q.size(2), v.size(1), v.size(2), _Torch().device()
+    _check_i32("linear_attn", dev, dict(cu=(cu, n_seq + 1), slots=(slots, n_seq)))
+    f32 = _Torch.float32
     for name, t in (("state_in", state_in), ("state_out", state_out)):
-        if t is not None and (str(t.dtype) != "torch.float32" or tuple(t.shape) != want or not t.is_contiguous()):
-            raise ValueError(f"linear_attn: {name} must be contiguous float32 {list(want)}")
-    if str(g.dtype) != "torch.float32" or g.shape[-1] != v.shape[1] or (g.stride(-1) != 1 and g.shape[-1] > 1) \
-            or g.dim() not in (1, 2) or (g.dim() == 2 and g.shape[0] < n_tok):
-        raise ValueError("linear_attn: g must be float32 [n_tok, n_v] or [n_v]")
+        if t is not None and (t.dtype is not f32 or t.get_device() != dev or not t.is_contiguous() or
+                              t.shape != (state_out.size(0), n_v, dk, dv)):
+            raise ValueError(f"linear_attn: {name} must be contiguous float32 [n_slots, {n_v}, {dk}, {dv}] on the current device")
+    if g.dtype is not f32 or g.get_device() != dev or g.size(-1) != n_v or (g.stride(-1) != 1 and n_v > 1) \
+            or g.dim() not in (1, 2) or (g.dim() == 2 and g.size(0) < n_tok):
+        raise ValueError(f"linear_attn: g must be float32 [{n_tok}, {n_v}] or [{n_v}] on the current device")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        if t.get_device() != dev:
+            raise ValueError(f"linear_attn: {name} must be on the current device ({dev})")
     scale = dk ** -0.5 if scale is None else scale
-    qv, kv, vv, ov = (heads_view(x) for x in (q, k, v, out))
+    r = ctypes.byref
     return check(load().qwfn_linear_attn(
-        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0,
-        cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.shape[0],
-        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, ctypes.byref(ov), *_ws(ws),
-        _stream(stream)))
+        r(heads_view(q)), r(heads_view(k)), r(heads_view(v)), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0,
+        cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.size(0),
+        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, r(heads_view(out)), *_ws(ws),
+        _stream_on(stream, dev)))
