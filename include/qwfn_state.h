@@ -258,8 +258,8 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  * tensors (cu: device I32 [n_seq + 1], cu_new of qwfn_paged_extend), none to
  * max_len of them:
  *   q, k  F32, F16 or BF16 [dk, n_k_heads, n_tok]; v, dst [dv, n_v_heads, n_tok] of
- *         q's type; rows contiguous, any token and head strides that are multiples
- *         of 16 bytes; dst contiguous
+ *         q's type; rows contiguous, head and token strides multiples of 16 bytes,
+ *         the token's below 2^24; dst contiguous
  *   g     F32 log decays (at most 0 in use; -inf forgets everything), token t's at
  *         g + t * g_token_stride floats; a stride of 0 gives every token the same
  *         n_v_heads decays

@@ -179,6 +179,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // k_linear_join makes the state before each part of them, and the third launch runs
 // the parts from there.
 typedef __bf16   v8b __attribute__((ext_vector_type(8)));
+typedef __bf16   v2b __attribute__((ext_vector_type(2)));
 typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
@@ -221,7 +222,6 @@ template <int C> __device__ __forceinline__ int lc_col(int row, int unit) {
     return row * (C * 2) + ((unit ^ ((row ^ (row >> 3)) & (C / 8 - 1))) * 16);
 }
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
-    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, v2b{(__bf16) x, (__bf16) y});
 }
 // x and y as NT bf16 terms, packed by term
@@ -305,7 +305,8 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     constexpr int C = F::C;
     __shared__ __attribute__((aligned(16))) uint8_t lds[F::LDS];
     __shared__ double G[C];                    // log2 of the decay from the chunk's start
-    __shared__ float eG[C], wG[C];             // 2^G, 2^(G_end - G)
+    __shared__ float eG[C], wG[C];             // scale 2^G, 2^(G_end - G)
+    __shared__ float eEnd;                     // 2^G_end
     __shared__ int32_t sh[12];
     __shared__ int32_t odd_v[2];               // a chunk, by parity, holds a non-finite v
     const la_args & a = x.a;
@@ -325,51 +326,69 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     // the next chunk on its way: unit i of the thread: 8 values from 8 eu of tokens 2 ta and 2 ta + 1
     v4w rq[F::KU][2][F::LPU], rk[F::KU][2][F::LPU], rv[F::VU][2][F::LPU];
     float rg = 0.f;
-    const char * pq[F::KU], * pk[F::KU], * pv[F::VU];      // the units' places in the first chunk
+    // A unit's place behind the chunk's first token, 32 bits (the host checks the strides): a whole chunk's loads are a
+    // uniform base and an offset.
+    uint32_t oq[F::KU], ok[F::KU], ov[F::VU];
 #pragma unroll
     for (int i = 0; i < F::KU; i++) {
-        const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8));
-        const int64_t t = part.t0 + 2 * (u / (DK / 8));
-        pq[i] = qh + t * a.q_nb2 + e8 * F::ES;
-        pk[i] = kh + t * a.k_nb2 + e8 * F::ES;
+        const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = 2 * (u / (DK / 8));
+        oq[i] = (uint32_t) (t * a.q_nb2 + e8 * F::ES);
+        ok[i] = (uint32_t) (t * a.k_nb2 + e8 * F::ES);
     }
 #pragma unroll
     for (int i = 0; i < F::VU; i++) {
         const int u = tid + F::THREADS * i;
-        pv[i] = vh + (int64_t) (part.t0 + 2 * (u / (F::COLS / 8))) * a.v_nb2 + (c0 + 8 * (u % (F::COLS / 8))) * F::ES;
+        ov[i] = (uint32_t) (2 * (u / (F::COLS / 8)) * a.v_nb2 + (c0 + 8 * (u % (F::COLS / 8))) * F::ES);
     }
-    // token t of the unit and the one behind it; past the part the last token is read (and not used)
-    auto load_unit = [&](v4w (&r)[2][F::LPU], const char * p, int64_t nb2, int t, int e8, int d) {
-        const int64_t back = t < part.len ? 0 : (int64_t) (part.len - 1 - t) * nb2;
-        const char * p0 = p + back, * p1 = t + 1 < part.len ? p0 + nb2 : p0;
-#pragma unroll
-        for (int j = 0; j < F::LPU; j++) {
-            r[0][j] = r[1][j] = v4w{0, 0, 0, 0};
-            if (e8 + j * (8 / F::LPU) < d) {
-                r[0][j] = *(const v4w *) (p0 + 16 * j);
-                r[1][j] = *(const v4w *) (p1 + 16 * j);
-            }
-        }
-    };
+    const bool plain = a.dk == DK && c0 + F::COLS <= a.dv && F::KN >= F::THREADS;
     auto load = [&](int t0) {
-        const int64_t dq = t0 * a.q_nb2, dk = t0 * a.k_nb2, dv = t0 * a.v_nb2;
+        const char * qb = qh + (int64_t) (part.t0 + t0) * a.q_nb2, * kb = kh + (int64_t) (part.t0 + t0) * a.k_nb2,
+                   * vb = vh + (int64_t) (part.t0 + t0) * a.v_nb2;
+        auto whole = [&](v4w (&r)[2][F::LPU], const char * base, uint32_t off, int64_t nb2) {
 #pragma unroll
-        for (int i = 0; i < F::KU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = t0 + 2 * (u / (DK / 8));
-            if (F::KN < F::THREADS && u >= F::KN) break;
-            if (!STATES) load_unit(rq[i], pq[i] + dq, a.q_nb2, t, e8, a.dk);
-            load_unit(rk[i], pk[i] + dk, a.k_nb2, t, e8, a.dk);
-        }
+            for (int j = 0; j < F::LPU; j++) {
+                r[0][j] = *(const v4w *) (base + off + 16 * j);
+                r[1][j] = *(const v4w *) (base + nb2 + off + 16 * j);
+            }
+        };
+        // zeros past the part, the head's rows and columns
+        auto some = [&](v4w (&r)[2][F::LPU], const char * base, uint32_t off, int64_t nb2, int t, int e8, int d) {
 #pragma unroll
-        for (int i = 0; i < F::VU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), t = t0 + 2 * (u / (F::COLS / 8));
-            load_unit(rv[i], pv[i] + dv, a.v_nb2, t, c0 + e8, a.dv);
+            for (int j = 0; j < F::LPU; j++) {
+                r[0][j] = r[1][j] = v4w{0, 0, 0, 0};
+                if (e8 + j * (8 / F::LPU) < d) {
+                    if (t < part.len) r[0][j] = *(const v4w *) (base + off + 16 * j);
+                    if (t + 1 < part.len) r[1][j] = *(const v4w *) (base + nb2 + off + 16 * j);
+                }
+            }
+        };
+        if (plain && t0 + C <= part.len) {
+#pragma unroll
+            for (int i = 0; i < F::KU; i++) {
+                if (!STATES) whole(rq[i], qb, oq[i], a.q_nb2);
+                whole(rk[i], kb, ok[i], a.k_nb2);
+            }
+#pragma unroll
+            for (int i = 0; i < F::VU; i++) whole(rv[i], vb, ov[i], a.v_nb2);
+        } else {
+#pragma unroll
+            for (int i = 0; i < F::KU; i++) {
+                const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = t0 + 2 * (u / (DK / 8));
+                if (F::KN < F::THREADS && u >= F::KN) break;
+                if (!STATES) some(rq[i], qb, oq[i], a.q_nb2, t, e8, a.dk);
+                some(rk[i], kb, ok[i], a.k_nb2, t, e8, a.dk);
+            }
+#pragma unroll
+            for (int i = 0; i < F::VU; i++) {
+                const int u = tid + F::THREADS * i;
+                some(rv[i], vb, ov[i], a.v_nb2, t0 + 2 * (u / (F::COLS / 8)), c0 + 8 * (u % (F::COLS / 8)), a.dv);
+            }
         }
         const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
         if (w == 0) rg = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
     };
-    // 8 values of a staged token as NT terms of 4 packed pairs; zeros past the part
-    auto terms = [&](const v4w (&r)[F::LPU], bool on, uint32_t (&o)[NT][4]) {
+    // 8 values of a staged token as NT terms of 4 packed pairs
+    auto terms = [&](const v4w (&r)[F::LPU], uint32_t (&o)[NT][4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             uint32_t t[NT];
@@ -385,7 +404,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                 bf16_terms<NT>(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1), t);
             }
 #pragma unroll
-            for (int n = 0; n < NT; n++) o[n][i] = on ? t[n] : 0u;
+            for (int n = 0; n < NT; n++) o[n][i] = t[n];
         }
     };
     auto rows = [&](int at, int token, int e8, const uint32_t (&o)[NT][4]) {      // q, k: two groups of 4 values
@@ -407,20 +426,20 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             }
     };
     auto stage = [&](int t0) {
-        uint32_t odd = 0;                     // a non-finite v
+        float odd = 0.f;                      // NaN with a non-finite v (times 0)
 #pragma unroll
         for (int i = 0; i < F::KU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), pair = u / (DK / 8), t = t0 + 2 * pair;
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), pair = u / (DK / 8);
             if (F::KN < F::THREADS && u >= F::KN) break;
             uint32_t o0[NT][4], o1[NT][4];
             if (!STATES) {
-                terms(rq[i][0], t < part.len, o0);
-                terms(rq[i][1], t + 1 < part.len, o1);
+                terms(rq[i][0], o0);
+                terms(rq[i][1], o1);
                 rows(F::OQ, 2 * pair, e8, o0);
                 rows(F::OQ, 2 * pair + 1, e8, o1);
             }
-            terms(rk[i][0], t < part.len, o0);
-            terms(rk[i][1], t + 1 < part.len, o1);
+            terms(rk[i][0], o0);
+            terms(rk[i][1], o1);
             if (!STATES) {
                 rows(F::OK, 2 * pair, e8, o0);
                 rows(F::OK, 2 * pair + 1, e8, o1);
@@ -429,16 +448,18 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         }
 #pragma unroll
         for (int i = 0; i < F::VU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), pair = u / (F::COLS / 8), t = t0 + 2 * pair;
+            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), pair = u / (F::COLS / 8);
             uint32_t o0[NT][4], o1[NT][4];
-            terms(rv[i][0], t < part.len, o0);
-            terms(rv[i][1], t + 1 < part.len, o1);
+            terms(rv[i][0], o0);
+            terms(rv[i][1], o1);
             columns(F::OV, F::V, pair, e8, o0, o1);
 #pragma unroll
-            for (int j = 0; j < 4; j++)          // an exponent of all ones carries into the sign's place
-                odd |= ((o0[0][j] & 0x7f807f80u) + 0x00800080u) | ((o1[0][j] & 0x7f807f80u) + 0x00800080u);
+            for (int j = 0; j < 4; j++) {
+                odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o0[0][j]), v2b{}, odd, false);
+                odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o1[0][j]), v2b{}, odd, false);
+            }
         }
-        if (!STATES && __ballot(odd & 0x80008000u) && lane == 0) odd_v[t0 / C & 1] = 1;
+        if (!STATES && __ballot(odd != odd) && lane == 0) odd_v[t0 / C & 1] = 1;
         if (w == 0) {
             float gt = t0 + lane < part.len && lane < C ? rg : 0.f;
             gt = gt < LC_FLOOR ? LC_FLOOR : gt;
@@ -451,8 +472,9 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             const double end = __shfl(s, C - 1);
             if (lane < C) {
                 G[lane] = s;
-                eG[lane] = __builtin_amdgcn_exp2f((float) s);
+                eG[lane] = __builtin_amdgcn_exp2f((float) s) * a.scale;
                 wG[lane] = __builtin_amdgcn_exp2f((float) (end - s));
+                if (lane == 0) eEnd = __builtin_amdgcn_exp2f((float) end);
             }
         }
     };
@@ -501,7 +523,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         stage(t0);
         __syncthreads();
         if (t0 + C < part.len) load(t0 + C);
-        const float cend = eG[C - 1];
+        const float cend = eEnd;
         if (STATES) total += G[C - 1];
         if constexpr (!STATES) {
             const bool odd = odd_v[t0 / C & 1] != 0;
@@ -537,7 +559,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int j = 16 * jt[x] + 4 * g + r;
-                    p[x][r] = j <= i ? p[x][r] * __builtin_amdgcn_exp2f((float) (gi - G[j])) : 0.f;
+                    p[x][r] = j <= i ? p[x][r] * (__builtin_amdgcn_exp2f((float) (gi - G[j])) * a.scale) : 0.f;
                 }
             }
 #pragma unroll
@@ -628,7 +650,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     const int t = t0 + 16 * i + m, c = c0 + LC_WCOLS * w + 8 * g;
                     if (t < part.len && c < a.dv) {
                         char * p = a.out + ((int64_t) (part.t0 + t) * a.n_v * a.dv + (int64_t) h * a.dv + c) * F::ES;
-                        const v4f y0 = o[i][0] * a.scale, y1 = o[i][1] * a.scale;
+                        const v4f y0 = o[i][0], y1 = o[i][1];
                         if constexpr (NT == 3) {
                             *(v4f *) p = y0;
                             *(v4f *) (p + 16) = y1;
@@ -873,6 +895,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             (uintptr_t) state_out < (uintptr_t) state_in + states)
             return set_error(QWFN_EINVAL, "linear_attn: state_in and state_out must be equal or not overlap");
         if (n_tok == 0) return QWFN_OK;
+        if ((q->nb[2] | k->nb[2] | v->nb[2]) >> 24) return set_error(QWFN_ENOTSUP, "linear_attn: token strides of 2^24 bytes or more");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
         if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");

@@ -142,6 +142,7 @@ def test_linear_attention_refusals():
     refused(linear(dst=heads(128, 6, 100, stride=128 * 6 * 2 + 16)), K.EINVAL, "contiguous")
     refused(linear(q=heads(128, 2, 100, at=FAKE + 8)), K.EALIGN, "16-byte")
     refused(linear(q=heads(128, 2, 100, stride=520)), K.EALIGN, "16-byte")
+    refused(linear(k=heads(128, 2, 100, stride=1 << 24)), K.ENOTSUP, "token strides")
     refused(linear(n_seq=0), K.EINVAL, "n_seq")
     refused(linear(max_len=0), K.EINVAL, "max_len")
     refused(linear(g_ts=5), K.EINVAL, "g_token_stride")
