@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace qwfn {
 namespace {
@@ -162,14 +163,15 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // A decay below e^-1000 counts as e^-1000, which is 0 in F32, so -inf is exact.
 //
 // A workgroup takes 32 columns a wave, its state in the waves' accumulators: lane m
-// of wave w, tile u holds column 32 w + 8 (m >> 2) + 4 u + (m & 3), rows 4 (l >> 4) + r
-// of each 16-row tile. As the state lies it is the A operand of S^T q (rows of a
-// 32-row block in the order of the registers; q and k lie in LDS in that order), and
+// of wave w, tile u holds column 32 w + 8 (m >> 2) + 4 u + (m & 3), rows
+// 32 (t / 2) + 8 (l >> 4) + 4 (t & 1) + r of 16-row tile t. So the state is the A
+// operand of S^T q as it lies, two tiles the 32 rows of a block in their order, and
 // O^T has 8 consecutive columns of a token in a lane: no data moves between the
-// products but the scores, which the waves share through LDS. q, k (rows), k^T and v^T
-// lie in LDS, a 16-byte unit at the place of an exclusive or with its row, so that
-// neither the row reads nor the transposed writes meet a bank often. The next chunk
-// is loaded into registers meanwhile. Three barriers a chunk.
+// products but the scores, which the waves share through LDS. q, k and v lie in LDS as
+// in memory, by rows; k^T and v^T are read by the transposing LDS reads, so each
+// value is stored once (with written transposes F32 of dk 128 had one workgroup a CU
+// instead of two, and 16 ragged F16 sequences of 32 heads of 64 took 122 us for 102). The next
+// chunk is loaded into registers meanwhile. Three barriers a chunk.
 //
 // A non-finite v_j must not reach tokens before j: a chunk that holds one takes its
 // scores times v by plain sums over j <= i.
@@ -196,28 +198,32 @@ struct lc_args {
 };
 
 template <int NT, int DK, int NW> struct lc_cfg {
-    static constexpr int C = NT == 1 ? 64 : 32;          // tokens of a chunk
+    static constexpr int C = NT == 1 && NW == 4 ? 64 : 32;          // tokens of a chunk (the next one waits in registers)
     static constexpr int IT = C / 16;                    // 16-token tiles
     static constexpr int JB = C / 32;                    // 32-token blocks of a sum
     static constexpr int KT = DK / 16, KB = DK / 32;
     static constexpr int COLS = LC_WCOLS * NW, THREADS = 64 * NW;
     static constexpr int ES = NT == 3 ? 4 : 2;           // bytes of a value
     static constexpr int LPU = NT == 3 ? 2 : 1;          // 16-byte loads of 8 values
-    // a staged unit: 8 values of two tokens
-    static constexpr int KN = C / 2 * (DK / 8), VN = C / 2 * (COLS / 8);
-    static constexpr int KU = (KN + THREADS - 1) / THREADS, VU = VN / THREADS;
-    static constexpr int QK = C * DK * 2, T = DK * C * 2, V = COLS * C * 2, P = C * C * 2;   // bytes of a term
-    static constexpr int OQ = 0, OK = OQ + NT * QK, OKT = OK + NT * QK, OV = OKT + NT * T, OP = OV + NT * V,
-                         LDS = OP + NT * P;
-    // workgroups of a CU: by LDS, and 8 waves (two a SIMD, 256 registers each)
-    static constexpr int PER_CU = 160 * 1024 / (LDS + 1280) < 8 / NW ? 160 * 1024 / (LDS + 1280) : 8 / NW;
+    // a staged unit: 8 values of a token; a thread's units of q and of k, and of v
+    static constexpr int KU = C * (DK / 8) / THREADS, VU = C * (COLS / 8) / THREADS;
+    static constexpr int QK = C * DK * 2, V = C * COLS * 2, P = C * C * 2;       // bytes of a term
+    static constexpr int OQ = 0, OK = OQ + NT * QK, OV = OK + NT * QK, OP = OV + NT * V, LDS = OP + NT * P;
+    // workgroups of a CU: by LDS, and two waves a SIMD, 256 registers each (one with a state of 256 rows)
+    static constexpr int WAVES = DK == 256 ? 4 : 8;
+    static constexpr int PER_CU = 160 * 1024 / (LDS + 1280) < WAVES / NW ? 160 * 1024 / (LDS + 1280) : WAVES / NW;
     static constexpr int WAVES_EU = (PER_CU * NW + 3) / 4;
-    static_assert((KN % THREADS == 0 || KU == 1) && VN % THREADS == 0, "whole units a thread, or one for some");
+    static_assert(KU * THREADS == C * (DK / 8) && VU * THREADS == C * (COLS / 8), "whole units a thread");
     static_assert(LDS + 2048 <= 160 * 1024, "LDS of a CU");
 };
 
-// Byte of a 16-byte unit in the rows of q and k ([token][dk]) and in k^T and v^T ([row][token]).
-template <int DK> __device__ __forceinline__ int lc_row(int row, int unit) { return row * (DK * 2) + ((unit ^ (row & 7)) * 16); }
+// Byte of a 16-byte unit in the rows of q, k and v ([token][W values]): the 16 rows of a row read, and the 4 rows by 4
+// units of 16 lanes of a transposing read, lie in different banks.
+template <int W> __device__ __forceinline__ int lc_row(int row, int unit) {
+    const int x = W == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+    return row * (W * 2) + ((unit ^ x) * 16);
+}
+// Byte of a 16-byte unit in the scores ([token i][token j]).
 template <int C> __device__ __forceinline__ int lc_col(int row, int unit) {
     return row * (C * 2) + ((unit ^ ((row ^ (row >> 3)) & (C / 8 - 1))) * 16);
 }
@@ -234,6 +240,16 @@ template <int NT> __device__ __forceinline__ void bf16_terms(float x, float y, u
             y -= __builtin_bit_cast(float, t[i] & 0xffff0000u);
         }
     }
+}
+// Lane m of 16-lane group g: column 8 (m >> 2) + 4 half + (m & 3) of the 32 columns from unit 4 ub, of the 8 rows from
+// `row` (8 g from a 32-row block): ds_read_b64_tr_b16 takes 4 rows of 16 values, 4 a lane, and gives a lane a column.
+template <int W> __device__ __forceinline__ v4w lc_transposed(uint8_t * rows, int row, int ub, int half, int m) {
+    typedef int16_t v4h __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4h * lp;
+    const int r = row + (m >> 2), u = 4 * ub + (m & 3);
+    const v2w x = __builtin_bit_cast(v2w, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp) (rows + lc_row<W>(r, u) + 8 * half)));
+    const v2w y = __builtin_bit_cast(v2w, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp) (rows + lc_row<W>(r + 4, u) + 8 * half)));
+    return v4w{x[0], x[1], y[0], y[1]};
 }
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __builtin_bit_cast(float, u & 0xffff0000u); }
@@ -323,69 +339,41 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     const int hk = h / a.rep, c0 = cb * F::COLS;
     const char * qh = a.q + (int64_t) hk * a.q_nb1, * kh = a.k + (int64_t) hk * a.k_nb1;
     const char * vh = a.v + (int64_t) h * a.v_nb1;
-    // the next chunk on its way: unit i of the thread: 8 values from 8 eu of tokens 2 ta and 2 ta + 1
-    v4w rq[F::KU][2][F::LPU], rk[F::KU][2][F::LPU], rv[F::VU][2][F::LPU];
+    // the next chunk on its way: unit i of the thread: 8 values of a token
+    v4w rq[F::KU][F::LPU], rk[F::KU][F::LPU], rv[F::VU][F::LPU];
     float rg = 0.f;
-    // A unit's place behind the chunk's first token, 32 bits (the host checks the strides): a whole chunk's loads are a
-    // uniform base and an offset.
-    uint32_t oq[F::KU], ok[F::KU], ov[F::VU];
-#pragma unroll
-    for (int i = 0; i < F::KU; i++) {
-        const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = 2 * (u / (DK / 8));
-        oq[i] = (uint32_t) (t * a.q_nb2 + e8 * F::ES);
-        ok[i] = (uint32_t) (t * a.k_nb2 + e8 * F::ES);
-    }
-#pragma unroll
-    for (int i = 0; i < F::VU; i++) {
-        const int u = tid + F::THREADS * i;
-        ov[i] = (uint32_t) (2 * (u / (F::COLS / 8)) * a.v_nb2 + (c0 + 8 * (u % (F::COLS / 8))) * F::ES);
-    }
-    const bool plain = a.dk == DK && c0 + F::COLS <= a.dv && F::KN >= F::THREADS;
+    // A thread's first unit behind the chunk's first token, 32 bits (the host checks the strides); its further ones lie
+    // a fixed number of tokens behind: a whole chunk's loads are uniform bases and one offset.
+    constexpr int KR = F::THREADS / (DK / 8), VR = F::THREADS / (F::COLS / 8);
+    const uint32_t oq = (uint32_t) (tid / (DK / 8) * a.q_nb2 + 8 * (tid % (DK / 8)) * F::ES);
+    const uint32_t ok = (uint32_t) (tid / (DK / 8) * a.k_nb2 + 8 * (tid % (DK / 8)) * F::ES);
+    const uint32_t ov = (uint32_t) (tid / (F::COLS / 8) * a.v_nb2 + (c0 + 8 * (tid % (F::COLS / 8))) * F::ES);
+    const bool plain = a.dk == DK && c0 + F::COLS <= a.dv;
     auto load = [&](int t0) {
-        const char * qb = qh + (int64_t) (part.t0 + t0) * a.q_nb2, * kb = kh + (int64_t) (part.t0 + t0) * a.k_nb2,
-                   * vb = vh + (int64_t) (part.t0 + t0) * a.v_nb2;
-        auto whole = [&](v4w (&r)[2][F::LPU], const char * base, uint32_t off, int64_t nb2) {
+        auto get = [&](auto & r, const char * base, uint32_t off, int64_t nb2, int step, int t, int e8, int d) {
+            constexpr int N = sizeof(r) / sizeof(r[0]);
+            if (plain && t0 + C <= part.len) {
 #pragma unroll
-            for (int j = 0; j < F::LPU; j++) {
-                r[0][j] = *(const v4w *) (base + off + 16 * j);
-                r[1][j] = *(const v4w *) (base + nb2 + off + 16 * j);
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < F::LPU; j++) r[i][j] = *(const v4w *) (base + i * step * nb2 + off + 16 * j);
+            } else {                              // zeros past the part, the head's rows and columns
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < F::LPU; j++) {
+                        r[i][j] = v4w{0, 0, 0, 0};
+                        if (e8 + j * (8 / F::LPU) < d && t + i * step < part.len) r[i][j] = *(const v4w *) (base + i * step * nb2 + off + 16 * j);
+                    }
             }
         };
-        // zeros past the part, the head's rows and columns
-        auto some = [&](v4w (&r)[2][F::LPU], const char * base, uint32_t off, int64_t nb2, int t, int e8, int d) {
-#pragma unroll
-            for (int j = 0; j < F::LPU; j++) {
-                r[0][j] = r[1][j] = v4w{0, 0, 0, 0};
-                if (e8 + j * (8 / F::LPU) < d) {
-                    if (t < part.len) r[0][j] = *(const v4w *) (base + off + 16 * j);
-                    if (t + 1 < part.len) r[1][j] = *(const v4w *) (base + nb2 + off + 16 * j);
-                }
-            }
-        };
-        if (plain && t0 + C <= part.len) {
-#pragma unroll
-            for (int i = 0; i < F::KU; i++) {
-                if (!STATES) whole(rq[i], qb, oq[i], a.q_nb2);
-                whole(rk[i], kb, ok[i], a.k_nb2);
-            }
-#pragma unroll
-            for (int i = 0; i < F::VU; i++) whole(rv[i], vb, ov[i], a.v_nb2);
-        } else {
-#pragma unroll
-            for (int i = 0; i < F::KU; i++) {
-                const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), t = t0 + 2 * (u / (DK / 8));
-                if (F::KN < F::THREADS && u >= F::KN) break;
-                if (!STATES) some(rq[i], qb, oq[i], a.q_nb2, t, e8, a.dk);
-                some(rk[i], kb, ok[i], a.k_nb2, t, e8, a.dk);
-            }
-#pragma unroll
-            for (int i = 0; i < F::VU; i++) {
-                const int u = tid + F::THREADS * i;
-                some(rv[i], vb, ov[i], a.v_nb2, t0 + 2 * (u / (F::COLS / 8)), c0 + 8 * (u % (F::COLS / 8)), a.dv);
-            }
-        }
-        const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
-        if (w == 0) rg = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
+        const int64_t t = part.t0 + t0;
+        const int tk = t0 + tid / (DK / 8), ek = 8 * (tid % (DK / 8));
+        if (!STATES) get(rq, qh + t * a.q_nb2, oq, a.q_nb2, KR, tk, ek, a.dk);
+        get(rk, kh + t * a.k_nb2, ok, a.k_nb2, KR, tk, ek, a.dk);
+        get(rv, vh + t * a.v_nb2, ov, a.v_nb2, VR, t0 + tid / (F::COLS / 8), c0 + 8 * (tid % (F::COLS / 8)), a.dv);
+        const int tg = t0 + lane < part.len ? t0 + lane : part.len - 1;
+        if (w == 0) rg = a.g[(int64_t) (part.t0 + tg) * a.g_ts + h];
     };
     // 8 values of a staged token as NT terms of 4 packed pairs
     auto terms = [&](const v4w (&r)[F::LPU], uint32_t (&o)[NT][4]) {
@@ -407,58 +395,26 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             for (int n = 0; n < NT; n++) o[n][i] = t[n];
         }
     };
-    auto rows = [&](int at, int token, int e8, const uint32_t (&o)[NT][4]) {      // q, k: two groups of 4 values
-        const int kb = e8 >> 5, uu = (e8 & 31) >> 3;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                *(v2w *) (lds + at + n * F::QK + lc_row<DK>(token, 4 * kb + (2 * uu & 3) + i) + 8 * (uu >> 1)) = v2w{o[n][2 * i], o[n][2 * i + 1]};
-    };
-    auto columns = [&](int at, int size, int pair, int e8, const uint32_t (&o0)[NT][4], const uint32_t (&o1)[NT][4]) {   // k^T, v^T
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t lo = __builtin_amdgcn_perm(o1[n][i], o0[n][i], 0x05040100u), hi = __builtin_amdgcn_perm(o1[n][i], o0[n][i], 0x07060302u);
-                *(uint32_t *) (lds + at + n * size + lc_col<C>(e8 + 2 * i, pair >> 2) + 4 * (pair & 3)) = lo;
-                *(uint32_t *) (lds + at + n * size + lc_col<C>(e8 + 2 * i + 1, pair >> 2) + 4 * (pair & 3)) = hi;
-            }
-    };
     auto stage = [&](int t0) {
         float odd = 0.f;                      // NaN with a non-finite v (times 0)
+        auto put = [&](auto wide, auto & r, int at, bool v) {
+            constexpr int W = decltype(wide)::value, N = sizeof(r) / sizeof(r[0]), STEP = F::THREADS / (W / 8);
 #pragma unroll
-        for (int i = 0; i < F::KU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (DK / 8)), pair = u / (DK / 8);
-            if (F::KN < F::THREADS && u >= F::KN) break;
-            uint32_t o0[NT][4], o1[NT][4];
-            if (!STATES) {
-                terms(rq[i][0], o0);
-                terms(rq[i][1], o1);
-                rows(F::OQ, 2 * pair, e8, o0);
-                rows(F::OQ, 2 * pair + 1, e8, o1);
-            }
-            terms(rk[i][0], o0);
-            terms(rk[i][1], o1);
-            if (!STATES) {
-                rows(F::OK, 2 * pair, e8, o0);
-                rows(F::OK, 2 * pair + 1, e8, o1);
-            }
-            columns(F::OKT, F::T, pair, e8, o0, o1);
-        }
+            for (int i = 0; i < N; i++) {
+                uint32_t o[NT][4];
+                terms(r[i], o);
 #pragma unroll
-        for (int i = 0; i < F::VU; i++) {
-            const int u = tid + F::THREADS * i, e8 = 8 * (u % (F::COLS / 8)), pair = u / (F::COLS / 8);
-            uint32_t o0[NT][4], o1[NT][4];
-            terms(rv[i][0], o0);
-            terms(rv[i][1], o1);
-            columns(F::OV, F::V, pair, e8, o0, o1);
+                for (int n = 0; n < NT; n++)
+                    *(v4w *) (lds + at + n * C * W * 2 + lc_row<W>(tid / (W / 8) + i * STEP, tid % (W / 8))) = v4w{o[n][0], o[n][1], o[n][2], o[n][3]};
+                if (v) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o0[0][j]), v2b{}, odd, false);
-                odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o1[0][j]), v2b{}, odd, false);
+                    for (int j = 0; j < 4; j++) odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o[0][j]), v2b{}, odd, false);
+                }
             }
-        }
+        };
+        if (!STATES) put(std::integral_constant<int, DK>{}, rq, F::OQ, false);
+        put(std::integral_constant<int, DK>{}, rk, F::OK, false);
+        put(std::integral_constant<int, F::COLS>{}, rv, F::OV, true);
         if (!STATES && __ballot(odd != odd) && lane == 0) odd_v[t0 / C & 1] = 1;
         if (w == 0) {
             float gt = t0 + lane < part.len && lane < C ? rg : 0.f;
@@ -480,7 +436,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     };
     load(0);
 
-    // the state of the lane: [row tile][column tile] of rows 16 t + 4 g + r
+    // the state of the lane: [row tile][column tile] of rows 32 (t / 2) + 8 g + 4 (t % 2) + r
     v4f S[F::KT][2];
     const size_t hs = (size_t) a.dk * a.dv, per = (size_t) a.n_v * hs;
     int col[2];
@@ -496,7 +452,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int row = 16 * t + 4 * g + r;
+                        const int row = 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r;
                         if (inside(row, col[u])) fn(S[t][u], r, (size_t) row * a.dv + col[u]);
                     }
         };
@@ -522,7 +478,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         asm volatile("" : "+v"(tid), "+v"(lane), "+v"(m), "+v"(g));
         stage(t0);
         __syncthreads();
-        if (t0 + C < part.len) load(t0 + C);
+        if (STATES && t0 + C < part.len) load(t0 + C);
         const float cend = eEnd;
         if (STATES) total += G[C - 1];
         if constexpr (!STATES) {
@@ -599,6 +555,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     }
                 }
             }
+            if (t0 + C < part.len) load(t0 + C);       // (here the scores' and S^T q's registers are free)
             __syncthreads();                   // the scores
             if (live) {
 #pragma unroll
@@ -614,7 +571,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
                         for (int u = 0; u < 2; u++)
 #pragma unroll
-                            for (int t = 0; t < NT; t++) vx[u][t] = *(const v4w *) (lds + F::OV + t * F::V + lc_col<C>(col[u] - c0, 4 * jb + g));
+                            for (int t = 0; t < NT; t++) vx[u][t] = lc_transposed<F::COLS>(lds + F::OV + t * F::V, 32 * jb + 8 * g, w, u, m);
 #pragma unroll
                         for (int i = 2 * jb; i < F::IT; i++) {
                             v4w px[NT];
@@ -625,18 +582,17 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                         }
                     }
                 } else {
-                    auto value = [&](int at, int size, int row, int t) {
+                    auto sum = [&](int at, int size) {
                         float f = 0.f;
-                        for (int n = 0; n < NT; n++)
-                            f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size + lc_col<C>(row, t >> 3) + 2 * (t & 7)) << 16);
+                        for (int n = 0; n < NT; n++) f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size) << 16);
                         return f;
                     };
                     for (int i = 0; i < F::IT; i++)
                         for (int j = 0; j <= 16 * i + m; j++) {
-                            const float p = value(F::OP, F::P, 16 * i + m, j);
+                            const float p = sum(F::OP + lc_col<C>(16 * i + m, j >> 3) + 2 * (j & 7), F::P);
                             for (int u = 0; u < 2; u++)
                                 for (int r = 0; r < 4; r++) {
-                                    const float v = value(F::OV, F::V, LC_WCOLS * w + 8 * g + 4 * u + r, j);
+                                    const float v = sum(F::OV + lc_row<F::COLS>(j, 4 * w + g) + 8 * u + 2 * r, F::V);
                                     // (the index is not a constant: written out for each of the tiles)
 #pragma unroll
                                     for (int ii = 0; ii < F::IT; ii++)
@@ -675,7 +631,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                 for (int u = 0; u < 2; u++) {
                     v4w vt[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) vt[t] = *(const v4w *) (lds + F::OV + t * F::V + lc_col<C>(col[u] - c0, 4 * jb + g));
+                    for (int t = 0; t < NT; t++) vt[t] = lc_transposed<F::COLS>(lds + F::OV + t * F::V, 32 * jb + 8 * g, w, u, m);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         float lo = 0.f, hi = 0.f;
@@ -701,7 +657,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     for (int t = 0; t < TG; t++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
-                            kx[t][n] = *(const v4w *) (lds + F::OKT + n * F::T + lc_col<C>(16 * (t0g + t) + m, 4 * jb + g));
+                            kx[t][n] = lc_transposed<DK>(lds + F::OK + n * F::QK, 32 * jb + 8 * g, (t0g + t) >> 1, t & 1, m);
 #pragma unroll
                     for (int d = 2; d >= 0; d--)
 #pragma unroll
@@ -804,8 +760,7 @@ struct lc_plan {
 template <int NT> int per_cu(int DK, int NW) {
     if (DK == 64) return NW == 2 ? lc_cfg<NT, 64, 2>::PER_CU : lc_cfg<NT, 64, 4>::PER_CU;
     if (DK == 128) return NW == 2 ? lc_cfg<NT, 128, 2>::PER_CU : lc_cfg<NT, 128, 4>::PER_CU;
-    if constexpr (NT < 3) return NW == 2 ? lc_cfg<NT, 256, 2>::PER_CU : lc_cfg<NT, 256, 4>::PER_CU;
-    return 1;
+    return NW == 2 ? lc_cfg<NT, 256, 2>::PER_CU : lc_cfg<NT, 256, 4>::PER_CU;
 }
 
 // Parts of a sequence: as many as fill the CUs once, so that no workgroup waits for another (4096 tokens of 48 heads
@@ -818,12 +773,11 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     const int64_t dk = q->ne[0], dv = v->ne[0], n_v = v->ne[1], n_tok = q->ne[2];
     p.NT = q->type == QWFN_TYPE_BF16 ? 1 : q->type == QWFN_TYPE_F16 ? 2 : 3;
     p.DK = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
-    // three terms of 256 rows of q, k and k^T are more than the LDS of a CU
-    p.step = max_len <= LC_STEP_MAX || (p.NT == 3 && p.DK == 256);
+    p.step = max_len <= LC_STEP_MAX;
     if (p.step) return p;
     p.NW = dv <= 2 * LC_WCOLS ? 2 : 4;
     p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
-    const int64_t longest = std::min<int64_t>(max_len, n_tok), C = p.NT == 1 ? 64 : 32;
+    const int64_t longest = std::min<int64_t>(max_len, n_tok), C = p.NT == 1 && p.NW == 4 ? 64 : 32;
     const int64_t room = LC_CUS * (p.NT == 1 ? per_cu<1>(p.DK, p.NW) : p.NT == 2 ? per_cu<2>(p.DK, p.NW) : per_cu<3>(p.DK, p.NW)) /
                          (n_v * p.ct);
     // a sequence's last part is half of one on average
@@ -856,8 +810,7 @@ template <int NT>
 int launch_type(const lc_args & x, const lc_plan & p, hipStream_t s) {
     if (p.DK == 64)  return p.NW == 2 ? launch_chunks<NT, 64, 2>(x, p, s) : launch_chunks<NT, 64, 4>(x, p, s);
     if (p.DK == 128) return p.NW == 2 ? launch_chunks<NT, 128, 2>(x, p, s) : launch_chunks<NT, 128, 4>(x, p, s);
-    if constexpr (NT < 3) return p.NW == 2 ? launch_chunks<NT, 256, 2>(x, p, s) : launch_chunks<NT, 256, 4>(x, p, s);
-    return QWFN_ENOTSUP;
+    return p.NW == 2 ? launch_chunks<NT, 256, 2>(x, p, s) : launch_chunks<NT, 256, 4>(x, p, s);
 }
 
 }  // namespace
