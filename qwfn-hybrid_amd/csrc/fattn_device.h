@@ -97,5 +97,19 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// A wave-wide LDS DMA: lane i copies the 16 bytes at base + off to LDS[at + 16 i] (base and at the same for all lanes).
+// Inline asm, so that the compiler neither moves memory operations across it nor waits for it: wait_vmem does. (m0 is
+// read one wait state after its write at the earliest; the compiler keeps nothing in it.)
+__device__ __forceinline__ void lds_dma16(const void * base, uint32_t off, uint32_t at) {
+    const uint64_t b = (uint64_t) (uintptr_t) base;
+    const uint64_t s = (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (b >> 32)) << 32 |
+                       (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) b);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(s), "s"(__builtin_amdgcn_readfirstlane((int) at)) : "memory");
+}
+// Waits for the wave's vector-memory operations.
+__device__ __forceinline__ void wait_vmem() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void * p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) p; }
+
 }  // namespace
 }  // namespace qwfn

@@ -170,8 +170,14 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // products but the scores, which the waves share through LDS. q, k and v lie in LDS as
 // in memory, by rows; k^T and v^T are read by the transposing LDS reads, so each
 // value is stored once (with written transposes F32 of dk 128 had one workgroup a CU
-// instead of two, and 16 ragged F16 sequences of 32 heads of 64 took 122 us for 102). The next
-// chunk is loaded into registers meanwhile. Three barriers a chunk.
+// instead of two, and 16 ragged F16 sequences of 32 heads of 64 took 122 us for 102).
+// bf16 goes to LDS as it is, by LDS DMA into two buffers, a chunk ahead: no registers
+// hold it and a chunk has two barriers. f16 and f32 are taken apart on the way, the
+// next chunk waits in registers, and a chunk has three.
+// What bounds it: 4096 bf16 tokens of 48 heads of 128 move 134 MB of q, k, v and o and
+// the parts' states another 190 MB, 63 us at the rate of a copy, and take 107; the
+// vector units are busy 40 % of the loop (the state's scaling and its roundings), the
+// matrix cores 20 %, the rest are the waits between a chunk's dependent products.
 //
 // A non-finite v_j must not reach tokens before j: a chunk that holds one takes its
 // scores times v by plain sums over j <= i.
@@ -193,40 +199,40 @@ constexpr float LC_FLOOR = -1000.f;
 struct lc_args {
     la_args   a;
     int32_t   L;                       // tokens of a part, a multiple of the chunk; 0: sequences are whole
-    float *   U;                       // [part][n_v][dk][dv]
+    int32_t   KT, US;                  // row tiles of a state, values of one in the workspace
+    float *   U;                       // [part][n_v][wave's columns][row tile][column tile][lane][4], as the lanes hold them
     double *  G;                       // [part][n_v]: log2 of the part's decay
 };
 
+constexpr int LC_C = 32;               // tokens of a chunk: the sum of one MFMA
+
 template <int NT, int DK, int NW> struct lc_cfg {
-    static constexpr int C = NT == 1 && NW == 4 ? 64 : 32;          // tokens of a chunk (the next one waits in registers)
-    static constexpr int IT = C / 16;                    // 16-token tiles
-    static constexpr int JB = C / 32;                    // 32-token blocks of a sum
     static constexpr int KT = DK / 16, KB = DK / 32;
     static constexpr int COLS = LC_WCOLS * NW, THREADS = 64 * NW;
     static constexpr int ES = NT == 3 ? 4 : 2;           // bytes of a value
     static constexpr int LPU = NT == 3 ? 2 : 1;          // 16-byte loads of 8 values
+    static constexpr bool DMA = NT == 1;                 // bf16 goes to LDS as it is
     // a staged unit: 8 values of a token; a thread's units of q and of k, and of v
-    static constexpr int KU = C * (DK / 8) / THREADS, VU = C * (COLS / 8) / THREADS;
-    static constexpr int QK = C * DK * 2, V = C * COLS * 2, P = C * C * 2;       // bytes of a term
-    static constexpr int OQ = 0, OK = OQ + NT * QK, OV = OK + NT * QK, OP = OV + NT * V, LDS = OP + NT * P;
-    // workgroups of a CU: by LDS, and two waves a SIMD, 256 registers each (one with a state of 256 rows)
-    static constexpr int WAVES = DK == 256 ? 4 : 8;
+    static constexpr int KU = LC_C * (DK / 8) / THREADS, VU = LC_C * (COLS / 8) / THREADS;
+    static constexpr int QK = LC_C * DK * 2, V = LC_C * COLS * 2, P = LC_C * LC_C * 2;     // bytes of a term
+    static constexpr int OQ = 0, OK = OQ + NT * QK, OV = OK + NT * QK, BUF = OV + NT * V, OP = (DMA ? 2 : 1) * BUF, LDS = OP + NT * P;
+    // workgroups of a CU: by LDS, and three waves a SIMD (168 registers each), two with a chunk in registers, one with a
+    // state of 256 rows
+    static constexpr int WAVES = DK == 256 ? 4 : DMA ? 12 : 8;
     static constexpr int PER_CU = 160 * 1024 / (LDS + 1280) < WAVES / NW ? 160 * 1024 / (LDS + 1280) : WAVES / NW;
     static constexpr int WAVES_EU = (PER_CU * NW + 3) / 4;
-    static_assert(KU * THREADS == C * (DK / 8) && VU * THREADS == C * (COLS / 8), "whole units a thread");
+    static_assert(KU * THREADS == LC_C * (DK / 8) && VU * THREADS == LC_C * (COLS / 8), "whole units a thread");
     static_assert(LDS + 2048 <= 160 * 1024, "LDS of a CU");
 };
 
 // Byte of a 16-byte unit in the rows of q, k and v ([token][W values]): the 16 rows of a row read, and the 4 rows by 4
 // units of 16 lanes of a transposing read, lie in different banks.
-template <int W> __device__ __forceinline__ int lc_row(int row, int unit) {
-    const int x = W == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
-    return row * (W * 2) + ((unit ^ x) * 16);
+template <int W> __device__ __forceinline__ int lc_place(int row) {       // exclusive or of a row's units
+    return W == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
 }
+template <int W> __device__ __forceinline__ int lc_row(int row, int unit) { return row * (W * 2) + ((unit ^ lc_place<W>(row)) * 16); }
 // Byte of a 16-byte unit in the scores ([token i][token j]).
-template <int C> __device__ __forceinline__ int lc_col(int row, int unit) {
-    return row * (C * 2) + ((unit ^ ((row ^ (row >> 3)) & (C / 8 - 1))) * 16);
-}
+__device__ __forceinline__ int lc_score(int row, int unit) { return row * (LC_C * 2) + ((unit ^ (row >> 1 & 3)) * 16); }
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
     return __builtin_bit_cast(uint32_t, v2b{(__bf16) x, (__bf16) y});
 }
@@ -297,34 +303,38 @@ __device__ lc_part find_part(const lc_args & x, int want, bool report, int threa
             for (int i = 0; i < c; i++) {
                 const int b = tid * c + i;
                 const int32_t n = b < a.n_seq ? (la_sequence(a, b, false).len + x.L - 1) / x.L : 0;
-                if (want >= at && want < at + n) { sh[8] = b; sh[9] = want - at; sh[10] = n; }
+                if (want >= at && want < at + n) {
+                    const la_seq s = la_sequence(a, b, false);
+                    sh[8] = b; sh[9] = want - at; sh[10] = n; sh[11] = s.t0; sh[12] = s.len; sh[13] = s.slot;
+                }
                 at += n;
             }
         }
         __syncthreads();
-        p.b = __builtin_amdgcn_readfirstlane(sh[8]);
+        auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(sh[i]); };
+        p.b = get(8);
         if (p.b < 0) return p;
-        p.before = __builtin_amdgcn_readfirstlane(sh[9]);
-        p.after = __builtin_amdgcn_readfirstlane(sh[10]) - p.before - 1;
+        p.before = get(9);
+        p.after = get(10) - p.before - 1;
+        p.t0 = get(11) + p.before * x.L;
+        p.len = p.after > 0 ? x.L : get(12) - p.before * x.L;
+        p.slot = get(13);
+        return p;
     }
-    const la_seq s = la_sequence(a, p.b, report && x.L == 0 && threadIdx.x == 0);
-    p.t0 = s.t0 + p.before * x.L;
-    p.len = p.after > 0 ? x.L : s.len - p.before * x.L;
-    p.slot = s.slot;
-    return p;
+    const la_seq s = la_sequence(a, want, report && threadIdx.x == 0);
+    return {want, s.t0, s.len, 0, 0, want, s.slot};
 }
 
 // STATES: only what the part adds to the state, to the workspace.
 template <int NT, int DK, int NW, bool STATES>
 __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_linear_chunks(lc_args x) {
     using F = lc_cfg<NT, DK, NW>;
-    constexpr int C = F::C;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[F::LDS];
-    __shared__ double G[C];                    // log2 of the decay from the chunk's start
-    __shared__ float eG[C], wG[C];             // scale 2^G, 2^(G_end - G)
-    __shared__ float eEnd;                     // 2^G_end
-    __shared__ int32_t sh[12];
-    __shared__ int32_t odd_v[2];               // a chunk, by parity, holds a non-finite v
+    constexpr int C = LC_C;
+    __shared__ __attribute__((aligned(256))) uint8_t lds[F::LDS];
+    // by the chunk's parity: log2 of the decay from the chunk's start, scale 2^G, 2^(G_end - G), 2^G_end
+    __shared__ double G[2][C];
+    __shared__ float eG[2][C], wG[2][C], eEnd[2];
+    __shared__ int32_t sh[14];
     const la_args & a = x.a;
     int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -339,41 +349,46 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     const int hk = h / a.rep, c0 = cb * F::COLS;
     const char * qh = a.q + (int64_t) hk * a.q_nb1, * kh = a.k + (int64_t) hk * a.k_nb1;
     const char * vh = a.v + (int64_t) h * a.v_nb1;
-    // the next chunk on its way: unit i of the thread: 8 values of a token
-    v4w rq[F::KU][F::LPU], rk[F::KU][F::LPU], rv[F::VU][F::LPU];
-    float rg = 0.f;
-    // A thread's first unit behind the chunk's first token, 32 bits (the host checks the strides); its further ones lie
-    // a fixed number of tokens behind: a whole chunk's loads are uniform bases and one offset.
-    constexpr int KR = F::THREADS / (DK / 8), VR = F::THREADS / (F::COLS / 8);
-    const uint32_t oq = (uint32_t) (tid / (DK / 8) * a.q_nb2 + 8 * (tid % (DK / 8)) * F::ES);
-    const uint32_t ok = (uint32_t) (tid / (DK / 8) * a.k_nb2 + 8 * (tid % (DK / 8)) * F::ES);
-    const uint32_t ov = (uint32_t) (tid / (F::COLS / 8) * a.v_nb2 + (c0 + 8 * (tid % (F::COLS / 8))) * F::ES);
+    // Unit i of the thread: 16 bytes of LDS at 16 (tid + THREADS i) of the tensor, its token, its 8 values from `e8`.
+    // Its place behind the chunk's first token has 32 bits (the host checks the strides): loads are a uniform base and
+    // an offset.
+    struct unit { int token, e8; };
+    auto q_unit = [&](int i) { const int u = tid + F::THREADS * i, t = u / (DK / 8); return unit{t, 8 * (u % (DK / 8) ^ lc_place<DK>(t))}; };
+    auto v_unit = [&](int i) {
+        const int u = tid + F::THREADS * i, t = u / (F::COLS / 8);
+        return unit{t, c0 + 8 * (u % (F::COLS / 8) ^ lc_place<F::COLS>(t))};
+    };
+    uint32_t oq[F::KU], ok[F::KU], ov[F::VU];
+#pragma unroll
+    for (int i = 0; i < F::KU; i++) {
+        const unit u = q_unit(i);
+        oq[i] = (uint32_t) (u.token * a.q_nb2 + u.e8 * F::ES);
+        ok[i] = (uint32_t) (u.token * a.k_nb2 + u.e8 * F::ES);
+    }
+#pragma unroll
+    for (int i = 0; i < F::VU; i++) {
+        const unit u = v_unit(i);
+        ov[i] = (uint32_t) (u.token * a.v_nb2 + u.e8 * F::ES);
+    }
     const bool plain = a.dk == DK && c0 + F::COLS <= a.dv;
-    auto load = [&](int t0) {
-        auto get = [&](auto & r, const char * base, uint32_t off, int64_t nb2, int step, int t, int e8, int d) {
-            constexpr int N = sizeof(r) / sizeof(r[0]);
-            if (plain && t0 + C <= part.len) {
+    auto get = [&](auto & r, const char * base, const auto & off, auto unit_of, int t0, int d) {
+        constexpr int N = sizeof(r) / sizeof(r[0]);
+        if (plain && t0 + C <= part.len) {
 #pragma unroll
-                for (int i = 0; i < N; i++)
+            for (int i = 0; i < N; i++)
 #pragma unroll
-                    for (int j = 0; j < F::LPU; j++) r[i][j] = *(const v4w *) (base + i * step * nb2 + off + 16 * j);
-            } else {                              // zeros past the part, the head's rows and columns
+                for (int j = 0; j < F::LPU; j++) r[i][j] = *(const v4w *) (base + off[i] + 16 * j);
+        } else {                                  // zeros past the part, the head's rows and columns
 #pragma unroll
-                for (int i = 0; i < N; i++)
+            for (int i = 0; i < N; i++) {
+                const unit u = unit_of(i);
 #pragma unroll
-                    for (int j = 0; j < F::LPU; j++) {
-                        r[i][j] = v4w{0, 0, 0, 0};
-                        if (e8 + j * (8 / F::LPU) < d && t + i * step < part.len) r[i][j] = *(const v4w *) (base + i * step * nb2 + off + 16 * j);
-                    }
+                for (int j = 0; j < F::LPU; j++) {
+                    r[i][j] = v4w{0, 0, 0, 0};
+                    if (u.e8 + j * (8 / F::LPU) < d && t0 + u.token < part.len) r[i][j] = *(const v4w *) (base + off[i] + 16 * j);
+                }
             }
-        };
-        const int64_t t = part.t0 + t0;
-        const int tk = t0 + tid / (DK / 8), ek = 8 * (tid % (DK / 8));
-        if (!STATES) get(rq, qh + t * a.q_nb2, oq, a.q_nb2, KR, tk, ek, a.dk);
-        get(rk, kh + t * a.k_nb2, ok, a.k_nb2, KR, tk, ek, a.dk);
-        get(rv, vh + t * a.v_nb2, ov, a.v_nb2, VR, t0 + tid / (F::COLS / 8), c0 + 8 * (tid % (F::COLS / 8)), a.dv);
-        const int tg = t0 + lane < part.len ? t0 + lane : part.len - 1;
-        if (w == 0) rg = a.g[(int64_t) (part.t0 + tg) * a.g_ts + h];
+        }
     };
     // 8 values of a staged token as NT terms of 4 packed pairs
     auto terms = [&](const v4w (&r)[F::LPU], uint32_t (&o)[NT][4]) {
@@ -395,46 +410,77 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             for (int n = 0; n < NT; n++) o[n][i] = t[n];
         }
     };
-    auto stage = [&](int t0) {
-        float odd = 0.f;                      // NaN with a non-finite v (times 0)
-        auto put = [&](auto wide, auto & r, int at, bool v) {
-            constexpr int W = decltype(wide)::value, N = sizeof(r) / sizeof(r[0]), STEP = F::THREADS / (W / 8);
+    auto put = [&](const auto & r, int at, int size) {
+        constexpr int N = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                uint32_t o[NT][4];
-                terms(r[i], o);
+        for (int i = 0; i < N; i++) {
+            uint32_t o[NT][4];
+            terms(r[i], o);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-                    *(v4w *) (lds + at + n * C * W * 2 + lc_row<W>(tid / (W / 8) + i * STEP, tid % (W / 8))) = v4w{o[n][0], o[n][1], o[n][2], o[n][3]};
-                if (v) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, o[0][j]), v2b{}, odd, false);
-                }
-            }
-        };
-        if (!STATES) put(std::integral_constant<int, DK>{}, rq, F::OQ, false);
-        put(std::integral_constant<int, DK>{}, rk, F::OK, false);
-        put(std::integral_constant<int, F::COLS>{}, rv, F::OV, true);
-        if (!STATES && __ballot(odd != odd) && lane == 0) odd_v[t0 / C & 1] = 1;
-        if (w == 0) {
-            float gt = t0 + lane < part.len && lane < C ? rg : 0.f;
-            gt = gt < LC_FLOOR ? LC_FLOOR : gt;
-            double s = (double) gt * LC_LOG2E;
-#pragma unroll
-            for (int d = 1; d < C; d <<= 1) {
-                const double y = __shfl_up(s, d);
-                if (lane >= d) s += y;
-            }
-            const double end = __shfl(s, C - 1);
-            if (lane < C) {
-                G[lane] = s;
-                eG[lane] = __builtin_amdgcn_exp2f((float) s) * a.scale;
-                wG[lane] = __builtin_amdgcn_exp2f((float) (end - s));
-                if (lane == 0) eEnd = __builtin_amdgcn_exp2f((float) end);
-            }
+            for (int n = 0; n < NT; n++) *(v4w *) (lds + at + n * size + 16 * (tid + F::THREADS * i)) = v4w{o[n][0], o[n][1], o[n][2], o[n][3]};
         }
     };
-    load(0);
+    auto q_at = [&](int t0) { return qh + (int64_t) (part.t0 + t0) * a.q_nb2; };
+    auto k_at = [&](int t0) { return kh + (int64_t) (part.t0 + t0) * a.k_nb2; };
+    auto v_at = [&](int t0) { return vh + (int64_t) (part.t0 + t0) * a.v_nb2; };
+    // bf16: a chunk to the buffer at `to`, under way when the call returns but for ragged chunks
+    auto send = [&](int t0, int to) {
+        if (plain && t0 + C <= part.len) {
+            const uint32_t at = lds_address(lds) + to + 1024 * w;
+            if (!STATES) {
+#pragma unroll
+                for (int i = 0; i < F::KU; i++) lds_dma16(q_at(t0), oq[i], at + F::OQ + 16 * F::THREADS * i);
+            }
+#pragma unroll
+            for (int i = 0; i < F::KU; i++) lds_dma16(k_at(t0), ok[i], at + F::OK + 16 * F::THREADS * i);
+#pragma unroll
+            for (int i = 0; i < F::VU; i++) lds_dma16(v_at(t0), ov[i], at + F::OV + 16 * F::THREADS * i);
+        } else {
+            v4w rk[F::KU][F::LPU], rv[F::VU][F::LPU];
+            if (!STATES) {
+                get(rk, q_at(t0), oq, q_unit, t0, a.dk);
+                put(rk, to + F::OQ, F::QK);
+            }
+            get(rk, k_at(t0), ok, q_unit, t0, a.dk);
+            put(rk, to + F::OK, F::QK);
+            get(rv, v_at(t0), ov, v_unit, t0, a.dv);
+            put(rv, to + F::OV, F::V);
+        }
+    };
+    // f16 and f32: the next chunk waits in registers, and is taken apart on its way to LDS
+    v4w rq[F::DMA ? 1 : F::KU][F::LPU], rk[F::DMA ? 1 : F::KU][F::LPU], rv[F::DMA ? 1 : F::VU][F::LPU];
+    auto load = [&](int t0) {
+        if (!STATES) get(rq, q_at(t0), oq, q_unit, t0, a.dk);
+        get(rk, k_at(t0), ok, q_unit, t0, a.dk);
+        get(rv, v_at(t0), ov, v_unit, t0, a.dv);
+    };
+    // the decays of the chunk from t0, by the last wave (which has no scores to make); the next chunk's g is loaded ahead
+    float gt = 0.f;
+    auto load_g = [&](int t0) {
+        const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
+        gt = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
+    };
+    auto decays = [&](int t0) {
+        const int at = t0 / C & 1;
+        float x = t0 + lane < part.len && lane < C ? gt : 0.f;
+        x = x < LC_FLOOR ? LC_FLOOR : x;
+        double s = (double) x * LC_LOG2E;
+#pragma unroll
+        for (int d = 1; d < C; d <<= 1) {
+            const double y = __shfl_up(s, d);
+            if (lane >= d) s += y;
+        }
+        const double end = __shfl(s, C - 1);
+        if (lane < C) {
+            G[at][lane] = s;
+            eG[at][lane] = __builtin_amdgcn_exp2f((float) s) * a.scale;
+            wG[at][lane] = __builtin_amdgcn_exp2f((float) (end - s));
+            if (lane == 0) eEnd[at] = __builtin_amdgcn_exp2f((float) end);
+        }
+    };
+    if (w == NW - 1) load_g(0);
+    if constexpr (F::DMA) send(0, 0);
+    else load(0);
 
     // the state of the lane: [row tile][column tile] of rows 32 (t / 2) + 8 g + 4 (t % 2) + r
     v4f S[F::KT][2];
@@ -444,6 +490,10 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     for (int u = 0; u < 2; u++) col[u] = c0 + LC_WCOLS * w + 8 * (m >> 2) + 4 * u + (m & 3);
     const bool live = c0 + LC_WCOLS * w < a.dv;            // the wave has columns
     const bool whole = a.dk == DK && c0 + LC_WCOLS * (w + 1) <= a.dv;      // no row or column past the head's
+    // the lane's values of a state in the workspace
+    auto in_u = [&](size_t index, int t, int u) -> v4f & {
+        return *(v4f *) (x.U + (index * a.n_v + h) * x.US + ((((size_t) cb * NW + w) * F::KT + t) * 2 + u) * 256 + 4 * lane);
+    };
     auto each = [&](auto fn) {                             // fn(value, its element, element of a head's state)
         auto all = [&](auto inside) {
 #pragma unroll
@@ -463,74 +513,89 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
     for (int t = 0; t < F::KT; t++) S[t][0] = S[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
     if (!STATES) {
-        const float * s0 = part.before > 0 ? x.U + ((size_t) (part.index - 1) * a.n_v + h) * hs
-                           : part.slot >= 0 && a.s_in ? a.s_in + part.slot * per + h * hs : nullptr;
-        if (s0) each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
-        // the scores of tokens behind a 32-token block's last one stay 0
+        if (part.before > 0) {
+#pragma unroll
+            for (int t = 0; t < F::KT; t++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) S[t][u] = in_u(part.index - 1, t, u);
+        } else if (part.slot >= 0 && a.s_in) {
+            const float * s0 = a.s_in + part.slot * per + h * hs;
+            each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
+        }
+        // the scores of the tokens behind the first 16 stay 0 in their rows
         for (int i = tid; i < NT * F::P / 16; i += F::THREADS) *(v4w *) (lds + F::OP + 16 * i) = v4w{0, 0, 0, 0};
-        if (tid < 2) odd_v[tid] = 0;
+    }
+    if (w == NW - 1) {
+        decays(0);
+        load_g(C);
     }
     double total = 0.;
-    __syncthreads();
 
     for (int t0 = 0; t0 < part.len; t0 += C) {
         // the thread's places are computed anew in every chunk: kept over the loop they cost registers, spilled
         asm volatile("" : "+v"(tid), "+v"(lane), "+v"(m), "+v"(g));
-        stage(t0);
+        const int even = t0 / C & 1, buf = F::DMA ? even * F::BUF : 0;
+        if constexpr (F::DMA) {
+            wait_vmem();
+        } else {
+            if (!STATES) put(rq, F::OQ, F::QK);
+            put(rk, F::OK, F::QK);
+            put(rv, F::OV, F::V);
+        }
         __syncthreads();
-        if (STATES && t0 + C < part.len) load(t0 + C);
-        const float cend = eEnd;
-        if (STATES) total += G[C - 1];
+        if (w == NW - 1 && t0 + C < part.len) {
+            decays(t0 + C);
+            load_g(t0 + 2 * C);
+        }
+        if constexpr (F::DMA) {
+            if (t0 + C < part.len) send(t0 + C, F::BUF - buf);
+        } else if (STATES && t0 + C < part.len) {
+            load(t0 + C);
+        }
+        const float cend = eEnd[even];
+        if (STATES) total += G[even][C - 1];
+        v4w vx[2][NT];                         // v^T of the wave's columns
+        auto load_v = [&]() {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) vx[u][t] = lc_transposed<F::COLS>(lds + buf + F::OV + t * F::V, 8 * g, w, u, m);
+        };
         if constexpr (!STATES) {
-            const bool odd = odd_v[t0 / C & 1] != 0;
-            if (tid == 0) odd_v[~(t0 / C) & 1] = 0;            // read in the chunk before, written in the next
-            // the scores, 16 x 16 tiles of tokens (j rows, i columns) with j <= i, PT a wave (the last tile by more than
-            // one wave where they do not come out even)
-            constexpr int TILES = F::IT * (F::IT + 1) / 2, PT = (TILES + NW - 1) / NW;
-            v4f p[PT];
-            int it[PT], jt[PT];
+            // the scores, 16 x 16 tiles of tokens (j rows, i columns): the three with j <= i
+            constexpr int PT = NW == 2 ? 2 : 1;
 #pragma unroll
             for (int x = 0; x < PT; x++) {
-                const int n = w + NW * x < TILES ? w + NW * x : TILES - 1;
-                it[x] = (n >= 1) + (n >= 3) + (n >= 6);
-                jt[x] = n - it[x] * (it[x] + 1) / 2;
-                p[x] = v4f{0.f, 0.f, 0.f, 0.f};
-            }
+                const int n = w + NW * x;
+                if (n >= 3) break;
+                const int it = n > 0, jt = n > 1;
+                v4f p{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kb = 0; kb < F::KB; kb++)
-#pragma unroll
-                for (int x = 0; x < PT; x++) {
+                for (int kb = 0; kb < F::KB; kb++) {
                     v4w kx[NT], qx[NT];
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        kx[t] = *(const v4w *) (lds + F::OK + t * F::QK + lc_row<DK>(16 * jt[x] + m, 4 * kb + g));
-                        qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * it[x] + m, 4 * kb + g));
+                        kx[t] = *(const v4w *) (lds + buf + F::OK + t * F::QK + lc_row<DK>(16 * jt + m, 4 * kb + g));
+                        qx[t] = *(const v4w *) (lds + buf + F::OQ + t * F::QK + lc_row<DK>(16 * it + m, 4 * kb + g));
                     }
-                    p[x] = mfma_terms<NT, NT, NT>(kx, qx, p[x]);
+                    p = mfma_terms<NT, NT, NT>(kx, qx, p);
                 }
-#pragma unroll
-            for (int x = 0; x < PT; x++) {
-                const int i = 16 * it[x] + m;
-                const double gi = G[i];
+                const int i = 16 * it + m;
+                const double gi = G[even][i];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int j = 16 * jt[x] + 4 * g + r;
-                    p[x][r] = j <= i ? p[x][r] * (__builtin_amdgcn_exp2f((float) (gi - G[j])) * a.scale) : 0.f;
+                    const int j = 16 * jt + 4 * g + r;
+                    p[r] = j <= i ? p[r] * (__builtin_amdgcn_exp2f((float) (gi - G[even][j])) * a.scale) : 0.f;
                 }
-            }
-#pragma unroll
-            for (int x = 0; x < PT; x++) {
                 uint32_t lo[NT], hi[NT];
-                bf16_terms<NT>(p[x][0], p[x][1], lo);
-                bf16_terms<NT>(p[x][2], p[x][3], hi);
+                bf16_terms<NT>(p[0], p[1], lo);
+                bf16_terms<NT>(p[2], p[3], hi);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
-                    *(v2w *) (lds + F::OP + t * F::P + lc_col<C>(16 * it[x] + m, 2 * jt[x] + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
+                    *(v2w *) (lds + F::OP + t * F::P + lc_score(i, 2 * jt + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
             }
             // S^T q
-            v4f o[F::IT][2];
-#pragma unroll
-            for (int i = 0; i < F::IT; i++) o[i][0] = o[i][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            v4f o[2][2] = {};
             if (live) {
 #pragma unroll
                 for (int kb = 0; kb < F::KB; kb++) {
@@ -546,40 +611,43 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                             for (int n = 0; n < NT; n++) sx[u][n][i] = t[n];
                         }
 #pragma unroll
-                    for (int i = 0; i < F::IT; i++) {
+                    for (int i = 0; i < 2; i++) {
                         v4w qx[NT];
 #pragma unroll
-                        for (int t = 0; t < NT; t++) qx[t] = *(const v4w *) (lds + F::OQ + t * F::QK + lc_row<DK>(16 * i + m, 4 * kb + g));
+                        for (int t = 0; t < NT; t++) qx[t] = *(const v4w *) (lds + buf + F::OQ + t * F::QK + lc_row<DK>(16 * i + m, 4 * kb + g));
                         o[i][0] = mfma_terms<NT, NT, NT>(sx[0], qx, o[i][0]);
                         o[i][1] = mfma_terms<NT, NT, NT>(sx[1], qx, o[i][1]);
                     }
                 }
             }
-            if (t0 + C < part.len) load(t0 + C);       // (here the scores' and S^T q's registers are free)
+            if constexpr (!F::DMA) {
+                if (t0 + C < part.len) load(t0 + C);       // (here the scores' and S^T q's registers are free)
+            }
             __syncthreads();                   // the scores
             if (live) {
+                load_v();
+                float odd = 0.f;               // NaN with a non-finite v (times 0)
 #pragma unroll
-                for (int i = 0; i < F::IT; i++) {
-                    const float e = eG[16 * i + m];
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t y = vx[u][0][i];
+                        odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, y), v2b{}, odd, false);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float e = eG[even][16 * i + m];
                     o[i][0] *= e;
                     o[i][1] *= e;
                 }
-                if (!odd) {
+                if (__ballot(odd != odd) == 0) {
 #pragma unroll
-                    for (int jb = 0; jb < F::JB; jb++) {
-                        v4w vx[2][NT];
+                    for (int i = 0; i < 2; i++) {
+                        v4w px[NT];
 #pragma unroll
-                        for (int u = 0; u < 2; u++)
-#pragma unroll
-                            for (int t = 0; t < NT; t++) vx[u][t] = lc_transposed<F::COLS>(lds + F::OV + t * F::V, 32 * jb + 8 * g, w, u, m);
-#pragma unroll
-                        for (int i = 2 * jb; i < F::IT; i++) {
-                            v4w px[NT];
-#pragma unroll
-                            for (int t = 0; t < NT; t++) px[t] = *(const v4w *) (lds + F::OP + t * F::P + lc_col<C>(16 * i + m, 4 * jb + g));
-                            o[i][0] = mfma_terms<NT, NT, NT>(vx[0], px, o[i][0]);
-                            o[i][1] = mfma_terms<NT, NT, NT>(vx[1], px, o[i][1]);
-                        }
+                        for (int t = 0; t < NT; t++) px[t] = *(const v4w *) (lds + F::OP + t * F::P + lc_score(16 * i + m, g));
+                        o[i][0] = mfma_terms<NT, NT, NT>(vx[0], px, o[i][0]);
+                        o[i][1] = mfma_terms<NT, NT, NT>(vx[1], px, o[i][1]);
                     }
                 } else {
                     auto sum = [&](int at, int size) {
@@ -587,22 +655,24 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                         for (int n = 0; n < NT; n++) f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size) << 16);
                         return f;
                     };
-                    for (int i = 0; i < F::IT; i++)
-                        for (int j = 0; j <= 16 * i + m; j++) {
-                            const float p = sum(F::OP + lc_col<C>(16 * i + m, j >> 3) + 2 * (j & 7), F::P);
-                            for (int u = 0; u < 2; u++)
-                                for (int r = 0; r < 4; r++) {
-                                    const float v = sum(F::OV + lc_row<F::COLS>(j, 4 * w + g) + 8 * u + 2 * r, F::V);
-                                    // (the index is not a constant: written out for each of the tiles)
+                    for (int j = 0; j <= 16 + m; j++) {
 #pragma unroll
-                                    for (int ii = 0; ii < F::IT; ii++)
-                                        if (ii == i) o[ii][u][r] = __fmaf_rn(p, v, o[ii][u][r]);
+                        for (int i = 0; i < 2; i++) {
+                            if (j > 16 * i + m) continue;
+                            const float p = sum(F::OP + lc_score(16 * i + m, j >> 3) + 2 * (j & 7), F::P);
+#pragma unroll
+                            for (int u = 0; u < 2; u++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++) {
+                                    const float v = sum(buf + F::OV + lc_row<F::COLS>(j, 4 * w + g) + 8 * u + 2 * r, F::V);
+                                    o[i][u][r] = __fmaf_rn(p, v, o[i][u][r]);
                                 }
                         }
+                    }
                 }
                 // 8 columns of a token
 #pragma unroll
-                for (int i = 0; i < F::IT; i++) {
+                for (int i = 0; i < 2; i++) {
                     const int t = t0 + 16 * i + m, c = c0 + LC_WCOLS * w + 8 * g;
                     if (t < part.len && c < a.dv) {
                         char * p = a.out + ((int64_t) (part.t0 + t) * a.n_v * a.dv + (int64_t) h * a.dv + c) * F::ES;
@@ -618,64 +688,57 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     }
                 }
             }
+        } else {
+            load_v();
         }
         // the state at the chunk's end
         if (live) {
-            v4w vx[F::JB][2][3];
+            v4w vw[2][3];
+            float wt[8];
 #pragma unroll
-            for (int jb = 0; jb < F::JB; jb++) {
-                float wt[8];
+            for (int i = 0; i < 8; i++) wt[i] = wG[even][8 * g + i];
 #pragma unroll
-                for (int i = 0; i < 8; i++) wt[i] = wG[32 * jb + 8 * g + i];
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    v4w vt[NT];
+                for (int i = 0; i < 4; i++) {
+                    float lo = 0.f, hi = 0.f;
 #pragma unroll
-                    for (int t = 0; t < NT; t++) vt[t] = lc_transposed<F::COLS>(lds + F::OV + t * F::V, 32 * jb + 8 * g, w, u, m);
+                    for (int t = NT - 1; t >= 0; t--) { lo += bf16_lo(vx[u][t][i]); hi += bf16_hi(vx[u][t][i]); }
+                    uint32_t t3[3];
+                    bf16_terms<3>(lo * wt[2 * i], hi * wt[2 * i + 1], t3);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float lo = 0.f, hi = 0.f;
-#pragma unroll
-                        for (int t = NT - 1; t >= 0; t--) { lo += bf16_lo(vt[t][i]); hi += bf16_hi(vt[t][i]); }
-                        uint32_t t3[3];
-                        bf16_terms<3>(lo * wt[2 * i], hi * wt[2 * i + 1], t3);
-#pragma unroll
-                        for (int t = 0; t < 3; t++) vx[jb][u][t][i] = t3[t];
-                    }
+                    for (int t = 0; t < 3; t++) vw[u][t][i] = t3[t];
                 }
-            }
             // (TG row tiles at a time: a sum's products are 2 TG MFMAs apart)
             constexpr int TG = 4;
 #pragma unroll
             for (int t0g = 0; t0g < F::KT; t0g += TG) {
+                v4w kx[TG][NT];
+#pragma unroll
+                for (int t = 0; t < TG; t++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        kx[t][n] = lc_transposed<DK>(lds + buf + F::OK + n * F::QK, 8 * g, (t0g + t) >> 1, t & 1, m);
 #pragma unroll
                 for (int t = t0g; t < t0g + TG; t++) { S[t][0] *= cend; S[t][1] *= cend; }
 #pragma unroll
-                for (int jb = 0; jb < F::JB; jb++) {
-                    v4w kx[TG][NT];
+                for (int d = 2; d >= 0; d--)
 #pragma unroll
-                    for (int t = 0; t < TG; t++)
+                    for (int n = 0; n < NT && n <= d; n++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
-                            kx[t][n] = lc_transposed<DK>(lds + F::OK + n * F::QK, 32 * jb + 8 * g, (t0g + t) >> 1, t & 1, m);
+                        for (int t = 0; t < TG; t++)
 #pragma unroll
-                    for (int d = 2; d >= 0; d--)
-#pragma unroll
-                        for (int n = 0; n < NT && n <= d; n++)
-#pragma unroll
-                            for (int t = 0; t < TG; t++)
-#pragma unroll
-                                for (int u = 0; u < 2; u++) S[t0g + t][u] = mfma_bf16(kx[t][n], vx[jb][u][d - n], S[t0g + t][u]);
-                }
+                            for (int u = 0; u < 2; u++) S[t0g + t][u] = mfma_bf16(kx[t][n], vw[u][d - n], S[t0g + t][u]);
             }
         }
-        __syncthreads();
+        if constexpr (!F::DMA) __syncthreads();
     }
     if constexpr (STATES) {
-        const size_t at = (size_t) part.index * a.n_v + h;
-        float * up = x.U + at * hs;
-        each([&](v4f & s, int r, size_t e) { up[e] = s[r]; });
-        if (tid == 0 && cb == 0) x.G[at] = total;
+#pragma unroll
+        for (int t = 0; t < F::KT; t++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) in_u(part.index, t, u) = S[t][u];
+        if (tid == 0 && cb == 0) x.G[(size_t) part.index * a.n_v + h] = total;
     } else if (part.after == 0 && part.slot >= 0) {
         float * so = a.s_out + part.slot * per + h * hs;
         each([&](v4f & s, int r, size_t e) { so[e] = s[r]; });
@@ -687,18 +750,25 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 constexpr int LJ_AHEAD = 4;
 
 __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
-    __shared__ int32_t sh[12];
+    __shared__ int32_t sh[14];
     const la_args & a = x.a;
-    const int64_t hs = (int64_t) a.dk * a.dv, per = hs * a.n_v;
-    const int blocks = (int) ((hs / 4 + LA_THREADS - 1) / LA_THREADS);
+    const int blocks = (x.US / 4 + LA_THREADS - 1) / LA_THREADS;
     const int eb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.n_v;
     const lc_part part = find_part(x, blockIdx.x / blocks / a.n_v, false, LA_THREADS, sh);
     if (part.b < 0 || part.before > 0 || part.after == 0) return;
-    const int64_t e = 4 * ((int64_t) eb * LA_THREADS + threadIdx.x);
-    if (e >= hs) return;
+    const int e = eb * LA_THREADS + threadIdx.x;
+    if (4 * e >= x.US) return;
     v4f s{0.f, 0.f, 0.f, 0.f};
-    if (part.slot >= 0 && a.s_in) s = *(const v4f *) (a.s_in + part.slot * per + h * hs + e);
-    float * up = x.U + ((int64_t) part.index * a.n_v + h) * hs + e;
+    if (part.slot >= 0 && a.s_in) {
+        const int lane = e & 63, m = lane & 15, g = lane >> 4, u = e >> 6 & 1, t = (e >> 7) % x.KT, w = (e >> 7) / x.KT;
+        const int col = LC_WCOLS * w + 8 * (m >> 2) + 4 * u + (m & 3), row = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+        const float * s0 = a.s_in + ((int64_t) part.slot * a.n_v + h) * a.dk * a.dv + col;
+        if (col < a.dv && row < a.dk)              // (dk is a multiple of 16)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[r] = s0[(int64_t) (row + r) * a.dv];
+    }
+    const int64_t per = (int64_t) x.US * a.n_v;
+    float * up = x.U + ((int64_t) part.index * a.n_v + h) * x.US + 4 * (int64_t) e;
     const double * gp = x.G + (int64_t) part.index * a.n_v + h;
     for (int p0 = 0; p0 < part.after; p0 += LJ_AHEAD) {
         v4f u[LJ_AHEAD];
@@ -752,7 +822,7 @@ int check_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, in
 
 struct lc_plan {
     bool    step;                      // token by token
-    int32_t NT, DK, NW, ct, L;
+    int32_t NT, DK, NW, ct, L, US;
     int64_t parts;                     // blocks along the tokens, at most
     size_t  off_g, bytes;
 };
@@ -760,13 +830,15 @@ struct lc_plan {
 template <int NT> int per_cu(int DK, int NW) {
     if (DK == 64) return NW == 2 ? lc_cfg<NT, 64, 2>::PER_CU : lc_cfg<NT, 64, 4>::PER_CU;
     if (DK == 128) return NW == 2 ? lc_cfg<NT, 128, 2>::PER_CU : lc_cfg<NT, 128, 4>::PER_CU;
-    return NW == 2 ? lc_cfg<NT, 256, 2>::PER_CU : lc_cfg<NT, 256, 4>::PER_CU;
+    if constexpr (NT < 3) if (NW == 2) return lc_cfg<NT, 256, 2>::PER_CU;
+    return lc_cfg<NT, 256, 4>::PER_CU;
 }
 
-// Parts of a sequence: as many as fill the CUs once, so that no workgroup waits for another (4096 tokens of 48 heads
-// in 6 parts, 288 workgroups: 189 us where 5 parts take 100), but no shorter than LC_MIN_PART tokens: a part costs its
-// state's way through the workspace and a second pass over its k and v.
-constexpr int64_t LC_CUS = 256, LC_MIN_PART = 256;
+// Parts of a sequence: as many as fill the CUs once with two waves a SIMD, so that no workgroup waits for another (4096
+// bf16 tokens of 48 heads of 128: 107 us in 10 parts, 125 in 5, 130 in 16, three waves a SIMD: a part's state goes
+// through the workspace three times), but no shorter than LC_MIN_PART tokens: a part costs a second pass over its k and v
+// (two f32 sequences of 509: 83 us with parts of 128, 97 of 256).
+constexpr int64_t LC_CUS = 256, LC_MIN_PART = 128;
 
 lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
     lc_plan p{};
@@ -775,11 +847,11 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     p.DK = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
     p.step = max_len <= LC_STEP_MAX;
     if (p.step) return p;
-    p.NW = dv <= 2 * LC_WCOLS ? 2 : 4;
+    p.NW = dv <= 2 * LC_WCOLS && (p.NT < 3 || p.DK < 256) ? 2 : 4;         // (256 rows of F32 for two waves are spilled)
     p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
-    const int64_t longest = std::min<int64_t>(max_len, n_tok), C = p.NT == 1 && p.NW == 4 ? 64 : 32;
-    const int64_t room = LC_CUS * (p.NT == 1 ? per_cu<1>(p.DK, p.NW) : p.NT == 2 ? per_cu<2>(p.DK, p.NW) : per_cu<3>(p.DK, p.NW)) /
-                         (n_v * p.ct);
+    const int64_t longest = std::min<int64_t>(max_len, n_tok), C = LC_C;
+    const int per = p.NT == 1 ? per_cu<1>(p.DK, p.NW) : p.NT == 2 ? per_cu<2>(p.DK, p.NW) : per_cu<3>(p.DK, p.NW);
+    const int64_t room = LC_CUS * std::min(per, 8 / p.NW) / (n_v * p.ct);
     // a sequence's last part is half of one on average
     const int64_t whole = std::max<int64_t>(1, room - n_seq / 2);
     const int64_t L = (std::max<int64_t>(LC_MIN_PART, (n_tok + whole - 1) / whole) + C - 1) / C * C;
@@ -787,7 +859,8 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     if (L < longest) {
         p.L = (int32_t) L;
         p.parts = n_seq + n_tok / L;
-        p.off_g = ((size_t) p.parts * n_v * dk * dv * sizeof(float) + 255) / 256 * 256;
+        p.US = p.DK * LC_WCOLS * p.NW * p.ct;
+        p.off_g = (size_t) p.parts * n_v * p.US * sizeof(float);
         p.bytes = p.off_g + (size_t) p.parts * n_v * sizeof(double);
     }
     return p;
@@ -799,7 +872,7 @@ int launch_chunks(const lc_args & x, const lc_plan & p, hipStream_t s) {
     if (p.L > 0) {
         hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, true>), grid, blk, 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
-        const int64_t blocks = ((int64_t) x.a.dk * x.a.dv / 4 + LA_THREADS - 1) / LA_THREADS;
+        const int64_t blocks = (x.US / 4 + LA_THREADS - 1) / LA_THREADS;
         hipLaunchKernelGGL(k_linear_join, dim3((unsigned) (p.parts * x.a.n_v * blocks)), dim3(LA_THREADS), 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
     }
@@ -810,7 +883,8 @@ template <int NT>
 int launch_type(const lc_args & x, const lc_plan & p, hipStream_t s) {
     if (p.DK == 64)  return p.NW == 2 ? launch_chunks<NT, 64, 2>(x, p, s) : launch_chunks<NT, 64, 4>(x, p, s);
     if (p.DK == 128) return p.NW == 2 ? launch_chunks<NT, 128, 2>(x, p, s) : launch_chunks<NT, 128, 4>(x, p, s);
-    return p.NW == 2 ? launch_chunks<NT, 256, 2>(x, p, s) : launch_chunks<NT, 256, 4>(x, p, s);
+    if constexpr (NT < 3) if (p.NW == 2) return launch_chunks<NT, 256, 2>(x, p, s);
+    return launch_chunks<NT, 256, 4>(x, p, s);
 }
 
 }  // namespace
@@ -862,9 +936,9 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         a.type = q->type; a.n_seq = n_seq; a.max_len = max_len; a.n_slots = n_slots; a.n_tok = (int32_t) n_tok;
         a.n_k = (int32_t) q->ne[1]; a.n_v = (int32_t) n_v; a.rep = a.n_v / a.n_k; a.dk = (int32_t) dk; a.dv = (int32_t) dv;
         if (!pl.step) {
-            if (pl.parts * n_v * std::max<int64_t>(pl.ct, dk * dv / (4 * LA_THREADS) + 1) > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
+            if (pl.parts * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1) > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
             a.ct = pl.ct;
-            const lc_args x{a, pl.L, (float *) ws, (double *) ((char *) ws + pl.off_g)};
+            const lc_args x{a, pl.L, pl.DK / 16, pl.US, (float *) ws, (double *) ((char *) ws + pl.off_g)};
             return pl.NT == 1 ? launch_type<1>(x, pl, as_stream(stream)) : pl.NT == 2 ? launch_type<2>(x, pl, as_stream(stream))
                                                                                       : launch_type<3>(x, pl, as_stream(stream));
         }
