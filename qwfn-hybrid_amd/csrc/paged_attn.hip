@@ -14,7 +14,10 @@
 // workgroup; the parts of the others go to the workspace as (O, M, l) and
 // k_paged_merge joins them in the order of the runs, so results repeat bit for bit.
 // The KV heads and row groups of one run are blocks next to each other on one XCD:
-// the cache lines that two heads share come from one L2.
+// the cache lines that two heads share come from one L2, and so do the rows that more
+// than 16 query rows need again (a workgroup of 32 query rows leaves one wave a SIMD:
+// 3 tokens of 8 requests with 12295 keys took 62 us that way, 55 this way, and 25 and 19
+// at 2 requests with 3000 keys).
 //
 // Inside a workgroup the 4 waves take every fourth tile of the run, each on its
 // own: no barrier, and no wave waits for another's data. A tile's rows come by LDS
@@ -54,7 +57,7 @@ constexpr int PA_THREADS = PA_WAVES * 64;
 constexpr int PA_TILE = 32;            // keys of a tile
 constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
 constexpr int PA_LEAD = 8;             // tiles that a request counts more than it has
-constexpr int PA_CUS = 256;            // two workgroups a CU of one row tile, one of two (registers)
+constexpr int PA_CUS = 256;            // two workgroups a CU (registers)
 constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
@@ -94,7 +97,7 @@ struct pa_args {
     uint32_t *      status;
 };
 
-template <int D, int NS> struct pa_cfg {
+template <int D> struct pa_cfg {
     static constexpr int NBLK = D / QK;
     static constexpr int SEG = NBLK * QBLOCK;            // bytes of a head row
     // a row goes to LDS in units of a DMA lane, 16 bytes where a head row is whole ones; UPR of them a row
@@ -105,11 +108,11 @@ template <int D, int NS> struct pa_cfg {
     static constexpr int UMUL = 65536 / UPR + 1;         // i / UPR = i UMUL >> 16 for i < UNITS
     static constexpr int ROWS = PA_TILE * LS;            // of a tensor's tile in LDS
     static constexpr int OROW = D + 4;                   // floats of a row of O in LDS: rows from other banks
-    // of a wave: NS stages of K and V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
-    static constexpr int OA = NS * 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
+    // of a wave: a tile of K and of V, row addresses, table entries (a lane each), each key's largest dv, K's and V's scales
+    static constexpr int OA = 2 * ROWS, OE = OA + PA_TILE * 8, OM = OE + 256, OS = OM + 2 * PA_TILE;
     static constexpr int WAVE = OS + 2 * NBLK * PA_TILE * 2;
-    static constexpr int IMG = 16 * NBLK * 64;           // the query windows of a row tile
-    static constexpr int QI = NBLK / 2;                  // 4-value groups a thread quantises, a row tile
+    static constexpr int IMG = 16 * NBLK * 64;           // the query windows
+    static constexpr int QI = NBLK / 2;                  // 4-value groups a thread quantises
     static_assert(IMG + 16 * NBLK * 4 <= ROWS && WAVE >= 16 * OROW * 4 && WAVE % 16 == 0, "the query images fit, and a wave's O in its part");
     static_assert((UNITS - 1) * (UMUL * UPR - 65536) < 65536, "the division is exact");
     static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
@@ -323,15 +326,12 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
     return r;
 }
 
-template <int D, int RT>
-__global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
-    // one row tile: one stage a wave, two waves a SIMD; two: one wave a SIMD, and two stages (head size 128 would
-    // have more DMAs in flight than the counter of a wave holds)
-    constexpr int NS = RT == 2 && 4 * pa_cfg<D, 1>::DMAS + 1 < 63 ? 2 : 1;
-    using C = pa_cfg<D, NS>;
-    constexpr int NBLK = C::NBLK, ND = C::DMAS, ROWS = 16 * RT;
+template <int D>
+__global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
+    using C = pa_cfg<D>;
+    constexpr int NBLK = C::NBLK, ND = C::DMAS;
     __shared__ __attribute__((aligned(16))) uint8_t lds[PA_WAVES * C::WAVE];
-    __shared__ float2 ml[PA_WAVES][ROWS];
+    __shared__ float2 ml[PA_WAVES][16];
     __shared__ int32_t sh[PA_WAVES + 3];
     const int tid = threadIdx.x;
     int lane = tid & 63, ln = lane & 15, lg = lane >> 4;
@@ -349,10 +349,8 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
     uint16_t * const kscl = (uint16_t *) (my + C::OS);
     uint16_t * const vscl = kscl + NBLK * PA_TILE;
     const uint32_t at_k = pa_lds(my), at_v = at_k + C::ROWS, at_e = at_k + C::OE;
-    // the query image of row tile rt, at image + rt IMG_STEP: with one stage in wave rt's V (sent for when the image is
-    // read), with two in the first wave's second stage (K's part, V's part)
-    constexpr int IMG_STEP = NS == 1 ? C::WAVE : C::ROWS;
-    uint8_t * const image = lds + (NS == 1 ? C::ROWS : 2 * C::ROWS);
+    // the query image: in the first wave's V, sent for when the image is read
+    uint8_t * const image = lds + C::ROWS;
     const char * kh = a.k + (size_t) kvh * a.nb2;
     const char * vh = a.v + (size_t) kvh * a.nb2;
     const uint64_t v_k = (uint64_t) (vh - kh);
@@ -412,19 +410,17 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         auto send_v = [&](uint32_t at) { units([&](int i, int) { pa_dma_plus<C::UB>(from[i], v_k, at + 64 * C::UB * i); }); };
         __syncthreads();                                   // the LDS of the part before is read
         // query values on their way: 8 lanes a q8_0 block
-        float qx[RT][C::QI][4];
+        float qx[C::QI][4];
         const int sub = tid & 7;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int i = 0; i < C::QI; i++) {
-                const int x = (tid >> 3) + 32 * i, r = x / NBLK, blk = x % NBLK;
-                int rr = ROWS * rg + 16 * rt + r;
-                rr = rr < a.R ? rr : a.R - 1;
-                const uint32_t t = div_by((uint32_t) rr, a.f_rep), h = (uint32_t) (kvh * a.rep + rr) - t * (uint32_t) a.rep;
-                load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 + (size_t) (blk * QK + sub * 4) * es,
-                      a.type, qx[rt][i]);
-            }
+        for (int i = 0; i < C::QI; i++) {
+            const int x = (tid >> 3) + 32 * i, r = x / NBLK, blk = x % NBLK;
+            int rr = 16 * rg + r;
+            rr = rr < a.R ? rr : a.R - 1;
+            const uint32_t t = div_by((uint32_t) rr, a.f_rep), h = (uint32_t) (kvh * a.rep + rr) - t * (uint32_t) a.rep;
+            load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 + (size_t) (blk * QK + sub * 4) * es,
+                  a.type, qx[i]);
+        }
         uint32_t live = 0, live_next = 0;                  // the tile's keys that exist
         if (wave < nt) {
             entries(wave);
@@ -433,94 +429,58 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         }
         // (they have come with the entries: a wait for them behind the rows' DMA would wait for the rows too)
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int i = 0; i < C::QI; i++)
 #pragma unroll
-            for (int i = 0; i < C::QI; i++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) asm volatile("" : "+v"(qx[rt][i][k]));
+            for (int k = 0; k < 4; k++) asm volatile("" : "+v"(qx[i][k]));
         if (wave < nt) {
             wave_lds_sync();
-            if constexpr (NS == 1) {
-                send_k(at_k);
-                entries(wave + PA_WAVES);
-            } else {
-                entries(wave + PA_WAVES);
-                send_k(at_k);
-                send_v(at_v);
-            }
+            send_k(at_k);
+            entries(wave + PA_WAVES);
         }
         // the query image: rows requantised, each block at its place of a window that is zero elsewhere
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int i = 0; i < C::QI; i++)
-                *(uint2 *) (image + rt * IMG_STEP + ((tid >> 3) + 32 * i) * 64 + sub * 8) = make_uint2(0u, 0u);
+        for (int i = 0; i < C::QI; i++)
+            *(uint2 *) (image + ((tid >> 3) + 32 * i) * 64 + sub * 8) = make_uint2(0u, 0u);
         wave_lds_sync();                                   // a block's 8 lanes zero its window, then write into it
+        float * const dql = (float *) (image + C::IMG);
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            uint8_t * const img = image + rt * IMG_STEP;
-            float * dql = (float *) (img + C::IMG);
-#pragma unroll
-            for (int i = 0; i < C::QI; i++) {
-                const int x = (tid >> 3) + 32 * i, blk = x % NBLK;
-                uint16_t d16;
-                float dq;
-                const uint32_t q4 = dev::q8_quantize_lane4(qx[rt][i], a.x86 != 0, &d16, &dq);
-                uint16_t * qp = (uint16_t *) (img + x * 64 + (QBLOCK * blk + 2) % 16 + sub * 4);
-                qp[0] = (uint16_t) q4;
-                qp[1] = (uint16_t) (q4 >> 16);
-                if (sub == 0) dql[x] = dq;
-            }
+        for (int i = 0; i < C::QI; i++) {
+            const int x = (tid >> 3) + 32 * i, blk = x % NBLK;
+            uint16_t d16;
+            float dq;
+            const uint32_t q4 = dev::q8_quantize_lane4(qx[i], a.x86 != 0, &d16, &dq);
+            uint16_t * qp = (uint16_t *) (image + x * 64 + (QBLOCK * blk + 2) % 16 + sub * 4);
+            qp[0] = (uint16_t) q4;
+            qp[1] = (uint16_t) (q4 >> 16);
+            if (sub == 0) dql[x] = dq;
         }
         __syncthreads();
-        v4i qw[RT][NBLK];
-        float dq[RT][NBLK];                                // dq c to 22 bits: PA_IBIAS dq is exact
+        v4i qw[NBLK];
+        float dq[NBLK];                                    // dq c to 22 bits: PA_IBIAS dq is exact
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const uint8_t * img = image + rt * IMG_STEP;
-#pragma unroll
-            for (int blk = 0; blk < NBLK; blk++) {
-                qw[rt][blk] = *(const v4i *) (img + (ln * NBLK + blk) * 64 + 16 * lg);
-                const uint32_t x = __builtin_bit_cast(uint32_t, ((const float *) (img + C::IMG))[ln * NBLK + blk] * a.c);
-                dq[rt][blk] = __builtin_bit_cast(float, (x + 2u) & ~3u);
-            }
+        for (int blk = 0; blk < NBLK; blk++) {
+            qw[blk] = *(const v4i *) (image + (ln * NBLK + blk) * 64 + 16 * lg);
+            const uint32_t x = __builtin_bit_cast(uint32_t, dql[ln * NBLK + blk] * a.c);
+            dq[blk] = __builtin_bit_cast(float, (x + 2u) & ~3u);
         }
         __syncthreads();
 
-        v4f O[RT][NBLK][2] = {};
-        float M[RT], l[RT];
-        int32_t limit[RT];                                 // the lane's row sees keys below it
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            M[rt] = -INFINITY;
-            l[rt] = 0.f;
-            limit[rt] = n - a.T + (int32_t) div_by((uint32_t) (ROWS * rg + 16 * rt + ln), a.f_rep) + 1;
-        }
-        if (NS == 1 && wave < nt) {
+        v4f O[NBLK][2] = {};
+        float M = -INFINITY, l = 0.f;
+        // the lane's row sees keys below it
+        const int32_t limit = n - a.T + (int32_t) div_by((uint32_t) (16 * rg + ln), a.f_rep) + 1;
+        if (wave < nt) {
             pa_wait_lds();
             send_v(at_v);
         }
-        // in flight at the top, in this order: with one stage K of the tile, the entries of the next, V of the tile;
-        // with two the entries of the next tile, K and V of this one
-        int stage = 0;                                     // bytes
+        // in flight at the top, in this order: K of the tile, the entries of the next, V of the tile
         for (int t = wave; t < nt; t += PA_WAVES) {
             // the lane's places are computed anew in every tile: kept over the loop they cost 40 registers, spilled
             asm volatile("" : "+v"(lane), "+v"(ln), "+v"(lg));
             const int32_t key0 = (run.off + t) * PA_TILE;
             const bool masked = live != 0xffffffffu || key0 + PA_TILE > n - a.T + 1;
-            if constexpr (NS == 1) {
-                pa_wait<ND + 1>();
-            } else {
-                pa_wait<2 * ND>();
-                live_next = rows_of(t + PA_WAVES);
-                wave_lds_sync();
-                pa_wait_lds();
-                entries(t + 2 * PA_WAVES);
-                send_k(at_k + (2 * C::ROWS - stage));
-                send_v(at_v + (2 * C::ROWS - stage));
-                pa_wait<3 * ND + 1>();
-            }
-            const uint8_t * const kt = my + stage, * const vt = kt + C::ROWS;
+            pa_wait<ND + 1>();
+            const uint8_t * const kt = my, * const vt = kt + C::ROWS;
             {   // K's scales by block and key
                 const int key = lane & 31, half = lane >> 5;
 #pragma unroll
@@ -533,7 +493,7 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
 
             // S^T: lane (row ln, keys 16 u + 4 lg + r). An integer dot comes out of the MFMA on top of the bits of
             // PA_IBIAS, so it is PA_IBIAS + dot as a float, and one fused step makes dot dq of it.
-            float s[RT][2][4] = {};
+            float s[2][4] = {};
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const uint8_t * kl = kt + (16 * u + ln) * C::LS + 16 * lg;
@@ -541,29 +501,24 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                 for (int blk = 0; blk < NBLK; blk++) {
                     const v4i kw = *(const v4i *) (kl + 16 * pa_win(blk));
                     const uint2 dk = *(const uint2 *) (kscl + blk * PA_TILE + 16 * u + 4 * lg);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[rt][blk], v4i{PA_IBITS, PA_IBITS, PA_IBITS, PA_IBITS}, 0, 0, 0);
-                        const int d0 = d[0], d1 = d[1], d2 = d[2], d3 = d[3];
-                        const float f = dq[rt][blk], nb = -PA_IBIAS * f;
-                        s[rt][u][0] = fma_f16lo(dk.x, __fmaf_rn(__builtin_bit_cast(float, d0), f, nb), s[rt][u][0]);
-                        s[rt][u][1] = fma_f16hi(dk.x, __fmaf_rn(__builtin_bit_cast(float, d1), f, nb), s[rt][u][1]);
-                        s[rt][u][2] = fma_f16lo(dk.y, __fmaf_rn(__builtin_bit_cast(float, d2), f, nb), s[rt][u][2]);
-                        s[rt][u][3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), f, nb), s[rt][u][3]);
-                    }
+                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(kw, qw[blk], v4i{PA_IBITS, PA_IBITS, PA_IBITS, PA_IBITS}, 0, 0, 0);
+                    const int d0 = d[0], d1 = d[1], d2 = d[2], d3 = d[3];
+                    const float f = dq[blk], nb = -PA_IBIAS * f;
+                    s[u][0] = fma_f16lo(dk.x, __fmaf_rn(__builtin_bit_cast(float, d0), f, nb), s[u][0]);
+                    s[u][1] = fma_f16hi(dk.x, __fmaf_rn(__builtin_bit_cast(float, d1), f, nb), s[u][1]);
+                    s[u][2] = fma_f16lo(dk.y, __fmaf_rn(__builtin_bit_cast(float, d2), f, nb), s[u][2]);
+                    s[u][3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), f, nb), s[u][3]);
                 }
             }
-            if constexpr (NS == 1) {                       // the next tile's K
-                pa_wait<ND>();
-                live_next = rows_of(t + PA_WAVES);
-                wave_lds_sync();
-                pa_wait_lds();
-                send_k(at_k);
-                entries(t + 2 * PA_WAVES);
-            }
+            pa_wait<ND>();                                 // the next tile's K
+            live_next = rows_of(t + PA_WAVES);
+            wave_lds_sync();
+            pa_wait_lds();
+            send_k(at_k);
+            entries(t + 2 * PA_WAVES);
             // V's scales; its largest of each key and of the tile. One that is not finite counts as 0 here and in
             // the products, and is added by itself below.
-            pa_wait<(2 * NS - 1) * ND + 1>();
+            pa_wait<ND + 1>();
             uint32_t dmax = 0;
             bool odd = false;
             {
@@ -583,44 +538,41 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
             }
             dmax = umax_rows(umax_row(dmax));
             wave_lds_sync();
-            float p[RT][2][4];
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                uint32_t top_d = dmax;
-                if (masked) {
-                    top_d = 0;                             // of the keys that the row sees
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int k = 16 * u + 4 * lg + r;
-                            if (!(live >> k & 1) || key0 + k >= limit[rt]) s[rt][u][r] = -INFINITY;
-                            else top_d = max(top_d, (uint32_t) vtop[k]);
-                        }
-                    top_d = umax_halves(umax_rows(top_d));
-                }
-                float top = vmax(vmax(s[rt][0][0], s[rt][0][1]), vmax(s[rt][0][2], s[rt][0][3]));
-                top = vmax(top, vmax(vmax(s[rt][1][0], s[rt][1][1]), vmax(s[rt][1][2], s[rt][1][3])));
-                top = xmax_lanes16_32(top);
-                const int e = (int) (top_d >> 10) < 1 ? 1 : (int) (top_d >> 10);      // d < 2^(e - 14)
-                const float ref = top + (float) (e - 14 - PA_BIAS);
-                if (__ballot(ref > M[rt] + PA_SLACK)) {
-                    const float to = fmaxf(M[rt], ref);
-                    const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M[rt] - to);
-                    M[rt] = to;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int blk = 0; blk < NBLK; blk++) { O[rt][blk][0] *= f; O[rt][blk][1] *= f; }
-                }
-                const float m = M[rt] == -INFINITY ? 0.f : M[rt];
+            float p[2][4];
+            uint32_t top_d = dmax;
+            if (masked) {
+                top_d = 0;                                 // of the keys that the row sees
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        p[rt][u][r] = __builtin_amdgcn_exp2f(s[rt][u][r] - m);       // 2^-inf = 0
-                        l[rt] += p[rt][u][r];
+                        const int k = 16 * u + 4 * lg + r;
+                        if (!(live >> k & 1) || key0 + k >= limit) s[u][r] = -INFINITY;
+                        else top_d = max(top_d, (uint32_t) vtop[k]);
                     }
+                top_d = umax_halves(umax_rows(top_d));
             }
+            float top = vmax(vmax(s[0][0], s[0][1]), vmax(s[0][2], s[0][3]));
+            top = vmax(top, vmax(vmax(s[1][0], s[1][1]), vmax(s[1][2], s[1][3])));
+            top = xmax_lanes16_32(top);
+            const int e = (int) (top_d >> 10) < 1 ? 1 : (int) (top_d >> 10);      // d < 2^(e - 14)
+            const float ref = top + (float) (e - 14 - PA_BIAS);
+            if (__ballot(ref > M + PA_SLACK)) {
+                const float to = fmaxf(M, ref);
+                const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - to);
+                M = to;
+                l *= f;
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) { O[blk][0] *= f; O[blk][1] *= f; }
+            }
+            const float m = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[u][r] = __builtin_amdgcn_exp2f(s[u][r] - m);       // 2^-inf = 0
+                    l += p[u][r];
+                }
             // O^T: A lane (dims 2 ln + e of the block, keys 4 lg + r of both halves)
 #pragma unroll
             for (int blk = 0; blk < NBLK; blk++) {
@@ -636,103 +588,91 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
                 v4u a0, a1;
                 cvt_v8(av, a0, a1);
                 const v8h A0 = __builtin_bit_cast(v8h, a0), A1 = __builtin_bit_cast(v8h, a1);
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    v4u bh, bl;
-                    hilo(p[rt], dv, bh, bl);
-                    const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
-                    O[rt][blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[rt][blk][0], 0, 0, 0);
-                    O[rt][blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[rt][blk][1], 0, 0, 0);
-                    O[rt][blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[rt][blk][0], 0, 0, 0);
-                    O[rt][blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[rt][blk][1], 0, 0, 0);
-                }
+                v4u bh, bl;
+                hilo(p, dv, bh, bl);
+                const v8h H = __builtin_bit_cast(v8h, bh), L = __builtin_bit_cast(v8h, bl);
+                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, H, O[blk][0], 0, 0, 0);
+                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, H, O[blk][1], 0, 0, 0);
+                O[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, L, O[blk][0], 0, 0, 0);
+                O[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, L, O[blk][1], 0, 0, 0);
             }
             if (__builtin_expect(__ballot(odd) != 0, 0)) {
                 // blocks of V whose scale is not finite, for the rows that see their key
+                for (int k = 0; k < PA_TILE; k++) {
+                    const int from = (k >> 2 & 3) * 16 + ln;
+                    float pk = 0.f;
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-                    for (int k = 0; k < PA_TILE; k++) {
-                        const int from = (k >> 2 & 3) * 16 + ln;
-                        float pk = 0.f;
+                    for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int u = 0; u < 2; u++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const float y = __shfl(p[rt][u][r], from);
-                                if (k == 16 * u + (k & 12) + r) pk = y;
-                            }
-#pragma unroll
-                        for (int blk = 0; blk < NBLK; blk++) {
-                            const uint8_t * vb = vt + k * C::LS + QBLOCK * blk;
-                            const uint16_t d = *(const uint16_t *) vb;
-                            if ((d & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
-#pragma unroll
-                            for (int e2 = 0; e2 < 2; e2++)
-#pragma unroll
-                                for (int r = 0; r < 4; r++)
-                                    if (pk != 0.f)
-                                        O[rt][blk][e2][r] += pk * dev::f16_bits_to_f32(d) * (float) *(const int8_t *) (vb + 2 + 2 * (4 * lg + r) + e2);
+                        for (int r = 0; r < 4; r++) {
+                            const float y = __shfl(p[u][r], from);
+                            if (k == 16 * u + (k & 12) + r) pk = y;
                         }
+#pragma unroll
+                    for (int blk = 0; blk < NBLK; blk++) {
+                        const uint8_t * vb = vt + k * C::LS + QBLOCK * blk;
+                        const uint16_t d = *(const uint16_t *) vb;
+                        if ((d & 0x7fffu) < 0x7c00u || !(live >> k & 1)) continue;
+#pragma unroll
+                        for (int e2 = 0; e2 < 2; e2++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (pk != 0.f)
+                                    O[blk][e2][r] += pk * dev::f16_bits_to_f32(d) * (float) *(const int8_t *) (vb + 2 + 2 * (4 * lg + r) + e2);
                     }
+                }
             }
-            if constexpr (NS == 1) {
-                pa_wait_lds();
-                send_v(at_v);
-            } else {
-                stage = 2 * C::ROWS - stage;
-            }
+            pa_wait_lds();
+            send_v(at_v);
             live = live_next;
         }
         pa_wait<0>();
 
-        // the waves' parts meet in LDS, a row tile at a time: O[row][dim] of each
+        // the waves' parts meet in LDS: O[row][dim] of each
+        const float ls = sum_lanes16_32(l);
+        __syncthreads();
+        float * ob = (float *) (lds + wave * C::WAVE) + ln * C::OROW;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const float ls = sum_lanes16_32(l[rt]);
-            __syncthreads();
-            float * ob = (float *) (lds + wave * C::WAVE) + ln * C::OROW;
+        for (int blk = 0; blk < NBLK; blk++)
 #pragma unroll
-            for (int blk = 0; blk < NBLK; blk++)
+            for (int r = 0; r < 4; r += 2)
+                *(float4 *) (ob + QK * blk + 8 * lg + 2 * r) =
+                    make_float4(O[blk][0][r], O[blk][1][r], O[blk][0][r + 1], O[blk][1][r + 1]);
+        if (lg == 0) ml[wave][ln] = make_float2(M, ls);
+        __syncthreads();
+        const int r = tid >> 4, rr = 16 * rg + r;
+        float2 e[PA_WAVES];
+        float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-                for (int r = 0; r < 4; r += 2)
-                    *(float4 *) (ob + QK * blk + 8 * lg + 2 * r) =
-                        make_float4(O[rt][blk][0][r], O[rt][blk][1][r], O[rt][blk][0][r + 1], O[rt][blk][1][r + 1]);
-            if (lg == 0) ml[wave][ln] = make_float2(M[rt], ls);
-            __syncthreads();
-            const int r = tid >> 4, rr = ROWS * rg + 16 * rt + r;
-            float2 e[PA_WAVES];
-            float mm = -INFINITY, ll = 0.f;
+        for (int w = 0; w < PA_WAVES; w++) { e[w] = ml[w][r]; mm = fmaxf(mm, e[w].x); }
 #pragma unroll
-            for (int w = 0; w < PA_WAVES; w++) { e[w] = ml[w][r]; mm = fmaxf(mm, e[w].x); }
+        for (int w = 0; w < PA_WAVES; w++) {
+            e[w].x = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - mm);
+            ll += e[w].x * e[w].y;                         // a NaN stays one
+        }
+        if (rr < a.R) {
+            const size_t elem = element(b, rr), part = ((size_t) (g + b) * a.nh_kv + kvh) * a.R + rr;
+            const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
 #pragma unroll
-            for (int w = 0; w < PA_WAVES; w++) {
-                e[w].x = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - mm);
-                ll += e[w].x * e[w].y;                     // a NaN stays one
-            }
-            if (rr < a.R) {
-                const size_t elem = element(b, rr), part = ((size_t) (g + b) * a.nh_kv + kvh) * a.R + rr;
-                const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
+            for (int i = 0; i < D / 64; i++) {
+                const int d0 = 4 * (tid & 15) + 64 * i;
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < D / 64; i++) {
-                    const int d0 = 4 * (tid & 15) + 64 * i;
-                    float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int w = 0; w < PA_WAVES; w++) {
-                        const float4 x = *(const float4 *) ((const float *) (lds + w * C::WAVE) + r * C::OROW + d0);
-                        if (e[w].x != 0.f) {
-                            o[0] += e[w].x * x.x; o[1] += e[w].x * x.y; o[2] += e[w].x * x.z; o[3] += e[w].x * x.w;
-                        }
-                    }
-                    if (whole) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) o[k] *= inv;
-                        finish4(a, elem + d0, o);
-                    } else {
-                        *(float4 *) (a.part_o + part * D + d0) = make_float4(o[0], o[1], o[2], o[3]);
+                for (int w = 0; w < PA_WAVES; w++) {
+                    const float4 x = *(const float4 *) ((const float *) (lds + w * C::WAVE) + r * C::OROW + d0);
+                    if (e[w].x != 0.f) {
+                        o[0] += e[w].x * x.x; o[1] += e[w].x * x.y; o[2] += e[w].x * x.z; o[3] += e[w].x * x.w;
                     }
                 }
-                if (!whole && (tid & 15) == 0) a.part_ml[part] = make_float2(mm, ll);
+                if (whole) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) o[k] *= inv;
+                    finish4(a, elem + d0, o);
+                } else {
+                    *(float4 *) (a.part_o + part * D + d0) = make_float4(o[0], o[1], o[2], o[3]);
+                }
             }
+            if (!whole && (tid & 15) == 0) a.part_ml[part] = make_float2(mm, ll);
         }
         if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(g, (run.pos + tiles - 1) / run.per);
         run.left -= nt;
@@ -748,10 +688,10 @@ __global__ __launch_bounds__(PA_THREADS, 3 - RT) void k_paged_attn(pa_args a) {
         if (n != clip_len(a, n) && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
         if (n > 0) continue;
         const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = tid >> 4; r < ROWS; r += PA_THREADS / 16)
-            if (ROWS * rg + r < a.R)
+        for (int r = tid >> 4; r < 16; r += PA_THREADS / 16)
+            if (16 * rg + r < a.R)
 #pragma unroll
-                for (int i = 0; i < D / 64; i++) store4(a.dst + (element(b, ROWS * rg + r) + 4 * (tid & 15) + 64 * i) * es, a.type, z);
+                for (int i = 0; i < D / 64; i++) store4(a.dst + (element(b, 16 * rg + r) + 4 * (tid & 15) + 64 * i) * es, a.type, z);
         if (hr == 0 && tid == 0) a.span[b] = make_int2(0, 0);
     }
 }
@@ -835,21 +775,19 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
 // ---------------------------------------------------------------- host
 
 struct pa_plan {
-    int32_t RT, groups, runs;          // row tiles of a workgroup, row groups
+    int32_t groups, runs;              // row groups
     size_t  off_o, off_ml, bytes;
 };
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Runs: as many as fill the CUs (two workgroups each, or one of two row tiles), whole rounds of the 8 XCDs; no
-// more than the longest requests could need.
+// Runs: as many as fill the CUs, whole rounds of the 8 XCDs; no more than the longest requests could need.
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    p.RT = R > 16 ? 2 : 1;
-    p.groups = (int32_t) ((R + 16 * p.RT - 1) / (16 * p.RT));
+    p.groups = (int32_t) ((R + 15) / 16);
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
-    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(PA_CUS * (3 - p.RT) / (nh_kv * p.groups), most));
+    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * PA_CUS / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
     p.off_o = round256((size_t) n_seq * sizeof(int2));
     p.off_ml = p.off_o + round256(parts * D * sizeof(float));
@@ -889,8 +827,7 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
 template <int D>
 int launch_paged(const pa_args & a, const pa_plan & p, hipStream_t s) {
     const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * p.groups));
-    if (p.RT == 1) hipLaunchKernelGGL((k_paged_attn<D, 1>), grid, dim3(PA_THREADS), 0, s, a);
-    else           hipLaunchKernelGGL((k_paged_attn<D, 2>), grid, dim3(PA_THREADS), 0, s, a);
+    hipLaunchKernelGGL(k_paged_attn<D>, grid, dim3(PA_THREADS), 0, s, a);
     if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
     // the requests' parts: on average runs / n_seq each, with long requests among short ones more
     const int64_t units = (int64_t) a.n_seq * a.nh_kv * a.R * (D / 64);
