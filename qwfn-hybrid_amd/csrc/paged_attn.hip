@@ -510,15 +510,20 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                     s[u][3] = fma_f16hi(dk.y, __fmaf_rn(__builtin_bit_cast(float, d3), f, nb), s[u][3]);
                 }
             }
-            pa_wait<ND>();                                 // the next tile's K
-            live_next = rows_of(t + PA_WAVES);
-            wave_lds_sync();
-            pa_wait_lds();
-            send_k(at_k);
-            entries(t + 2 * PA_WAVES);
+            const bool more = t + PA_WAVES < nt;
+            pa_wait<ND>();
+            if (more) {                                    // the next tile's K
+                live_next = rows_of(t + PA_WAVES);
+                wave_lds_sync();
+                pa_wait_lds();
+                send_k(at_k);
+                entries(t + 2 * PA_WAVES);
+                pa_wait<ND + 1>();
+            } else {
+                pa_wait<0>();
+            }
             // V's scales; its largest of each key and of the tile. One that is not finite counts as 0 here and in
             // the products, and is added by itself below.
-            pa_wait<ND + 1>();
             uint32_t dmax = 0;
             bool odd = false;
             {
@@ -622,8 +627,10 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                     }
                 }
             }
-            pa_wait_lds();
-            send_v(at_v);
+            if (more) {
+                pa_wait_lds();
+                send_v(at_v);
+            }
             live = live_next;
         }
         pa_wait<0>();
