@@ -454,15 +454,20 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         get(rk, k_at(t0), ok, q_unit, t0, a.dk);
         get(rv, v_at(t0), ov, v_unit, t0, a.dv);
     };
-    // the decays of the chunk from t0, by the last wave (which has no scores to make); the next chunk's g is loaded ahead
+    // The part's chunks in their order; backwards for STATES, where a chunk's weights then hold all the decay behind it and
+    // the sum is never scaled (these parts are whole chunks).
+    auto place = [&](int t0) { return STATES ? part.len - C - t0 : t0; };
+    // the decays of a chunk, by the last wave (which has no scores to make); the next chunk's g is loaded ahead
     float gt = 0.f;
+    double after = 0.;                     // STATES: of the chunks behind
     auto load_g = [&](int t0) {
-        const int t = t0 + lane < part.len ? t0 + lane : part.len - 1;
-        gt = a.g[(int64_t) (part.t0 + t) * a.g_ts + h];
+        int t = place(t0) + (lane & (C - 1));
+        t = t < part.len ? t : part.len - 1;
+        gt = a.g[(int64_t) (part.t0 + (t < 0 ? 0 : t)) * a.g_ts + h];
     };
     auto decays = [&](int t0) {
         const int at = t0 / C & 1;
-        float x = t0 + lane < part.len && lane < C ? gt : 0.f;
+        float x = place(t0) + lane < part.len && lane < C ? gt : 0.f;
         x = x < LC_FLOOR ? LC_FLOOR : x;
         double s = (double) x * LC_LOG2E;
 #pragma unroll
@@ -471,7 +476,10 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             if (lane >= d) s += y;
         }
         const double end = __shfl(s, C - 1);
-        if (lane < C) {
+        if constexpr (STATES) {
+            if (lane < C) wG[at][lane] = __builtin_amdgcn_exp2f((float) (end - s + after));
+            after += end;
+        } else if (lane < C) {
             G[at][lane] = s;
             eG[at][lane] = __builtin_amdgcn_exp2f((float) s) * a.scale;
             wG[at][lane] = __builtin_amdgcn_exp2f((float) (end - s));
@@ -479,8 +487,8 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         }
     };
     if (w == NW - 1) load_g(0);
-    if constexpr (F::DMA) send(0, 0);
-    else load(0);
+    if constexpr (F::DMA) send(place(0), 0);
+    else load(place(0));
 
     // the state of the lane: [row tile][column tile] of rows 32 (t / 2) + 8 g + 4 (t % 2) + r
     v4f S[F::KT][2];
@@ -529,7 +537,6 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         decays(0);
         load_g(C);
     }
-    double total = 0.;
 
     for (int t0 = 0; t0 < part.len; t0 += C) {
         // the thread's places are computed anew in every chunk: kept over the loop they cost registers, spilled
@@ -548,12 +555,10 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             load_g(t0 + 2 * C);
         }
         if constexpr (F::DMA) {
-            if (t0 + C < part.len) send(t0 + C, F::BUF - buf);
+            if (t0 + C < part.len) send(place(t0 + C), F::BUF - buf);
         } else if (STATES && t0 + C < part.len) {
-            load(t0 + C);
+            load(place(t0 + C));
         }
-        const float cend = eEnd[even];
-        if (STATES) total += G[even][C - 1];
         v4w vx[2][NT];                         // v^T of the wave's columns
         auto load_v = [&]() {
 #pragma unroll
@@ -694,7 +699,8 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         // the state at the chunk's end
         if (live) {
             v4w vw[2][3];
-            float wt[8];
+            float wt[8], cend = 1.f;
+            if (!STATES) cend = eEnd[even];
 #pragma unroll
             for (int i = 0; i < 8; i++) wt[i] = wG[even][8 * g + i];
 #pragma unroll
@@ -720,7 +726,8 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     for (int n = 0; n < NT; n++)
                         kx[t][n] = lc_transposed<DK>(lds + buf + F::OK + n * F::QK, 8 * g, (t0g + t) >> 1, t & 1, m);
 #pragma unroll
-                for (int t = t0g; t < t0g + TG; t++) { S[t][0] *= cend; S[t][1] *= cend; }
+                for (int t = t0g; t < t0g + TG; t++)
+                    if (!STATES) { S[t][0] *= cend; S[t][1] *= cend; }
 #pragma unroll
                 for (int d = 2; d >= 0; d--)
 #pragma unroll
@@ -738,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
         for (int t = 0; t < F::KT; t++)
 #pragma unroll
             for (int u = 0; u < 2; u++) in_u(part.index, t, u) = S[t][u];
-        if (tid == 0 && cb == 0) x.G[(size_t) part.index * a.n_v + h] = total;
+        if (tid == F::THREADS - 64 && cb == 0) x.G[(size_t) part.index * a.n_v + h] = after;
     } else if (part.after == 0 && part.slot >= 0) {
         float * so = a.s_out + part.slot * per + h * hs;
         each([&](v4f & s, int r, size_t e) { so[e] = s[r]; });
