@@ -199,6 +199,7 @@ constexpr float LC_FLOOR = -1000.f;
 struct lc_args {
     la_args   a;
     int32_t   L;                       // tokens of a part, a multiple of the chunk; 0: sequences are whole
+    int32_t   parts;                   // that the workspace has room for
     int32_t   KT, US;                  // row tiles of a state, values of one in the workspace
     float *   U;                       // [part][n_v][wave's columns][row tile][column tile][lane][4], as the lanes hold them
     double *  G;                       // [part][n_v]: log2 of the part's decay
@@ -276,7 +277,8 @@ template <int NX, int NY, int NT> __device__ __forceinline__ v4f mfma_terms(cons
 // its place in the workspace, and the state's slot.
 struct lc_part { int32_t b, t0, len, before, after, index, slot; };
 
-// Part `want` of the batch, parts in order of the sequences.
+// Part `want` of the batch, parts in order of the sequences. Offsets that descend may let sequences share tokens and so
+// have more parts than the workspace: a sequence whose parts pass it is left out, by every launch alike.
 __device__ lc_part find_part(const lc_args & x, int want, bool report, int threads, int32_t * sh) {
     const la_args & a = x.a;
     lc_part p{want, 0, 0, 0, 0, want, -1};
@@ -303,7 +305,7 @@ __device__ lc_part find_part(const lc_args & x, int want, bool report, int threa
             for (int i = 0; i < c; i++) {
                 const int b = tid * c + i;
                 const int32_t n = b < a.n_seq ? (la_sequence(a, b, false).len + x.L - 1) / x.L : 0;
-                if (want >= at && want < at + n) {
+                if (want >= at && want < at + n && at + n <= x.parts) {
                     const la_seq s = la_sequence(a, b, false);
                     sh[8] = b; sh[9] = want - at; sh[10] = n; sh[11] = s.t0; sh[12] = s.len; sh[13] = s.slot;
                 }
@@ -945,7 +947,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         if (!pl.step) {
             if (pl.parts * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1) > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
             a.ct = pl.ct;
-            const lc_args x{a, pl.L, pl.DK / 16, pl.US, (float *) ws, (double *) ((char *) ws + pl.off_g)};
+            const lc_args x{a, pl.L, (int32_t) pl.parts, pl.DK / 16, pl.US, (float *) ws, (double *) ((char *) ws + pl.off_g)};
             return pl.NT == 1 ? launch_type<1>(x, pl, as_stream(stream)) : pl.NT == 2 ? launch_type<2>(x, pl, as_stream(stream))
                                                                                       : launch_type<3>(x, pl, as_stream(stream));
         }

@@ -251,6 +251,30 @@ def test_bad_sequences_and_slots(gpu):
             assert (np.abs(host(o) - zr[0]) <= z.bounds(zr)[0]).all()
 
 
+def test_descending_offsets_stay_in_the_workspace(gpu):
+    """Sequences that share their tokens have more parts together than the workspace has room for."""
+    K, n, d, n_v = gpu, 1000, 64, 2
+    c = Case([n], 1, n_v, d, d, seed=21)
+    cu = dev(np.array([0, n, 0, n, 0, n], np.int32))
+    q, k, v, g = c.q.cuda(), c.k.cuda(), c.v.cuda(), dev(c.g)
+    s_in = dev(np.repeat(c.state[c.slots], 5, axis=0))
+    s_out, o = torch.full_like(s_in, 5.0), torch.full_like(v, 7.0)
+    need = K.linear_attn_workspace_size(q, v, 5, n)
+    assert need > 0
+    ws = torch.full((need + (1 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    say("linear attention: sequences that share tokens")
+    K.device_status()
+    K.linear_attn(q, k, v, g, cu, n, s_in, s_out, o, scale=c.scale, ws=ws[:need])
+    torch.cuda.synchronize()
+    assert K.device_status() == K.DEVERR_SET_ROWS_INDEX
+    assert bool((ws[need:] == 0xA5).all())
+    ref, _ = c.reference()
+    tol, st = c.bounds(ref)
+    assert (np.abs(host(s_out)[0] - ref[2][0]) <= st[0]).all()
+    assert (host(s_out)[[1, 3]] == 5.0).all()
+    assert (np.abs(host(o) - ref[0]) <= tol).all()         # every sequence has the same tokens and the same state
+
+
 def test_repeats_and_graphs(gpu):
     """The same bits twice; two captured graphs with workspaces of their own, replayed with other lengths."""
     K = gpu
