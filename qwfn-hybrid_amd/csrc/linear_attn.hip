@@ -523,11 +523,13 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 #pragma unroll
     for (int t = 0; t < F::KT; t++) S[t][0] = S[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
     if (!STATES) {
-        if (part.before > 0) {
+        // (in place the last part may be done before the first begins: it finds its state in the workspace too)
+        if (part.before > 0 || (part.after > 0 && a.s_in == a.s_out)) {
+            const int at = part.before > 0 ? part.index - 1 : part.index + part.after;
 #pragma unroll
             for (int t = 0; t < F::KT; t++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) S[t][u] = in_u(part.index - 1, t, u);
+                for (int u = 0; u < 2; u++) S[t][u] = in_u(at, t, u);
         } else if (part.slot >= 0 && a.s_in) {
             const float * s0 = a.s_in + part.slot * per + h * hs;
             each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
@@ -754,8 +756,9 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     }
 }
 
-// The states behind the parts of a sequence (but the last), in the place of their U: S = 2^G_p S + U_p. A thread per 4
-// elements of a head's state; the parts' values are loaded LJ_AHEAD at a time.
+// The states behind the parts of a sequence (but the last), in the place of their U: S = 2^G_p S + U_p; in place the
+// state before the first part in the last one's. A thread per 4 elements of a head's state; the parts' values are loaded
+// LJ_AHEAD at a time.
 constexpr int LJ_AHEAD = 4;
 
 __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
@@ -778,6 +781,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
     }
     const int64_t per = (int64_t) x.US * a.n_v;
     float * up = x.U + ((int64_t) part.index * a.n_v + h) * x.US + 4 * (int64_t) e;
+    if (a.s_in == a.s_out) *(v4f *) (up + part.after * per) = s;
     const double * gp = x.G + (int64_t) part.index * a.n_v + h;
     for (int p0 = 0; p0 < part.after; p0 += LJ_AHEAD) {
         v4f u[LJ_AHEAD];

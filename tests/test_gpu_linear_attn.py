@@ -251,6 +251,17 @@ def test_bad_sequences_and_slots(gpu):
             assert (np.abs(host(o) - zr[0]) <= z.bounds(zr)[0]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_in_place_is_the_same_bits(gpu, dtype):
+    """More parts than run at once, states updated in place: no part reads what the sequence's last one wrote."""
+    K = gpu
+    say(f"linear attention {dtype}: in place")
+    c = Case([300] * 40, 4, 16, 64, 64, dtype, seed=22)
+    a, b = c.on_gpu(K), c.on_gpu(K, in_place=True)
+    assert torch.equal(a[0], b[0])
+    assert torch.equal(a[1][c.slots.tolist()], b[1][c.slots.tolist()])
+
+
 def test_descending_offsets_stay_in_the_workspace(gpu):
     """Sequences that share their tokens have more parts together than the workspace has room for."""
     K, n, d, n_v = gpu, 1000, 64, 2
