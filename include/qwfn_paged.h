@@ -61,7 +61,8 @@ size_t qwfn_paged_workspace_size(int32_t n_seq);
  * Any request not served, a negative n_past or n_new (taken as 0) and an n_free
  * outside [0, free_cap] (clipped) set bit 2 of qwfn_device_status. A table entry
  * of a partly filled page that names no row below 2^31 gives pad_slot and sets
- * the same bit. n_seq <= 65536, max_pages * page_size < 2^31; apart from the two
+ * the same bit. n_seq <= 65536, max_pages * page_size and table_stride (entries
+ * from one request's row to the next) < 2^31; apart from the two
  * in-place pairs no output may overlap an input or another output. One launch,
  * two where n_tok is more than 8 tokens a request. */
 int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size, int32_t * table,
@@ -92,8 +93,9 @@ int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq,
  *   n_kv device I32 [n_seq]: query t of request b is its token n_kv[b] - T + t and
  *        sees the tokens up to itself; a query before the first token gives 0, and
  *        so does a request of length 0 (a padded batch)
- *   dst  [D, n_head, T, n_seq] contiguous, 16-byte aligned, q's type
- *   gate NULL or dst's type and shape: dst = attention * sigmoid(gate)
+ *   dst  [D, n_head, T, n_seq] contiguous, 16-byte aligned, q's type, not
+ *        overlapping q
+ *   gate NULL or dst's type and shape: dst = attention * sigmoid(gate); may be dst
  * D 64, 128 or 256; n_head a multiple of n_head_kv, T * n_head / n_head_kv <= 64;
  * head rows and strides aligned to D / 16 bytes. Arithmetic as
  * qwfn_flash_attn_ext_q8_0: Q requantised to q8_0 with `variant`, exact integer

@@ -259,7 +259,7 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  * max_len of them:
  *   q, k  F32, F16 or BF16 [dk, n_k_heads, n_tok]; v, dst [dv, n_v_heads, n_tok] of
  *         q's type; rows contiguous, head and token strides multiples of 16 bytes,
- *         the token's below 2^24; dst contiguous
+ *         the token's below 2^24; dst contiguous, not overlapping q, k or v
  *   g     F32 log decays (at most 0 in use; -inf forgets everything), token t's at
  *         g + t * g_token_stride floats; a stride of 0 gives every token the same
  *         n_v_heads decays
@@ -272,7 +272,8 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  *         with rejected drafts is taken back by running the accepted tokens again
  *         from state_in.
  * dk and dv multiples of 16, dk <= 256, dv <= 512. States, decays and sums are F32
- * (sums of decays inside a chunk F64); the 16-bit types' products are exact, what
+ * (sums of decays inside a chunk F64; in chunks an F32 value above 3.39e38 counts as
+ * infinite); the 16-bit types' products are exact, what
  * is rounded on the way to an output is stated at the kernels; outputs are
  * rounded once. Tokens outside every sequence (cu[0] > 0, past cu[n_seq]) are not
  * read and their dst rows not written. cu is read as clipped to [0, n_tok] and to

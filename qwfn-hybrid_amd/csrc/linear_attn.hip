@@ -811,7 +811,7 @@ int check_heads(const qwfn_tensor * t, int32_t type, const char * name, bool pac
     if (t->ne[0] < 1 || t->ne[1] < 1 || t->ne[2] < 0 || t->ne[3] != 1) return err(QWFN_EINVAL, " must be [d, n_heads, n_tok]");
     if (t->nb[0] != es) return err(QWFN_EINVAL, " rows must be contiguous");
     if (!is_aligned(t->data, 16) || t->nb[1] % 16 || t->nb[2] % 16) return err(QWFN_EALIGN, " must be 16-byte aligned, its strides too");
-    if (packed && (t->nb[1] != t->ne[0] * es || t->nb[2] != t->ne[0] * t->ne[1] * es)) return err(QWFN_EINVAL, " must be contiguous");
+    if (packed && ((t->ne[1] > 1 && t->nb[1] != t->ne[0] * es) || (t->ne[2] > 1 && t->nb[2] != t->ne[0] * t->ne[1] * es))) return err(QWFN_EINVAL, " must be contiguous");
     if (t->ne[1] > 1 && t->nb[1] < t->ne[0] * es) return err(QWFN_EINVAL, " heads overlap");
     return QWFN_OK;
 }
@@ -936,6 +936,8 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             return set_error(QWFN_EINVAL, "linear_attn: state_in and state_out must be equal or not overlap");
         if (n_tok == 0) return QWFN_OK;
         if ((q->nb[2] | k->nb[2] | v->nb[2]) >> 24) return set_error(QWFN_ENOTSUP, "linear_attn: token strides of 2^24 bytes or more");
+        for (const qwfn_tensor * t : {q, k, v})
+            if (overlaps(dst->data, tensor_extent(dst), t->data, tensor_extent(t))) return set_error(QWFN_EINVAL, "linear_attn: dst overlaps q, k or v");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
         if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");

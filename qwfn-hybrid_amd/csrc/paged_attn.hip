@@ -900,6 +900,11 @@ extern "C" int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_
             if (!is_aligned(t->data, 16)) return err(QWFN_EALIGN, g ? ": gate must be 16-byte aligned" : ": dst must be 16-byte aligned");
         }
         if (table_stride < max_pages && B > 1) return err(QWFN_EINVAL, ": table rows overlap (table_stride < max_pages)");
+        if (table_stride > 0x7fffffff) return err(QWFN_EINVAL, ": table_stride must be below 2^31");
+        // (a request's queries are read by several workgroups, and one of them may be done before another begins)
+        const size_t out = tensor_extent(dst);
+        if (overlaps(dst->data, out, q->data, tensor_extent(q))) return err(QWFN_EINVAL, ": dst overlaps q");
+        if (gate && gate->data != dst->data && overlaps(dst->data, out, gate->data, out)) return err(QWFN_EINVAL, ": dst overlaps gate");
         if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
         if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
         if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");

@@ -258,25 +258,20 @@ __global__ __launch_bounds__(ROW_THREADS) void k_trim_pages(trim_args a) {
 
 int scan_threads(int32_t n_seq) { return std::min(PT_THREADS, (n_seq + 63) / 64 * 64); }
 
-bool overlaps(const void * a, size_t an, const void * b, size_t bn) {
-    const uintptr_t x = (uintptr_t) a, y = (uintptr_t) b;
-    return a && b && an && bn && x < y + bn && y < x + an;
-}
-
 struct span { const void * p; size_t n; const char * name; };
 
-int check_tables(const char * op, int32_t n_seq, int32_t page_size, const int32_t * table, int64_t table_stride,
-                 int32_t max_pages, int32_t free_cap, const void * ws, size_t ws_bytes) {
+int check_tables(const char * op, int32_t n_seq, int32_t page_size, int64_t table_stride, int32_t max_pages,
+                 int32_t free_cap, const void * ws, size_t ws_bytes) {
     const std::string o(op);
     if (n_seq < 1 || n_seq > PT_MAX_SEQ) return set_error(QWFN_EINVAL, o + ": n_seq must lie in [1, 65536]");
     if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff)
         return set_error(QWFN_EINVAL, o + ": page_size and max_pages must be positive, their product below 2^31");
     if (table_stride < max_pages) return set_error(QWFN_EINVAL, o + ": table rows overlap (table_stride < max_pages)");
+    if (table_stride > 0x7fffffff) return set_error(QWFN_EINVAL, o + ": table_stride must be below 2^31");
     if (free_cap < 0) return set_error(QWFN_EINVAL, o + ": free_cap must not be negative");
     if (!ws || ws_bytes < qwfn_paged_workspace_size(n_seq))
         return set_error(QWFN_ENOMEM, o + ": ws must hold qwfn_paged_workspace_size bytes");
     if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, o + ": ws must be 16-byte aligned");
-    (void) table;
     return QWFN_OK;
 }
 
@@ -314,7 +309,7 @@ extern "C" int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, 
     return ::qwfn::abi_call("paged_extend", [&]() -> int {
         if (!n_past || !n_new || !table || !free_pages || !n_free || !n_free_out || !n_kv || !cu_new || (!slots && n_tok))
             return set_error(QWFN_EINVAL, "paged_extend: NULL pointer");
-        if (int rc = check_tables("paged_extend", n_seq, page_size, table, table_stride, max_pages, free_cap, ws, ws_bytes))
+        if (int rc = check_tables("paged_extend", n_seq, page_size, table_stride, max_pages, free_cap, ws, ws_bytes))
             return rc;
         if (n_tok < 0 || n_tok > 0x7fffffff) return set_error(QWFN_EINVAL, "paged_extend: n_tok must lie in [0, 2^31)");
         const size_t per = (size_t) n_seq * 4, tok = (size_t) n_tok * 4;
@@ -350,7 +345,7 @@ extern "C" int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int
     return ::qwfn::abi_call("paged_trim", [&]() -> int {
         if (!n_keep || !n_kv || !table || !free_pages || !n_free || !n_free_out || !n_kv_out)
             return set_error(QWFN_EINVAL, "paged_trim: NULL pointer");
-        if (int rc = check_tables("paged_trim", n_seq, page_size, table, table_stride, max_pages, free_cap, ws, ws_bytes))
+        if (int rc = check_tables("paged_trim", n_seq, page_size, table_stride, max_pages, free_cap, ws, ws_bytes))
             return rc;
         const size_t per = (size_t) n_seq * 4, tab = ((size_t) (n_seq - 1) * table_stride + max_pages) * 4;
         const span in[] = {{n_keep, per, "n_keep"}, {n_kv_out == n_kv ? nullptr : n_kv, per, "n_kv"}, {table, tab, "table"},

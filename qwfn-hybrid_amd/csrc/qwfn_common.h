@@ -91,6 +91,20 @@ inline hipStream_t as_stream(void * s) { return reinterpret_cast<hipStream_t>(s)
 
 inline bool is_aligned(const void * p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+inline bool overlaps(const void * a, size_t an, const void * b, size_t bn) {
+    const uintptr_t x = (uintptr_t) a, y = (uintptr_t) b;
+    return a && b && an && bn && x < y + bn && y < x + an;
+}
+// Bytes from a tensor's first element to behind its last.
+inline size_t tensor_extent(const qwfn_tensor * t) {
+    size_t n = t->nb[0];
+    for (int i = 0; i < 4; i++) {
+        if (t->ne[i] < 1) return 0;
+        n += (size_t) (t->ne[i] - 1) * t->nb[i];
+    }
+    return n;
+}
+
 inline const char * type_name(int32_t t) {
     switch (t) {
         case QWFN_TYPE_F32:  return "f32";

@@ -793,8 +793,12 @@ def _check_i32(op, dev, vectors, table=None, rows=0):
             raise ValueError(f"{op}: table must be [{rows}, max_pages] with contiguous rows")
 
 
-def _ws(ws):
-    return (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (None, 0)
+def _ws(ws, dev):
+    if ws is None:
+        return None, 0
+    if ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError(f"ws must be a contiguous tensor on the current device ({dev})")
+    return ws.data_ptr(), ws.numel() * ws.element_size()
 
 
 def paged_workspace_size(n_seq: int) -> int:
@@ -815,7 +819,7 @@ def paged_extend(n_past, n_new, page_size: int, table, free_pages, n_free, n_fre
         n_past.data_ptr(), n_new.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1),
         free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(), n_kv.data_ptr(),
         cu_new.data_ptr(), slots.data_ptr(), pos.data_ptr() if pos is not None else None,
-        seq.data_ptr() if seq is not None else None, n_tok, pad_slot, *_ws(ws), _stream_on(stream, dev)))
+        seq.data_ptr() if seq is not None else None, n_tok, pad_slot, *_ws(ws, dev), _stream_on(stream, dev)))
 
 
 def paged_trim(n_keep, n_kv, page_size: int, table, free_pages, n_free, n_free_out, n_kv_out, ws=None, stream=None):
@@ -827,7 +831,7 @@ def paged_trim(n_keep, n_kv, page_size: int, table, free_pages, n_free, n_free_o
         n_free_out=(n_free_out, 1), n_kv_out=(n_kv_out, n_seq)), table, n_seq)
     return check(load().qwfn_paged_trim(n_keep.data_ptr(), n_kv.data_ptr(), n_seq, page_size, table.data_ptr(),
                                         table.stride(0), table.size(1), free_pages.data_ptr(), free_pages.numel(),
-                                        n_free.data_ptr(), n_free_out.data_ptr(), n_kv_out.data_ptr(), *_ws(ws),
+                                        n_free.data_ptr(), n_free_out.data_ptr(), n_kv_out.data_ptr(), *_ws(ws, dev),
                                         _stream_on(stream, dev)))
 
 
@@ -848,7 +852,7 @@ def flash_attn_ext_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: i
     gv = out_view(gate) if gate is not None else None
     return check(load().qwfn_flash_attn_ext_q8_0_paged(
         ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.size(1), page_size,
-        n_kv.data_ptr(), scale, ctypes.byref(gv) if gv is not None else None, ctypes.byref(ov), variant, *_ws(ws),
+        n_kv.data_ptr(), scale, ctypes.byref(gv) if gv is not None else None, ctypes.byref(ov), variant, *_ws(ws, dev),
         _stream_on(stream, dev)))
 
 
@@ -882,5 +886,5 @@ def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=No
     return check(load().qwfn_linear_attn(
         r(heads_view(q)), r(heads_view(k)), r(heads_view(v)), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0,
         cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.size(0),
-        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, r(heads_view(out)), *_ws(ws),
+        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, r(heads_view(out)), *_ws(ws, dev),
         _stream_on(stream, dev)))

@@ -121,6 +121,26 @@ def test_shapes_and_types(gpu, dtype, lens, n_k, n_v, dk, dv):
     Case(lens, n_k, n_v, dk, dv, dtype, seed=dk + dv).check(gpu)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [SINGLE, LONG, [600]])
+@pytest.mark.parametrize("n_k,n_v,dk,dv", [(1, 2, 240, 112), (1, 1, 256, 256), (1, 1, 144, 400), (2, 2, 48, 128), (1, 2, 160, 32)])
+def test_wide_heads(gpu, dtype, lens, n_k, n_v, dk, dv):
+    say(f"linear attention {dtype} lens={lens} heads {n_k}/{n_v} dk={dk} dv={dv}")
+    Case(lens, n_k, n_v, dk, dv, dtype, seed=dk + dv).check(gpu)
+
+
+def test_random_draws(gpu):
+    """Shapes and lengths drawn over their ranges."""
+    rng = np.random.default_rng(31)
+    for i in range(18):
+        n_k = int(rng.integers(1, 4))
+        n_v, dk, dv = n_k * int(rng.integers(1, 4)), 16 * int(rng.integers(1, 17)), 16 * int(rng.integers(1, 17))
+        lens = [int(np.exp(rng.uniform(0, np.log(700)))) - 1 for _ in range(int(rng.integers(1, 9)))]
+        dtype = [torch.float32, torch.float16, torch.bfloat16][i % 3]
+        say(f"linear attention draw {i}: {dtype} heads {n_k}/{n_v} dk={dk} dv={dv} lens={lens}")
+        Case(lens, n_k, n_v, dk, dv, dtype, seed=200 + i, fixed=bool(i & 1), gap=i % 3).check(gpu, in_place=bool(i & 2))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("lens", [[1], [4], [1500], [700, 5, 900], [16], [129]])
 def test_lengths(gpu, dtype, lens):

@@ -391,6 +391,112 @@ def test_attention_graphs_with_moving_lengths(gpu):
             assert torch.equal(got, t["out"])
 
 
+def test_attention_random_draws(gpu):
+    """Shapes, lengths and page sizes drawn over their ranges."""
+    rng = np.random.default_rng(23)
+    for i in range(14):
+        D, kvh, T = int(rng.choice([64, 128, 256])), int(rng.integers(1, 9)), int(rng.integers(1, 9))
+        rep, page = int(rng.integers(1, 64 // T + 1)), int(np.exp(rng.uniform(0, np.log(300))))
+        lens = [int(np.exp(rng.uniform(0, np.log(3000)))) - 1 for _ in range(int(np.exp(rng.uniform(0, np.log(24)))))]
+        dtype = [torch.float32, torch.float16, torch.bfloat16][i % 3]
+        say(f"paged attention draw {i}: D={D} kvh={kvh} rep={rep} T={T} page={page} lens={lens} {dtype}")
+        Case(lens, D, kvh, rep, T, page, seed=100 + i, dtype=dtype).check(gpu, gate=bool(i & 1))
+
+
+def test_attention_gate_in_place(gpu):
+    say("paged attention: the gate's tensor is the output")
+    K, c = gpu, Case([3000, 0, 70, 5], 128, 2, 6, 2, 16, seed=24)
+    want = c.on_gpu(K, gate=True)
+    o, q, td, nd = c.gate.cuda(), c.q.cuda(), dev(c.table), dev(np.asarray(c.lens, np.int32))
+    kv, vv = K.cache_attn_view(c.kd, c.n_rows, 2, 128), K.cache_attn_view(c.vd, c.n_rows, 2, 128)
+    K.flash_attn_ext_paged(K.q_view(q), kv, vv, td, 16, nd, c.scale, K.out_view(o), gate=o)
+    torch.cuda.synchronize()
+    assert torch.equal(o, want)
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Calls under way on two streams, each with its workspaces, beside work on the default one: the bits of calls alone."""
+    say("paged attention: two streams")
+    K, cases = gpu, [Case([4000, 90, 700], 256, 2, 8, 1, 16, seed=s) for s in (25, 26)]
+    want = [c.on_gpu(K) for c in cases]
+    streams, runs = [torch.cuda.Stream() for _ in cases], []
+    for c in cases:
+        q, td, nd = c.q.cuda(), dev(c.table), dev(np.asarray(c.lens, np.int32))
+        kv, vv = K.cache_attn_view(c.kd, c.n_rows, 2), K.cache_attn_view(c.vd, c.n_rows, 2)
+        o = torch.full_like(q, 3.0)
+        runs.append((q, td, nd, kv, vv, o, ws_of(K.fattn_workspace_size_paged(K.q_view(q), kv, vv, td, 16))))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, c, (q, td, nd, kv, vv, o, ws) in zip(streams, cases, runs):
+            with torch.cuda.stream(st):
+                o.fill_(3.0)
+                K.flash_attn_ext_paged(K.q_view(q), kv, vv, td, 16, nd, c.scale, K.out_view(o), ws=ws)
+    torch.cuda.synchronize()
+    for (*_, o, _), w in zip(runs, want):
+        assert torch.equal(o, w)
+
+
+def test_tables_captured_in_place(gpu):
+    """A step's extend and trim in one graph, lengths and stack in place: every replay as the eager calls."""
+    say("page tables: captured in place")
+    K, B, page = gpu, 70, 16
+    i32 = lambda x: dev(np.asarray(x, np.int32))  # noqa: E731
+    rng = np.random.default_rng(27)
+    start = dict(n_kv=i32(rng.integers(0, 40, B) // page * 0), table=i32(np.full((B, 9), -1)), free=i32(rng.permutation(500)),
+                 n_free=i32([500]))
+    new, keep = i32([0] * B), i32([0] * B)
+    sets = []
+    for _ in range(2):
+        t = {k: x.clone() for k, x in start.items()}
+        t.update(cu=i32([0] * (B + 1)), slots=i32([0] * 900), seq=i32([0] * 900), ws=ws_of(K.paged_workspace_size(B)))
+        sets.append(t)
+
+    def step(t):
+        K.paged_extend(t["n_kv"], new, page, t["table"], t["free"], t["n_free"], t["n_free"], t["n_kv"], t["cu"], t["slots"],
+                       seq=t["seq"], ws=t["ws"])
+        K.paged_trim(keep, t["n_kv"], page, t["table"], t["free"], t["n_free"], t["n_free"], t["n_kv"], ws=t["ws"])
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(sets[0])
+    for i in range(6):
+        new.copy_(i32(rng.integers(0, 12, B)))
+        keep.copy_(i32(rng.integers(0, 60, B) if i % 2 else [1 << 20] * B))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        step(sets[1])
+        torch.cuda.synchronize()
+        for name in ("n_kv", "table", "n_free", "cu", "slots", "seq", "free"):
+            assert torch.equal(sets[0][name], sets[1][name]), (i, name)
+
+
+def test_wrappers_refuse_tensors_elsewhere(gpu):
+    """Host tensors and other types where the calls read device int32, before anything is launched."""
+    K, c = gpu, Case([30], 256, 2, 8, 1, 16, seed=28)
+    c.on_gpu(K)
+    q, td, nd = c.q.cuda(), dev(c.table), dev(np.asarray(c.lens, np.int32))
+    kv = K.cache_attn_view(c.kd, c.n_rows, 2)
+    call = lambda table=td, n=nd, ws=None: K.flash_attn_ext_paged(  # noqa: E731
+        K.q_view(q), kv, kv, table, 16, n, 1 / 16, K.out_view(torch.empty_like(q)), ws=ws)
+    for kw in (dict(table=td.cpu()), dict(table=td.long()), dict(n=nd.cpu()), dict(n=nd[:0]), dict(table=td[0]),
+               dict(ws=torch.empty(1 << 20, dtype=torch.uint8))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    # the transposed table is one of one page a request: a call like another, its request clipped to that page
+    K.device_status()
+    call(table=td.t())
+    assert K.device_status() == K.DEVERR_GET_ROWS_INDEX
+    v = torch.zeros((4, 2, 64), device="cuda")
+    s, cu = torch.zeros((1, 2, 64, 64), device="cuda"), dev(np.array([0, 4], np.int32))
+    for kw in (dict(q=v.cpu()), dict(g=torch.zeros(2)), dict(cu=cu.long()), dict(s=s.cpu()), dict(g=torch.zeros(3, device="cuda"))):
+        a = dict(q=v, g=torch.zeros(2, device="cuda"), cu=cu, s=s)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            K.linear_attn(a["q"], v, v, a["g"], a["cu"], 4, a["s"], a["s"], torch.empty_like(v))
+
+
 def test_null_workspace_is_refused_in_capture(gpu):
     say("paged attention: ws NULL under capture")
     c = Case([30], 256, 2, 8, 1, 16, seed=17)

@@ -125,6 +125,26 @@ def linear(q=None, k=None, v=None, g=FAKE, g_ts=6, cu=FAKE, n_seq=3, max_len=50,
                                      ws, ws_bytes, None)
 
 
+def test_results_over_inputs_and_wide_strides_refused():
+    """Results that would be written over what other workgroups still read, and strides that pass the address space."""
+    for call in (extend, trim):
+        refused(call(stride=1 << 31), K.EINVAL, "table_stride")
+    q, k, o = paged_views()
+    refused(paged(q, k, o, stride=1 << 31), K.EINVAL, "table_stride")
+    q.data = o.data
+    refused(paged(q, k, o), K.EINVAL, "dst overlaps q")
+    q.data = o.data + 4 * 16 * 256 * 4 - 16                # the last 16 bytes of dst
+    refused(paged(q, k, o), K.EINVAL, "dst overlaps q")
+    q, k, o = paged_views()
+    gate = paged_views()[2]
+    gate.data = o.data + 16
+    refused(paged(q, k, o, gate=gate), K.EINVAL, "dst overlaps gate")
+    at = FAKE + 3 * GB
+    for name, d, n in (("q", 128, 2), ("k", 128, 2), ("v", 128, 6)):
+        refused(linear(**{name: heads(d, n, 100, at=at + 100 * 6 * 128 * 2 - 16)}, dst=heads(128, 6, 100, at=at)), K.EINVAL,
+                "dst overlaps")
+
+
 def test_linear_attention_refusals():
     refused(linear(g=None), K.EINVAL, "NULL")
     refused(linear(cu=None), K.EINVAL, "NULL")
