@@ -277,9 +277,9 @@ template <int NX, int NY, int NT> __device__ __forceinline__ v4f mfma_terms(cons
 // its place in the workspace, and the state's slot.
 struct lc_part { int32_t b, t0, len, before, after, index, slot; };
 
-// Part `want` of the batch, parts in order of the sequences. Offsets that descend may let sequences share tokens and so
+// Part `want` of the batch, parts in order of the sequences (by_seq: the first part of sequence `want`). Offsets that descend may let sequences share tokens and so
 // have more parts than the workspace: a sequence whose parts pass it is left out, by every launch alike.
-__device__ lc_part find_part(const lc_args & x, int want, bool report, int threads, int32_t * sh) {
+__device__ lc_part find_part(const lc_args & x, int want, bool by_seq, bool report, int threads, int32_t * sh) {
     const la_args & a = x.a;
     lc_part p{want, 0, 0, 0, 0, want, -1};
     if (x.L > 0) {
@@ -300,14 +300,14 @@ __device__ lc_part find_part(const lc_args & x, int want, bool report, int threa
         if (tid == 0) sh[8] = -1;
         __syncthreads();
         for (int i = 0; i < w; i++) incl += sh[i];
-        if (want >= incl - sum && want < incl) {
+        if (by_seq ? want / c == tid : want >= incl - sum && want < incl) {
             int32_t at = incl - sum;
             for (int i = 0; i < c; i++) {
                 const int b = tid * c + i;
                 const int32_t n = b < a.n_seq ? (la_sequence(a, b, false).len + x.L - 1) / x.L : 0;
-                if (want >= at && want < at + n && at + n <= x.parts) {
+                if ((by_seq ? b == want && n > 0 : want >= at && want < at + n) && at + n <= x.parts) {
                     const la_seq s = la_sequence(a, b, false);
-                    sh[8] = b; sh[9] = want - at; sh[10] = n; sh[11] = s.t0; sh[12] = s.len; sh[13] = s.slot;
+                    sh[8] = b; sh[9] = by_seq ? 0 : want - at; sh[14] = by_seq ? at : want; sh[10] = n; sh[11] = s.t0; sh[12] = s.len; sh[13] = s.slot;
                 }
                 at += n;
             }
@@ -321,6 +321,7 @@ __device__ lc_part find_part(const lc_args & x, int want, bool report, int threa
         p.t0 = get(11) + p.before * x.L;
         p.len = p.after > 0 ? x.L : get(12) - p.before * x.L;
         p.slot = get(13);
+        p.index = get(14);
         return p;
     }
     const la_seq s = la_sequence(a, want, report && threadIdx.x == 0);
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     // by the chunk's parity: log2 of the decay from the chunk's start, scale 2^G, 2^(G_end - G), 2^G_end
     __shared__ double G[2][C];
     __shared__ float eG[2][C], wG[2][C], eEnd[2];
-    __shared__ int32_t sh[14];
+    __shared__ int32_t sh[15];
     const la_args & a = x.a;
     int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     int blk = blockIdx.x;
     if (gridDim.x % 8 == 0) blk = (blk % 8) * (int) (gridDim.x / 8) + blk / 8;
     const int cb = blk % a.ct, h = blk / a.ct % a.n_v;
-    const lc_part part = find_part(x, blk / a.ct / a.n_v, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
+    const lc_part part = find_part(x, blk / a.ct / a.n_v, false, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
     if (part.b < 0) return;
     if (part.len <= 0 || (STATES && part.after == 0)) return;
 
@@ -762,12 +763,12 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
 constexpr int LJ_AHEAD = 4;
 
 __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
-    __shared__ int32_t sh[14];
+    __shared__ int32_t sh[15];
     const la_args & a = x.a;
     const int blocks = (x.US / 4 + LA_THREADS - 1) / LA_THREADS;
     const int eb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.n_v;
-    const lc_part part = find_part(x, blockIdx.x / blocks / a.n_v, false, LA_THREADS, sh);
-    if (part.b < 0 || part.before > 0 || part.after == 0) return;
+    const lc_part part = find_part(x, blockIdx.x / blocks / a.n_v, true, false, LA_THREADS, sh);
+    if (part.b < 0 || part.after == 0) return;
     const int e = eb * LA_THREADS + threadIdx.x;
     if (4 * e >= x.US) return;
     v4f s{0.f, 0.f, 0.f, 0.f};
@@ -886,7 +887,7 @@ int launch_chunks(const lc_args & x, const lc_plan & p, hipStream_t s) {
         hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, true>), grid, blk, 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
         const int64_t blocks = (x.US / 4 + LA_THREADS - 1) / LA_THREADS;
-        hipLaunchKernelGGL(k_linear_join, dim3((unsigned) (p.parts * x.a.n_v * blocks)), dim3(LA_THREADS), 0, s, x);
+        hipLaunchKernelGGL(k_linear_join, dim3((unsigned) (x.a.n_seq * x.a.n_v * blocks)), dim3(LA_THREADS), 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
     }
     hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, false>), grid, blk, 0, s, x);
