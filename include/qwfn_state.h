@@ -279,9 +279,10 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  * read and their dst rows not written. cu is read as clipped to [0, n_tok] and to
  * max_len tokens a sequence; a cu that descends or that is clipped sets bit 0 of
  * qwfn_device_status (a descending pair: no tokens, and sequences that then share
- * tokens with others may be left out). A sequence's results do not depend on the rest of the batch beyond rounding. max_len <= 8 runs token by
- * token; longer ones in chunks, long sequences cut into parts that are joined
- * through ws.
+ * tokens with others may be left out). A sequence's results do not depend on the
+ * rest of the batch beyond rounding. A max_len of a few tokens (4 of bf16, 6 of
+ * f16, 8 of f32) runs token by token; longer ones in chunks, long sequences cut
+ * into parts that are joined through ws.
  * ws: device memory of at least qwfn_linear_attn_workspace_size bytes, 16-byte
  * aligned (NULL where that is 0). */
 size_t qwfn_linear_attn_workspace_size(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len);

@@ -7,8 +7,9 @@
 // rows rg + 16 i; the state stays in registers for the sequence's tokens and is
 // read and written once. The output's sum over rows is finished across the lanes
 // (permlane swaps) and the waves (LDS), in a fixed order, one barrier a token.
-// What bounds it: the state, 8 dk dv bytes a head and sequence. Longer sequences run
-// in chunks (below).
+// What bounds it: the state, 8 dk dv bytes a head and sequence (64 sequences of one
+// bf16 token, 48 heads of 128: 407 MB in 82 us, 5.0 TB/s, a copy's rate). Calls of
+// more than a few tokens a sequence run in chunks (below).
 #include "fattn_device.h"
 #include "qwfn_common.h"
 #include "qwfn_state.h"
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // hold it and a chunk has two barriers. f16 and f32 are taken apart on the way, the
 // next chunk waits in registers, and a chunk has three.
 // What bounds it: 4096 bf16 tokens of 48 heads of 128 move 134 MB of q, k, v and o and
-// the parts' states another 190 MB, 63 us at the rate of a copy, and take 107; the
+// the parts' states another 190 MB, 63 us at the rate of a copy, and take 101; the
 // vector units are busy 40 % of the loop (the state's scaling and its roundings), the
 // matrix cores 20 %, the rest are the waits between a chunk's dependent products.
 //
@@ -192,7 +193,6 @@ typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
 constexpr int LC_WCOLS = 32;           // columns of a wave
-constexpr int LC_STEP_MAX = 8;         // up to this length token by token
 constexpr double LC_LOG2E = 1.4426950408889634;
 constexpr float LC_FLOOR = -1000.f;
 
@@ -849,9 +849,9 @@ template <int NT> int per_cu(int DK, int NW) {
 }
 
 // Parts of a sequence: as many as fill the CUs once with two waves a SIMD, so that no workgroup waits for another (4096
-// bf16 tokens of 48 heads of 128: 107 us in 10 parts, 125 in 5, 130 in 16, three waves a SIMD: a part's state goes
+// bf16 tokens of 48 heads of 128: 99 us in 10 parts, 120 in 5, 121 in 16, three waves a SIMD: a part's state goes
 // through the workspace three times), but no shorter than LC_MIN_PART tokens: a part costs a second pass over its k and v
-// (two f32 sequences of 509: 83 us with parts of 128, 97 of 256).
+// (two f32 sequences of 509: 78 us with parts of 128, 93 of 256).
 constexpr int64_t LC_CUS = 256, LC_MIN_PART = 128;
 
 lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
@@ -859,7 +859,10 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     const int64_t dk = q->ne[0], dv = v->ne[0], n_v = v->ne[1], n_tok = q->ne[2];
     p.NT = q->type == QWFN_TYPE_BF16 ? 1 : q->type == QWFN_TYPE_F16 ? 2 : 3;
     p.DK = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
-    p.step = max_len <= LC_STEP_MAX;
+    // Short calls go token by token: 1.2 us a token and 4 sequences (16 bf16 heads of 128 for 48), against a chunk whatever it
+    // holds: 12.5 us and 11.3 at 4 bf16 tokens, 14.9 and 13.6 at 6 of f16, 16.8 and 15.3 at 8 of f32; 10.1, 10.2 and 10.1
+    // against 11.3, 13.6 and 15.3 at 2. At 64 sequences the sides meet at 5 bf16, 6 f16 and 8 f32 tokens.
+    p.step = max_len <= 2 + 2 * p.NT;
     if (p.step) return p;
     p.NW = dv <= 2 * LC_WCOLS && (p.NT < 3 || p.DK < 256) ? 2 : 4;         // (256 rows of F32 for two waves are spilled)
     p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
