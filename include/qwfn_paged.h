@@ -63,8 +63,9 @@ size_t qwfn_paged_workspace_size(int32_t n_seq);
  * of a partly filled page that names no row below 2^31 gives pad_slot and sets
  * the same bit. n_seq <= 65536, max_pages * page_size and table_stride (entries
  * from one request's row to the next) < 2^31; apart from the two
- * in-place pairs no output may overlap an input or another output. One launch,
- * two where n_tok is more than 8 tokens a request. */
+ * in-place pairs no output may overlap an input or another output. One launch;
+ * two where n_tok is more than 8 tokens a request and a pair is in place or n_seq
+ * above 1024. */
 int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size, int32_t * table,
                       int64_t table_stride, int32_t max_pages, const int32_t * free_pages, int32_t free_cap,
                       const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv, int32_t * cu_new, int32_t * slots,
@@ -79,7 +80,8 @@ int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, int32_t n_s
  * become unused. A request whose pages would pass free_cap (counting those of
  * the requests before it) keeps its length and its pages and sets bit 2 of
  * qwfn_device_status, as do a negative n_kv, one above max_pages * page_size
- * (taken as 0 and as that) and an n_free outside [0, free_cap]. */
+ * (taken as 0 and as that) and an n_free outside [0, free_cap]. One launch; two
+ * where a pair is in place or n_seq above 1024. */
 int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq, int32_t page_size, const int32_t * table,
                     int64_t table_stride, int32_t max_pages, int32_t * free_pages, int32_t free_cap,
                     const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv_out, void * ws, size_t ws_bytes,

@@ -128,6 +128,28 @@ def test_trim_against_loop(gpu, in_place):
         check_trim(gpu, keep, n, page, max_pages, int(rng.integers(0, 3)) if cap > 3 else 0, cap, seed, in_place)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_tables_on_both_sides_of_a_workgroup(gpu, in_place):
+    """1023 to 1025 requests with many and few tokens, and every irregular length, in place and not."""
+    for B in (1023, 1024, 1025):
+        for most in (3, 40):
+            say(f"tables: B={B} new<={most} in_place={in_place}")
+            rng = np.random.default_rng(B + most)
+            past, new = rng.integers(0, 60, B), rng.integers(0, most + 1, B)
+            need = sum(-(-(p + f) // 16) - -(-p // 16) for p, f in zip(past, new))
+            for n_free in (need, need // 2):
+                check_extend(gpu, past, new, 16, 8, n_free, int(new.sum()) - 5, seed=B, in_place=in_place)
+        n = rng.integers(0, 120 * 16 + 1, B)
+        keep = np.where(rng.random(B) < 0.3, 0, n - rng.integers(0, 40, B))
+        check_trim(gpu, keep, n, 16, 120, 3, 120 * B, B, in_place)
+        check_trim(gpu, keep, n, 16, 120, 3, 9 * B, B, in_place)
+    check_extend(gpu, [-5, 4, 2 ** 31 - 1], [3, -2, 2 ** 31 - 1], 4, 8, 20, 50, in_place=in_place)
+    check_extend(gpu, [0, 3], [5, 5], 4, 8, -3, 50, in_place=in_place)
+    check_extend(gpu, [0, 3], [5, 5], 4, 8, 900, 50, cap=10, in_place=in_place)
+    check_trim(gpu, [-1, 5, 100], [10, -3, 40], 4, 8, 0, 40, in_place=in_place)
+    check_trim(gpu, [0, 0], [8, 8], 4, 8, -2, 40, in_place=in_place)
+
+
 def test_trim_bad_lengths(gpu):
     say("trim: lengths and stack out of range")
     check_trim(gpu, [-1, 5, 100], [10, -3, 40], 4, 8, 0, 40)
