@@ -24,6 +24,7 @@ namespace {
 constexpr int LA_THREADS = 256;
 constexpr int LA_COLS = 64;            // columns of a workgroup
 constexpr int LA_TC = 8;               // tokens whose q and k are brought in at once
+constexpr int64_t LA_BLOCKS = 0xffffff;    // of a launch: below 2^32 threads
 
 struct la_args {
     const char * q; const char * k; const char * v; char * out;
@@ -944,6 +945,9 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         for (const qwfn_tensor * t : {q, k, v})
             if (overlaps(dst->data, tensor_extent(dst), t->data, tensor_extent(t))) return set_error(QWFN_EINVAL, "linear_attn: dst overlaps q, k or v");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
+        const int64_t ct = (dv + LA_COLS - 1) / LA_COLS;       // token by token
+        const int64_t blocks = pl.step ? n_seq * n_v * ct : pl.parts * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1);
+        if (blocks > LA_BLOCKS) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
         if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");
         if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, "linear_attn: ws must be 16-byte aligned");
@@ -956,15 +960,12 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         a.type = q->type; a.n_seq = n_seq; a.max_len = max_len; a.n_slots = n_slots; a.n_tok = (int32_t) n_tok;
         a.n_k = (int32_t) q->ne[1]; a.n_v = (int32_t) n_v; a.rep = a.n_v / a.n_k; a.dk = (int32_t) dk; a.dv = (int32_t) dv;
         if (!pl.step) {
-            if (pl.parts * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1) > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
             a.ct = pl.ct;
             const lc_args x{a, pl.L, (int32_t) pl.parts, pl.DK / 16, pl.US, (float *) ws, (double *) ((char *) ws + pl.off_g)};
             return pl.NT == 1 ? launch_type<1>(x, pl, as_stream(stream)) : pl.NT == 2 ? launch_type<2>(x, pl, as_stream(stream))
                                                                                       : launch_type<3>(x, pl, as_stream(stream));
         }
-        a.ct = (int32_t) ((dv + LA_COLS - 1) / LA_COLS);
-        const int64_t blocks = (int64_t) n_seq * n_v * a.ct;
-        if (blocks > 0x7fffffff) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
+        a.ct = (int32_t) ct;
         const dim3 grid((unsigned) blocks), blk(LA_THREADS);
         if (dk <= 64)       hipLaunchKernelGGL(k_linear_step<64>, grid, blk, 0, as_stream(stream), a);
         else if (dk <= 128) hipLaunchKernelGGL(k_linear_step<128>, grid, blk, 0, as_stream(stream), a);

@@ -824,7 +824,8 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
         return err(QWFN_EINVAL, ": page_size and max_pages must be positive, their product below 2^31 - 256");
     if (B > 65536 || B * ((int64_t) page_size * max_pages / PA_TILE + 1 + PA_LEAD) > 0x7ffff000)
         return err(QWFN_ENOTSUP, ": at most 65536 requests and 2^31 tiles of 32 keys");
-    if (B * nh * T * (D / 64) > 0x7ffff000) return err(QWFN_ENOTSUP, ": too many query rows");
+    // (a wave of the merge a row and 64 dims, and a launch has below 2^32 threads)
+    if (B * nh * T * (D / 64) >= 1 << 26) return err(QWFN_ENOTSUP, ": too many query rows");
     if (k->ne[1] < page_size) return err(QWFN_EINVAL, ": the pool holds no whole page");
     if (k->ne[1] > 0x7fffffff) return err(QWFN_ENOTSUP, ": a pool of at most 2^31 - 1 rows");
     *pl = plan_paged(D, T, nh, nh_kv, B, (int64_t) page_size * max_pages);

@@ -271,6 +271,19 @@ def test_bad_sequences_and_slots(gpu):
             assert (np.abs(host(o) - zr[0]) <= z.bounds(zr)[0]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_sequences_in_parts(gpu, dtype):
+    """More sequences than a workgroup has threads, most of them short or empty, a few in parts."""
+    rng = np.random.default_rng(32)
+    lens = [int(x) for x in rng.integers(0, 9, 600)]
+    for b in (0, 255, 256, 511, 599):
+        lens[b] = int(rng.integers(300, 700))
+    say(f"linear attention {dtype}: 600 sequences, {sum(lens)} tokens")
+    c = Case(lens, 1, 2, 64, 64, dtype, seed=32)
+    assert gpu.linear_attn_workspace_size(c.q, c.v, 600, max(lens)) > 0
+    c.check(gpu, in_place=True)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_in_place_is_the_same_bits(gpu, dtype):
     """More parts than run at once, states updated in place: no part reads what the sequence's last one wrote."""

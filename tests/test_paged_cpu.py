@@ -145,6 +145,14 @@ def test_results_over_inputs_and_wide_strides_refused():
                 "dst overlaps")
 
 
+def test_more_work_than_a_launch_has_threads():
+    refused(paged(*paged_views(D=64, nh=2048, kvh=32, B=65536), cols=1, stride=1), K.ENOTSUP, "too many query rows")
+    far = dict(q=heads(16, 1, 100), k=heads(16, 1, 100), v=heads(16, 1024, 100, at=FAKE + GB), g_ts=1024, n_seq=65535,
+               n_slots=65535, s_in=None, s_out=FAKE + 8 * GB, dst=heads(16, 1024, 100, at=FAKE + 2 * GB))
+    for max_len in (1, 50):
+        refused(linear(max_len=max_len, ws_bytes=1 << 60, **far), K.ENOTSUP, "too many sequences")
+
+
 def test_linear_attention_refusals():
     refused(linear(g=None), K.EINVAL, "NULL")
     refused(linear(cu=None), K.EINVAL, "NULL")
