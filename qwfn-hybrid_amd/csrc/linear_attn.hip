@@ -343,11 +343,12 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     const la_args & a = x.a;
     int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // consecutive blocks (the heads of a key head) on one XCD
-    int blk = blockIdx.x;
-    if (gridDim.x % 8 == 0) blk = (blk % 8) * (int) (gridDim.x / 8) + blk / 8;
-    const int cb = blk % a.ct, h = blk / a.ct % a.n_v;
-    const lc_part part = find_part(x, blk / a.ct / a.n_v, false, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
+    // the heads of a key head on one XCD, key heads and parts in turn on all of them
+    const int share = a.rep * a.ct, near = (int) blockIdx.x >> 3;
+    const int blk = (near / share * 8 + (int) (blockIdx.x & 7)) * share + near % share;
+    const int cb = blk % a.ct, h = blk / a.ct % a.n_v, want = blk / a.ct / a.n_v;
+    if (want >= x.parts) return;
+    const lc_part part = find_part(x, want, false, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
     if (part.b < 0) return;
     if (part.len <= 0 || (STATES && part.after == 0)) return;
 
@@ -887,7 +888,8 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
 
 template <int NT, int DK, int NW>
 int launch_chunks(const lc_args & x, const lc_plan & p, hipStream_t s) {
-    const dim3 grid((unsigned) (p.parts * x.a.n_v * p.ct)), blk(64 * NW);
+    const int64_t share = (int64_t) x.a.rep * p.ct;                // (whole rounds of the 8 XCDs)
+    const dim3 grid((unsigned) ((p.parts * x.a.n_k + 7) / 8 * 8 * share)), blk(64 * NW);
     if (p.L > 0) {
         hipLaunchKernelGGL((k_linear_chunks<NT, DK, NW, true>), grid, blk, 0, s, x);
         if (int rc = hip_check(hipGetLastError(), "linear_attn launch")) return rc;
@@ -946,7 +948,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             if (overlaps(dst->data, tensor_extent(dst), t->data, tensor_extent(t))) return set_error(QWFN_EINVAL, "linear_attn: dst overlaps q, k or v");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
         const int64_t ct = (dv + LA_COLS - 1) / LA_COLS;       // token by token
-        const int64_t blocks = pl.step ? n_seq * n_v * ct : pl.parts * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1);
+        const int64_t blocks = pl.step ? n_seq * n_v * ct : (pl.parts + 8) * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1);
         if (blocks > LA_BLOCKS) return set_error(QWFN_ENOTSUP, "linear_attn: too many sequences and heads");
         if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");
