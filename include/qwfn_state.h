@@ -273,8 +273,8 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  *         from state_in.
  * dk and dv multiples of 16, dk <= 256, dv <= 512. States, decays and sums are F32
  * (sums of decays inside a chunk F64; in chunks an F32 value above 3.39e38 counts as
- * infinite); the 16-bit types' products are exact, what
- * is rounded on the way to an output is stated at the kernels; outputs are
+ * infinite); the 16-bit types' products are exact, and on the way to
+ * an output the state and the scores keep 16 bits at least (24 of F32); outputs are
  * rounded once. Tokens outside every sequence (cu[0] > 0, past cu[n_seq]) are not
  * read and their dst rows not written. cu is read as clipped to [0, n_tok] and to
  * max_len tokens a sequence; a cu that descends or that is clipped sets bit 0 of

@@ -160,8 +160,9 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // the pairs of terms that reach NT terms' accuracy. The state's update always
 // takes three terms of e^{G_C - G_j} v_j, so the state stays an F32 sum whatever the
 // type; on the way to an output the state and the weighted scores are rounded to NT
-// terms (bf16: once to bf16 each, as the output itself is: 2.3e-3 of the result for the
-// 1.7e-3 of its own rounding; two terms of both took 113 us for 101 at 4096 tokens).
+// terms, two at least (2^-16 of each: an output is off by its own rounding, 1.7e-3 of the
+// result in bf16, whether its tokens run in chunks or one by one; with one term it was
+// 2.3e-3, and 101 us for 113 at 4096 tokens).
 // G and its differences are F64: a chunk's strong decays leave the weak ones exact.
 // A decay below e^-1000 counts as e^-1000, which is 0 in F32, so -inf is exact.
 //
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // hold it and a chunk has two barriers. f16 and f32 are taken apart on the way, the
 // next chunk waits in registers, and a chunk has three.
 // What bounds it: 4096 bf16 tokens of 48 heads of 128 move 134 MB of q, k, v and o and
-// the parts' states another 190 MB, 63 us at the rate of a copy, and take 101; the
+// the parts' states another 190 MB, 63 us at the rate of a copy, and take 113; the
 // vector units are busy 40 % of the loop (the state's scaling and its roundings), the
 // matrix cores 20 %, the rest are the waits between a chunk's dependent products.
 //
@@ -212,13 +213,14 @@ constexpr int LC_C = 32;               // tokens of a chunk: the sum of one MFMA
 template <int NT, int DK, int NW> struct lc_cfg {
     static constexpr int KT = DK / 16, KB = DK / 32;
     static constexpr int COLS = LC_WCOLS * NW, THREADS = 64 * NW;
+    static constexpr int OT = NT == 1 ? 2 : NT;          // terms of the state and of the scores on their way to an output
     static constexpr int ES = NT == 3 ? 4 : 2;           // bytes of a value
     static constexpr int LPU = NT == 3 ? 2 : 1;          // 16-byte loads of 8 values
     static constexpr bool DMA = NT == 1;                 // bf16 goes to LDS as it is
     // a staged unit: 8 values of a token; a thread's units of q and of k, and of v
     static constexpr int KU = LC_C * (DK / 8) / THREADS, VU = LC_C * (COLS / 8) / THREADS;
     static constexpr int QK = LC_C * DK * 2, V = LC_C * COLS * 2, P = LC_C * LC_C * 2;     // bytes of a term
-    static constexpr int OQ = 0, OK = OQ + NT * QK, OV = OK + NT * QK, BUF = OV + NT * V, OP = (DMA ? 2 : 1) * BUF, LDS = OP + NT * P;
+    static constexpr int OQ = 0, OK = OQ + NT * QK, OV = OK + NT * QK, BUF = OV + NT * V, OP = (DMA ? 2 : 1) * BUF, LDS = OP + OT * P;
     // workgroups of a CU: by LDS, and three waves a SIMD (168 registers each), two with a chunk in registers, one with a
     // state of 256 rows
     static constexpr int WAVES = DK == 256 ? 4 : DMA ? 12 : 8;
@@ -334,7 +336,7 @@ __device__ lc_part find_part(const lc_args & x, int want, bool by_seq, bool repo
 template <int NT, int DK, int NW, bool STATES>
 __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_linear_chunks(lc_args x) {
     using F = lc_cfg<NT, DK, NW>;
-    constexpr int C = LC_C;
+    constexpr int C = LC_C, OT = F::OT;
     __shared__ __attribute__((aligned(256))) uint8_t lds[F::LDS];
     // by the chunk's parity: log2 of the decay from the chunk's start, scale 2^G, 2^(G_end - G), 2^G_end
     __shared__ double G[2][C];
@@ -539,7 +541,7 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             each([&](v4f & s, int r, size_t e) { s[r] = s0[e]; });
         }
         // the scores of the tokens behind the first 16 stay 0 in their rows
-        for (int i = tid; i < NT * F::P / 16; i += F::THREADS) *(v4w *) (lds + F::OP + 16 * i) = v4w{0, 0, 0, 0};
+        for (int i = tid; i < OT * F::P / 16; i += F::THREADS) *(v4w *) (lds + F::OP + 16 * i) = v4w{0, 0, 0, 0};
     }
     if (w == NW - 1) {
         decays(0);
@@ -600,11 +602,11 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                     const int j = 16 * jt + 4 * g + r;
                     p[r] = j <= i ? p[r] * (__builtin_amdgcn_exp2f((float) (gi - G[even][j])) * a.scale) : 0.f;
                 }
-                uint32_t lo[NT], hi[NT];
-                bf16_terms<NT>(p[0], p[1], lo);
-                bf16_terms<NT>(p[2], p[3], hi);
+                uint32_t lo[OT], hi[OT];
+                bf16_terms<OT>(p[0], p[1], lo);
+                bf16_terms<OT>(p[2], p[3], hi);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int t = 0; t < OT; t++)
                     *(v2w *) (lds + F::OP + t * F::P + lc_score(i, 2 * jt + (g >> 1)) + 8 * (g & 1)) = v2w{lo[t], hi[t]};
             }
             // S^T q
@@ -612,24 +614,24 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
             if (live) {
 #pragma unroll
                 for (int kb = 0; kb < F::KB; kb++) {
-                    v4w sx[2][NT];
+                    v4w sx[2][OT];
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const v4f & s = S[2 * kb + (i >> 1)][u];
-                            uint32_t t[NT];
-                            bf16_terms<NT>(s[2 * (i & 1)], s[2 * (i & 1) + 1], t);
+                            uint32_t t[OT];
+                            bf16_terms<OT>(s[2 * (i & 1)], s[2 * (i & 1) + 1], t);
 #pragma unroll
-                            for (int n = 0; n < NT; n++) sx[u][n][i] = t[n];
+                            for (int n = 0; n < OT; n++) sx[u][n][i] = t[n];
                         }
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         v4w qx[NT];
 #pragma unroll
                         for (int t = 0; t < NT; t++) qx[t] = *(const v4w *) (lds + buf + F::OQ + t * F::QK + lc_row<DK>(16 * i + m, 4 * kb + g));
-                        o[i][0] = mfma_terms<NT, NT, NT>(sx[0], qx, o[i][0]);
-                        o[i][1] = mfma_terms<NT, NT, NT>(sx[1], qx, o[i][1]);
+                        o[i][0] = mfma_terms<OT, NT, OT>(sx[0], qx, o[i][0]);
+                        o[i][1] = mfma_terms<OT, NT, OT>(sx[1], qx, o[i][1]);
                     }
                 }
             }
@@ -656,28 +658,28 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
                 if (__ballot(odd != odd) == 0) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        v4w px[NT];
+                        v4w px[OT];
 #pragma unroll
-                        for (int t = 0; t < NT; t++) px[t] = *(const v4w *) (lds + F::OP + t * F::P + lc_score(16 * i + m, g));
-                        o[i][0] = mfma_terms<NT, NT, NT>(vx[0], px, o[i][0]);
-                        o[i][1] = mfma_terms<NT, NT, NT>(vx[1], px, o[i][1]);
+                        for (int t = 0; t < OT; t++) px[t] = *(const v4w *) (lds + F::OP + t * F::P + lc_score(16 * i + m, g));
+                        o[i][0] = mfma_terms<NT, OT, OT>(vx[0], px, o[i][0]);
+                        o[i][1] = mfma_terms<NT, OT, OT>(vx[1], px, o[i][1]);
                     }
                 } else {
-                    auto sum = [&](int at, int size) {
+                    auto sum = [&](int at, int size, int terms) {
                         float f = 0.f;
-                        for (int n = 0; n < NT; n++) f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size) << 16);
+                        for (int n = 0; n < terms; n++) f += __builtin_bit_cast(float, (uint32_t) *(const uint16_t *) (lds + at + n * size) << 16);
                         return f;
                     };
                     for (int j = 0; j <= 16 + m; j++) {
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             if (j > 16 * i + m) continue;
-                            const float p = sum(F::OP + lc_score(16 * i + m, j >> 3) + 2 * (j & 7), F::P);
+                            const float p = sum(F::OP + lc_score(16 * i + m, j >> 3) + 2 * (j & 7), F::P, OT);
 #pragma unroll
                             for (int u = 0; u < 2; u++)
 #pragma unroll
                                 for (int r = 0; r < 4; r++) {
-                                    const float v = sum(buf + F::OV + lc_row<F::COLS>(j, 4 * w + g) + 8 * u + 2 * r, F::V);
+                                    const float v = sum(buf + F::OV + lc_row<F::COLS>(j, 4 * w + g) + 8 * u + 2 * r, F::V, NT);
                                     o[i][u][r] = __fmaf_rn(p, v, o[i][u][r]);
                                 }
                         }
@@ -863,8 +865,9 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     p.NT = q->type == QWFN_TYPE_BF16 ? 1 : q->type == QWFN_TYPE_F16 ? 2 : 3;
     p.DK = dk <= 64 ? 64 : dk <= 128 ? 128 : 256;
     // Short calls go token by token: 1.2 us a token and 4 sequences (16 bf16 heads of 128 for 48), against a chunk whatever it
-    // holds: 12.5 us and 11.3 at 4 bf16 tokens, 14.9 and 13.6 at 6 of f16, 16.8 and 15.3 at 8 of f32; 10.1, 10.2 and 10.1
-    // against 11.3, 13.6 and 15.3 at 2. At 64 sequences the sides meet at 5 bf16, 6 f16 and 8 f32 tokens.
+    // holds: 11.9 us and 11.3 at 4 bf16 tokens, 14.9 and 13.6 at 6 of f16, 16.8 and 15.3 at 8 of f32; 9.6, 10.2 and 10.1
+    // against 11.3, 13.6 and 15.3 at 2. At 64 sequences the sides meet at 6 f16 and 8 f32 tokens, and 4 bf16 tokens take 84
+    // against 95.
     p.step = max_len <= 2 + 2 * p.NT;
     if (p.step) return p;
     p.NW = dv <= 2 * LC_WCOLS && (p.NT < 3 || p.DK < 256) ? 2 : 4;         // (256 rows of F32 for two waves are spilled)

@@ -383,3 +383,34 @@ def test_hybrid_step(gpu):
         ref, mag = r[2], r[3]
         assert (np.abs(host(state[0]) - ref) <= 2 * (3 * 100 + 200) * 2.0 ** -24 * r[3] + 1e-30).all()
     assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [LONG, [600, 40], [1500]])
+@pytest.mark.parametrize("n_k,n_v,dk,dv", [(1, 3, 128, 128), (2, 2, 64, 64), (1, 2, 256, 48), (1, 1, 256, 256)])
+def test_outputs_in_chunks_are_rounded_once(gpu, dtype, lens, n_k, n_v, dk, dv):
+    """A 16-bit output differs from the recurrence by its own rounding, an f32 one by the roundings of f32 sums.
+
+    By element: a value x in two bf16 terms is off by 2^-16 |x|, and a product of two such values without its last pair of
+    terms by another 2^-16. bf16: the state and the scores are in two terms, all else is exact: 2^-16 of mag. f16: q, k and v
+    are exact in two; the state's product 2, the scores' and the weighted scores' together 3: 3 2^-16 of mag.
+    In the 2-norm: an error before the rounding of e adds to it as sqrt(r^2 + e^2); e is below 3 2^-16, r of f16 (uniform in a
+    step of 2^-10 to 2^-11 of the value) at least 2^-11 / sqrt(12) = 1.4e-4: at most 5 % more. With a term less e is 2^-9.
+    f32: 3 roundings a chunk, dk / 16 sums and the split's 6, each 2^-24 / sqrt(3) in the mean: sqrt(3 47 + 16 + 6) / sqrt(3) = 7.4
+    steps of 2^-24 at 1500 tokens; 16 allowed. With a term less it is 2^-17."""
+    say(f"linear attention in chunks {dtype} lens={lens} heads {n_k}/{n_v} dk={dk} dv={dv}")
+    c = Case(lens, n_k, n_v, dk, dv, dtype, seed=dk + dv + 1, decay=0.05)
+    o, _ = c.on_gpu(gpu, max_len=max(lens))
+    (out, mag, _, _), _ = c.reference()
+    o = o.float().cpu().numpy().astype(np.float64)
+    err = np.linalg.norm(o - out) / np.linalg.norm(out)
+    if dtype == torch.float32:
+        assert err <= 2.0 ** -20, err
+        return
+    once = torch.from_numpy(out).to(dtype).double().numpy()
+    assert err <= 1.05 * np.linalg.norm(once - out) / np.linalg.norm(out), err
+    h, e = HALF_STEP[dtype], np.zeros((len(mag), 1, 1))
+    for t0, m in zip(c.starts, c.lens):
+        e[t0:t0 + m] = (3 * m + 64 + dk) * 2.0 ** -24 + (1 if dtype == torch.bfloat16 else 3) * 2.0 ** -16
+    tol = h * np.abs(out) + (1 + h) * e * mag + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
+    assert (np.abs(o - out) <= tol).all(), np.max(np.abs(o - out) / tol)
