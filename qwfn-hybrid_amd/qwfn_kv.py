@@ -847,8 +847,11 @@ def flash_attn_ext_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: i
     int32 [n_seq]; times sigmoid(gate) when gate (laid out as the output) is given."""
     n_seq, dev = qv.ne[3], _Torch().device()
     _check_i32("flash_attn_ext_paged", dev, dict(n_kv=(n_kv, n_seq)), table, n_seq)
-    if gate is not None and not gate.is_contiguous():
-        raise ValueError("flash_attn_ext_paged: gate must be contiguous")
+    if gate is not None:
+        if gate.get_device() != dev:
+            raise ValueError(f"flash_attn_ext_paged: gate must be on the current device ({dev})")
+        if not gate.is_contiguous():
+            raise ValueError("flash_attn_ext_paged: gate must be contiguous")
     gv = out_view(gate) if gate is not None else None
     return check(load().qwfn_flash_attn_ext_q8_0_paged(
         ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.size(1), page_size,

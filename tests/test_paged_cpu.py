@@ -179,3 +179,42 @@ def test_linear_attention_refusals():
     refused(linear(s_in=FAKE + 4), K.EALIGN, "16-byte")
     refused(linear(s_in=FAKE + GB + 4096), K.EINVAL, "overlap")
     assert linear(q=heads(128, 2, 0), k=heads(128, 2, 0), v=heads(128, 6, 0), dst=heads(128, 6, 0)) == K.OK   # no tokens
+
+
+class Elsewhere:
+    """A [4, 1, 16, 256] float32 tensor of another device, as far as the wrappers look."""
+    shape = (4, 1, 16, 256)
+
+    def __init__(self, device=3):
+        import torch
+        self.dtype, self.device = torch.float32, device
+
+    def dim(self):
+        return 4
+
+    def is_contiguous(self):
+        return True
+
+    def element_size(self):
+        return 4
+
+    def data_ptr(self):
+        return FAKE + 5 * GB
+
+    def get_device(self):
+        return self.device
+
+
+def test_a_gate_on_another_device_is_refused(monkeypatch):
+    """Host tensors stand in for those of the current device; dst is NULL, so that the library refuses the call that passes."""
+    import torch
+    monkeypatch.setattr(K._Torch(), "device", staticmethod(lambda: -1))
+    q, k, o = paged_views()
+    o.data = None
+    table, n_kv = torch.zeros((4, 40), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    call = lambda gate: K.flash_attn_ext_paged(q, k, k, table, 16, n_kv, 0.0625, o, gate=gate, stream=0)  # noqa: E731
+    for gate in (None, Elsewhere(device=-1)):
+        with pytest.raises(K.QwfnError, match="dst is NULL"):
+            call(gate)
+    with pytest.raises(ValueError, match="gate must be on the current device"):
+        call(Elsewhere())
