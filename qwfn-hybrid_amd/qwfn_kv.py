@@ -359,9 +359,10 @@ class _Torch:
             import torch
             cls.int32, cls.float32 = torch.int32, torch.float32
             cls.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-            cls.device, cls.mod = staticmethod(torch.cuda.current_device), torch
+            cls.device = staticmethod(torch.cuda.current_device)
             raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
             cls.stream = staticmethod(raw or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+            cls.mod = torch                              # last: another thread that sees it finds the rest
         return cls
 
 

@@ -218,3 +218,35 @@ def test_a_gate_on_another_device_is_refused(monkeypatch):
             call(gate)
     with pytest.raises(ValueError, match="gate must be on the current device"):
         call(Elsewhere())
+
+
+@pytest.mark.parametrize("at", range(9))
+def test_first_use_from_two_threads(monkeypatch, at):
+    """A second thread that comes at the first's `at`-th question to torch, while it still fills what the wrappers keep of
+    the answers, finds all of them, or fills them itself."""
+    import sys
+    import threading
+
+    import torch
+    names, found, asked = ("int32", "float32", "types", "device", "stream"), [], []
+    K._Torch()
+    for name in names:
+        monkeypatch.delattr(K._Torch, name)
+    monkeypatch.setattr(K._Torch, "mod", None)
+
+    def second():
+        t = K._Torch()
+        found.append([n for n in names if not hasattr(t, n)])
+
+    class Slow:
+        def __getattr__(self, name):
+            asked.append(name)
+            if len(asked) == at + 1:
+                th = threading.Thread(target=second)
+                th.start()
+                th.join()
+            return getattr(torch, name)
+
+    monkeypatch.setitem(sys.modules, "torch", Slow())
+    K._Torch()
+    assert found in ([[]], []) and (found or len(asked) <= at), (found, asked)
