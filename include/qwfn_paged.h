@@ -107,7 +107,8 @@ int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq,
  * not depend on the other requests of the batch beyond float rounding (the
  * split points), and repeat bit for bit on the same inputs.
  * ws: at least qwfn_fattn_workspace_size_paged bytes, 16-byte aligned, or NULL for
- * the library's buffer (see qwfn_flash_attn_ext_q8_0). */
+ * the library's buffer (see qwfn_flash_attn_ext_q8_0). dst and ws overlap no other tensor
+ * but dst the gate. */
 size_t qwfn_fattn_workspace_size_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
                                        int32_t max_pages, int32_t page_size);
 int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,

@@ -284,7 +284,7 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  * f16, 8 of f32) runs token by token; longer ones in chunks, long sequences cut
  * into parts that are joined through ws.
  * ws: device memory of at least qwfn_linear_attn_workspace_size bytes, 16-byte
- * aligned (NULL where that is 0). */
+ * aligned (NULL where that is 0). dst, state_out and ws overlap no other tensor. */
 size_t qwfn_linear_attn_workspace_size(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len);
 int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const float * g,
                      int64_t g_token_stride, const int32_t * cu, int32_t n_seq, int32_t max_len, const int32_t * slots,

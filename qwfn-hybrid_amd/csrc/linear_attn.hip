@@ -947,8 +947,6 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             return set_error(QWFN_EINVAL, "linear_attn: state_in and state_out must be equal or not overlap");
         if (n_tok == 0) return QWFN_OK;
         if ((q->nb[2] | k->nb[2] | v->nb[2]) >> 24) return set_error(QWFN_ENOTSUP, "linear_attn: token strides of 2^24 bytes or more");
-        for (const qwfn_tensor * t : {q, k, v})
-            if (overlaps(dst->data, tensor_extent(dst), t->data, tensor_extent(t))) return set_error(QWFN_EINVAL, "linear_attn: dst overlaps q, k or v");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
         const int64_t ct = (dv + LA_COLS - 1) / LA_COLS;       // token by token
         const int64_t blocks = pl.step ? n_seq * n_v * ct : (pl.parts + 8) * n_v * std::max<int64_t>(pl.ct, pl.US / (4 * LA_THREADS) + 1);
@@ -956,6 +954,11 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         if (pl.bytes > 0 && (!ws || ws_bytes < pl.bytes))
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");
         if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, "linear_attn: ws must be 16-byte aligned");
+        const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, tensor_extent(k), "k"}, {v->data, tensor_extent(v), "v"},
+                           {g, (size_t) ((n_tok - 1) * g_token_stride + n_v) * 4, "g"}, {cu, (size_t) (n_seq + 1) * 4, "cu"},
+                           {slots, (size_t) n_seq * 4, "slots"}, {state_in != state_out ? state_in : nullptr, states, "state_in"}};
+        const span out[] = {{dst->data, tensor_extent(dst), "dst"}, {state_out, states, "state_out"}, {ws, pl.bytes, "ws"}};
+        if (int rc = check_overlaps("linear_attn", in, 7, out, 3)) return rc;
         la_args a{};
         if (int rc = status_word(&a.status)) return rc;
         a.q = (const char *) q->data; a.k = (const char *) k->data; a.v = (const char *) v->data; a.out = (char *) dst->data;

@@ -902,13 +902,16 @@ extern "C" int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_
         }
         if (table_stride < max_pages && B > 1) return err(QWFN_EINVAL, ": table rows overlap (table_stride < max_pages)");
         if (table_stride > 0x7fffffff) return err(QWFN_EINVAL, ": table_stride must be below 2^31");
-        // (a request's queries are read by several workgroups, and one of them may be done before another begins)
-        const size_t out = tensor_extent(dst);
-        if (overlaps(dst->data, out, q->data, tensor_extent(q))) return err(QWFN_EINVAL, ": dst overlaps q");
-        if (gate && gate->data != dst->data && overlaps(dst->data, out, gate->data, out)) return err(QWFN_EINVAL, ": dst overlaps gate");
         if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
         if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
         if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");
+        // (a request's queries are read by several workgroups, and one of them may be done before another begins)
+        const size_t rows = tensor_extent(dst);
+        const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, view_bytes(*k), "k"}, {v->data, view_bytes(*v), "v"},
+                           {gate && gate->data != dst->data ? gate->data : nullptr, rows, "gate"},
+                           {table, ((size_t) (B - 1) * table_stride + max_pages) * 4, "table"}, {n_kv, (size_t) B * 4, "n_kv"}};
+        const span out[] = {{dst->data, rows, "dst"}, {ws, pl.bytes, "ws"}};
+        if (int rc = check_overlaps("flash_attn_ext_paged", in, 6, out, 2)) return rc;
         if (!ws) {
             size_t got = 0;
             if (int rc = library_workspace(pl.bytes, pl.bytes, as_stream(stream), &ws, &got)) return rc;

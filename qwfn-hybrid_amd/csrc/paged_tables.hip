@@ -355,8 +355,6 @@ __global__ __launch_bounds__(PT_THREADS) void k_trim_once(trim_args a) {
 
 int scan_threads(int32_t n_seq) { return std::min(PT_THREADS, (n_seq + 63) / 64 * 64); }
 
-struct span { const void * p; size_t n; const char * name; };
-
 int check_tables(const char * op, int32_t n_seq, int32_t page_size, int64_t table_stride, int32_t max_pages,
                  int32_t free_cap, const void * ws, size_t ws_bytes) {
     const std::string o(op);
@@ -378,15 +376,7 @@ int check_spans(const char * op, const span * in, int n_in, const span * out, in
         const span & s = i < n_in ? in[i] : out[i - n_in];
         if (!is_aligned(s.p, 4)) return set_error(QWFN_EALIGN, std::string(op) + ": " + s.name + " must be 4-byte aligned");
     }
-    for (int i = 0; i < n_out; i++) {
-        for (int j = 0; j < n_in; j++)
-            if (overlaps(out[i].p, out[i].n, in[j].p, in[j].n))
-                return set_error(QWFN_EINVAL, std::string(op) + ": " + out[i].name + " overlaps " + in[j].name);
-        for (int j = 0; j < i; j++)
-            if (overlaps(out[i].p, out[i].n, out[j].p, out[j].n))
-                return set_error(QWFN_EINVAL, std::string(op) + ": " + out[i].name + " overlaps " + out[j].name);
-    }
-    return QWFN_OK;
+    return check_overlaps(op, in, n_in, out, n_out);
 }
 
 }  // namespace

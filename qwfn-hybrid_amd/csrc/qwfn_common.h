@@ -105,6 +105,19 @@ inline size_t tensor_extent(const qwfn_tensor * t) {
     return n;
 }
 
+// A call's tensors in memory: QWFN_EINVAL where one of `out` lies over another span. In-place pairs are passed once, and
+// what the call does not have is a NULL or of no bytes.
+struct span { const void * p; size_t n; const char * name; };
+inline int check_overlaps(const char * op, const span * in, int n_in, const span * out, int n_out) {
+    for (int i = 0; i < n_out; i++)
+        for (int j = 0; j < n_in + i; j++) {
+            const span & s = j < n_in ? in[j] : out[j - n_in];
+            if (overlaps(out[i].p, out[i].n, s.p, s.n))
+                return set_error(QWFN_EINVAL, std::string(op) + ": " + out[i].name + " overlaps " + s.name);
+        }
+    return QWFN_OK;
+}
+
 inline const char * type_name(int32_t t) {
     switch (t) {
         case QWFN_TYPE_F32:  return "f32";

@@ -250,3 +250,64 @@ def test_first_use_from_two_threads(monkeypatch, at):
     monkeypatch.setitem(sys.modules, "torch", Slow())
     K._Torch()
     assert found in ([[]], []) and (found or len(asked) <= at), (found, asked)
+
+
+def spans_linear():
+    """A call of linear_attn in parts, each tensor at a place of its own: the arguments, and each one's place and bytes."""
+    n, n_slots = 5000, 4
+    at = {name: FAKE + i * GB for i, name in enumerate(("q", "k", "v", "dst", "g", "cu", "slots", "s_in", "s_out", "ws"))}
+    size = dict(q=n * 256 * 2, k=n * 256 * 2, v=n * 768 * 2, dst=n * 768 * 2, g=n * 6 * 4, cu=16, slots=12,
+                s_in=n_slots * 6 * 128 * 128 * 4, s_out=n_slots * 6 * 128 * 128 * 4)
+    a = dict(q=heads(128, 2, n, at=at["q"]), k=heads(128, 2, n, at=at["k"]), v=heads(128, 6, n, at=at["v"]),
+             dst=heads(128, 6, n, at=at["dst"]), g=at["g"], cu=at["cu"], slots=at["slots"], s_in=at["s_in"], s_out=at["s_out"],
+             ws=at["ws"], max_len=n, n_slots=n_slots)
+    size["ws"] = K.load().qwfn_linear_attn_workspace_size(ctypes.byref(a["q"]), ctypes.byref(a["v"]), 3, n)
+    assert size["ws"] > 0
+    return a, at, size
+
+
+@pytest.mark.parametrize("out", ["dst", "s_out", "ws"])
+def test_linear_attention_outputs_over_other_tensors_refused(out):
+    """dst, the states and the workspace over the last bytes of every other tensor."""
+    label = dict(s_in="state_in", s_out="state_out")
+    _, at, size = spans_linear()
+    for name in at:
+        if name == out:
+            continue
+        a, at, size = spans_linear()
+        place = at[name] + (size[name] + 15) // 16 * 16 - 16
+        if out == "dst":
+            a["dst"].data = place
+        else:
+            a[out] = place
+        refused(linear(**a), K.EINVAL, "overlap")
+        msg = K.load().qwfn_last_error().decode()
+        assert label.get(out, out) in msg and label.get(name, name) in msg, msg
+
+
+@pytest.mark.parametrize("out", ["dst", "ws"])
+def test_paged_attention_outputs_over_other_tensors_refused(out):
+    def spans():
+        q, k, o = paged_views()
+        v = paged_views()[1]
+        gate = paged_views()[2]
+        at = {name: FAKE + i * GB for i, name in enumerate(("q", "k", "v", "dst", "gate", "table", "n_kv", "ws"))}
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "dst"), (gate, "gate")):
+            t.data = at[name]
+        row = 4 * 16 * 256 * 4
+        size = dict(q=row, k=640 * 544, v=640 * 544, dst=row, gate=row, table=(3 * 43 + 40) * 4, n_kv=16,
+                    ws=K.load().qwfn_fattn_workspace_size_paged(ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), 40, 16))
+        return dict(q=q, k=k, v=v, o=o, gate=gate, table=at["table"], stride=43, n_kv=at["n_kv"], ws=at["ws"]), at, size
+
+    for name in ("q", "k", "v", "dst", "gate", "table", "n_kv", "ws"):
+        if name == out:
+            continue
+        a, at, size = spans()
+        place = at[name] + (size[name] + 15) // 16 * 16 - 16
+        if out == "dst":
+            a["o"].data = place
+        else:
+            a["ws"] = place
+        refused(paged(**a), K.EINVAL, "overlap")
+        msg = K.load().qwfn_last_error().decode()
+        assert out in msg and name in msg, msg
