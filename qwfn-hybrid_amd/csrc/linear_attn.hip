@@ -811,7 +811,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
 
 int check_heads(const qwfn_tensor * t, int32_t type, const char * name, bool packed) {
     auto err = [&](int code, const char * what) { return set_error(code, std::string("linear_attn: ") + name + what); };
-    if (!t || !t->data) return err(QWFN_EINVAL, " is NULL");
+    if (!t || (!t->data && t->ne[2] != 0)) return err(QWFN_EINVAL, " is NULL");        // (no tokens, no address)
     if (t->type != type) return err(QWFN_EINVAL, " must be f32, f16 or bf16, one type for q, k, v and dst");
     const size_t es = type == QWFN_TYPE_F32 ? 4 : 2;
     if (t->ne[0] < 1 || t->ne[1] < 1 || t->ne[2] < 0 || t->ne[3] != 1) return err(QWFN_EINVAL, " must be [d, n_heads, n_tok]");
@@ -934,7 +934,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             if (k->ne[i] != q->ne[i]) return set_error(QWFN_EINVAL, "linear_attn: q and k must have the same shape");
         for (int i = 0; i < 3; i++)
             if (dst->ne[i] != v->ne[i]) return set_error(QWFN_EINVAL, "linear_attn: dst must have v's shape");
-        if (!g || !cu || !state_out) return set_error(QWFN_EINVAL, "linear_attn: g, cu or state_out is NULL");
+        if ((!g && q->ne[2] != 0) || !cu || !state_out) return set_error(QWFN_EINVAL, "linear_attn: g, cu or state_out is NULL");
         const int64_t n_v = v->ne[1], dk = q->ne[0], dv = v->ne[0], n_tok = q->ne[2];
         if (g_token_stride != 0 && g_token_stride < n_v) return set_error(QWFN_EINVAL, "linear_attn: g_token_stride must be 0 or at least n_v_heads");
         if (n_slots < 1 || (!slots && n_slots < n_seq)) return set_error(QWFN_EINVAL, "linear_attn: too few state slots");

@@ -311,3 +311,17 @@ def test_paged_attention_outputs_over_other_tensors_refused(out):
         refused(paged(**a), K.EINVAL, "overlap")
         msg = K.load().qwfn_last_error().decode()
         assert out in msg and name in msg, msg
+
+
+def test_linear_attention_without_tokens_has_no_addresses():
+    """An empty tensor of torch's has the address 0: a call of no tokens with it is one like another."""
+    import torch
+    assert torch.empty((0, 2, 64)).data_ptr() == 0
+    none = lambda h: heads(128, h, 0, at=None)  # noqa: E731
+    a = dict(q=none(2), k=none(2), v=none(6), dst=none(6))
+    assert linear(**a) == K.OK
+    assert linear(ws=None, ws_bytes=0, **a) == K.OK
+    assert linear(g=None, **a) == K.OK
+    assert K.load().qwfn_linear_attn_workspace_size(ctypes.byref(a["q"]), ctypes.byref(a["v"]), 3, 50) == 0
+    refused(linear(**{**a, "max_len": 0}), K.EINVAL, "max_len")
+    refused(linear(q=heads(128, 2, 100, at=None)), K.EINVAL, "q is NULL")
