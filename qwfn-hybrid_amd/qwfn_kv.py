@@ -440,7 +440,7 @@ def out_view(out) -> Tensor:
 def heads_view(x) -> Tensor:
     """Packed tokens torch [n_tok, n_heads, d] (contiguous rows) = ggml [d, n_heads, n_tok]."""
     n, h, d = x.shape
-    s, e = x.stride(), x.element_size()
+    s, e = x.stride() if n else (h * d, d, 1), x.element_size()          # (an empty tensor may have any strides)
     return _tensor4(x.data_ptr(), float_type(x), (d, h, n, 1), (s[2] * e, s[1] * e, s[0] * e, (n or 1) * s[0] * e))
 
 
@@ -879,7 +879,7 @@ def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=No
         if t is not None and (t.dtype is not f32 or t.get_device() != dev or not t.is_contiguous() or
                               t.shape != (state_out.size(0), n_v, dk, dv)):
             raise ValueError(f"linear_attn: {name} must be contiguous float32 [n_slots, {n_v}, {dk}, {dv}] on the current device")
-    if g.dtype is not f32 or g.get_device() != dev or g.size(-1) != n_v or (g.stride(-1) != 1 and n_v > 1) \
+    if g.dtype is not f32 or g.get_device() != dev or g.size(-1) != n_v or (g.stride(-1) != 1 and n_v > 1 and n_tok > 0) \
             or g.dim() not in (1, 2) or (g.dim() == 2 and g.size(0) < n_tok):
         raise ValueError(f"linear_attn: g must be float32 [{n_tok}, {n_v}] or [{n_v}] on the current device")
     for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
@@ -888,7 +888,7 @@ def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=No
     scale = dk ** -0.5 if scale is None else scale
     r = ctypes.byref
     return check(load().qwfn_linear_attn(
-        r(heads_view(q)), r(heads_view(k)), r(heads_view(v)), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0,
+        r(heads_view(q)), r(heads_view(k)), r(heads_view(v)), g.data_ptr(), g.stride(0) if g.dim() == 2 and n_tok > 0 else 0,
         cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.size(0),
         state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, r(heads_view(out)), *_ws(ws, dev),
         _stream_on(stream, dev)))

@@ -325,3 +325,15 @@ def test_linear_attention_without_tokens_has_no_addresses():
     assert K.load().qwfn_linear_attn_workspace_size(ctypes.byref(a["q"]), ctypes.byref(a["v"]), 3, 50) == 0
     refused(linear(**{**a, "max_len": 0}), K.EINVAL, "max_len")
     refused(linear(q=heads(128, 2, 100, at=None)), K.EINVAL, "q is NULL")
+
+
+def test_linear_attention_takes_empty_tensors_of_any_strides(monkeypatch):
+    """An empty tensor out of numpy has strides of 0: they say nothing, as there is nothing to step over."""
+    import numpy as np
+    import torch
+    empty = lambda *s: torch.from_numpy(np.zeros(s, np.float32))  # noqa: E731
+    assert empty(0, 4).stride() == (0, 0)
+    monkeypatch.setattr(K._Torch(), "device", staticmethod(lambda: -1))         # host tensors stand in; nothing is launched
+    q, v, g, state = empty(0, 2, 64), empty(0, 4, 64), empty(0, 4), torch.zeros((3, 4, 64, 64))
+    assert K.linear_attn_workspace_size(q, v, 3, 50) == 0
+    K.linear_attn(q, q, v, g, torch.zeros(4, dtype=torch.int32), 50, state, state, empty(0, 4, 64), stream=0)
