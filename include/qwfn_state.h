@@ -268,9 +268,13 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  *         slot at most once in a call; NULL: slot b). state_in NULL: zero states. A
  *         slot of -1: a zero state, and none is written; another slot outside
  *         [0, n_slots): the same, and bit 0 of qwfn_device_status. A sequence of no
- *         tokens leaves its slot of state_out unwritten. With two buffers, a step
- *         with rejected drafts is taken back by running the accepted tokens again
- *         from state_in.
+ *         tokens leaves its slot of state_out unwritten. -2 - s leaves the sequence out
+ *         whatever its length: its tokens are not read, their dst rows not written, and
+ *         slot s (which it counts as) is kept: with two buffers it is copied to
+ *         state_out (zeros without a state_in). With two buffers, a step with rejected drafts is taken back by
+ *         running the accepted tokens again from state_in; when the buffers then change
+ *         places, state_out has to hold every state that goes on: give the sequences
+ *         without tokens as -2 - s, as qwfn_paged_extend_states does, or copy their slots.
  * dk and dv multiples of 16, dk <= 256, dv <= 512. States, decays and sums are F32
  * (sums of decays inside a chunk F64; in chunks an F32 value above 3.39e38 counts as
  * infinite); the 16-bit types' products are exact, and on the way to

@@ -58,20 +58,35 @@ __device__ __forceinline__ void la_store4(char * p, int32_t type, float4 x) {
     else *(uint2 *) p = make_uint2(la_pack2(x.x, x.y, type), la_pack2(x.z, x.w, type));
 }
 
-// Sequence b: its first token and its length, and its state's slot (-1: none).
-struct la_seq { int32_t t0, len, slot; };
+// Sequence b: its first token and its length, its state's slot (-1: none), and the slot of a sequence that is left out
+// (then len is 0; -1: none).
+struct la_seq { int32_t t0, len, slot, held; };
 __device__ __forceinline__ la_seq la_sequence(const la_args & a, int b, bool report) {
     auto clip = [&](int32_t x) { return x < 0 ? 0 : x > a.n_tok ? a.n_tok : x; };
     const int32_t c0 = a.cu[b], c1 = a.cu[b + 1], lo = clip(c0), hi = clip(c1);
     int32_t len = hi - lo, slot = a.slots ? a.slots[b] : b;
     bool bad = lo != c0 || hi != c1 || len < 0 || len > a.max_len;
     len = len < 0 ? 0 : len > a.max_len ? a.max_len : len;
+    int32_t held = -1;
     if (slot < 0 || slot >= a.n_slots) {
-        bad |= slot != -1;
+        if (slot < -1 && -2 - slot < a.n_slots) {
+            held = -2 - slot;
+            len = 0;
+        } else {
+            bad |= slot != -1;
+        }
         slot = -1;
     }
     if (bad && report) atomicOr(a.status, DEVERR_SET_ROWS_INDEX);
-    return {lo, len, slot};
+    return {lo, len, slot, held};
+}
+
+// The state of head h of a sequence that is left out, from one buffer to the other: thread i of n.
+__device__ __forceinline__ void la_carry(const la_args & a, int32_t held, int h, int i, int n) {
+    if (held < 0 || a.s_in == a.s_out) return;
+    const size_t head = ((size_t) held * a.n_v + h) * a.dk * a.dv;
+    for (int e = i; 4 * e < a.dk * a.dv; e += n)
+        *(float4 *) (a.s_out + head + 4 * e) = a.s_in ? *(const float4 *) (a.s_in + head + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int DK>
@@ -82,7 +97,10 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, cq = tid & 15, rg = tid >> 4;
     const int cb = blockIdx.x % a.ct, h = blockIdx.x / a.ct % a.n_v, b = blockIdx.x / a.ct / a.n_v;
     const la_seq s = la_sequence(a, b, tid == 0 && cb == 0 && h == 0);
-    if (s.len == 0) return;
+    if (s.len == 0) {
+        la_carry(a, s.held, h, cb * LA_THREADS + tid, a.ct * LA_THREADS);
+        return;
+    }
     const int c = cb * LA_COLS + 4 * cq;
     const bool on = c < a.dv;                  // dv is a multiple of 16
     const size_t state = (size_t) a.n_v * a.dk * a.dv;
@@ -278,14 +296,15 @@ template <int NX, int NY, int NT> __device__ __forceinline__ v4f mfma_terms(cons
 }
 
 // A part of a sequence: its first token and length, how many parts of the sequence come before and after,
-// its place in the workspace, and the state's slot.
-struct lc_part { int32_t b, t0, len, before, after, index, slot; };
+// its place in the workspace, the state's slot, and that of a sequence that is left out (of no tokens: only where
+// sequences are whole).
+struct lc_part { int32_t b, t0, len, before, after, index, slot, held; };
 
 // Part `want` of the batch, parts in order of the sequences (by_seq: the first part of sequence `want`). Offsets that descend may let sequences share tokens and so
 // have more parts than the workspace: a sequence whose parts pass it is left out, by every launch alike.
 __device__ lc_part find_part(const lc_args & x, int want, bool by_seq, bool report, int threads, int32_t * sh) {
     const la_args & a = x.a;
-    lc_part p{want, 0, 0, 0, 0, want, -1};
+    lc_part p{want, 0, 0, 0, 0, want, -1, -1};
     if (x.L > 0) {
         // every thread counts the parts of a few sequences
         const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = (a.n_seq + threads - 1) / threads;
@@ -329,7 +348,7 @@ __device__ lc_part find_part(const lc_args & x, int want, bool by_seq, bool repo
         return p;
     }
     const la_seq s = la_sequence(a, want, report && threadIdx.x == 0);
-    return {want, s.t0, s.len, 0, 0, want, s.slot};
+    return {want, s.t0, s.len, 0, 0, want, s.slot, s.held};
 }
 
 // STATES: only what the part adds to the state, to the workspace.
@@ -352,7 +371,11 @@ __global__ __launch_bounds__(64 * NW, (lc_cfg<NT, DK, NW>::WAVES_EU)) void k_lin
     if (want >= x.parts) return;
     const lc_part part = find_part(x, want, false, !STATES && (x.L > 0 ? blk == 0 : cb == 0 && h == 0), F::THREADS, sh);
     if (part.b < 0) return;
-    if (part.len <= 0 || (STATES && part.after == 0)) return;
+    if (part.len <= 0) {
+        la_carry(a, part.held, h, cb * F::THREADS + tid, a.ct * F::THREADS);
+        return;
+    }
+    if (STATES && part.after == 0) return;
 
     const int hk = h / a.rep, c0 = cb * F::COLS;
     const char * qh = a.q + (int64_t) hk * a.q_nb1, * kh = a.k + (int64_t) hk * a.k_nb1;
@@ -772,8 +795,13 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
     const la_args & a = x.a;
     const int blocks = (x.US / 4 + LA_THREADS - 1) / LA_THREADS;
     const int eb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.n_v;
-    const lc_part part = find_part(x, blockIdx.x / blocks / a.n_v, true, false, LA_THREADS, sh);
-    if (part.b < 0 || part.after == 0) return;
+    const int b = blockIdx.x / blocks / a.n_v;
+    const lc_part part = find_part(x, b, true, false, LA_THREADS, sh);
+    if (part.b < 0) {
+        la_carry(a, la_sequence(a, b, false).held, h, eb * LA_THREADS + threadIdx.x, blocks * LA_THREADS);
+        return;
+    }
+    if (part.after == 0) return;
     const int e = eb * LA_THREADS + threadIdx.x;
     if (4 * e >= x.US) return;
     v4f s{0.f, 0.f, 0.f, 0.f};
@@ -868,7 +896,7 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     // holds: 11.9 us and 11.3 at 4 bf16 tokens, 14.9 and 13.6 at 6 of f16, 16.8 and 15.3 at 8 of f32; 9.6, 10.2 and 10.1
     // against 11.3, 13.6 and 15.3 at 2. At 64 sequences the sides meet at 6 f16 and 8 f32 tokens, and 4 bf16 tokens take 84
     // against 95.
-    p.step = max_len <= 2 + 2 * p.NT;
+    p.step = max_len <= 2 + 2 * p.NT || n_tok == 0;
     if (p.step) return p;
     p.NW = dv <= 2 * LC_WCOLS && (p.NT < 3 || p.DK < 256) ? 2 : 4;         // (256 rows of F32 for two waves are spilled)
     p.ct = (int32_t) ((dv + LC_WCOLS * p.NW - 1) / (LC_WCOLS * p.NW));
@@ -945,7 +973,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         if (state_in && state_in != state_out && (uintptr_t) state_in < (uintptr_t) state_out + states &&
             (uintptr_t) state_out < (uintptr_t) state_in + states)
             return set_error(QWFN_EINVAL, "linear_attn: state_in and state_out must be equal or not overlap");
-        if (n_tok == 0) return QWFN_OK;
+        if (n_tok == 0 && (!slots || state_in == state_out)) return QWFN_OK;
         if ((q->nb[2] | k->nb[2] | v->nb[2]) >> 24) return set_error(QWFN_ENOTSUP, "linear_attn: token strides of 2^24 bytes or more");
         const lc_plan pl = plan_linear(q, v, n_seq, max_len);
         const int64_t ct = (dv + LA_COLS - 1) / LA_COLS;       // token by token
@@ -955,7 +983,7 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
             return set_error(QWFN_ENOMEM, "linear_attn: ws must hold qwfn_linear_attn_workspace_size bytes");
         if (!is_aligned(ws, 16)) return set_error(QWFN_EALIGN, "linear_attn: ws must be 16-byte aligned");
         const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, tensor_extent(k), "k"}, {v->data, tensor_extent(v), "v"},
-                           {g, (size_t) ((n_tok - 1) * g_token_stride + n_v) * 4, "g"}, {cu, (size_t) (n_seq + 1) * 4, "cu"},
+                           {g, n_tok > 0 ? (size_t) ((n_tok - 1) * g_token_stride + n_v) * 4 : 0, "g"}, {cu, (size_t) (n_seq + 1) * 4, "cu"},
                            {slots, (size_t) n_seq * 4, "slots"}, {state_in != state_out ? state_in : nullptr, states, "state_in"}};
         const span out[] = {{dst->data, tensor_extent(dst), "dst"}, {state_out, states, "state_out"}, {ws, pl.bytes, "ws"}};
         if (int rc = check_overlaps("linear_attn", in, 7, out, 3)) return rc;

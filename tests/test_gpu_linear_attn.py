@@ -414,3 +414,73 @@ def test_outputs_in_chunks_are_rounded_once(gpu, dtype, lens, n_k, n_v, dk, dv):
         e[t0:t0 + m] = (3 * m + 64 + dk) * 2.0 ** -24 + (1 if dtype == torch.bfloat16 else 3) * 2.0 ** -16
     tol = h * np.abs(out) + (1 + h) * e * mag + (2.0 ** -25 if dtype == torch.float16 else 1e-30)
     assert (np.abs(o - out) <= tol).all(), np.max(np.abs(o - out) / tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,held", [(SINGLE, (1, 3, 4)), (LONG, (0, 1, 5)), ([700, 0, 40, 500], (1, 3)), ([5], (0,)),
+                                       ([900], (0,)), ([0, 0], (0, 1))])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (112, 208)])
+def test_sequences_left_out_keep_their_states(gpu, dtype, lens, held, dk, dv):
+    """Slots of -2 - s, for sequences with and without tokens: no output, the state as it was, in the other buffer too."""
+    for kw, case in ((dict(), {}), (dict(in_place=True), {}), (dict(), dict(zero=True))):
+        say(f"linear attention {dtype}: left out {held} of {lens} {kw} {case} dk={dk} dv={dv}")
+        c = Case(lens, 2, 4, dk, dv, dtype, seed=40, **case)
+        (out, mag, S, A), at = c.reference()
+        tol, st = c.bounds((out, mag, S, A))
+        c.slots = c.slots.copy()
+        for b in held:
+            c.slots[b] = -2 - c.slots[b]
+        gpu.device_status()
+        o, s = c.on_gpu(gpu, **kw)
+        assert gpu.device_status() == 0
+        o, s = o.float().cpu().numpy().astype(np.float64), s.cpu().numpy()
+        for b, (t0, m) in enumerate(zip(c.starts, c.lens)):
+            if b in held:
+                assert (o[t0:t0 + m] == 7.0).all()
+                assert np.array_equal(s[at[b]], c.state[at[b]] * np.float32(0 if c.zero else 1))
+            elif m:
+                assert (np.abs(o - out) <= tol)[t0:t0 + m].all()
+                assert (np.abs(s[at[b]] - S[b]) <= st[b]).all()
+        rest = [i for i in range(len(s)) if i not in set(at)]
+        assert np.array_equal(s[rest], c.state[rest] if kw else np.full_like(s[rest], 5.0))
+
+
+def test_left_out_slots_outside_the_states(gpu):
+    """-2 - s of a slot that is not there: a zero state that is not kept, and reported, as another bad slot."""
+    for lens in ([3, 1], [60, 40]):
+        say(f"linear attention: left-out slots outside, lens {lens}")
+        c = Case(lens, 1, 2, 64, 64, seed=41)
+        for bad in (-2 - len(c.state), -2 ** 31):
+            z = Case(lens, 1, 2, 64, 64, seed=41)
+            c.slots[0], z.state[z.slots[0]] = bad, 0
+            gpu.device_status()
+            o, s = c.on_gpu(gpu)
+            assert gpu.device_status() == gpu.DEVERR_SET_ROWS_INDEX
+            ref, at = z.reference()
+            assert (np.abs(host(o) - ref[0]) <= z.bounds(ref)[0]).all()
+            assert np.array_equal(host(s)[at[0]], np.full_like(host(s)[0], 5.0))
+
+
+@pytest.mark.parametrize("max_len", [1, 700])
+def test_no_tokens_at_all(gpu, max_len):
+    """An idle step of a batch: empty tensors; states that go on are carried over, the others left alone."""
+    K = gpu
+    say(f"linear attention: no tokens, max_len {max_len}")
+    q, v = (torch.zeros((0, h, 64), device="cuda", dtype=torch.bfloat16) for h in (1, 2))
+    g, cu = torch.zeros((0, 2), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    s_in = torch.randn((5, 2, 64, 64), device="cuda")
+    K.device_status()
+    for slots, want in ((None, []), ([2, 0, 4], []), ([2, -2, -6], [0, 4]), ([-1, -1, -5], [3])):
+        for src in (s_in, None):
+            out = torch.full_like(s_in, 5.0)
+            ws = torch.empty(16, dtype=torch.uint8, device="cuda")
+            K.linear_attn(q, q, v, g, cu, max_len, src, out, torch.empty_like(v), ws=ws,
+                          slots=None if slots is None else torch.tensor(slots, dtype=torch.int32, device="cuda"))
+            torch.cuda.synchronize()
+            ref = torch.full_like(s_in, 5.0)
+            ref[want] = s_in[want] if src is not None else 0.0
+            assert torch.equal(out, ref)
+    same = s_in.clone()
+    K.linear_attn(q, q, v, g, cu, max_len, same, same, torch.empty_like(v), slots=torch.tensor([2, -2, -6], dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(same, s_in) and K.device_status() == 0
