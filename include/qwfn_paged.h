@@ -11,7 +11,8 @@
  * request's ceil(length / page_size) pages are never read and may hold anything.
  * Free pages are a stack free_pages[0 .. n_free) in device memory.
  *
- * A decoding step: qwfn_paged_extend makes room and lists the new tokens' slots;
+ * A decoding step: qwfn_paged_extend makes room and lists the new tokens' slots
+ * (qwfn_paged_extend_states those of recurrent states too);
  * qwfn_set_rows_q8_0_kv (qwfn_kv.h) with idx = slots appends their K and V rows
  * in every layer; qwfn_flash_attn_ext_q8_0_paged attends; qwfn_paged_trim gives
  * back the pages of finished requests and rejected drafts. For a prompt,
@@ -71,6 +72,21 @@ int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, int32_t n_s
                       const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv, int32_t * cu_new, int32_t * slots,
                       int32_t * pos, int32_t * seq, int64_t n_tok, int32_t pad_slot, void * ws, size_t ws_bytes,
                       void * stream);
+
+/* The same, and for recurrent layers beside the cache (qwfn_linear_attn of
+ * qwfn_state.h, which takes cu_new) the state slots of the step:
+ *   states       I32 [n_seq] or NULL: the request's state slot, -1 for none (NULL: b)
+ *   state_slots  I32 [n_seq]: that slot where the request is served and has new
+ *                tokens, else -2 - slot, which leaves the request out there and
+ *                keeps its state (a negative slot is passed on as it is)
+ * cu_new lists the tokens of requests that are not served too: with other slots a
+ * layer would add them to states whose request stays where it was, and once more
+ * when it is asked again. */
+int qwfn_paged_extend_states(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size, int32_t * table,
+                             int64_t table_stride, int32_t max_pages, const int32_t * free_pages, int32_t free_cap,
+                             const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv, int32_t * cu_new, int32_t * slots,
+                             int32_t * pos, int32_t * seq, int64_t n_tok, int32_t pad_slot, const int32_t * states,
+                             int32_t * state_slots, void * ws, size_t ws_bytes, void * stream);
 
 /* The inverse: request b keeps its first n_keep[b] tokens (a negative count as 0,
  * one above n_kv[b] as n_kv[b]; 0 ends the request), and the pages behind them go

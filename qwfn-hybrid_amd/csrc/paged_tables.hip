@@ -55,6 +55,7 @@ struct ext_args {
     int64_t         n_tok;
     int32_t         n_seq, page, max_pages, pad_slot;
     int32_t         lists;             // the scan writes the lists and the table
+    const int32_t * states; int32_t * state_slots;        // NULL: slot b; not wanted
     pt_head *       head;
     pt_req *        req;
     uint32_t *      status;
@@ -111,6 +112,14 @@ __device__ __forceinline__ int32_t stack_size(const int32_t * n_free, int32_t ca
     return x;
 }
 
+// Request b's entry of state_slots: its slot, or -2 - its slot where the step adds nothing to its state. A negative slot is
+// none to mark.
+__device__ __forceinline__ void put_state(const ext_args & a, int64_t b, bool runs) {
+    if (!a.state_slots) return;
+    const int32_t s = a.states ? a.states[b] : (int32_t) b;
+    a.state_slots[b] = s < 0 || runs ? s : (int32_t) (0xfffffffeu - (uint32_t) s);
+}
+
 // Request b, a thread each, behind requests whose new tokens and needs sum to `before`.
 struct ext_sums { pt_req r; int64_t total, cu0, cu1, need, c; };
 __device__ __forceinline__ ext_sums extend_sums(const ext_args & a, int64_t b, int32_t n_free, pair64 before,
@@ -150,6 +159,7 @@ __global__ __launch_bounds__(PT_THREADS) void k_extend_scan(ext_args a) {
         if (in) {
             if (r.served) given += x.need;
             a.n_kv[b] = r.served ? (int32_t) x.total : r.past;
+            put_state(a, b, r.served && cu1 > cu0);
             if (b == 0) a.cu[0] = 0;
             a.cu[b + 1] = (int32_t) (cu1 < a.n_tok ? cu1 : a.n_tok);
             a.req[b] = r;
@@ -227,6 +237,7 @@ __global__ __launch_bounds__(PT_THREADS) void k_extend_once(ext_args a) {
     if (blockIdx.x == 0) {
         if (tid < a.n_seq) {
             a.n_kv[tid] = x.r.served ? (int32_t) x.total : x.r.past;
+            put_state(a, tid, x.r.served && x.cu1 > x.cu0);
             if (tid == 0) a.cu[0] = 0;
             a.cu[tid + 1] = end;
         }
@@ -379,6 +390,46 @@ int check_spans(const char * op, const span * in, int n_in, const span * out, in
     return check_overlaps(op, in, n_in, out, n_out);
 }
 
+int extend(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size, int32_t * table, int64_t table_stride,
+           int32_t max_pages, const int32_t * free_pages, int32_t free_cap, const int32_t * n_free, int32_t * n_free_out,
+           int32_t * n_kv, int32_t * cu_new, int32_t * slots, int32_t * pos, int32_t * seq, int64_t n_tok, int32_t pad_slot,
+           const int32_t * states, int32_t * state_slots, void * ws, size_t ws_bytes, void * stream) {
+    if (!n_past || !n_new || !table || !free_pages || !n_free || !n_free_out || !n_kv || !cu_new || (!slots && n_tok))
+        return set_error(QWFN_EINVAL, "paged_extend: NULL pointer");
+    if (int rc = check_tables("paged_extend", n_seq, page_size, table_stride, max_pages, free_cap, ws, ws_bytes))
+        return rc;
+    if (n_tok < 0 || n_tok > 0x7fffffff) return set_error(QWFN_EINVAL, "paged_extend: n_tok must lie in [0, 2^31)");
+    const size_t per = (size_t) n_seq * 4, tok = (size_t) n_tok * 4;
+    const size_t tab = ((size_t) (n_seq - 1) * table_stride + max_pages) * 4;
+    const span in[] = {{n_kv == n_past ? nullptr : n_past, per, "n_past"}, {n_new, per, "n_new"},
+                       {free_pages, (size_t) free_cap * 4, "free_pages"}, {states, per, "states"},
+                       {n_free_out == n_free ? nullptr : n_free, 4, "n_free"}};
+    const span out[] = {{table, tab, "table"}, {n_free_out, 4, "n_free_out"}, {n_kv, per, "n_kv"},
+                        {cu_new, per + 4, "cu_new"}, {slots, tok, "slots"}, {pos, tok, "pos"}, {seq, tok, "seq"},
+                        {state_slots, per, "state_slots"}, {ws, qwfn_paged_workspace_size(n_seq), "ws"}};
+    if (int rc = check_spans("paged_extend", in, 5, out, 9)) return rc;
+    ext_args a{};
+    if (int rc = status_word(&a.status)) return rc;
+    a.past = n_past; a.fresh = n_new; a.table = table; a.t_stride = table_stride;
+    a.free_pages = free_pages; a.free_cap = free_cap; a.n_free = n_free; a.n_free_out = n_free_out;
+    a.n_kv = n_kv; a.cu = cu_new; a.slots = slots; a.pos = pos; a.seq = seq; a.n_tok = n_tok;
+    a.states = states; a.state_slots = state_slots;
+    a.n_seq = n_seq; a.page = page_size; a.max_pages = max_pages; a.pad_slot = pad_slot;
+    a.head = (pt_head *) ws; a.req = (pt_req *) ((char *) ws + sizeof(pt_head));
+    a.lists = n_tok <= (int64_t) EXT_FEW * n_seq;
+    if (!a.lists && n_seq <= PT_THREADS && n_kv != n_past && n_free_out != n_free) {
+        const int threads = std::max(scan_threads(n_seq), ROW_THREADS);
+        hipLaunchKernelGGL(k_extend_once, dim3((unsigned) ((n_tok + threads - 1) / threads)), dim3(threads), 0, as_stream(stream), a);
+        return hip_check(hipGetLastError(), "paged_extend launch");
+    }
+    hipLaunchKernelGGL(k_extend_scan, dim3(1), dim3(scan_threads(n_seq)), 0, as_stream(stream), a);
+    if (int rc = hip_check(hipGetLastError(), "paged_extend launch")) return rc;
+    if (a.lists) return QWFN_OK;
+    hipLaunchKernelGGL(k_extend_lists, dim3((unsigned) ((n_tok + ROW_THREADS - 1) / ROW_THREADS)), dim3(ROW_THREADS), 0,
+                       as_stream(stream), a);
+    return hip_check(hipGetLastError(), "paged_extend launch");
+}
+
 }  // namespace
 }  // namespace qwfn
 
@@ -394,39 +445,21 @@ extern "C" int qwfn_paged_extend(const int32_t * n_past, const int32_t * n_new, 
                                  int32_t * cu_new, int32_t * slots, int32_t * pos, int32_t * seq, int64_t n_tok,
                                  int32_t pad_slot, void * ws, size_t ws_bytes, void * stream) {
     return ::qwfn::abi_call("paged_extend", [&]() -> int {
-        if (!n_past || !n_new || !table || !free_pages || !n_free || !n_free_out || !n_kv || !cu_new || (!slots && n_tok))
-            return set_error(QWFN_EINVAL, "paged_extend: NULL pointer");
-        if (int rc = check_tables("paged_extend", n_seq, page_size, table_stride, max_pages, free_cap, ws, ws_bytes))
-            return rc;
-        if (n_tok < 0 || n_tok > 0x7fffffff) return set_error(QWFN_EINVAL, "paged_extend: n_tok must lie in [0, 2^31)");
-        const size_t per = (size_t) n_seq * 4, tok = (size_t) n_tok * 4;
-        const size_t tab = ((size_t) (n_seq - 1) * table_stride + max_pages) * 4;
-        const span in[] = {{n_kv == n_past ? nullptr : n_past, per, "n_past"}, {n_new, per, "n_new"},
-                           {free_pages, (size_t) free_cap * 4, "free_pages"},
-                           {n_free_out == n_free ? nullptr : n_free, 4, "n_free"}};
-        const span out[] = {{table, tab, "table"}, {n_free_out, 4, "n_free_out"}, {n_kv, per, "n_kv"},
-                            {cu_new, per + 4, "cu_new"}, {slots, tok, "slots"}, {pos, tok, "pos"}, {seq, tok, "seq"},
-                            {ws, qwfn_paged_workspace_size(n_seq), "ws"}};
-        if (int rc = check_spans("paged_extend", in, 4, out, 8)) return rc;
-        ext_args a{};
-        if (int rc = status_word(&a.status)) return rc;
-        a.past = n_past; a.fresh = n_new; a.table = table; a.t_stride = table_stride;
-        a.free_pages = free_pages; a.free_cap = free_cap; a.n_free = n_free; a.n_free_out = n_free_out;
-        a.n_kv = n_kv; a.cu = cu_new; a.slots = slots; a.pos = pos; a.seq = seq; a.n_tok = n_tok;
-        a.n_seq = n_seq; a.page = page_size; a.max_pages = max_pages; a.pad_slot = pad_slot;
-        a.head = (pt_head *) ws; a.req = (pt_req *) ((char *) ws + sizeof(pt_head));
-        a.lists = n_tok <= (int64_t) EXT_FEW * n_seq;
-        if (!a.lists && n_seq <= PT_THREADS && n_kv != n_past && n_free_out != n_free) {
-            const int threads = std::max(scan_threads(n_seq), ROW_THREADS);
-            hipLaunchKernelGGL(k_extend_once, dim3((unsigned) ((n_tok + threads - 1) / threads)), dim3(threads), 0, as_stream(stream), a);
-            return hip_check(hipGetLastError(), "paged_extend launch");
-        }
-        hipLaunchKernelGGL(k_extend_scan, dim3(1), dim3(scan_threads(n_seq)), 0, as_stream(stream), a);
-        if (int rc = hip_check(hipGetLastError(), "paged_extend launch")) return rc;
-        if (a.lists) return QWFN_OK;
-        hipLaunchKernelGGL(k_extend_lists, dim3((unsigned) ((n_tok + ROW_THREADS - 1) / ROW_THREADS)), dim3(ROW_THREADS), 0,
-                           as_stream(stream), a);
-        return hip_check(hipGetLastError(), "paged_extend launch");
+        return extend(n_past, n_new, n_seq, page_size, table, table_stride, max_pages, free_pages, free_cap, n_free, n_free_out,
+                      n_kv, cu_new, slots, pos, seq, n_tok, pad_slot, nullptr, nullptr, ws, ws_bytes, stream);
+    });
+}
+
+extern "C" int qwfn_paged_extend_states(const int32_t * n_past, const int32_t * n_new, int32_t n_seq, int32_t page_size,
+                                        int32_t * table, int64_t table_stride, int32_t max_pages, const int32_t * free_pages,
+                                        int32_t free_cap, const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv,
+                                        int32_t * cu_new, int32_t * slots, int32_t * pos, int32_t * seq, int64_t n_tok,
+                                        int32_t pad_slot, const int32_t * states, int32_t * state_slots, void * ws,
+                                        size_t ws_bytes, void * stream) {
+    return ::qwfn::abi_call("paged_extend", [&]() -> int {
+        if (!state_slots) return set_error(QWFN_EINVAL, "paged_extend: NULL pointer");
+        return extend(n_past, n_new, n_seq, page_size, table, table_stride, max_pages, free_pages, free_cap, n_free, n_free_out,
+                      n_kv, cu_new, slots, pos, seq, n_tok, pad_slot, states, state_slots, ws, ws_bytes, stream);
     });
 }
 

@@ -159,7 +159,7 @@ EXPORTS = [
     "qwfn_qsa_pool_cfg_default", "qwfn_set_rows_f16", "qwfn_qsa_pool_decode", "qwfn_qsa_pool_rebuild",
     "qwfn_gated_delta_net", "qwfn_linear_attn_workspace_size", "qwfn_linear_attn",
     # include/qwfn_paged.h
-    "qwfn_paged_workspace_size", "qwfn_paged_extend", "qwfn_paged_trim", "qwfn_fattn_workspace_size_paged",
+    "qwfn_paged_workspace_size", "qwfn_paged_extend", "qwfn_paged_extend_states", "qwfn_paged_trim", "qwfn_fattn_workspace_size_paged",
     "qwfn_flash_attn_ext_q8_0_paged",
 ]
 
@@ -292,6 +292,8 @@ def load(path: str = LIB_PATH):
     L.qwfn_paged_workspace_size.argtypes = [i32]
     L.qwfn_paged_workspace_size.restype = sz
     L.qwfn_paged_extend.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp, sz, vp]
+    L.qwfn_paged_extend_states.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, vp, vp, vp,
+                                           sz, vp]
     L.qwfn_paged_trim.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp, sz, vp]
     L.qwfn_fattn_workspace_size_paged.argtypes = [T, T, T, i32, i32]
     L.qwfn_fattn_workspace_size_paged.restype = sz
@@ -807,20 +809,27 @@ def paged_workspace_size(n_seq: int) -> int:
 
 
 def paged_extend(n_past, n_new, page_size: int, table, free_pages, n_free, n_free_out, n_kv, cu_new, slots, pos=None,
-                 seq=None, pad_slot: int = -1, ws=None, stream=None):
+                 seq=None, pad_slot: int = -1, ws=None, stream=None, states=None, state_slots=None):
     """Pages and cache rows for n_new[b] more tokens of each request: device int32 n_past, n_new, n_kv [n_seq] (n_kv may
     be n_past), table [n_seq, max_pages], free_pages [free_cap], n_free, n_free_out [1] (may be one tensor), cu_new
-    [n_seq + 1], slots, pos, seq [n_tok]."""
+    [n_seq + 1], slots, pos, seq [n_tok]; state_slots [n_seq], if given: the slots of linear_attn in this step, out of
+    states [n_seq] (None: b)."""
     n_seq, n_tok, dev = n_past.numel(), slots.numel(), _Torch().device()
     _check_i32("paged_extend", dev, dict(
         n_past=(n_past, n_seq), n_new=(n_new, n_seq), free_pages=(free_pages, 0), n_free=(n_free, 1),
         n_free_out=(n_free_out, 1), n_kv=(n_kv, n_seq), cu_new=(cu_new, n_seq + 1), slots=(slots, n_tok), pos=(pos, n_tok),
-        seq=(seq, n_tok)), table, n_seq)
-    return check(load().qwfn_paged_extend(
+        seq=(seq, n_tok), states=(states, n_seq), state_slots=(state_slots, n_seq)), table, n_seq)
+    if states is not None and state_slots is None:
+        raise ValueError("paged_extend: states without state_slots")
+    args = (
         n_past.data_ptr(), n_new.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1),
         free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(), n_kv.data_ptr(),
         cu_new.data_ptr(), slots.data_ptr(), pos.data_ptr() if pos is not None else None,
-        seq.data_ptr() if seq is not None else None, n_tok, pad_slot, *_ws(ws, dev), _stream_on(stream, dev)))
+        seq.data_ptr() if seq is not None else None, n_tok, pad_slot)
+    if state_slots is None:
+        return check(load().qwfn_paged_extend(*args, *_ws(ws, dev), _stream_on(stream, dev)))
+    return check(load().qwfn_paged_extend_states(*args, states.data_ptr() if states is not None else None, state_slots.data_ptr(),
+                                                 *_ws(ws, dev), _stream_on(stream, dev)))
 
 
 def paged_trim(n_keep, n_kv, page_size: int, table, free_pages, n_free, n_free_out, n_kv_out, ws=None, stream=None):

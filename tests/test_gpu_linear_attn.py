@@ -484,3 +484,66 @@ def test_no_tokens_at_all(gpu, max_len):
     K.linear_attn(q, q, v, g, cu, max_len, same, same, torch.empty_like(v), slots=torch.tensor([2, -2, -6], dtype=torch.int32, device="cuda"))
     torch.cuda.synchronize()
     assert torch.equal(same, s_in) and K.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("two_buffers", [False, True])
+def test_hybrid_steps_of_a_short_pool(gpu, dtype, two_buffers):
+    """Steps whose pool has no room for some requests, which come again later, and of idle requests: a layer's states hold the
+    tokens of the served steps once each, in place and with two buffers that change places after every step."""
+    K, rng = gpu, np.random.default_rng(50)
+    B, n_k, n_v, d, page, n_pages = 4, 1, 2, 64, 16, 20
+    i32 = lambda x: dev(np.asarray(x, np.int32))  # noqa: E731
+    n_kv, table, free, n_free = i32([0] * B), i32(np.full((B, 40), -1)), i32(rng.permutation(n_pages)), i32([n_pages])
+    states, state_slots = i32([3, 0, 4, 1]), i32([0] * B)
+    at = host(states)
+    ws = torch.empty(K.paged_workspace_size(B), dtype=torch.uint8, device="cuda")
+    first = torch.full((5, n_v, d, d), float("nan"), device="cuda")           # (slot 2 belongs to nobody)
+    first[at.tolist()] = 0.0
+    buf = [first, torch.full_like(first, float("nan")) if two_buffers else first]
+    ref = mag = np.zeros((B, n_v, d, d))
+    lens, n_seen = [0] * B, 0
+    refused = []
+    #        prompts; the third does not fit      again, others decode       idle ones       room is made   single tokens, one refused
+    steps = [([100, 0, 250, 90], None), ([1, 40, 250, 1], None), ([1, 0, 0, 3], [0, 41, 0, 93]), ([0, 1, 130, 0], None),
+             ([1, 1, 1, 1], None), ([5, 9, 200, 2], [0, 51, 0, 80]), ([2, 0, 60, 1], None)]
+    for step, (new, keep) in enumerate(steps):
+        n, longest = sum(new), max(new)
+        cu, slots = i32([0] * (B + 1)), i32([0] * n)
+        K.paged_extend(n_kv, i32(new), page, table, free, n_free, n_free, n_kv, cu, slots, ws=ws, states=states, state_slots=state_slots)
+        after = list(host(n_kv))
+        runs = [m if a == x + m else 0 for m, a, x in zip(new, after, lens)]
+        refused.append([b for b in range(B) if new[b] != runs[b]])
+        say(f"hybrid step {step} {dtype} two_buffers={two_buffers}: lens {lens} new {new} refused {refused[-1]}")
+        c = Case(new, n_k, n_v, d, d, dtype, seed=60 + step)
+        out = torch.full_like(c.v, 7.0, device="cuda")
+        lw = torch.empty(max(16, K.linear_attn_workspace_size(c.q.cuda(), c.v.cuda(), B, longest)), dtype=torch.uint8, device="cuda")
+        K.linear_attn(c.q.cuda(), c.k.cuda(), c.v.cuda(), dev(c.g), cu, longest, buf[0], buf[1], out, slots=state_slots, scale=c.scale, ws=lw)
+        buf.reverse()
+        starts = list(np.cumsum([0] + new[:-1]))
+        o = host(out.float())
+        r = reference(*(x.float().numpy() for x in (c.q, c.k, c.v)), c.g, runs, starts, ref, c.scale, mag)
+        ref, mag, n_seen = r[2], r[3], n_seen + longest
+        # the bounds of Case.bounds over all the tokens there were; 16-bit outputs 2 2^-16 of the state's and scores' split
+        rel, h = (3 * n_seen + 64 * (step + 1) + d) * 2.0 ** -24, HALF_STEP[dtype]
+        for b, (t0, m) in enumerate(zip(starts, new)):
+            if runs[b]:
+                tol = h * np.abs(r[0]) + (1 + h) * (rel + (0 if dtype == torch.float32 else 2 * 2.0 ** -16)) * r[1] + 1e-30
+                assert (np.abs(o - r[0]) <= tol)[t0:t0 + m].all(), (step, b)
+            else:
+                assert (o[t0:t0 + m] == 7.0).all(), (step, b)
+        s = host(buf[0])
+        assert (np.abs(s[at] - ref) <= rel * mag + 1e-30).all(), step
+        assert np.isnan(s[2]).all()
+        lens = after
+        if keep is not None:                               # requests end: their cache rows go; their states start anew
+            K.paged_trim(i32(keep), n_kv, page, table, free, n_free, n_free, n_kv, ws=ws)
+            lens = [min(x, m) for x, m in zip(lens, keep)]
+            for b in range(B):
+                if keep[b] == 0:
+                    buf[0][at[b]] = 0.0
+                    ref, mag = ref.copy(), mag.copy()
+                    ref[b] = mag[b] = 0.0
+            assert list(host(n_kv)) == lens
+    assert any(refused) and not all(refused), refused
+    assert K.device_status() == K.DEVERR_PAGES

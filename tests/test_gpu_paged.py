@@ -602,3 +602,38 @@ def quantised(x):
     out[..., :2] = (amax[..., 0] / np.float32(127)).astype(np.float16)[..., None].view(np.uint8).reshape(len(x), 16, 2)
     out[..., 2:] = q.view(np.uint8)
     return out.reshape(len(x), 544)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("with_states", [False, True])
+@pytest.mark.parametrize("B,most_new", [(5, 3), (5, 90), (300, 2), (300, 40), (1024, 40), (1030, 40), (1030, 3)])
+def test_extend_state_slots(gpu, B, most_new, with_states, in_place):
+    """The slots of a step's recurrent states, by every way the lists are made; all else as without them."""
+    say(f"extend: state slots, B={B} new<={most_new} states={with_states} in_place={in_place}")
+    K, rng, page = gpu, np.random.default_rng(B + most_new), 16
+    past, new = rng.integers(0, 70, B), rng.integers(0, most_new + 1, B)
+    past[B // 2], new[B // 3] = -1, -1                     # (as lengths of 0)
+    max_pages, n_tok = 8, int(np.maximum(new, 0).sum()) - 2
+    free = rng.permutation(4 * B + 9).astype(np.int32)
+    n_free = sum(-(-(max(p, 0) + max(f, 0)) // page) - -(-max(p, 0) // page) for p, f in zip(past, new)) * 2 // 3
+    states = rng.permutation(B + 3)[:B].astype(np.int32)
+    states[rng.random(B) < 0.1] = -1
+    states[0] = -4
+    i32 = lambda x: dev(np.asarray(x, np.int32))  # noqa: E731
+    ids, got = rng.permutation(B * max_pages).reshape(B, max_pages), []
+    for slots_too in (False, True):
+        d = dict(past=i32(past), table=i32(ids), n_free=i32([n_free]), cu=i32([0] * (B + 1)), slots=i32([0] * n_tok),
+                 pos=i32([0] * n_tok), seq=i32([0] * n_tok), state_slots=torch.full((B + 2,), -99, dtype=torch.int32, device="cuda"))
+        d["n_kv"], d["nfo"] = (d["past"], d["n_free"]) if in_place else (i32([0] * B), i32([0]))
+        kw = dict(state_slots=d["state_slots"][1:B + 1], states=i32(states) if with_states else None) if slots_too else {}
+        K.paged_extend(d["past"], i32(new), page, d["table"], i32(free), d["n_free"], d["nfo"], d["n_kv"], d["cu"], d["slots"],
+                       pos=d["pos"], seq=d["seq"], ws=ws_of(K.paged_workspace_size(B)), **kw)
+        got.append({k: host(x) for k, x in d.items()})
+    K.device_status()
+    assert all(np.array_equal(got[0][k], got[1][k]) for k in got[0] if k != "state_slots")
+    p, f = np.maximum(past, 0), np.maximum(new, 0)
+    runs = (got[1]["n_kv"] == p + f) & (f > 0)
+    assert 0 < runs.sum() < B and ((got[1]["n_kv"] == p) & (f > 0)).any()
+    own = states if with_states else np.arange(B)
+    want = np.where(runs | (own < 0), own, -2 - own)
+    assert np.array_equal(got[1]["state_slots"], np.concatenate([[-99], want, [-99]]))

@@ -337,3 +337,19 @@ def test_linear_attention_takes_empty_tensors_of_any_strides(monkeypatch):
     q, v, g, state = empty(0, 2, 64), empty(0, 4, 64), empty(0, 4), torch.zeros((3, 4, 64, 64))
     assert K.linear_attn_workspace_size(q, v, 3, 50) == 0
     K.linear_attn(q, q, v, g, torch.zeros(4, dtype=torch.int32), 50, state, state, empty(0, 4, 64), stream=0)
+
+
+def test_extend_states_refusals():
+    def call(states=FAKE + 10 * GB, state_slots=FAKE + 11 * GB, **kw):
+        a = dict(past=FAKE, new=FAKE + GB, n_seq=4, page=16, table=FAKE + 2 * GB, stride=8, cols=8, free=FAKE + 3 * GB, cap=10,
+                 n_free=FAKE + 4 * GB, n_free_out=FAKE + 5 * GB, n_kv=FAKE + 6 * GB, cu=FAKE + 7 * GB, slots=FAKE + 8 * GB,
+                 pos=None, seq=None, n_tok=9, pad=-1)
+        a.update(kw)
+        return K.load().qwfn_paged_extend_states(*a.values(), states, state_slots, FAKE + 9 * GB, 1 << 20, None)
+    refused(call(state_slots=None), K.EINVAL, "NULL")
+    refused(call(n_seq=0), K.EINVAL, "n_seq")
+    refused(call(state_slots=FAKE + 11 * GB + 2), K.EALIGN, "state_slots")
+    refused(call(states=FAKE + 10 * GB + 1), K.EALIGN, "states")
+    refused(call(states=FAKE + 11 * GB + 12), K.EINVAL, "state_slots overlaps states")
+    refused(call(state_slots=FAKE + 4), K.EINVAL, "state_slots overlaps n_past")
+    refused(call(state_slots=FAKE + 8 * GB + 32), K.EINVAL, "state_slots overlaps slots")
