@@ -277,7 +277,8 @@ int qwfn_gated_delta_net(const float * q, int64_t q_token_stride, const float * 
  *         without tokens as -2 - s, as qwfn_paged_extend_states does, or copy their slots.
  * dk and dv multiples of 16, dk <= 256, dv <= 512. States, decays and sums are F32
  * (sums of decays inside a chunk F64; in chunks an F32 value above 3.39e38 counts as
- * infinite); the 16-bit types' products are exact, and on the way to
+ * infinite, and what an infinite value enters becomes NaN, where token by token it may
+ * become infinite); the 16-bit types' products are exact, and on the way to
  * an output the state and the scores keep 16 bits at least (24 of F32); outputs are
  * rounded once. Tokens outside every sequence (cu[0] > 0, past cu[n_seq]) are not
  * read and their dst rows not written. cu is read as clipped to [0, n_tok] and to

@@ -180,7 +180,7 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // type; on the way to an output the state and the weighted scores are rounded to NT
 // terms, two at least (2^-16 of each: an output is off by its own rounding, 1.7e-3 of the
 // result in bf16, whether its tokens run in chunks or one by one; with one term it was
-// 2.3e-3, and 101 us for 113 at 4096 tokens).
+// 2.3e-3, and 4096 tokens took 101 us for 113, replayed from a graph).
 // G and its differences are F64: a chunk's strong decays leave the weak ones exact.
 // A decay below e^-1000 counts as e^-1000, which is 0 in F32, so -inf is exact.
 //
@@ -197,12 +197,14 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_step(la_args a) {
 // hold it and a chunk has two barriers. f16 and f32 are taken apart on the way, the
 // next chunk waits in registers, and a chunk has three.
 // What bounds it: 4096 bf16 tokens of 48 heads of 128 move 134 MB of q, k, v and o and
-// the parts' states another 190 MB, 63 us at the rate of a copy, and take 113; the
-// vector units are busy 40 % of the loop (the state's scaling and its roundings), the
-// matrix cores 20 %, the rest are the waits between a chunk's dependent products.
+// the parts' states another 190 MB, 63 us at the rate of a copy, and take 104 in calls one
+// after another; the vector units are busy 45 % of the last launch (the state's scaling and
+// its roundings), the matrix cores 21 %, the rest are the waits between a chunk's
+// dependent products.
 //
 // A non-finite v_j must not reach tokens before j: a chunk that holds one takes its
-// scores times v by plain sums over j <= i.
+// scores times v by plain sums over j <= i. (The rest of a term of an infinity is NaN, so an
+// infinity comes out as NaN in its column where the recurrence may leave an infinity.)
 //
 // A long sequence is cut into parts that run at once: k_linear_chunks<.., true> leaves
 // each part's own contribution U to the state and its decay in the workspace,
@@ -882,9 +884,9 @@ template <int NT> int per_cu(int DK, int NW) {
 }
 
 // Parts of a sequence: as many as fill the CUs once with two waves a SIMD, so that no workgroup waits for another (4096
-// bf16 tokens of 48 heads of 128: 99 us in 10 parts, 120 in 5, 121 in 16, three waves a SIMD: a part's state goes
-// through the workspace three times), but no shorter than LC_MIN_PART tokens: a part costs a second pass over its k and v
-// (two f32 sequences of 509: 78 us with parts of 128, 93 of 256).
+// bf16 tokens of 48 heads of 128, with one term of the state and the scores: 99 us in 10 parts, 120 in 5, 121 in 16, three
+// waves a SIMD: a part's state goes through the workspace three times), but no shorter than LC_MIN_PART tokens: a part costs
+// a second pass over its k and v (two f32 sequences of 509: 78 us with parts of 128, 93 of 256).
 constexpr int64_t LC_CUS = 256, LC_MIN_PART = 128;
 
 lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq, int32_t max_len) {
@@ -903,7 +905,9 @@ lc_plan plan_linear(const qwfn_tensor * q, const qwfn_tensor * v, int32_t n_seq,
     const int64_t longest = std::min<int64_t>(max_len, n_tok), C = LC_C;
     const int per = p.NT == 1 ? per_cu<1>(p.DK, p.NW) : p.NT == 2 ? per_cu<2>(p.DK, p.NW) : per_cu<3>(p.DK, p.NW);
     const int64_t room = LC_CUS * std::min(per, 8 / p.NW) / (n_v * p.ct);
-    // a sequence's last part is half of one on average
+    // A sequence's last part is half of one on average (16 ragged f16 sequences: 75.8 us with the n_seq / 2, 73.8 without). So
+    // a batch of more than about 2 room sequences is not cut, however long one of them is: with 48 heads of 128 (room 10)
+    // from 18 sequences on.
     const int64_t whole = std::max<int64_t>(1, room - n_seq / 2);
     const int64_t L = (std::max<int64_t>(LC_MIN_PART, (n_tok + whole - 1) / whole) + C - 1) / C * C;
     p.parts = n_seq;

@@ -16,8 +16,9 @@
 // The KV heads and row groups of one run are blocks next to each other on one XCD:
 // the cache lines that two heads share come from one L2, and so do the rows that more
 // than 16 query rows need again (a workgroup of 32 query rows leaves one wave a SIMD:
-// 3 tokens of 8 requests with 12295 keys took 62 us that way, 55 this way, and 25 and 19
-// at 2 requests with 3000 keys).
+// 3 tokens of 8 requests with 12295 keys took 62 us that way and 52 this way, and 25 and 19
+// at 2 requests with 3000 keys). The rows of two row groups go from the L2 to the LDS twice:
+// those 8 requests 214 MB in 46 us, the 4.7 TB/s of one group's long requests.
 //
 // Inside a workgroup the 4 waves take every fourth tile of the run, each on its
 // own: no barrier, and no wave waits for another's data. A tile's rows come by LDS
@@ -788,7 +789,9 @@ struct pa_plan {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Runs: as many as fill the CUs, whole rounds of the 8 XCDs; no more than the longest requests could need.
+// Runs: as many as fill the CUs; no more than the longest requests could need. (Run g is on XCD g mod 8. Their number is
+// whole rounds of the 8 XCDs where heads and row groups divide 64; 85 runs, of 2 heads in 3 groups, leave some XCDs with 11
+// for the others' 10.)
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
