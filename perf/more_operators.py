@@ -362,7 +362,7 @@ def prepare(case, seed):
             s["kv"], s["vv"] = (K.cache_attn_view(c, c.shape[0], case["kvh"], case["D"]) for c in (s["kc"], s["vc"]))
             n = K.fattn_workspace_size_paged_tree(s["qv"], s["kv"], s["vv"], s["table"], case["page"])
         elif kind in ("fork", "release"):
-            n = K.paged_workspace_size(B)
+            n = K.paged_workspace_size(B) if kind == "fork" else K.paged_release_workspace_size(B, s["shared"].numel())
         elif kind == "compact":
             n = K.paged_compact_workspace_size(case["pages"])
         s["ws"] = torch.empty(max(256, n), dtype=torch.uint8, device=dev)
