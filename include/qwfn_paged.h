@@ -132,6 +132,140 @@ int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_tensor * k,
                                    const int32_t * n_kv, float scale, const qwfn_tensor * gate, const qwfn_tensor * dst,
                                    int variant, void * ws, size_t ws_bytes, void * stream);
 
+/* --------------------------------------------------------- shared pages
+ *
+ * Requests may hold pages together: shared[p] (I32 [n_pages], device memory, 0
+ * for a pool that starts) counts the requests that hold page p besides one, so
+ * qwfn_paged_extend, whose pages nobody else holds, has nothing to write there.
+ * Only whole pages are shared: the page that a request writes into is its own. A
+ * pool whose requests share pages gives them back by qwfn_paged_release, not by
+ * qwfn_paged_trim. shared_out, n_kv_out, n_free_out, table_out and free_out may be
+ * the array that they continue; apart from that no output overlaps an input or another
+ * output. n_seq <= 65536, max_pages * page_size, n_pages * page_size and
+ * table_stride < 2^31. */
+
+/* Requests that begin as copies of others (samples of one prompt, beams, a cached
+ * prefix): request b with from[b] = f >= 0 gets f's first n = n_tok[b] tokens
+ * (n_tok NULL: all). It is served if f < n_seq is itself not forked in this call
+ * (from[f] < 0), n_kv[b] is 0, 0 <= n <= n_kv[f], and n % page_size is 0 or a page is
+ * left: the requests that need one get them in order, the i-th
+ * free_pages[n_free - 1 - i]. Then, with F = n / page_size, r = n % page_size:
+ *   table[b][0 .. F)  f's, each page counted once more in shared_out
+ *   table[b][F]       the new page, if r > 0
+ *   moves[b]          I32 {source row, destination row, r} of qwfn_paged_copy, which
+ *                     brings the rest over in every layer; {0, 0, 0} where r = 0
+ *   state_moves[b]    (NULL: not wanted) {states[f], states[b], 1} for the recurrent
+ *                     states, if n = n_kv[f] and both slots are at least 0, else
+ *                     {0, 0, 0}; states NULL: request b has slot b
+ *   n_kv_out[b]       n; n_kv[b] for every request that is not served
+ * A request with from[b] >= 0 that is not served sets bit 2 of qwfn_device_status,
+ * as do a negative n_kv, one above max_pages * page_size (taken as 0 and as that), an
+ * n_free outside [0, free_cap] (clipped) and a shared page outside the pool (copied,
+ * not counted; its rest not moved). ws: qwfn_paged_workspace_size bytes. */
+int qwfn_paged_fork(const int32_t * from, const int32_t * n_tok, const int32_t * n_kv, int32_t n_seq, int32_t page_size,
+                    int32_t * table, int64_t table_stride, int32_t max_pages, const int32_t * shared, int32_t n_pages,
+                    const int32_t * free_pages, int32_t free_cap, const int32_t * n_free, int32_t * n_free_out,
+                    int32_t * n_kv_out, int32_t * shared_out, int32_t * moves, const int32_t * states, int32_t * state_moves,
+                    void * ws, size_t ws_bytes, void * stream);
+
+/* qwfn_paged_trim for pages that may be shared: request b keeps its first n_keep[b]
+ * tokens (0 ends it). Each page behind them counts one request less in shared_out;
+ * those that nobody holds any more go onto the stack, the lowest first. A request
+ * that would keep a part of a shared page (whose next token would be written into
+ * the others' page) keeps its length and its pages and sets bit 2 of
+ * qwfn_device_status; so do lengths and an n_free as in qwfn_paged_trim, a negative
+ * shared (taken as 0), and a page outside the pool (left out). free_cap at least n_pages;
+ * pages beyond it (of tables that hold one page more often than shared says) set the bit
+ * and are lost. */
+size_t qwfn_paged_release_workspace_size(int32_t n_seq, int32_t n_pages);
+int qwfn_paged_release(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq, int32_t page_size, const int32_t * table,
+                       int64_t table_stride, int32_t max_pages, const int32_t * shared, int32_t n_pages, int32_t * free_pages,
+                       int32_t free_cap, const int32_t * n_free, int32_t * n_free_out, int32_t * n_kv_out,
+                       int32_t * shared_out, void * ws, size_t ws_bytes, void * stream);
+
+/* Closes the pool's holes. The pages that are not on the stack are live, n_live of
+ * them; the live pages from n_live on move to the free pages below it, the k-th to the
+ * k-th. Writes:
+ *   page_map    I32 [n_pages]: where a live page is now, -1 for a free one (tables
+ *               of other requests over the same pool are renamed by it)
+ *   table_out   the ceil(n_kv / page_size) columns of every request, renamed (an entry
+ *               outside the pool, or on the stack, is kept and sets bit 2 of
+ *               qwfn_device_status)
+ *   shared_out  of the pages where they are now, 0 from n_live on
+ *   free_out    [0 .. n_pages - n_live): the pages from n_live on, the lowest on top
+ *   moves       I32 [n_moves][3] of qwfn_paged_copy: {source row, destination row,
+ *               page_size}, room for (n_pages + 1) / 2 of them; n_moves I32 [1]
+ * An n_free outside [0, free_cap], a stack entry outside the pool, one that is there twice
+ * and lengths as in qwfn_paged_trim set bit 2 too. free_cap at least n_pages. */
+size_t qwfn_paged_compact_workspace_size(int32_t n_pages);
+int qwfn_paged_compact(const int32_t * n_kv, int32_t n_seq, int32_t page_size, const int32_t * table, int64_t table_stride,
+                       int32_t max_pages, const int32_t * shared, int32_t n_pages, const int32_t * free_pages, int32_t free_cap,
+                       const int32_t * n_free, int32_t * table_out, int32_t * shared_out, int32_t * free_out,
+                       int32_t * n_free_out, int32_t * page_map, int32_t * moves, int32_t * n_moves, void * ws,
+                       size_t ws_bytes, void * stream);
+
+/* Rows copied inside each of n_caches tensors (the K and V of all layers, or the
+ * recurrent states with a slot a row): for every move {s, d, n} of the list rows
+ * s .. s + n - 1 go to d .. d + n - 1. caches: host array of tensors [ne0, n_rows] of one
+ * type, shape and row stride, rows contiguous, none over another. moves: device I32
+ * [cap][3]; n_moves: device I32 [1], how many of them count, or NULL for all cap. No
+ * row that a move writes may be read or written by another. A move with n = 0 is
+ * none; one with n outside [0, max_rows] or rows outside the tensor is left out and sets
+ * bit 0 of qwfn_device_status, as does an n_moves outside [0, cap] (clipped). One
+ * launch for up to 64 tensors. */
+int qwfn_paged_copy(const qwfn_tensor * caches, int32_t n_caches, const int32_t * moves, int32_t cap, const int32_t * n_moves,
+                    int32_t max_rows, void * stream);
+
+/* ------------------------------------------------ trees of drafted tokens
+ *
+ * A verify step over a tree: request b has T' = n_tree[b] <= T <= 64 drafted tokens
+ * (nodes; n_tree NULL: T, or all where it has fewer), its newest T' tokens in the cache (extend them as usual).
+ * Node t's parent precedes it; masks[b][t] (64-bit words, [n_seq][T]) has the bit of
+ * every node that t sees, t itself among them. Per step: qwfn_tree_masks; per
+ * attention layer qwfn_flash_attn_ext_q8_0_paged_tree, per recurrent layer
+ * qwfn_linear_attn_tree (qwfn_state.h); then qwfn_paged_accept keeps one path,
+ * qwfn_paged_trim (or _release) with its n_keep gives back the rest, and
+ * qwfn_linear_attn over the rows of path (qwfn_get_rows_i32) with cu_path brings
+ * the recurrent states forward. */
+
+/* parents I32 [n_seq][T]: -1 for a child of the context's last token, else an earlier
+ * node (another value counts as -1 and sets bit 2 of qwfn_device_status).
+ *   masks  the node and its ancestors; 0 for t >= n_tree[b]
+ *   pos    I32 [n_seq][T] or NULL: n_past[b] + the number of t's ancestors, for the
+ *          rope; -1 for t >= n_tree[b]. n_past NULL: 0
+ * An n_tree outside [0, T] is clipped and sets the bit. */
+int qwfn_tree_masks(const int32_t * parents, const int32_t * n_tree, const int32_t * n_past, int32_t n_seq, int32_t T,
+                    uint64_t * masks, int32_t * pos, void * stream);
+
+/* qwfn_flash_attn_ext_q8_0_paged with queries that are nodes of a tree: q [D, T, n_head,
+ * n_seq]; query t < n_tree[b] of request b sees the n_kv[b] - n_tree[b] tokens before the
+ * tree and the nodes in masks[b][t] (any bits; those from n_tree[b] on count for
+ * nothing), a query that sees nothing and queries from n_tree[b] on give 0. Arguments,
+ * limits and arithmetic as there, but T <= 64 and T * n_head / n_head_kv <= 1024. An n_tree
+ * outside [0, min(T, n_kv[b])] is clipped and sets bit 1 of qwfn_device_status. */
+size_t qwfn_fattn_workspace_size_paged_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                            int32_t max_pages, int32_t page_size);
+int qwfn_flash_attn_ext_q8_0_paged_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                        const int32_t * table, int64_t table_stride, int32_t max_pages, int32_t page_size,
+                                        const int32_t * n_kv, const int32_t * n_tree, const uint64_t * masks, float scale,
+                                        const qwfn_tensor * gate, const qwfn_tensor * dst, int variant, void * ws,
+                                        size_t ws_bytes, void * stream);
+
+/* The path from the context to node leaf[b] (-1: nothing is accepted), which is
+ * masks[b][leaf[b]], m nodes t_0 < t_1 < ..: with B = n_kv[b] - n_tree[b] token B + t_i becomes
+ * token B + i in every cache (as in qwfn_paged_copy: tensors [ne0, n_rows], at most 64).
+ *   n_keep   I32 [n_seq]: B + m, for qwfn_paged_trim / _release
+ *   cu_path  I32 [n_seq + 1] or NULL: the sums of m before each request
+ *   path     I32 [n_seq * T] or NULL (NULL if cu_path is): b * T + t_i at cu_path[b] + i; 0
+ *            behind cu_path[n_seq]
+ * A leaf outside [-1, n_tree[b]) counts as -1, an n_tree outside [0, min(T, n_kv)] and an
+ * n_kv outside [0, max_pages * page_size] are clipped, a row whose page lies outside the
+ * caches is not moved; each sets bit 2 of qwfn_device_status. One launch. */
+int qwfn_paged_accept(const qwfn_tensor * caches, int32_t n_caches, const int32_t * table, int64_t table_stride,
+                      int32_t max_pages, int32_t page_size, const int32_t * n_kv, const int32_t * n_tree,
+                      const uint64_t * masks, const int32_t * leaf, int32_t n_seq, int32_t T, int32_t * n_keep,
+                      int32_t * cu_path, int32_t * path, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -296,6 +296,24 @@ int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_te
                      int32_t n_slots, const float * state_in, float * state_out, float scale, const qwfn_tensor * dst,
                      void * ws, size_t ws_bytes, void * stream);
 
+/* The outputs of qwfn_linear_attn for the nodes of a tree of drafted tokens (qwfn_paged.h),
+ * without a step of the state: token b * T + t of the packed tensors is node t <
+ * n_tree[b] <= T <= 64 of request b (n_tree: device I32 or NULL for T), and with G_t the
+ * sum of g over the nodes of masks[b][t] (64-bit words [n_seq][T]; bits from n_tree[b] on
+ * count for nothing)
+ *   out[t] = scale (exp(G_t) S^T q_t + sum over j in masks[b][t] of exp(G_t - G_j) (q_t . k_j) v_j)
+ * which is the recurrence along the path to t where masks are qwfn_tree_masks'. Nodes
+ * from n_tree[b] on are not read and give 0. q, k, v, g, dst, the slots and the states as in
+ * qwfn_linear_attn (n_tok = n_seq * T; state may be NULL: zeros; a slot of -2 - s leaves the
+ * request out, its dst rows are not written). A decay below exp(-693) counts as that. F32
+ * products and sums for every type, sums of decays F64; what a node does not see never
+ * reaches it, infinite or not. An n_tree outside [0, T] is clipped and sets bit 0 of
+ * qwfn_device_status, as does a slot outside [-1 - n_slots, n_slots). One launch. */
+int qwfn_linear_attn_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const float * g,
+                          int64_t g_token_stride, const int32_t * n_tree, const uint64_t * masks, int32_t n_seq, int32_t T,
+                          const int32_t * slots, int32_t n_slots, const float * state, float scale, const qwfn_tensor * dst,
+                          void * stream);
+
 /* ------------------------------------------------- QSA index producer */
 
 /* The indexer's key geometry and the rope / norm constants of the model

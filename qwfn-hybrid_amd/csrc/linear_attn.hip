@@ -837,10 +837,220 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
     }
 }
 
+// ---------------------------------------------------------------- the nodes of a drafted tree
+//
+// With G_t the sum of g over what node t sees, S the state before the tree:
+//   o_t = scale (e^{G_t} S^T q_t + sum over j that t sees of e^{G_t - G_j} (q_t . k_j) v_j)
+// the chunk form above with the tree's masks in the place of j <= i, and no step of the state. What bounds it: the
+// states, read once, 4 dk dv bytes a head and request.
+//
+// A workgroup takes 64 CW columns of one head of one request, 4 / CW waves 64 of them each over a slice of the rows. Products
+// run on v_mfma_f32_16x16x4_f32, so every type is exact until a sum rounds: lane (m, l) holds for step i of a slice row
+// lo + l n + i (n = the slice's rows / 4), so that a lane's operands are consecutive in memory, and columns 4 m + j of
+// tile j, so that a row of the state is one 16-byte load a lane and 256 bytes a 16 lanes. The state's loads go out first and
+// come in while q, k and the scores are made.
+//
+// A v_j that is not finite must not reach nodes that do not see it (0 times infinity): a workgroup that holds one takes its
+// scores times v by plain sums over the masks.
+constexpr int LT_THREADS = 256;
+
+struct lt_args {
+    la_args          a;                // cu unused; max_len is T
+    const int32_t *  n_tree; const uint64_t * masks;
+};
+
+template <int DK, int TT, int CW> struct lt_cfg {
+    static constexpr int KS = 4 / CW;                    // slices of the rows
+    static constexpr int N = 16 * TT;                    // nodes, padded
+    static constexpr int RPL = DK / KS / 4;              // rows of a lane
+    static constexpr int QS = DK + 4, PS = N + 4;        // floats of a row of q and k, of the scores, in LDS
+    static constexpr int JPL = N / 4 / KS > 0 ? N / 4 / KS : 1;            // nodes of a lane in the scores' product
+    static constexpr int OQ = 0, OK = N * QS, OP = 2 * N * QS, RED = (KS - 1) * CW * TT * 4 * 64 * 4;
+    static constexpr int LDS = OP + N * PS > RED ? OP + N * PS : RED;      // floats
+    static_assert(JPL * 4 * KS == N, "whole nodes a lane");
+    static_assert(LDS * 4 + 1536 <= 160 * 1024, "LDS of a CU");
+};
+
+__device__ __forceinline__ v4f mfma_f32(float x, float y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, z, 0, 0, 0); }
+
+template <int DK, int TT, int CW>
+__global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
+    using F = lt_cfg<DK, TT, CW>;
+    __shared__ __attribute__((aligned(16))) float lds[F::LDS];
+    __shared__ double gl[64], G[64];
+    __shared__ float eG[64];
+    __shared__ int odd;
+    const la_args & a = x.a;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, l = lane >> 4, w = tid >> 6, cw = w % CW, ks = w / CW;
+    const int cb = blockIdx.x % a.ct, h = blockIdx.x / a.ct % a.n_v, b = blockIdx.x / a.ct / a.n_v, T = a.max_len;
+    int32_t nt = x.n_tree ? x.n_tree[b] : T, slot = a.slots ? a.slots[b] : b;
+    bool bad = nt < 0 || nt > T;
+    nt = nt < 0 ? 0 : nt > T ? T : nt;
+    const bool out = slot < -1 && -2 - slot < a.n_slots;                   // left out
+    if (slot < 0 || slot >= a.n_slots) {
+        bad |= slot != -1 && !out;
+        slot = -1;
+    }
+    if (bad && tid == 0 && cb == 0 && h == 0) atomicOr(a.status, DEVERR_SET_ROWS_INDEX);
+    if (out) return;
+    const int es = a.type == QWFN_TYPE_F32 ? 4 : 2;
+    const int c = (cb * CW + cw) * LA_COLS + 4 * m;
+    const bool on = c < a.dv;                                              // (dv is a multiple of 16)
+    const int64_t t0 = (int64_t) b * T;
+
+    // the state's rows of the lane
+    float4 S[F::RPL];
+    const int row0 = ks * (DK / F::KS) + l * F::RPL;
+    const float * sp = a.s_in + ((int64_t) (slot < 0 ? 0 : slot) * a.n_v + h) * a.dk * a.dv + c;
+#pragma unroll
+    for (int i = 0; i < F::RPL; i++) {
+        S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on && slot >= 0 && a.s_in && row0 + i < a.dk) S[i] = *(const float4 *) (sp + (int64_t) (row0 + i) * a.dv);
+    }
+    // v of the lane's nodes
+    float4 V[F::JPL];
+    const int j0 = (ks * 4 + l) * F::JPL;
+    const char * vh = a.v + (int64_t) h * a.v_nb1 + (int64_t) c * es;
+#pragma unroll
+    for (int i = 0; i < F::JPL; i++) {
+        V[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on && j0 + i < nt) V[i] = la_load4(vh + (t0 + j0 + i) * a.v_nb2, a.type);
+    }
+    // q and k
+    const char * qh = a.q + (int64_t) (h / a.rep) * a.q_nb1, * kh = a.k + (int64_t) (h / a.rep) * a.k_nb1;
+    for (int u = tid; u < 2 * F::N * (DK / 4); u += LT_THREADS) {
+        const int e4 = u % (DK / 4), t = u / (DK / 4) % F::N, which = u / (DK / 4) / F::N;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (4 * e4 < a.dk && t < nt) f = la_load4((which ? kh + (t0 + t) * a.k_nb2 : qh + (t0 + t) * a.q_nb2) + 4 * e4 * es, a.type);
+        *(float4 *) &lds[(which ? F::OK : F::OQ) + t * F::QS + 4 * e4] = f;
+    }
+    // decays
+    const uint64_t live = nt < 64 ? (1ull << nt) - 1 : ~0ull;
+    if (tid < 64) {
+        const double g = tid < nt ? (double) a.g[(t0 + tid) * a.g_ts + h] * LC_LOG2E : 0.;
+        gl[tid] = g < (double) LC_FLOOR ? (double) LC_FLOOR : g;
+    }
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    if (tid < 64) {
+        double sum = 0.;
+        if (tid < nt)
+            for (uint64_t k = x.masks[t0 + tid] & live; k; k &= k - 1) sum += gl[__builtin_ctzll(k)];
+        G[tid] = sum;
+        eG[tid] = __builtin_amdgcn_exp2f((float) sum);
+    }
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < F::JPL; i++)
+        fine = fine && fabsf(V[i].x) < INFINITY && fabsf(V[i].y) < INFINITY && fabsf(V[i].z) < INFINITY && fabsf(V[i].w) < INFINITY;
+    if (!fine) odd = 1;
+    __syncthreads();
+
+    // scores, a tile a wave in turn: lane (node j = m, nodes t = 4 l + r)
+    constexpr int SR = DK / 4;                                             // rows of a lane
+    for (int tile = w; tile < TT * TT; tile += 4) {
+        const int ti = tile / TT, tj = tile % TT;
+        v4f s{0.f, 0.f, 0.f, 0.f};
+        const float * qp = &lds[F::OQ + (16 * ti + m) * F::QS + l * SR], * kp = &lds[F::OK + (16 * tj + m) * F::QS + l * SR];
+#pragma unroll
+        for (int i = 0; i < SR; i += 4) {
+            const float4 y = *(const float4 *) (qp + i), z = *(const float4 *) (kp + i);
+            s = mfma_f32(y.x, z.x, s);
+            s = mfma_f32(y.y, z.y, s);
+            s = mfma_f32(y.z, z.z, s);
+            s = mfma_f32(y.w, z.w, s);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int t = 16 * ti + 4 * l + r, j = 16 * tj + m;
+            const bool sees = t < nt && ((x.masks[t0 + (t < nt ? t : 0)] & live) >> j & 1);
+            lds[F::OP + t * F::PS + j] = sees ? s[r] * __builtin_amdgcn_exp2f((float) (G[t] - G[j])) : 0.f;
+        }
+    }
+    // the state's part
+    v4f O[TT][4] = {};
+#pragma unroll
+    for (int i = 0; i < F::RPL; i += 4) {
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) {
+            const float4 y = *(const float4 *) &lds[F::OQ + (16 * tt + m) * F::QS + row0 + i];
+            const float q4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                O[tt][0] = mfma_f32(q4[k], S[i + k].x, O[tt][0]);
+                O[tt][1] = mfma_f32(q4[k], S[i + k].y, O[tt][1]);
+                O[tt][2] = mfma_f32(q4[k], S[i + k].z, O[tt][2]);
+                O[tt][3] = mfma_f32(q4[k], S[i + k].w, O[tt][3]);
+            }
+        }
+    }
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) O[tt][j][r] *= eG[16 * tt + 4 * l + r];
+    __syncthreads();
+    // the scores' part
+    if (!odd) {
+#pragma unroll
+        for (int i = 0; i < F::JPL; i++)
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) {
+                const float p = lds[F::OP + (16 * tt + m) * F::PS + j0 + i];
+                O[tt][0] = mfma_f32(p, V[i].x, O[tt][0]);
+                O[tt][1] = mfma_f32(p, V[i].y, O[tt][1]);
+                O[tt][2] = mfma_f32(p, V[i].z, O[tt][2]);
+                O[tt][3] = mfma_f32(p, V[i].w, O[tt][3]);
+            }
+    } else if (ks == 0 && on) {
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 16 * tt + 4 * l + r;
+                if (t >= nt) continue;
+                for (uint64_t k = x.masks[t0 + t] & live; k; k &= k - 1) {
+                    const int j = __builtin_ctzll(k);
+                    const float p = lds[F::OP + t * F::PS + j];
+                    const float4 v = la_load4(vh + (t0 + j) * a.v_nb2, a.type);
+                    O[tt][0][r] += p * v.x; O[tt][1][r] += p * v.y; O[tt][2][r] += p * v.z; O[tt][3][r] += p * v.w;
+                }
+            }
+    }
+    // the slices' sums meet
+    __syncthreads();
+    if (ks > 0) {
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) *(v4f *) &lds[(((((ks - 1) * CW + cw) * TT + tt) * 4 + j) * 64 + lane) * 4] = O[tt][j];
+    }
+    __syncthreads();
+    if (ks > 0 || !on) return;
+    char * oh = a.out + ((int64_t) h * a.dv + c) * es;
+    const int64_t o_ts = (int64_t) a.n_v * a.dv * es;
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++) {
+#pragma unroll
+        for (int k = 1; k < F::KS; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) O[tt][j] += *(const v4f *) &lds[(((((k - 1) * CW + cw) * TT + tt) * 4 + j) * 64 + lane) * 4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int t = 16 * tt + 4 * l + r;
+            if (t >= T) continue;
+            float4 o = make_float4(O[tt][0][r] * a.scale, O[tt][1][r] * a.scale, O[tt][2][r] * a.scale, O[tt][3][r] * a.scale);
+            if (t >= nt) o = make_float4(0.f, 0.f, 0.f, 0.f);
+            la_store4(oh + (t0 + t) * o_ts, a.type, o);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- host
 
-int check_heads(const qwfn_tensor * t, int32_t type, const char * name, bool packed) {
-    auto err = [&](int code, const char * what) { return set_error(code, std::string("linear_attn: ") + name + what); };
+int check_heads(const qwfn_tensor * t, int32_t type, const char * name, bool packed, const char * op = "linear_attn") {
+    auto err = [&](int code, const char * what) { return set_error(code, std::string(op) + ": " + name + what); };
     if (!t || (!t->data && t->ne[2] != 0)) return err(QWFN_EINVAL, " is NULL");        // (no tokens, no address)
     if (t->type != type) return err(QWFN_EINVAL, " must be f32, f16 or bf16, one type for q, k, v and dst");
     const size_t es = type == QWFN_TYPE_F32 ? 4 : 2;
@@ -943,6 +1153,22 @@ int launch_type(const lc_args & x, const lc_plan & p, hipStream_t s) {
     return launch_chunks<NT, 256, 4>(x, p, s);
 }
 
+template <int DK, int TT>
+void launch_tree(const lt_args & x, unsigned blocks, bool wide, hipStream_t s) {
+    if (wide) hipLaunchKernelGGL((k_linear_tree<DK, TT, 2>), dim3(blocks), dim3(LT_THREADS), 0, s, x);
+    else      hipLaunchKernelGGL((k_linear_tree<DK, TT, 1>), dim3(blocks), dim3(LT_THREADS), 0, s, x);
+}
+template <int DK>
+int launch_tree(const lt_args & x, unsigned blocks, bool wide, hipStream_t s) {
+    switch ((x.a.max_len + 15) / 16) {
+        case 1:  launch_tree<DK, 1>(x, blocks, wide, s); break;
+        case 2:  launch_tree<DK, 2>(x, blocks, wide, s); break;
+        case 3:  launch_tree<DK, 3>(x, blocks, wide, s); break;
+        default: launch_tree<DK, 4>(x, blocks, wide, s); break;
+    }
+    return hip_check(hipGetLastError(), "linear_attn_tree launch");
+}
+
 }  // namespace
 }  // namespace qwfn
 
@@ -1011,5 +1237,64 @@ extern "C" int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, co
         else if (dk <= 128) hipLaunchKernelGGL(k_linear_step<128>, grid, blk, 0, as_stream(stream), a);
         else                hipLaunchKernelGGL(k_linear_step<256>, grid, blk, 0, as_stream(stream), a);
         return hip_check(hipGetLastError(), "linear_attn launch");
+    });
+}
+
+extern "C" int qwfn_linear_attn_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const float * g,
+                                     int64_t g_token_stride, const int32_t * n_tree, const uint64_t * masks, int32_t n_seq,
+                                     int32_t T, const int32_t * slots, int32_t n_slots, const float * state, float scale,
+                                     const qwfn_tensor * dst, void * stream) {
+    return ::qwfn::abi_call("linear_attn_tree", [&]() -> int {
+        const char * op = "linear_attn_tree";
+        auto err = [&](int code, const char * what) { return set_error2(code, op, what); };
+        if (!q || !k || !v || !dst) return err(QWFN_EINVAL, ": q, k, v or dst is NULL");
+        if (q->type != QWFN_TYPE_F32 && q->type != QWFN_TYPE_F16 && q->type != QWFN_TYPE_BF16)
+            return err(QWFN_EINVAL, ": q must be f32, f16 or bf16");
+        if (int rc = check_heads(q, q->type, "q", false, op)) return rc;
+        if (int rc = check_heads(k, q->type, "k", false, op)) return rc;
+        if (int rc = check_heads(v, q->type, "v", false, op)) return rc;
+        if (int rc = check_heads(dst, q->type, "dst", true, op)) return rc;
+        if (n_seq < 1 || n_seq > 65535) return err(QWFN_EINVAL, ": n_seq must lie in [1, 65535]");
+        if (T < 1 || T > 64) return err(QWFN_ENOTSUP, ": T must lie in [1, 64]");
+        const int64_t n_v = v->ne[1], dk = q->ne[0], dv = v->ne[0], n_tok = q->ne[2];
+        if (n_tok != (int64_t) n_seq * T || v->ne[2] != n_tok) return err(QWFN_EINVAL, ": q, k and v must hold n_seq * T tokens");
+        for (int i = 0; i < 3; i++)
+            if (k->ne[i] != q->ne[i]) return err(QWFN_EINVAL, ": q and k must have the same shape");
+        for (int i = 0; i < 3; i++)
+            if (dst->ne[i] != v->ne[i]) return err(QWFN_EINVAL, ": dst must have v's shape");
+        if (dk % 16 || dv % 16 || dk > 256 || dv > 512) return err(QWFN_ENOTSUP, ": dk and dv must be multiples of 16, dk at most 256, dv at most 512");
+        if (n_v % q->ne[1]) return err(QWFN_EINVAL, ": n_v_heads must be a multiple of n_k_heads");
+        if (n_v > 1024) return err(QWFN_EINVAL, ": n_v_heads at most 1024");
+        if (!g || !masks) return err(QWFN_EINVAL, ": g or masks is NULL");
+        if (g_token_stride != 0 && g_token_stride < n_v) return err(QWFN_EINVAL, ": g_token_stride must be 0 or at least n_v_heads");
+        if (n_slots < 1 || (!slots && n_slots < n_seq)) return err(QWFN_EINVAL, ": too few state slots");
+        if (!std::isfinite(scale)) return err(QWFN_EINVAL, ": scale must be finite");
+        if (!is_aligned(g, 4) || !is_aligned(n_tree, 4) || !is_aligned(slots, 4) || !is_aligned(masks, 8) || !is_aligned(state, 16))
+            return err(QWFN_EALIGN, ": state must be 16-byte aligned, masks 8, g, n_tree and slots 4");
+        if ((q->nb[2] | k->nb[2] | v->nb[2]) >> 24) return err(QWFN_ENOTSUP, ": token strides of 2^24 bytes or more");
+        const bool wide = dv > LA_COLS;
+        const int64_t ct = (dv + (wide ? 2 : 1) * LA_COLS - 1) / ((wide ? 2 : 1) * LA_COLS), blocks = n_seq * n_v * ct;
+        if (blocks > LA_BLOCKS) return err(QWFN_ENOTSUP, ": too many requests and heads");
+        const size_t states = (size_t) n_slots * n_v * dk * dv * 4;
+        const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, tensor_extent(k), "k"}, {v->data, tensor_extent(v), "v"},
+                           {g, (size_t) ((n_tok - 1) * g_token_stride + n_v) * 4, "g"}, {n_tree, (size_t) n_seq * 4, "n_tree"},
+                           {masks, (size_t) n_tok * 8, "masks"}, {slots, (size_t) n_seq * 4, "slots"}, {state, states, "state"}};
+        const span out[] = {{dst->data, tensor_extent(dst), "dst"}};
+        if (int rc = check_overlaps(op, in, 8, out, 1)) return rc;
+        lt_args x{};
+        la_args & a = x.a;
+        if (int rc = status_word(&a.status)) return rc;
+        a.q = (const char *) q->data; a.k = (const char *) k->data; a.v = (const char *) v->data; a.out = (char *) dst->data;
+        a.q_nb1 = (int64_t) q->nb[1]; a.q_nb2 = (int64_t) q->nb[2]; a.k_nb1 = (int64_t) k->nb[1]; a.k_nb2 = (int64_t) k->nb[2];
+        a.v_nb1 = (int64_t) v->nb[1]; a.v_nb2 = (int64_t) v->nb[2];
+        a.g = g; a.g_ts = g_token_stride; a.slots = slots; a.s_in = state; a.scale = scale;
+        a.type = q->type; a.n_seq = n_seq; a.max_len = T; a.n_slots = n_slots; a.n_tok = (int32_t) n_tok;
+        a.n_k = (int32_t) q->ne[1]; a.n_v = (int32_t) n_v; a.rep = a.n_v / a.n_k; a.dk = (int32_t) dk; a.dv = (int32_t) dv;
+        a.ct = (int32_t) ct;
+        x.n_tree = n_tree; x.masks = masks;
+        const hipStream_t s = as_stream(stream);
+        if (dk <= 64)  return launch_tree<64>(x, (unsigned) blocks, wide, s);
+        if (dk <= 128) return launch_tree<128>(x, (unsigned) blocks, wide, s);
+        return launch_tree<256>(x, (unsigned) blocks, wide, s);
     });
 }

@@ -39,64 +39,13 @@
 // largest dv of the tile and down by 8: P dv then lies below 2^8 whatever the
 // scales of V are, and 33 bits of range lie below it in f16. It follows a rise
 // of up to 2^6 late (P dv < 2^15), so O is rescaled rarely.
-#include "fattn_device.h"
-#include "q8_device.h"
-#include "qwfn_common.h"
-#include "qwfn_paged.h"
+#include "paged_device.h"
 
 #include <algorithm>
 #include <cmath>
 
 namespace qwfn {
 namespace {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
-constexpr int PA_WAVES = 4;
-constexpr int PA_THREADS = PA_WAVES * 64;
-constexpr int PA_TILE = 32;            // keys of a tile
-constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
-constexpr int PA_LEAD = 8;             // tiles that a request counts more than it has
-constexpr int PA_CUS = 256;            // two workgroups a CU (registers)
-constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
-constexpr float PA_LOG2E = 1.4426950408889634f;
-constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
-constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M
-constexpr float PA_IBIAS = 12582912.f; // 1.5 2^23: an integer below 2^22 added to its bits is added to its value
-constexpr int PA_IBITS = 0x4b400000;   // (a block's dot is at most 32 128 128 = 2^19)
-
-// x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), is off by at
-// most d <= 2^s, and x (m d - 2^(31 + s)) < 2^(31 + s) keeps the quotient whole.
-struct fast_div { uint32_t d, m, s; };
-fast_div make_div(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) s++;
-    return {d, (uint32_t) (((1ull << (31 + s)) / d) + 1), s};
-}
-__device__ __forceinline__ uint32_t div_by(uint32_t x, fast_div f) { return f.s == 0 ? x : __umulhi(x, f.m) >> (f.s - 1); }
-
-struct pa_args {
-    const char *    q; size_t q_nb1, q_nb2, q_nb3;
-    const char *    k; const char * v;
-    uint32_t        nb1;               // bytes of a cache row
-    size_t          nb2;               // and of a head's offset
-    int64_t         n_pages;
-    const int32_t * table; int64_t t_stride;
-    const int32_t * n_kv;
-    int64_t         max_kv;            // max_pages * page
-    fast_div        page;
-    const char *    gate; char * dst;
-    int32_t         type;              // of q, gate and dst
-    int32_t         n_seq, T, nh, nh_kv, rep, R, x86;
-    int32_t         runs;              // runs the tiles are cut into, at most
-    fast_div        f_runs, f_inner, f_kv, f_rep;      // runs, blocks of a run, KV heads, rep
-    float           c;                 // scale * log2(e): scores are in log2 units
-    float *         part_o;            // [run + request][nh_kv][R][D]
-    float2 *        part_ml;           // [run + request][nh_kv][R]
-    int2 *          span;              // [request]: its first and last run
-    uint32_t *      status;
-};
 
 template <int D> struct pa_cfg {
     static constexpr int NBLK = D / QK;
@@ -119,65 +68,6 @@ template <int D> struct pa_cfg {
     static_assert((QBLOCK * (NBLK - 1) + 2) / 16 * 16 + 64 <= LS + 64, "a window ends in the next row, or V's first");
 };
 constexpr int pa_win(int b) { return (QBLOCK * b + 2) / 16; }              // first 16 bytes of block b's window
-
-// One wave-wide LDS DMA: lane i copies its UB bytes to LDS[at + UB i]. Inline asm, so that the compiler neither
-// moves memory operations across it nor waits for it: the kernel's own counts do. (m0 is read one wait state after
-// its write at the earliest; the compiler keeps nothing in it here.)
-template <int UB> __device__ __forceinline__ void pa_dma(uint64_t from, uint32_t at) {
-    if constexpr (UB == 16)
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(at) : "memory");
-    else
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(from), "s"(at) : "memory");
-}
-// The same from `from` + delta (delta the same for all lanes); the sum stands in m0's wait state.
-template <int UB> __device__ __forceinline__ void pa_dma_plus(uint64_t from, uint64_t delta, uint32_t at) {
-    uint64_t sum;
-    if constexpr (UB == 16)
-        asm volatile("s_mov_b32 m0, %3\n\tv_lshl_add_u64 %0, %1, 0, %2\n\tglobal_load_lds_dwordx4 %0, off"
-                     : "=&v"(sum) : "v"(from), "s"(delta), "s"(at) : "memory");
-    else
-        asm volatile("s_mov_b32 m0, %3\n\tv_lshl_add_u64 %0, %1, 0, %2\n\tglobal_load_lds_dword %0, off"
-                     : "=&v"(sum) : "v"(from), "s"(delta), "s"(at) : "memory");
-}
-// Waits until at most N vector-memory operations are in flight, or for this wave's LDS operations.
-template <int N> __device__ __forceinline__ void pa_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
-__device__ __forceinline__ void pa_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ uint32_t pa_lds(const void * p) { return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) p; }
-
-__device__ __forceinline__ void load4(const char * p, int32_t type, float x[4]) {
-    if (type == QWFN_TYPE_F32) {
-        const float4 f = *(const float4 *) p;
-        x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-    } else {
-        const uint2 u = *(const uint2 *) p;
-        const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            x[i] = type == QWFN_TYPE_F16 ? dev::f16_bits_to_f32((uint16_t) h[i]) : __builtin_bit_cast(float, h[i] << 16);
-    }
-}
-// bf16 of x, to nearest even; a NaN stays one
-__device__ __forceinline__ uint32_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16) x); }
-__device__ __forceinline__ void store4(char * p, int32_t type, const float x[4]) {
-    if (type == QWFN_TYPE_F32) {
-        *(float4 *) p = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = type == QWFN_TYPE_F16 ? dev::f32_to_f16_bits(x[i]) : bf16_bits(x[i]);
-        *(uint2 *) p = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-    }
-}
-__device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[4]) {
-    const size_t es = a.type == QWFN_TYPE_F32 ? 4 : 2;
-    if (a.gate) {
-        float g[4];
-        load4(a.gate + elem * es, a.type, g);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = x[i] / (1.f + expf(-g[i]));
-    }
-    store4(a.dst + elem * es, a.type, x);
-}
 
 // B operands of a V block: x = p d of the lane's 8 keys (p[u], d[u] packed) as f16 pairs, hi toward zero, lo = p d - hi from
 // one fused step each. One asm: a single pair of wait states before the MFMA (fattn_device.h) for all of it.
@@ -220,114 +110,8 @@ __device__ __forceinline__ void cvt_v8(const uint32_t (&v)[2][4], v4u & a0, v4u 
     a1 = v4u{y0, y1, y2, y3};
 }
 
-// Largest over lanes l and l ^ 32, l and l ^ 16, a row of 16, without LDS.
-__device__ __forceinline__ uint32_t umax_halves(uint32_t x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    unsigned p = r[0], q = r[1];
-    asm volatile("" : "+v"(p), "+v"(q));
-    return max(p, q);
-}
-__device__ __forceinline__ uint32_t umax_rows(uint32_t x) {           // lanes l and l ^ 16
-    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    unsigned p = r[0], q = r[1];
-    asm volatile("" : "+v"(p), "+v"(q));
-    return max(p, q);
-}
-__device__ __forceinline__ uint32_t umax_row(uint32_t x) {            // the 16 lanes of a row
-    x = max(x, dev::dpp_u32<dev::DPP_QUAD_1032>(x));
-    x = max(x, dev::dpp_u32<dev::DPP_QUAD_2301>(x));
-    x = max(x, dev::dpp_u32<dev::DPP_HALF_MIRROR>(x));
-    return max(x, dev::dpp_u32<0x140>(x));                            // row_mirror
-}
-
-// A block's run of the tiles of all requests: the request it starts in and its length, the tile there, the
-// tiles left, its place, how many tiles a run has. A request counts PA_LEAD tiles more than it has, in front of
-// its own (off starts at -PA_LEAD): what its queries and its output cost the workgroup that begins it. 48 ragged
-// requests without that: 99 us for 91, the workgroups with two requests last.
-struct pa_run { int32_t b, n, off, left, pos, per; };
-
-__device__ __forceinline__ int32_t clip_len(const pa_args & a, int32_t n) { return n <= 0 ? 0 : n < a.max_kv ? n : (int32_t) a.max_kv; }
-__device__ __forceinline__ int32_t tiles_of(int32_t n) { return (int32_t) (((uint32_t) n + PA_TILE - 1) / PA_TILE); }
-__device__ __forceinline__ int32_t cost_of(int32_t n) { return n > 0 ? tiles_of(n) + PA_LEAD : 0; }
-__device__ __forceinline__ int32_t run_len(const pa_args & a, int32_t total) {
-    const int32_t per = ((int32_t) div_by((uint32_t) (total + a.runs - 1), a.f_runs) + PA_WAVES - 1) / PA_WAVES * PA_WAVES;
-    return per < PA_MIN_TILES ? PA_MIN_TILES : per;         // whole rounds of the waves
-}
-
-// Where run g starts. Up to 64 requests: a lane each, every wave on its own. More: every thread sums the tiles of
-// a few requests.
-__device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * sh) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    pa_run r{0, 0, 0, 0, 0, 0};
-    if (a.n_seq <= 64) {
-        const int32_t n = lane < a.n_seq ? clip_len(a, a.n_kv[lane]) : 0, t = cost_of(n);
-        int32_t incl = t;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int32_t x = __shfl_up(incl, d);
-            if (lane >= d) incl += x;
-        }
-        const int32_t total = __builtin_amdgcn_readlane(incl, 63);
-        r.per = run_len(a, total);
-        const int64_t start = (int64_t) g * r.per;
-        if (start < total) {
-            r.b = __builtin_popcountll(__ballot(incl <= (int32_t) start));
-            r.n = __builtin_amdgcn_readlane(n, r.b);
-            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b) - PA_LEAD;
-            r.left = total - (int32_t) start < r.per ? total - (int32_t) start : r.per;
-            r.pos = (int32_t) start;
-        }
-        return r;
-    }
-    const int c = (a.n_seq + PA_THREADS - 1) / PA_THREADS;
-    int32_t sum = 0;
-    for (int i = 0; i < c; i++) {
-        const int b = tid * c + i;
-        if (b < a.n_seq) sum += cost_of(clip_len(a, a.n_kv[b]));
-    }
-    int32_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int32_t x = __shfl_up(incl, d);
-        if (lane >= d) incl += x;
-    }
-    if (lane == 63) sh[w] = incl;
-    __syncthreads();
-    int32_t before = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < PA_WAVES; i++) {
-        const int32_t x = sh[i];
-        if (i < w) before += x;
-        total += x;
-    }
-    incl += before;
-    r.per = run_len(a, total);
-    const int64_t start = (int64_t) g * r.per;
-    if (start >= incl - sum && start < incl) {
-        int32_t at = incl - sum;
-        for (int i = 0; i < c; i++) {
-            const int b = tid * c + i;
-            const int32_t n = b < a.n_seq ? clip_len(a, a.n_kv[b]) : 0, t = cost_of(n);
-            if (start >= at && start < at + t) {
-                sh[PA_WAVES] = b;
-                sh[PA_WAVES + 1] = n;
-                sh[PA_WAVES + 2] = (int32_t) (start - at);
-            }
-            at += t;
-        }
-    }
-    __syncthreads();
-    if (start < total) {
-        r.b = __builtin_amdgcn_readfirstlane(sh[PA_WAVES]);
-        r.n = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
-        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 2]) - PA_LEAD;
-        r.left = __builtin_amdgcn_readfirstlane(total - start < r.per ? (int32_t) (total - start) : r.per);
-        r.pos = (int32_t) start;
-    }
-    return r;
-}
-
-template <int D>
+// TREE: the queries are nodes of a tree, and their masks decide which of the last n_tree tokens they see.
+template <int D, bool TREE>
 __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     using C = pa_cfg<D>;
     constexpr int NBLK = C::NBLK, ND = C::DMAS;
@@ -341,7 +125,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     // blocks -> (run, KV head, row group): those of one run follow each other on one XCD
     const uint32_t j = blockIdx.x >> 3, jq = div_by(j, a.f_inner), hr = j - jq * a.f_inner.d;
     const int g = (int) jq * 8 + (int) (blockIdx.x & 7), rg = (int) div_by(hr, a.f_kv), kvh = (int) hr - rg * a.nh_kv;
-    pa_run run = find_run(a, g, sh);
+    auto length = [&](int32_t b) { return TREE ? tree_len(a, b, rg) : clip_len(a, a.n_kv[b]); };
+    pa_run run = find_run(a, g, sh, length);
 
     uint8_t * const my = lds + wave * C::WAVE;
     uint64_t * const addr = (uint64_t *) (my + C::OA);
@@ -422,6 +207,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             load4(a.q + (size_t) t * a.q_nb1 + (size_t) h * a.q_nb2 + (size_t) b * a.q_nb3 + (size_t) (blk * QK + sub * 4) * es,
                   a.type, qx[i]);
         }
+        // (a tree's: keys below base, and the nodes of its mask; rows without a node are dropped at the end)
+        const int32_t nodes = TREE ? tree_nodes(a, b, n) : a.T, base = n - nodes;
+        uint64_t mask = 0;
+        if constexpr (TREE) {
+            const int32_t t = (int32_t) div_by((uint32_t) (16 * rg + ln), a.f_rep);
+            if (t < nodes) mask = a.masks[(int64_t) b * a.T + t];
+        }
         uint32_t live = 0, live_next = 0;                  // the tile's keys that exist
         if (wave < nt) {
             entries(wave);
@@ -433,6 +225,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
         for (int i = 0; i < C::QI; i++)
 #pragma unroll
             for (int k = 0; k < 4; k++) asm volatile("" : "+v"(qx[i][k]));
+        if constexpr (TREE) asm volatile("" : "+v"(mask));
         if (wave < nt) {
             wave_lds_sync();
             send_k(at_k);
@@ -479,7 +272,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             // the lane's places are computed anew in every tile: kept over the loop they cost 40 registers, spilled
             asm volatile("" : "+v"(lane), "+v"(ln), "+v"(lg));
             const int32_t key0 = (run.off + t) * PA_TILE;
-            const bool masked = live != 0xffffffffu || key0 + PA_TILE > n - a.T + 1;
+            const bool masked = live != 0xffffffffu || key0 + PA_TILE > (TREE ? base : n - a.T + 1);
             pa_wait<ND + 1>();
             const uint8_t * const kt = my, * const vt = kt + C::ROWS;
             {   // K's scales by block and key
@@ -548,12 +341,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             uint32_t top_d = dmax;
             if (masked) {
                 top_d = 0;                                 // of the keys that the row sees
+                const uint32_t sees = TREE ? live & tree_sees(mask, key0, base) : live;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int k = 16 * u + 4 * lg + r;
-                        if (!(live >> k & 1) || key0 + k >= limit) s[u][r] = -INFINITY;
+                        if (!(sees >> k & 1) || (!TREE && key0 + k >= limit)) s[u][r] = -INFINITY;
                         else top_d = max(top_d, (uint32_t) vtop[k]);
                     }
                 top_d = umax_halves(umax_rows(top_d));
@@ -658,6 +452,12 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             e[w].x = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - mm);
             ll += e[w].x * e[w].y;                         // a NaN stays one
         }
+        if (TREE && rr >= nodes * a.rep) {
+            mm = -INFINITY;
+            ll = 0.f;
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; w++) e[w].x = 0.f;
+        }
         if (rr < a.R) {
             const size_t elem = element(b, rr), part = ((size_t) (g + b) * a.nh_kv + kvh) * a.R + rr;
             const float inv = ll > 0.f ? 1.f / ll : ll == ll ? 0.f : ll;
@@ -682,25 +482,28 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
             }
             if (!whole && (tid & 15) == 0) a.part_ml[part] = make_float2(mm, ll);
         }
-        if (run.off == 0 && hr == 0 && tid == 0) a.span[b] = make_int2(g, (run.pos + tiles - 1) / run.per);
+        if (run.off == 0 && (TREE ? kvh : (int) hr) == 0 && tid == 0)
+            a.span[TREE ? rg * a.n_seq + b : b] = make_int2(g, (run.pos + tiles - 1) / run.per);
         run.left -= nt;
         run.pos += nt;
         run.off = -PA_LEAD;
         if (run.left > 0)
-            do run.n = clip_len(a, a.n_kv[++run.b]);
+            do run.n = length(++run.b);
             while (run.n == 0);
     }
     // requests without a key, and lengths that were clipped
     for (int b = g; b < a.n_seq; b += (int) (gridDim.x / a.f_inner.d)) {
         const int32_t n = a.n_kv[b];
-        if (n != clip_len(a, n) && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
-        if (n > 0) continue;
+        bool bad = n != clip_len(a, n);
+        if (TREE && a.n_tree) bad |= a.n_tree[b] != tree_nodes(a, b, clip_len(a, n));
+        if (bad && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
+        if (length(b) > 0) continue;
         const float z[4] = {0.f, 0.f, 0.f, 0.f};
         for (int r = tid >> 4; r < 16; r += PA_THREADS / 16)
             if (16 * rg + r < a.R)
 #pragma unroll
                 for (int i = 0; i < D / 64; i++) store4(a.dst + (element(b, 16 * rg + r) + 4 * (tid & 15) + 64 * i) * es, a.type, z);
-        if (hr == 0 && tid == 0) a.span[b] = make_int2(0, 0);
+        if ((TREE ? kvh : (int) hr) == 0 && tid == 0) a.span[TREE ? rg * a.n_seq + b : b] = make_int2(0, 0);
     }
 }
 
@@ -709,7 +512,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
 // workgroup (16) where it has many. Requests of one part are done.
 constexpr int PM_BATCH = 8;
 
-template <int D, int GROUPS>
+template <int D, int GROUPS, bool TREE>
 __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
     __shared__ float4 acc[16][16];
     __shared__ float2 gl[16];
@@ -719,7 +522,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
     const uint32_t row = (uint32_t) (unit / (D / 64)), bk = row / (uint32_t) a.R, r = row - bk * (uint32_t) a.R;
     const uint32_t b = div_by(bk, a.f_kv), kvh = bk - b * (uint32_t) a.nh_kv;
     const bool on = b < (uint32_t) a.n_seq;
-    const int2 sp = on ? a.span[b] : make_int2(0, 0);
+    const int2 sp = on ? a.span[TREE ? (int64_t) div_by(r, a.f_group) * a.n_seq + b : b] : make_int2(0, 0);
     if (GROUPS == 16 && sp.x == sp.y) return;
     const int g = (int) (threadIdx.x >> 4) % GROUPS, q = threadIdx.x & 15;
     float M = -INFINITY, l = 0.f;
@@ -783,7 +586,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
 // ---------------------------------------------------------------- host
 
 struct pa_plan {
-    int32_t groups, runs;              // row groups
+    int32_t groups, runs, rows;        // row groups, of `rows` rows each
     size_t  off_o, off_ml, bytes;
 };
 
@@ -792,22 +595,25 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Runs: as many as fill the CUs; no more than the longest requests could need. (Run g is on XCD g mod 8. Their number is
 // whole rounds of the 8 XCDs where heads and row groups divide 64; 85 runs, of 2 heads in 3 groups, leave some XCDs with 11
 // for the others' 10.)
-pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv) {
+pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv, bool tree) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    p.groups = (int32_t) ((R + 15) / 16);
+    p.rows = 16;
+    p.groups = (int32_t) ((R + p.rows - 1) / p.rows);
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
     p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * PA_CUS / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
-    p.off_o = round256((size_t) n_seq * sizeof(int2));
+    p.off_o = round256((size_t) n_seq * (tree ? p.groups : 1) * sizeof(int2));
     p.off_ml = p.off_o + round256(parts * D * sizeof(float));
     p.bytes = p.off_ml + round256(parts * sizeof(float2));
     return p;
 }
 
+const char * paged_name(bool tree) { return tree ? "flash_attn_ext_paged_tree" : "flash_attn_ext_paged"; }
+
 int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, int32_t max_pages, int32_t page_size,
-                pa_plan * pl) {
-    const char * op = "flash_attn_ext_paged";
+                bool tree, pa_plan * pl) {
+    const char * op = paged_name(tree);
     auto err = [&](int code, const char * what) { return set_error2(code, op, what); };
     if (!q || !q->data || !k || !k->data || !v || !v->data) return err(QWFN_EINVAL, ": q, k or v is NULL");
     if (q->type != QWFN_TYPE_F32 && q->type != QWFN_TYPE_F16 && q->type != QWFN_TYPE_BF16)
@@ -820,7 +626,9 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
     if (k->ne[0] != D) return err(QWFN_EINVAL, ": q and k head sizes differ");
     if (k->ne[3] != 1) return err(QWFN_ENOTSUP, ": k and v are one pool (ne[3] == 1)");
     if (nh % nh_kv) return err(QWFN_EINVAL, ": n_head must be a multiple of n_head_kv");
-    if (T > PA_MAX_ROWS || T * (nh / nh_kv) > PA_MAX_ROWS)
+    if (tree && (T > 64 || T * (nh / nh_kv) > PA_MAX_TREE_ROWS))
+        return err(QWFN_ENOTSUP, ": at most 64 nodes and 1024 query rows per KV head (T * n_head / n_head_kv)");
+    if (!tree && (T > PA_MAX_ROWS || T * (nh / nh_kv) > PA_MAX_ROWS))
         return err(QWFN_ENOTSUP, ": at most 64 query rows per KV head (T * n_head / n_head_kv)");
     if (nh_kv > 128) return err(QWFN_ENOTSUP, ": at most 128 KV heads");
     if (page_size < 1 || max_pages < 1 || (int64_t) page_size * max_pages > 0x7fffffff - 2 * PA_TILE * PA_WAVES)
@@ -831,22 +639,105 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
     if (B * nh * T * (D / 64) >= 1 << 26) return err(QWFN_ENOTSUP, ": too many query rows");
     if (k->ne[1] < page_size) return err(QWFN_EINVAL, ": the pool holds no whole page");
     if (k->ne[1] > 0x7fffffff) return err(QWFN_ENOTSUP, ": a pool of at most 2^31 - 1 rows");
-    *pl = plan_paged(D, T, nh, nh_kv, B, (int64_t) page_size * max_pages);
+    *pl = plan_paged(D, T, nh, nh_kv, B, (int64_t) page_size * max_pages, tree);
     return QWFN_OK;
 }
 
-template <int D>
+template <int D, bool TREE>
 int launch_paged(const pa_args & a, const pa_plan & p, hipStream_t s) {
     const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * p.groups));
-    hipLaunchKernelGGL(k_paged_attn<D>, grid, dim3(PA_THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_paged_attn<D, TREE>), grid, dim3(PA_THREADS), 0, s, a);
     if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
     // the requests' parts: on average runs / n_seq each, with long requests among short ones more
     const int64_t units = (int64_t) a.n_seq * a.nh_kv * a.R * (D / 64);
     if (a.runs > 16 * (int64_t) a.n_seq)
-        hipLaunchKernelGGL((k_paged_merge<D, 16>), dim3((unsigned) units), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_paged_merge<D, 16, TREE>), dim3((unsigned) units), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_paged_merge<D, 4>), dim3((unsigned) ((units + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_paged_merge<D, 4, TREE>), dim3((unsigned) ((units + 3) / 4)), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "flash_attn_ext_paged launch");
+}
+
+// A call of either form.
+int paged_attention(bool tree, const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const int32_t * table,
+                    int64_t table_stride, int32_t max_pages, int32_t page_size, const int32_t * n_kv, const int32_t * n_tree,
+                    const uint64_t * masks, float scale, const qwfn_tensor * gate, const qwfn_tensor * dst, int variant, void * ws,
+                    size_t ws_bytes, void * stream) {
+    const char * op = paged_name(tree);
+    auto err = [&](int code, const char * what) { return set_error2(code, op, what); };
+    pa_plan pl;
+    if (int rc = check_paged(q, k, v, max_pages, page_size, tree, &pl)) return rc;
+    if (!table || !n_kv || !dst || !dst->data) return err(QWFN_EINVAL, ": table, n_kv or dst is NULL");
+    if (tree && !masks) return err(QWFN_EINVAL, ": masks is NULL");
+    if (!std::isfinite(scale)) return err(QWFN_EINVAL, ": scale must be finite");
+    if (variant != QWFN_Q8_REF && variant != QWFN_Q8_X86) return err(QWFN_EINVAL, ": unknown rounding variant");
+    const int64_t D = q->ne[0], T = q->ne[1], nh = q->ne[2], B = q->ne[3], nh_kv = k->ne[2];
+    const size_t es = q->type == QWFN_TYPE_F32 ? 4 : 2, seg = (size_t) D / QK * QBLOCK, al = (size_t) D / 16;
+    for (int i = 0; i < 4; i++)
+        if (v->ne[i] != k->ne[i] || (i < 3 && v->nb[i] != k->nb[i]))
+            return err(QWFN_EINVAL, ": k and v must have the same shape and strides");
+    if (k->nb[0] != QBLOCK) return err(QWFN_EINVAL, ": k and v nb[0] must be 34");
+    if (!is_aligned(k->data, al) || !is_aligned(v->data, al) || k->nb[1] % al || k->nb[2] % al)
+        return err(QWFN_EALIGN, ": k and v rows and strides must be aligned to head size / 16 bytes");
+    if (k->nb[1] > 0xffffffffu) return err(QWFN_ENOTSUP, ": a row stride of 2^32 bytes or more");
+    // heads inside a row, or rows inside a head
+    if (k->nb[1] < (size_t) (nh_kv - 1) * k->nb[2] + seg && k->nb[2] < (size_t) (k->ne[1] - 1) * k->nb[1] + seg)
+        return err(QWFN_EINVAL, ": k and v rows or heads overlap");
+    if (k->nb[1] < seg || (nh_kv > 1 && k->nb[2] < seg)) return err(QWFN_EINVAL, ": k and v rows or heads overlap");
+    if (q->nb[0] != es) return err(QWFN_EINVAL, ": q rows must be contiguous");
+    if (!is_aligned(q->data, 16) || q->nb[1] % 16 || q->nb[2] % 16 || q->nb[3] % 16)
+        return err(QWFN_EALIGN, ": q must be 16-byte aligned");
+    const int64_t ne[4] = {D, nh, T, B};
+    for (int g = 0; g < 2; g++) {
+        const qwfn_tensor * t = g ? gate : dst;
+        if (!t) continue;
+        if (!t->data || t->type != q->type) return err(QWFN_EINVAL, g ? ": gate must have q's type" : ": dst must have q's type");
+        size_t nb = es;
+        for (int i = 0; i < 4; i++) {
+            if (t->ne[i] != ne[i] || t->nb[i] != nb)
+                return err(QWFN_EINVAL, g ? ": gate must be contiguous [D, n_head, T, n_seq]" : ": dst must be contiguous [D, n_head, T, n_seq]");
+            nb *= (size_t) ne[i];
+        }
+        if (!is_aligned(t->data, 16)) return err(QWFN_EALIGN, g ? ": gate must be 16-byte aligned" : ": dst must be 16-byte aligned");
+    }
+    if (table_stride < max_pages && B > 1) return err(QWFN_EINVAL, ": table rows overlap (table_stride < max_pages)");
+    if (table_stride > 0x7fffffff) return err(QWFN_EINVAL, ": table_stride must be below 2^31");
+    if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
+    if (!is_aligned(n_tree, 4) || !is_aligned(masks, 8)) return err(QWFN_EALIGN, ": n_tree must be 4-byte aligned, masks 8");
+    if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
+    if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");
+    // (a request's queries are read by several workgroups, and one of them may be done before another begins)
+    const size_t rows = tensor_extent(dst);
+    const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, view_bytes(*k), "k"}, {v->data, view_bytes(*v), "v"},
+                       {gate && gate->data != dst->data ? gate->data : nullptr, rows, "gate"},
+                       {table, ((size_t) (B - 1) * table_stride + max_pages) * 4, "table"}, {n_kv, (size_t) B * 4, "n_kv"},
+                               {n_tree, (size_t) B * 4, "n_tree"}, {masks, (size_t) (B * T) * 8, "masks"}};
+    const span out[] = {{dst->data, rows, "dst"}, {ws, pl.bytes, "ws"}};
+    if (int rc = check_overlaps(op, in, 8, out, 2)) return rc;
+    if (!ws) {
+        size_t got = 0;
+        if (int rc = library_workspace(pl.bytes, pl.bytes, as_stream(stream), &ws, &got)) return rc;
+    }
+    pa_args a{};
+    if (int rc = status_word(&a.status)) return rc;
+    a.q = (const char *) q->data; a.q_nb1 = q->nb[1]; a.q_nb2 = q->nb[2]; a.q_nb3 = q->nb[3];
+    a.k = (const char *) k->data; a.v = (const char *) v->data; a.nb1 = (uint32_t) k->nb[1]; a.nb2 = k->nb[2];
+    a.n_pages = k->ne[1] / page_size;
+    a.table = table; a.t_stride = table_stride; a.n_kv = n_kv; a.max_kv = (int64_t) max_pages * page_size;
+    a.page = make_div((uint32_t) page_size);
+    a.gate = gate ? (const char *) gate->data : nullptr; a.dst = (char *) dst->data; a.type = q->type;
+    a.n_seq = (int32_t) B; a.T = (int32_t) T; a.nh = (int32_t) nh; a.nh_kv = (int32_t) nh_kv;
+    a.rep = (int32_t) (nh / nh_kv); a.R = a.T * a.rep; a.x86 = variant == QWFN_Q8_X86;
+    a.f_runs = make_div((uint32_t) pl.runs); a.f_inner = make_div((uint32_t) (nh_kv * pl.groups));
+    a.f_kv = make_div((uint32_t) nh_kv); a.f_rep = make_div((uint32_t) a.rep);
+    a.runs = pl.runs; a.c = scale * PA_LOG2E;
+    a.span = (int2 *) ws; a.part_o = (float *) ((char *) ws + pl.off_o); a.part_ml = (float2 *) ((char *) ws + pl.off_ml);
+    a.n_tree = n_tree; a.masks = masks; a.group = pl.rows; a.f_group = make_div((uint32_t) pl.rows);
+    const hipStream_t s = as_stream(stream);
+    switch (D) {
+        case 64:  return tree ? launch_paged<64, true>(a, pl, s) : launch_paged<64, false>(a, pl, s);
+        case 128: return tree ? launch_paged<128, true>(a, pl, s) : launch_paged<128, false>(a, pl, s);
+        default:  return tree ? launch_paged<256, true>(a, pl, s) : launch_paged<256, false>(a, pl, s);
+    }
 }
 
 }  // namespace
@@ -858,7 +749,15 @@ extern "C" size_t qwfn_fattn_workspace_size_paged(const qwfn_tensor * q, const q
                                                   int32_t max_pages, int32_t page_size) {
     return ::qwfn::abi_value<size_t>("fattn_workspace_size_paged", 0, [&]() -> size_t {
         pa_plan pl;
-        return check_paged(q, k, v, max_pages, page_size, &pl) ? 0 : pl.bytes;
+        return check_paged(q, k, v, max_pages, page_size, false, &pl) ? 0 : pl.bytes;
+    });
+}
+
+extern "C" size_t qwfn_fattn_workspace_size_paged_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                                       int32_t max_pages, int32_t page_size) {
+    return ::qwfn::abi_value<size_t>("fattn_workspace_size_paged_tree", 0, [&]() -> size_t {
+        pa_plan pl;
+        return check_paged(q, k, v, max_pages, page_size, true, &pl) ? 0 : pl.bytes;
     });
 }
 
@@ -868,75 +767,19 @@ extern "C" int qwfn_flash_attn_ext_q8_0_paged(const qwfn_tensor * q, const qwfn_
                                               const qwfn_tensor * dst, int variant, void * ws, size_t ws_bytes,
                                               void * stream) {
     return ::qwfn::abi_call("flash_attn_ext_paged", [&]() -> int {
-        auto err = [&](int code, const char * what) { return set_error2(code, "flash_attn_ext_paged", what); };
-        pa_plan pl;
-        if (int rc = check_paged(q, k, v, max_pages, page_size, &pl)) return rc;
-        if (!table || !n_kv || !dst || !dst->data) return err(QWFN_EINVAL, ": table, n_kv or dst is NULL");
-        if (!std::isfinite(scale)) return err(QWFN_EINVAL, ": scale must be finite");
-        if (variant != QWFN_Q8_REF && variant != QWFN_Q8_X86) return err(QWFN_EINVAL, ": unknown rounding variant");
-        const int64_t D = q->ne[0], T = q->ne[1], nh = q->ne[2], B = q->ne[3], nh_kv = k->ne[2];
-        const size_t es = q->type == QWFN_TYPE_F32 ? 4 : 2, seg = (size_t) D / QK * QBLOCK, al = (size_t) D / 16;
-        for (int i = 0; i < 4; i++)
-            if (v->ne[i] != k->ne[i] || (i < 3 && v->nb[i] != k->nb[i]))
-                return err(QWFN_EINVAL, ": k and v must have the same shape and strides");
-        if (k->nb[0] != QBLOCK) return err(QWFN_EINVAL, ": k and v nb[0] must be 34");
-        if (!is_aligned(k->data, al) || !is_aligned(v->data, al) || k->nb[1] % al || k->nb[2] % al)
-            return err(QWFN_EALIGN, ": k and v rows and strides must be aligned to head size / 16 bytes");
-        if (k->nb[1] > 0xffffffffu) return err(QWFN_ENOTSUP, ": a row stride of 2^32 bytes or more");
-        // heads inside a row, or rows inside a head
-        if (k->nb[1] < (size_t) (nh_kv - 1) * k->nb[2] + seg && k->nb[2] < (size_t) (k->ne[1] - 1) * k->nb[1] + seg)
-            return err(QWFN_EINVAL, ": k and v rows or heads overlap");
-        if (k->nb[1] < seg || (nh_kv > 1 && k->nb[2] < seg)) return err(QWFN_EINVAL, ": k and v rows or heads overlap");
-        if (q->nb[0] != es) return err(QWFN_EINVAL, ": q rows must be contiguous");
-        if (!is_aligned(q->data, 16) || q->nb[1] % 16 || q->nb[2] % 16 || q->nb[3] % 16)
-            return err(QWFN_EALIGN, ": q must be 16-byte aligned");
-        const int64_t ne[4] = {D, nh, T, B};
-        for (int g = 0; g < 2; g++) {
-            const qwfn_tensor * t = g ? gate : dst;
-            if (!t) continue;
-            if (!t->data || t->type != q->type) return err(QWFN_EINVAL, g ? ": gate must have q's type" : ": dst must have q's type");
-            size_t nb = es;
-            for (int i = 0; i < 4; i++) {
-                if (t->ne[i] != ne[i] || t->nb[i] != nb)
-                    return err(QWFN_EINVAL, g ? ": gate must be contiguous [D, n_head, T, n_seq]" : ": dst must be contiguous [D, n_head, T, n_seq]");
-                nb *= (size_t) ne[i];
-            }
-            if (!is_aligned(t->data, 16)) return err(QWFN_EALIGN, g ? ": gate must be 16-byte aligned" : ": dst must be 16-byte aligned");
-        }
-        if (table_stride < max_pages && B > 1) return err(QWFN_EINVAL, ": table rows overlap (table_stride < max_pages)");
-        if (table_stride > 0x7fffffff) return err(QWFN_EINVAL, ": table_stride must be below 2^31");
-        if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
-        if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
-        if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");
-        // (a request's queries are read by several workgroups, and one of them may be done before another begins)
-        const size_t rows = tensor_extent(dst);
-        const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, view_bytes(*k), "k"}, {v->data, view_bytes(*v), "v"},
-                           {gate && gate->data != dst->data ? gate->data : nullptr, rows, "gate"},
-                           {table, ((size_t) (B - 1) * table_stride + max_pages) * 4, "table"}, {n_kv, (size_t) B * 4, "n_kv"}};
-        const span out[] = {{dst->data, rows, "dst"}, {ws, pl.bytes, "ws"}};
-        if (int rc = check_overlaps("flash_attn_ext_paged", in, 6, out, 2)) return rc;
-        if (!ws) {
-            size_t got = 0;
-            if (int rc = library_workspace(pl.bytes, pl.bytes, as_stream(stream), &ws, &got)) return rc;
-        }
-        pa_args a{};
-        if (int rc = status_word(&a.status)) return rc;
-        a.q = (const char *) q->data; a.q_nb1 = q->nb[1]; a.q_nb2 = q->nb[2]; a.q_nb3 = q->nb[3];
-        a.k = (const char *) k->data; a.v = (const char *) v->data; a.nb1 = (uint32_t) k->nb[1]; a.nb2 = k->nb[2];
-        a.n_pages = k->ne[1] / page_size;
-        a.table = table; a.t_stride = table_stride; a.n_kv = n_kv; a.max_kv = (int64_t) max_pages * page_size;
-        a.page = make_div((uint32_t) page_size);
-        a.gate = gate ? (const char *) gate->data : nullptr; a.dst = (char *) dst->data; a.type = q->type;
-        a.n_seq = (int32_t) B; a.T = (int32_t) T; a.nh = (int32_t) nh; a.nh_kv = (int32_t) nh_kv;
-        a.rep = (int32_t) (nh / nh_kv); a.R = a.T * a.rep; a.x86 = variant == QWFN_Q8_X86;
-        a.f_runs = make_div((uint32_t) pl.runs); a.f_inner = make_div((uint32_t) (nh_kv * pl.groups));
-        a.f_kv = make_div((uint32_t) nh_kv); a.f_rep = make_div((uint32_t) a.rep);
-        a.runs = pl.runs; a.c = scale * PA_LOG2E;
-        a.span = (int2 *) ws; a.part_o = (float *) ((char *) ws + pl.off_o); a.part_ml = (float2 *) ((char *) ws + pl.off_ml);
-        switch (D) {
-            case 64:  return launch_paged<64>(a, pl, as_stream(stream));
-            case 128: return launch_paged<128>(a, pl, as_stream(stream));
-            default:  return launch_paged<256>(a, pl, as_stream(stream));
-        }
+        return paged_attention(false, q, k, v, table, table_stride, max_pages, page_size, n_kv, nullptr, nullptr, scale, gate, dst,
+                               variant, ws, ws_bytes, stream);
+    });
+}
+
+extern "C" int qwfn_flash_attn_ext_q8_0_paged_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v,
+                                                   const int32_t * table, int64_t table_stride, int32_t max_pages,
+                                                   int32_t page_size, const int32_t * n_kv, const int32_t * n_tree,
+                                                   const uint64_t * masks, float scale, const qwfn_tensor * gate,
+                                                   const qwfn_tensor * dst, int variant, void * ws, size_t ws_bytes,
+                                                   void * stream) {
+    return ::qwfn::abi_call("flash_attn_ext_paged_tree", [&]() -> int {
+        return paged_attention(true, q, k, v, table, table_stride, max_pages, page_size, n_kv, n_tree, masks, scale, gate, dst,
+                               variant, ws, ws_bytes, stream);
     });
 }

@@ -157,10 +157,12 @@ EXPORTS = [
     "qwfn_snap_pool_split", "qwfn_snap_pool_restore_or_reset",
     "qwfn_qsa_select_workspace_size", "qwfn_qsa_select_cells",
     "qwfn_qsa_pool_cfg_default", "qwfn_set_rows_f16", "qwfn_qsa_pool_decode", "qwfn_qsa_pool_rebuild",
-    "qwfn_gated_delta_net", "qwfn_linear_attn_workspace_size", "qwfn_linear_attn",
+    "qwfn_gated_delta_net", "qwfn_linear_attn_workspace_size", "qwfn_linear_attn", "qwfn_linear_attn_tree",
     # include/qwfn_paged.h
     "qwfn_paged_workspace_size", "qwfn_paged_extend", "qwfn_paged_extend_states", "qwfn_paged_trim", "qwfn_fattn_workspace_size_paged",
-    "qwfn_flash_attn_ext_q8_0_paged",
+    "qwfn_flash_attn_ext_q8_0_paged", "qwfn_paged_fork", "qwfn_paged_release_workspace_size", "qwfn_paged_release",
+    "qwfn_paged_compact_workspace_size", "qwfn_paged_compact", "qwfn_paged_copy", "qwfn_tree_masks",
+    "qwfn_fattn_workspace_size_paged_tree", "qwfn_flash_attn_ext_q8_0_paged_tree", "qwfn_paged_accept",
 ]
 
 _lib = None
@@ -299,6 +301,21 @@ def load(path: str = LIB_PATH):
     L.qwfn_fattn_workspace_size_paged.restype = sz
     L.qwfn_flash_attn_ext_q8_0_paged.argtypes = [T, T, T, vp, i64, i32, i32, vp, ctypes.c_float, T, T, ctypes.c_int, vp,
                                                  sz, vp]
+    L.qwfn_fattn_workspace_size_paged_tree.argtypes = [T, T, T, i32, i32]
+    L.qwfn_fattn_workspace_size_paged_tree.restype = sz
+    L.qwfn_flash_attn_ext_q8_0_paged_tree.argtypes = [T, T, T, vp, i64, i32, i32, vp, vp, vp, ctypes.c_float, T, T, ctypes.c_int,
+                                                      vp, sz, vp]
+    L.qwfn_paged_fork.argtypes = [vp, vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.qwfn_paged_release_workspace_size.argtypes = [i32, i32]
+    L.qwfn_paged_release_workspace_size.restype = sz
+    L.qwfn_paged_release.argtypes = [vp, vp, i32, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, sz, vp]
+    L.qwfn_paged_compact_workspace_size.argtypes = [i32]
+    L.qwfn_paged_compact_workspace_size.restype = sz
+    L.qwfn_paged_compact.argtypes = [vp, i32, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.qwfn_paged_copy.argtypes = [T, i32, vp, i32, vp, i32, vp]
+    L.qwfn_tree_masks.argtypes = [vp, vp, vp, i32, i32, vp, vp, vp]
+    L.qwfn_paged_accept.argtypes = [T, i32, vp, i64, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp]
+    L.qwfn_linear_attn_tree.argtypes = [T, T, T, vp, i64, vp, vp, i32, i32, vp, i32, vp, ctypes.c_float, T, vp]
     L.qwfn_qsa_select_workspace_size.argtypes = [i64, i32]
     L.qwfn_qsa_select_workspace_size.restype = sz
     L.qwfn_qsa_select_cells.argtypes = [vp, sz, i64, vp, i32, sz, vp, sz, i32, i32, vp, i32, vp, vp, vp, sz, vp]
@@ -869,6 +886,176 @@ def flash_attn_ext_paged(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: i
         _stream_on(stream, dev)))
 
 
+# --------------------------------------------------------------------- shared pages, drafted trees
+
+class CacheList:
+    """The descriptors of tensors whose rows are moved together, made once: torch tensors [n_rows, ...] with contiguous
+    rows, all of one shape, type and row stride (uint8: q8_0 rows)."""
+    def __init__(self, caches):
+        caches = list(caches)
+        arr = (Tensor * max(1, len(caches)))()
+        for i, c in enumerate(caches):
+            if c.dim() < 2 or not c[0].is_contiguous():
+                raise ValueError("cache_list: tensors must be [n_rows, ...] with contiguous rows")
+            if c.get_device() != caches[0].get_device():
+                raise ValueError("cache_list: tensors must be on one device")
+            n, e = c[0].numel(), c.element_size()
+            if str(c.dtype) == "torch.uint8":
+                if n % Q8_0_BLOCK:
+                    raise ValueError(f"cache_list: uint8 rows must be whole q8_0 blocks of {Q8_0_BLOCK} bytes")
+                typ, n, e = TYPE_Q8_0, n // Q8_0_BLOCK * QK8_0, Q8_0_BLOCK
+            else:
+                typ = TYPE_I32 if str(c.dtype) == "torch.int32" else float_type(c)
+            arr[i] = tensor(c.data_ptr(), typ, (n, c.size(0)), (e, c.stride(0) * c.element_size()))
+        self.arr, self.n, self.keep = arr, len(caches), caches
+        self.device = caches[0].get_device() if caches else None
+
+
+def cache_list(caches) -> CacheList:
+    return CacheList(caches)
+
+
+def _check_list(op, caches, dev):
+    if not isinstance(caches, CacheList):
+        caches = CacheList(caches)
+    if caches.n and caches.device != dev:
+        raise ValueError(f"{op}: the caches must be on the current device ({dev})")
+    return caches
+
+
+def _check_2d(op, dev, tensors):
+    """Contiguous int32 [rows, cols] tensors {name: (tensor or None, rows, cols)}, or int64 ones where the name is masks."""
+    for name, (t, rows, cols) in tensors.items():
+        if t is None:
+            continue
+        typ = _Torch.mod.int64 if name == "masks" else _Torch.int32
+        if t.dtype is not typ or t.get_device() != dev:
+            raise ValueError(f"{op}: {name} must be {'int64' if name == 'masks' else 'int32'} on the current device ({dev})")
+        if t.dim() != 2 or t.size(0) < rows or t.size(1) != cols or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous [{rows}, {cols}]")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def paged_fork(src, n_kv, page_size: int, table, shared, free_pages, n_free, n_free_out, n_kv_out, shared_out, moves, n_tok=None,
+               states=None, state_moves=None, ws=None, stream=None):
+    """Requests that begin as copies of others: src [n_seq] holds each one's parent or -1, n_tok [n_seq] how many tokens it
+    takes over (None: all); shared [n_pages]; moves, state_moves [n_seq, 3] for paged_copy; the other tensors as in
+    paged_extend. n_kv_out, n_free_out and shared_out may be n_kv, n_free and shared."""
+    n_seq, n_pages, dev = src.numel(), shared.numel(), _Torch().device()
+    _check_i32("paged_fork", dev, dict(
+        src=(src, n_seq), n_tok=(n_tok, n_seq), n_kv=(n_kv, n_seq), shared=(shared, n_pages), free_pages=(free_pages, 0),
+        n_free=(n_free, 1), n_free_out=(n_free_out, 1), n_kv_out=(n_kv_out, n_seq), shared_out=(shared_out, n_pages),
+        states=(states, n_seq)), table, n_seq)
+    _check_2d("paged_fork", dev, dict(moves=(moves, n_seq, 3), state_moves=(state_moves, n_seq, 3)))
+    return check(load().qwfn_paged_fork(
+        src.data_ptr(), _ptr(n_tok), n_kv.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1),
+        shared.data_ptr(), n_pages, free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(),
+        n_kv_out.data_ptr(), shared_out.data_ptr(), moves.data_ptr(), _ptr(states), _ptr(state_moves), *_ws(ws, dev),
+        _stream_on(stream, dev)))
+
+
+def paged_release_workspace_size(n_seq: int, n_pages: int) -> int:
+    return int(load().qwfn_paged_release_workspace_size(n_seq, n_pages))
+
+
+def paged_release(n_keep, n_kv, page_size: int, table, shared, free_pages, n_free, n_free_out, n_kv_out, shared_out, ws=None,
+                  stream=None):
+    """paged_trim over pages that requests may share: those that nobody holds any more go onto the stack, the lowest first."""
+    n_seq, n_pages, dev = n_kv.numel(), shared.numel(), _Torch().device()
+    _check_i32("paged_release", dev, dict(
+        n_keep=(n_keep, n_seq), n_kv=(n_kv, n_seq), shared=(shared, n_pages), free_pages=(free_pages, 0), n_free=(n_free, 1),
+        n_free_out=(n_free_out, 1), n_kv_out=(n_kv_out, n_seq), shared_out=(shared_out, n_pages)), table, n_seq)
+    return check(load().qwfn_paged_release(
+        n_keep.data_ptr(), n_kv.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1), shared.data_ptr(),
+        n_pages, free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(), n_kv_out.data_ptr(),
+        shared_out.data_ptr(), *_ws(ws, dev), _stream_on(stream, dev)))
+
+
+def paged_compact_workspace_size(n_pages: int) -> int:
+    return int(load().qwfn_paged_compact_workspace_size(n_pages))
+
+
+def paged_compact(n_kv, page_size: int, table, shared, free_pages, n_free, table_out, shared_out, free_out, n_free_out, page_map,
+                  moves, n_moves, ws=None, stream=None):
+    """The live pages of a pool moved to its front: page_map [n_pages], moves [>= (n_pages + 1) / 2, 3] and n_moves [1] for
+    paged_copy; table_out, shared_out, free_out and n_free_out may be the tensors they continue."""
+    n_seq, n_pages, dev = n_kv.numel(), shared.numel(), _Torch().device()
+    _check_i32("paged_compact", dev, dict(
+        n_kv=(n_kv, n_seq), shared=(shared, n_pages), free_pages=(free_pages, 0), n_free=(n_free, 1),
+        shared_out=(shared_out, n_pages), free_out=(free_out, free_pages.numel()), n_free_out=(n_free_out, 1),
+        page_map=(page_map, n_pages), n_moves=(n_moves, 1)), table, n_seq)
+    _check_i32("paged_compact", dev, {}, table_out, n_seq)
+    if table_out.size(1) != table.size(1) or table_out.stride(0) != table.stride(0):
+        raise ValueError("paged_compact: table_out must have table's shape and strides")
+    _check_2d("paged_compact", dev, dict(moves=(moves, (n_pages + 1) // 2, 3)))
+    return check(load().qwfn_paged_compact(
+        n_kv.data_ptr(), n_seq, page_size, table.data_ptr(), table.stride(0), table.size(1), shared.data_ptr(), n_pages,
+        free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), table_out.data_ptr(), shared_out.data_ptr(),
+        free_out.data_ptr(), n_free_out.data_ptr(), page_map.data_ptr(), moves.data_ptr(), n_moves.data_ptr(), *_ws(ws, dev),
+        _stream_on(stream, dev)))
+
+
+def paged_copy(caches, moves, max_rows: int, n_moves=None, stream=None):
+    """The rows of moves [cap, 3] ({source, destination, rows}) copied in every tensor of caches (a cache_list, or tensors);
+    n_moves: device int32 [1], how many count (None: all)."""
+    dev = _Torch().device()
+    caches = _check_list("paged_copy", caches, dev)
+    _check_2d("paged_copy", dev, dict(moves=(moves, 0, 3)))
+    _check_i32("paged_copy", dev, dict(n_moves=(n_moves, 1)))
+    return check(load().qwfn_paged_copy(caches.arr, caches.n, moves.data_ptr(), moves.size(0), _ptr(n_moves), max_rows,
+                                        _stream_on(stream, dev)))
+
+
+def tree_masks(parents, masks, n_tree=None, n_past=None, pos=None, stream=None):
+    """What each node of drafted trees sees: parents int32 [n_seq, T] (-1: the context), masks int64 [n_seq, T]; pos int32
+    [n_seq, T], if given: n_past[b] + the node's depth. n_tree int32 [n_seq]: the nodes of each tree (None: T)."""
+    (n_seq, T), dev = parents.shape, _Torch().device()
+    _check_2d("tree_masks", dev, dict(parents=(parents, n_seq, T), masks=(masks, n_seq, T), pos=(pos, n_seq, T)))
+    _check_i32("tree_masks", dev, dict(n_tree=(n_tree, n_seq), n_past=(n_past, n_seq)))
+    return check(load().qwfn_tree_masks(parents.data_ptr(), _ptr(n_tree), _ptr(n_past), n_seq, T, masks.data_ptr(), _ptr(pos),
+                                        _stream_on(stream, dev)))
+
+
+def fattn_workspace_size_paged_tree(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int) -> int:
+    return int(load().qwfn_fattn_workspace_size_paged_tree(ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.shape[1],
+                                                           page_size))
+
+
+def flash_attn_ext_paged_tree(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int, n_kv, masks, scale: float, ov: Tensor,
+                              n_tree=None, gate=None, variant: int = Q8_X86, ws=None, stream=None):
+    """flash_attn_ext_paged of the nodes of drafted trees: masks int64 [n_seq, T] (tree_masks), n_tree device int32 [n_seq] or
+    None (T nodes each); a request's nodes are its newest tokens in the cache."""
+    n_seq, T, dev = qv.ne[3], qv.ne[1], _Torch().device()
+    _check_i32("flash_attn_ext_paged_tree", dev, dict(n_kv=(n_kv, n_seq), n_tree=(n_tree, n_seq)), table, n_seq)
+    _check_2d("flash_attn_ext_paged_tree", dev, dict(masks=(masks, n_seq, T)))
+    if gate is not None:
+        if gate.get_device() != dev:
+            raise ValueError(f"flash_attn_ext_paged_tree: gate must be on the current device ({dev})")
+        if not gate.is_contiguous():
+            raise ValueError("flash_attn_ext_paged_tree: gate must be contiguous")
+    gv = out_view(gate) if gate is not None else None
+    return check(load().qwfn_flash_attn_ext_q8_0_paged_tree(
+        ctypes.byref(qv), ctypes.byref(kv), ctypes.byref(vv), table.data_ptr(), table.stride(0), table.size(1), page_size,
+        n_kv.data_ptr(), _ptr(n_tree), masks.data_ptr(), scale, ctypes.byref(gv) if gv is not None else None, ctypes.byref(ov),
+        variant, *_ws(ws, dev), _stream_on(stream, dev)))
+
+
+def paged_accept(caches, page_size: int, table, n_kv, masks, leaf, n_keep, n_tree=None, cu_path=None, path=None, stream=None):
+    """The path to node leaf[b] of each tree moved to the tree's front in every tensor of caches (a cache_list, or tensors):
+    n_keep int32 [n_seq] the tokens then kept, cu_path [n_seq + 1] and path [n_seq * T] the accepted nodes b * T + t."""
+    (n_seq, T), dev = masks.shape, _Torch().device()
+    caches = _check_list("paged_accept", caches, dev)
+    _check_i32("paged_accept", dev, dict(n_kv=(n_kv, n_seq), leaf=(leaf, n_seq), n_keep=(n_keep, n_seq), n_tree=(n_tree, n_seq),
+                                         cu_path=(cu_path, n_seq + 1), path=(path, n_seq * T)), table, n_seq)
+    _check_2d("paged_accept", dev, dict(masks=(masks, n_seq, T)))
+    return check(load().qwfn_paged_accept(
+        caches.arr, caches.n, table.data_ptr(), table.stride(0), table.size(1), page_size, n_kv.data_ptr(), _ptr(n_tree),
+        masks.data_ptr(), leaf.data_ptr(), n_seq, T, n_keep.data_ptr(), _ptr(cu_path), _ptr(path), _stream_on(stream, dev)))
+
+
 # --------------------------------------------------------------------- linear attention
 
 def linear_attn_workspace_size(q, v, n_seq: int, max_len: int) -> int:
@@ -901,3 +1088,29 @@ def linear_attn(q, k, v, g, cu, max_len: int, state_in, state_out, out, slots=No
         cu.data_ptr(), n_seq, max_len, slots.data_ptr() if slots is not None else None, state_out.size(0),
         state_in.data_ptr() if state_in is not None else None, state_out.data_ptr(), scale, r(heads_view(out)), *_ws(ws, dev),
         _stream_on(stream, dev)))
+
+
+def linear_attn_tree(q, k, v, g, masks, state, out, n_tree=None, slots=None, scale: float | None = None, stream=None):
+    """The outputs of linear_attn for the nodes of drafted trees, without a step of the state: q, k, v, out packed
+    [n_seq * T, heads, d]; masks int64 [n_seq, T]; state float32 [n_slots, n_v, dk, dv] or None; n_tree, slots device int32
+    [n_seq] or None."""
+    (n_seq, T), dk, n_v, dv, dev = masks.shape, q.size(2), v.size(1), v.size(2), _Torch().device()
+    n_tok = n_seq * T
+    _check_i32("linear_attn_tree", dev, dict(n_tree=(n_tree, n_seq), slots=(slots, n_seq)))
+    _check_2d("linear_attn_tree", dev, dict(masks=(masks, n_seq, T)))
+    f32 = _Torch.float32
+    if state is not None and (state.dtype is not f32 or state.get_device() != dev or not state.is_contiguous() or state.dim() != 4
+                              or state.shape[1:] != (n_v, dk, dv)):
+        raise ValueError(f"linear_attn_tree: state must be contiguous float32 [n_slots, {n_v}, {dk}, {dv}] on the current device")
+    if g.dtype is not f32 or g.get_device() != dev or g.size(-1) != n_v or (g.stride(-1) != 1 and n_v > 1) \
+            or g.dim() not in (1, 2) or (g.dim() == 2 and g.size(0) < n_tok):
+        raise ValueError(f"linear_attn_tree: g must be float32 [{n_tok}, {n_v}] or [{n_v}] on the current device")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        if t.get_device() != dev:
+            raise ValueError(f"linear_attn_tree: {name} must be on the current device ({dev})")
+    scale = dk ** -0.5 if scale is None else scale
+    n_slots = state.size(0) if state is not None else 0x7fffffff
+    r = ctypes.byref
+    return check(load().qwfn_linear_attn_tree(
+        r(heads_view(q)), r(heads_view(k)), r(heads_view(v)), g.data_ptr(), g.stride(0) if g.dim() == 2 else 0, _ptr(n_tree),
+        masks.data_ptr(), n_seq, T, _ptr(slots), n_slots, _ptr(state), scale, r(heads_view(out)), _stream_on(stream, dev)))
