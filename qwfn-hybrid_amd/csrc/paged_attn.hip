@@ -126,7 +126,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
     const uint32_t j = blockIdx.x >> 3, jq = div_by(j, a.f_inner), hr = j - jq * a.f_inner.d;
     const int g = (int) jq * 8 + (int) (blockIdx.x & 7), rg = (int) div_by(hr, a.f_kv), kvh = (int) hr - rg * a.nh_kv;
     auto length = [&](int32_t b) { return TREE ? tree_len(a, b, rg) : clip_len(a, a.n_kv[b]); };
-    pa_run run = find_run(a, g, sh, length);
+    pa_run run = find_run<PA_WAVES, PA_MIN_TILES, PA_LEAD>(a, g, sh, length);
 
     uint8_t * const my = lds + wave * C::WAVE;
     uint64_t * const addr = (uint64_t *) (my + C::OA);
@@ -587,6 +587,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
 
 struct pa_plan {
     int32_t groups, runs, rows;        // row groups, of `rows` rows each
+    bool    wide;
     size_t  off_o, off_ml, bytes;
 };
 
@@ -598,10 +599,23 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv, bool tree) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    p.rows = 16;
+    // A tree of many rows takes 256 rows a workgroup (paged_tree.hip), where that is faster than 16. It pays from 65 rows on
+    // (of head size 64: 129), and where each of 512 workgroups of 16 rows would have at least 48 tiles. us, 16 rows against 256,
+    // f32, 2 KV heads:
+    //                                    96 rows        128        256        512       1024
+    //   D 256,  1 request  of  3000      22 / 34    24 / 37    27 / 52    38 / 61    96 / 73
+    //   D 256,  1 request  of 12000      33 / 42    35 / 46    51 / 64    81 / 79   254 / 114
+    //   D 256, 16 requests of  3000     100 / 76    88 / 82   148 / 124  248 / 199  965 / 349
+    //   D 256, 16 requests of 12000    302 / 183  246 / 189  476 / 290  887 / 521  3532 / 978
+    //   D 128, 16 requests of  3000      70 / 57    60 / 61   103 / 81   173 / 130  666 / 225
+    //   D 64,  16 requests of  3000      35 / 45    37 / 46    61 / 60
+    // and of 700 keys 58 / 55 with 1024 rows, 28 / 46 with 512. (64 rows, 16 requests of 12000: 137 / 172.)
+    const int64_t tiles = (max_kv + PA_TILE - 1) / PA_TILE * n_seq, narrow = (R + 15) / 16 * nh_kv;
+    p.wide = tree && R > (D == 64 ? PA_NARROW_64 : PA_NARROW_ROWS) && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
+    p.rows = p.wide ? tree_rows() : 16;
     p.groups = (int32_t) ((R + p.rows - 1) / p.rows);
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
-    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * PA_CUS / (nh_kv * p.groups), most));
+    p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>((p.wide ? tree_per_cu(D) : 2) * PA_CUS / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
     p.off_o = round256((size_t) n_seq * (tree ? p.groups : 1) * sizeof(int2));
     p.off_ml = p.off_o + round256(parts * D * sizeof(float));
@@ -646,8 +660,12 @@ int check_paged(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor 
 template <int D, bool TREE>
 int launch_paged(const pa_args & a, const pa_plan & p, hipStream_t s) {
     const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * p.groups));
-    hipLaunchKernelGGL((k_paged_attn<D, TREE>), grid, dim3(PA_THREADS), 0, s, a);
-    if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
+    if (TREE && p.wide) {
+        if (int rc = launch_tree_attn(a, D, p.groups, s)) return rc;
+    } else {
+        hipLaunchKernelGGL((k_paged_attn<D, TREE>), grid, dim3(PA_THREADS), 0, s, a);
+        if (int rc = hip_check(hipGetLastError(), "flash_attn_ext_paged launch")) return rc;
+    }
     // the requests' parts: on average runs / n_seq each, with long requests among short ones more
     const int64_t units = (int64_t) a.n_seq * a.nh_kv * a.R * (D / 64);
     if (a.runs > 16 * (int64_t) a.n_seq)

@@ -10,24 +10,6 @@
 #include <algorithm>
 
 namespace qwfn {
-namespace {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
-constexpr int PA_WAVES = 4;
-constexpr int PA_THREADS = PA_WAVES * 64;
-constexpr int PA_TILE = 32;            // keys of a tile
-constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
-constexpr int PA_LEAD = 8;             // tiles that a request counts more than it has
-constexpr int PA_CUS = 256;            // two workgroups a CU (registers)
-constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
-constexpr int PA_MAX_TREE_ROWS = 1024;
-constexpr float PA_LOG2E = 1.4426950408889634f;
-constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
-constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M
-constexpr float PA_IBIAS = 12582912.f; // 1.5 2^23: an integer below 2^22 added to its bits is added to its value
-constexpr int PA_IBITS = 0x4b400000;   // (a block's dot is at most 32 128 128 = 2^19)
 
 // x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), is off by at
 // most d <= 2^s, and x (m d - 2^(31 + s)) < 2^(31 + s) keeps the quotient whole.
@@ -37,8 +19,6 @@ inline fast_div make_div(uint32_t d) {
     while ((1ull << s) < d) s++;
     return {d, (uint32_t) (((1ull << (31 + s)) / d) + 1), s};
 }
-__device__ __forceinline__ uint32_t div_by(uint32_t x, fast_div f) { return f.s == 0 ? x : __umulhi(x, f.m) >> (f.s - 1); }
-
 struct pa_args {
     const char *    q; size_t q_nb1, q_nb2, q_nb3;
     const char *    k; const char * v;
@@ -63,6 +43,33 @@ struct pa_args {
     int32_t         group; fast_div f_group;
     uint32_t *      status;
 };
+
+// The attention of a tree with 32 query rows a wave (paged_tree.hip): the rows of a workgroup, workgroups of a CU, and the launch.
+int tree_rows();
+int tree_per_cu(int64_t D);
+int launch_tree_attn(const pa_args & a, int64_t D, int groups, hipStream_t s);
+
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_THREADS = PA_WAVES * 64;
+constexpr int PA_TILE = 32;            // keys of a tile
+constexpr int PA_MIN_TILES = PA_WAVES; // of a run: one a wave
+constexpr int PA_LEAD = 8;             // tiles that a request counts more than it has
+constexpr int PA_CUS = 256;            // two workgroups a CU (registers)
+constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
+constexpr int PA_MAX_TREE_ROWS = 1024;
+constexpr int PA_NARROW_ROWS = 64, PA_NARROW_64 = 128, PA_WIDE_ROWS = 512, PA_WIDE_TILES = 48;      // plan_paged
+constexpr float PA_LOG2E = 1.4426950408889634f;
+constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
+constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M
+constexpr float PA_IBIAS = 12582912.f; // 1.5 2^23: an integer below 2^22 added to its bits is added to its value
+constexpr int PA_IBITS = 0x4b400000;   // (a block's dot is at most 32 128 128 = 2^19)
+
+__device__ __forceinline__ uint32_t div_by(uint32_t x, fast_div f) { return f.s == 0 ? x : __umulhi(x, f.m) >> (f.s - 1); }
 
 // One wave-wide LDS DMA: lane i copies its UB bytes to LDS[at + UB i]. Inline asm, so that the compiler neither
 // moves memory operations across it nor waits for it: the kernel's own counts do. (m0 is read one wait state after
@@ -112,15 +119,18 @@ __device__ __forceinline__ void store4(char * p, int32_t type, const float x[4])
         *(uint2 *) p = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     }
 }
+// TYPE: a.type where it is known (-1: it is not).
+template <int TYPE = -1>
 __device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[4]) {
-    const size_t es = a.type == QWFN_TYPE_F32 ? 4 : 2;
+    const int32_t type = TYPE >= 0 ? TYPE : a.type;
+    const size_t es = type == QWFN_TYPE_F32 ? 4 : 2;
     if (a.gate) {
         float g[4];
-        load4(a.gate + elem * es, a.type, g);
+        load4(a.gate + elem * es, type, g);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = x[i] / (1.f + expf(-g[i]));
     }
-    store4(a.dst + elem * es, a.type, x);
+    store4(a.dst + elem * es, type, x);
 }
 
 // Largest over lanes l and l ^ 32, l and l ^ 16, a row of 16, without LDS.
@@ -151,10 +161,10 @@ struct pa_run { int32_t b, n, off, left, pos, per; };
 
 __device__ __forceinline__ int32_t clip_len(const pa_args & a, int32_t n) { return n <= 0 ? 0 : n < a.max_kv ? n : (int32_t) a.max_kv; }
 __device__ __forceinline__ int32_t tiles_of(int32_t n) { return (int32_t) (((uint32_t) n + PA_TILE - 1) / PA_TILE); }
-__device__ __forceinline__ int32_t cost_of(int32_t n) { return n > 0 ? tiles_of(n) + PA_LEAD : 0; }
-__device__ __forceinline__ int32_t run_len(const pa_args & a, int32_t total) {
-    const int32_t per = ((int32_t) div_by((uint32_t) (total + a.runs - 1), a.f_runs) + PA_WAVES - 1) / PA_WAVES * PA_WAVES;
-    return per < PA_MIN_TILES ? PA_MIN_TILES : per;         // whole rounds of the waves
+template <int LEAD> __device__ __forceinline__ int32_t cost_of(int32_t n) { return n > 0 ? tiles_of(n) + LEAD : 0; }
+template <int ROUND> __device__ __forceinline__ int32_t run_len(const pa_args & a, int32_t total) {
+    const int32_t per = ((int32_t) div_by((uint32_t) (total + a.runs - 1), a.f_runs) + ROUND - 1) / ROUND * ROUND;
+    return per < ROUND ? ROUND : per;                       // whole rounds of the waves
 }
 
 // A tree's nodes in the cache, and the keys that row group rg of request b goes through: none where it has no node.
@@ -176,12 +186,12 @@ __device__ __forceinline__ uint32_t tree_sees(uint64_t mask, int32_t key0, int32
 
 // Where run g starts, requests of len(b) keys. Up to 64 requests: a lane each, every wave on its own. More: every thread sums
 // the tiles of a few requests.
-template <typename Len>
+template <int WAVES, int ROUND, int LEAD, typename Len>
 __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * sh, Len len) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     pa_run r{0, 0, 0, 0, 0, 0};
     if (a.n_seq <= 64) {
-        const int32_t n = lane < a.n_seq ? len(lane) : 0, t = cost_of(n);
+        const int32_t n = lane < a.n_seq ? len(lane) : 0, t = cost_of<LEAD>(n);
         int32_t incl = t;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -189,22 +199,22 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
             if (lane >= d) incl += x;
         }
         const int32_t total = __builtin_amdgcn_readlane(incl, 63);
-        r.per = run_len(a, total);
+        r.per = run_len<ROUND>(a, total);
         const int64_t start = (int64_t) g * r.per;
         if (start < total) {
             r.b = __builtin_popcountll(__ballot(incl <= (int32_t) start));
             r.n = __builtin_amdgcn_readlane(n, r.b);
-            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b) - PA_LEAD;
+            r.off = (int32_t) start - __builtin_amdgcn_readlane(incl - t, r.b) - LEAD;
             r.left = total - (int32_t) start < r.per ? total - (int32_t) start : r.per;
             r.pos = (int32_t) start;
         }
         return r;
     }
-    const int c = (a.n_seq + PA_THREADS - 1) / PA_THREADS;
+    const int c = (a.n_seq + (WAVES * 64) - 1) / (WAVES * 64);
     int32_t sum = 0;
     for (int i = 0; i < c; i++) {
         const int b = tid * c + i;
-        if (b < a.n_seq) sum += cost_of(len(b));
+        if (b < a.n_seq) sum += cost_of<LEAD>(len(b));
     }
     int32_t incl = sum;
 #pragma unroll
@@ -216,32 +226,32 @@ __device__ __forceinline__ pa_run find_run(const pa_args & a, int g, int32_t * s
     __syncthreads();
     int32_t before = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < PA_WAVES; i++) {
+    for (int i = 0; i < WAVES; i++) {
         const int32_t x = sh[i];
         if (i < w) before += x;
         total += x;
     }
     incl += before;
-    r.per = run_len(a, total);
+    r.per = run_len<ROUND>(a, total);
     const int64_t start = (int64_t) g * r.per;
     if (start >= incl - sum && start < incl) {
         int32_t at = incl - sum;
         for (int i = 0; i < c; i++) {
             const int b = tid * c + i;
-            const int32_t n = b < a.n_seq ? len(b) : 0, t = cost_of(n);
+            const int32_t n = b < a.n_seq ? len(b) : 0, t = cost_of<LEAD>(n);
             if (start >= at && start < at + t) {
-                sh[PA_WAVES] = b;
-                sh[PA_WAVES + 1] = n;
-                sh[PA_WAVES + 2] = (int32_t) (start - at);
+                sh[WAVES] = b;
+                sh[WAVES + 1] = n;
+                sh[WAVES + 2] = (int32_t) (start - at);
             }
             at += t;
         }
     }
     __syncthreads();
     if (start < total) {
-        r.b = __builtin_amdgcn_readfirstlane(sh[PA_WAVES]);
-        r.n = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 1]);
-        r.off = __builtin_amdgcn_readfirstlane(sh[PA_WAVES + 2]) - PA_LEAD;
+        r.b = __builtin_amdgcn_readfirstlane(sh[WAVES]);
+        r.n = __builtin_amdgcn_readfirstlane(sh[WAVES + 1]);
+        r.off = __builtin_amdgcn_readfirstlane(sh[WAVES + 2]) - LEAD;
         r.left = __builtin_amdgcn_readfirstlane(total - start < r.per ? (int32_t) (total - start) : r.per);
         r.pos = (int32_t) start;
     }
