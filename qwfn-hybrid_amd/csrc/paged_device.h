@@ -45,8 +45,7 @@ struct pa_args {
 };
 
 // The attention of a tree with 32 query rows a wave (paged_tree.hip): the rows of a workgroup, workgroups of a CU, and the launch.
-int tree_rows();
-int tree_per_cu(int64_t D);
+int tree_rows(int64_t D, int64_t R);
 int launch_tree_attn(const pa_args & a, int64_t D, int groups, hipStream_t s);
 
 namespace {

@@ -4,11 +4,11 @@
 //   out = sum_j 2^(s_j - M) v_j / sum_j 2^(s_j - M),   v_j = dv_jb vq_j,   c = scale log2(e)
 //
 // over the tokens before the tree and the nodes in the query's mask. A tree of 64 nodes at 8 heads a KV head has 512 rows:
-// 940 operations a byte of the cache, so the matrix and vector units bound it, not the rows.
+// 940 operations a byte of the cache, so the vector and matrix units bound it, not the rows.
 //
 // Work: as in k_paged_attn the requests' key tiles of 32 stand in one row, cut into equal runs; a workgroup takes one run for
-// one KV head and 32 query rows a wave. Its waves share a tile: its rows come by LDS DMA while the tile before is multiplied, and
-// are converted once for all the rows:
+// one KV head and 32 query rows a wave, two waves a SIMD. Its waves share a tile: its rows come by LDS DMA two tiles ahead, and
+// each wave converts 4 keys (of 4 waves: 8) for all the rows, between the matrix instructions of the tile before:
 //   K   quants to 16-byte units [block][half][key], the A operands of v_mfma_i32_32x32x32_i8, a whole q8_0 block each
 //   V   to f16 pairs hi + lo of vq dv 2^(22 - e), e the exponent of the key's largest dv (dv < 2^(e - 14)), transposed: a
 //       unit holds 8 keys of one dim, in the order in which S^T leaves them in the registers
@@ -17,7 +17,15 @@
 //       running maximum of the shifted scores less 8, so P lies below 2^8 (2^14 before M follows), as in k_paged_attn.
 //   O^T = V^T P^T, v_mfma_f32_32x32x16_f16: P, an f16 pair too, is the B operand as it lies; hi hi + hi lo + lo hi, 2^-22. bf16
 //       results take hi hi alone: 2^-11 of a term, an eighth of the result's own rounding.
-// Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256).
+// Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256). O takes 128
+// registers of D 256, so the queries' scales and five of their blocks lie in LDS.
+//
+// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 267 us with the parts' merge (252 without), 0.39 P operations/s: the
+// vector units are busy for 60 % of the cycles, the matrix units for a third. A tile takes a SIMD's two waves 10000 cycles: 3700
+// of vector instructions in the scores, then 3100 of matrix instructions in the product, then 1800 in sending and at the barrier.
+// Slower: one half of the waves a phase behind the other with two barriers a tile, so that a product stands beside scores
+// (292 us), 4 waves of 64 rows with the registers of a whole SIMD (spills), operands of the product read further ahead (spills),
+// the conversion before the scores (291 us).
 #include "paged_device.h"
 
 #include <type_traits>
@@ -33,26 +41,24 @@ typedef uint16_t v2us __attribute__((ext_vector_type(2)));
 constexpr int TA_LEAD = 4;             // tiles that a request counts more than it has
 constexpr int TA_E0 = 22;              // a key's dv are stored times 2^(TA_E0 - e), below 2^8
 
-constexpr int TA_WAVES = 8, TA_THREADS = 64 * TA_WAVES, TA_ROWS = 32 * TA_WAVES;
-
-template <int D, int NT> struct ta_cfg {
+template <int D, int NT, int WAVES> struct ta_cfg {
+    static constexpr int PER_CU = 8 / WAVES, THREADS = 64 * WAVES, ROWS = 32 * WAVES;      // workgroups a CU, by registers
+    static constexpr int GROUPS = 8 / WAVES;                              // of 4 keys of a tile, a wave
     static constexpr int NBLK = D / QK, SEG = NBLK * QBLOCK;
     static constexpr int UB = SEG % 16 == 0 ? 16 : 4, UV = SEG / UB;      // DMA units, as in k_paged_attn
     static constexpr int LS = (SEG + 15) / 16 * 16, UPR = LS / UB;
-    // a wave brings in 4 keys: their rows of K, then of V
-    static constexpr int UNITS = 8 * UPR, DMAS = (UNITS + 63) / 64;
+    // a wave brings in its groups' rows of K and V
+    static constexpr int UNITS = GROUPS * 8 * UPR, DMAS = (UNITS + 63) / 64;
     static constexpr int UMUL = 65536 / UPR + 1;
-    static constexpr int GROUP = 8 * LS, RAW = TA_WAVES * GROUP;
+    static constexpr int GROUP = GROUPS * 8 * LS, RAW = WAVES * GROUP;
     // an image: K, V, K's scales, the keys' shifts and their inverses
     static constexpr int OV = NBLK * 1024, OS = OV + NT * NBLK * 2048, OE = OS + NBLK * PA_TILE * 2, OW = OE + PA_TILE * 4, IMG = OW + PA_TILE * 4;
     static constexpr int OI = RAW, OA = OI + 2 * IMG;
     // and of the queries the scales [wave][block][row] and, of D 256, the later blocks [wave][block][lane], which the registers do not hold
-    static constexpr int QREG = NBLK == 8 ? 3 : NBLK, OQ = OA + TA_ROWS * NBLK * 4, LDS = OQ + TA_WAVES * (NBLK - QREG) * 1024;
-    static constexpr int PER_CU = 1;                        // workgroups, by registers
-    static constexpr int WAVES_EU = PER_CU * TA_WAVES / 4;
-    static_assert(4 * TA_WAVES == PA_TILE && (UNITS - 1) * (UMUL * UPR - 65536) < 65536, "all keys, the division is exact");
+    static constexpr int QREG = NBLK == 8 ? 3 : NBLK, OQ = OA + ROWS * NBLK * 4, LDS = OQ + WAVES * (NBLK - QREG) * 1024;
+    static_assert((UNITS - 1) * (UMUL * UPR - 65536) < 65536, "all keys, the division is exact");
     static_assert(RAW % 16 == 0 && OV % 16 == 0 && OS % 16 == 0 && OE % 16 == 0 && IMG % 16 == 0, "aligned");
-    static_assert(TA_WAVES * NBLK * 1024 <= OA, "the queries fit");
+    static_assert(WAVES * NBLK * 1024 <= OA, "the queries fit");
     static_assert(PER_CU * (LDS + 128) <= 160 * 1024, "LDS of a CU");
 };
 
@@ -92,7 +98,10 @@ template <int NT> __device__ __forceinline__ void split2(float x, float y, uint3
     if constexpr (NT == 2) {
         const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
         hi = __builtin_bit_cast(uint32_t, h);
-        lo = pk_f16(x - (float) h[0], y - (float) h[1]);
+        float x1, y1;                                      // (the compiler takes two instructions each)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x1) : "v"(hi), "v"(x));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y1) : "v"(hi), "v"(y));
+        lo = pk_f16(x1, y1);
     } else {
         typedef _Float16 v2h __attribute__((ext_vector_type(2)));
         hi = __builtin_bit_cast(uint32_t, v2h{(_Float16) x, (_Float16) y});
@@ -108,13 +117,13 @@ template <typename F, int... X> __device__ __forceinline__ void for_blocks(F & f
     (fn(std::integral_constant<int, X>{}), ...);
 }
 
-template <int D, int TYPE>
-__global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 : 2>::WAVES_EU)) void k_paged_tree(pa_args a) {
+template <int D, int TYPE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
     constexpr int NT = TYPE == QWFN_TYPE_BF16 ? 1 : 2;
-    using C = ta_cfg<D, NT>;
+    using C = ta_cfg<D, NT, WAVES>;
     constexpr int NBLK = C::NBLK;
     __shared__ __attribute__((aligned(16))) uint8_t lds[C::LDS];
-    __shared__ int32_t sh[TA_WAVES + 3], odd[4];
+    __shared__ int32_t sh[WAVES + 3], odd[4];
     int tid = threadIdx.x;
 #define lane (tid & 63)
 #define ln (tid & 31)
@@ -125,7 +134,7 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
     const uint32_t jb = blockIdx.x >> 3, jq = div_by(jb, a.f_inner), hr = jb - jq * a.f_inner.d;
     const int g = (int) jq * 8 + (int) (blockIdx.x & 7), rg = (int) div_by(hr, a.f_kv), kvh = (int) hr - rg * a.nh_kv;
     auto length = [&](int32_t b) { return tree_len(a, b, rg); };
-    pa_run run = find_run<TA_WAVES, 1, TA_LEAD>(a, g, sh, length);
+    pa_run run = find_run<WAVES, 1, TA_LEAD>(a, g, sh, length);
 
     const uint32_t at_raw = pa_lds(lds) + wave * C::GROUP;
     const char * kh = a.k + (size_t) kvh * a.nb2;
@@ -135,7 +144,7 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
     // the lane's query row
     struct place { int row; uint32_t node, head; };
     auto query = [&]() {
-        const int row = rg * TA_ROWS + 32 * wave + ln, at = row < a.R ? row : a.R - 1;
+        const int row = rg * C::ROWS + 32 * wave + ln, at = row < a.R ? row : a.R - 1;
         const uint32_t node = div_by((uint32_t) at, a.f_rep);
         return place{row, node, (uint32_t) (kvh * a.rep + at) - node * (uint32_t) a.rep};
     };
@@ -155,7 +164,7 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
         const int32_t * table = a.table + (int64_t) b * a.t_stride;
         const int32_t nodes = tree_nodes(a, b, n), base = n - nodes;
         asm volatile("" : "+v"(tid));
-        const bool busy = rg * TA_ROWS + 32 * wave < nodes * a.rep;                   // the wave has a row
+        const bool busy = rg * C::ROWS + 32 * wave < nodes * a.rep;                   // the wave has a row
 
         const int32_t end = (run.off + nt) * PA_TILE < n ? (run.off + nt) * PA_TILE : n;
         // (the divisor's parts from scalar registers each time: kept in vector ones over the loop they are spilled)
@@ -180,7 +189,7 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
 #pragma unroll
             for (int i = 0; i < C::DMAS; i++) {
                 const int x = lane + 64 * i, row = (x * C::UMUL) >> 16, u = x - row * C::UPR;
-                const uint32_t sl = (uint32_t) __shfl((int) slot, 4 * wave + (row & 3));
+                const uint32_t sl = (uint32_t) __shfl((int) slot, 4 * (wave + WAVES * (row >> 3)) + (row & 3));
                 from[i] = (uint64_t) (uintptr_t) kh + (uint64_t) sl * a.nb1 + (uint32_t) ((u < C::UV ? u : C::UV - 1) * C::UB) + (row & 4 ? v_k : 0ull);
             }
             if (t < nt)
@@ -258,7 +267,7 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
 #pragma unroll
         for (int i = 0; i < 16; i++) ib[i] = PA_IBITS;
 
-        // ---- the wave's 4 keys of a tile into its images, in 8 steps that stand between matrix instructions: a lane 4 values of
+        // ---- the wave's keys of a tile into its images, 4 in 8 steps that stand between matrix instructions: a lane 4 values of
         // each key's K, then of its V (of D 64 and 128 not all lanes)
         struct { uint32_t w[4], w2[4], dv[4]; float d[4]; } cv;
         constexpr bool all = D == 256;
@@ -279,26 +288,27 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
             for (int k = 0; k < 4; k++) cv.w[k] = __builtin_amdgcn_alignbyte(cv.w2[k], cv.w[k], sh8);
         };
         auto convert = [&](auto X, int t, uint32_t alive, uint8_t * img) {
-            constexpr int x = X.value;
+            constexpr int x = X.value & 7, first = X.value & ~7;
+            const int group = wave + WAVES * (X.value >> 3);
             if (!all && lane >= D / 4) return;
             const int blk = lane >> 3, j = lane & 7;
-            if constexpr (x == 0) cv_read(0);
+            if constexpr (x == 0) cv_read(first);
             if constexpr (x == 1) {
                 // K: word j & 3 of unit (block, half j >> 2, key), units of a plane turned by the plane's number
                 cv_align();
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    *(uint32_t *) (img + (lane >> 2) * 512 + ((4 * wave + k + (lane >> 2)) & 31) * 16 + (j & 3) * 4) = cv.w[k];
+                    *(uint32_t *) (img + (lane >> 2) * 512 + ((4 * group + k + (lane >> 2)) & 31) * 16 + (j & 3) * 4) = cv.w[k];
                 if (j == 0)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) *(uint16_t *) (img + C::OS + (blk * PA_TILE + 4 * wave + k) * 2) = (uint16_t) cv.dv[k];
-                cv_read(4);
+                    for (int k = 0; k < 4; k++) *(uint16_t *) (img + C::OS + (blk * PA_TILE + 4 * group + k) * 2) = (uint16_t) cv.dv[k];
+                cv_read(first + 4);
             }
             if constexpr (x == 2) {
                 bool bad = false;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const bool on = alive >> (4 * wave + k) & 1, fine = (cv.dv[k] & 0x7fffu) < 0x7c00u;
+                    const bool on = alive >> (4 * group + k) & 1, fine = (cv.dv[k] & 0x7fffu) < 0x7c00u;
                     bad |= on && !fine;
                     cv.dv[k] = on && fine ? cv.dv[k] : 0u;
                 }
@@ -320,15 +330,15 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
                     const float up = __builtin_bit_cast(float, (127 + TA_E0 - e1) << 23);
                     cv.d[k] = dev::f16_bits_to_f32((uint16_t) cv.dv[k]) * up;
                     if (lane == k) {
-                        *(float *) (img + C::OE + 4 * (4 * wave + k)) = (float) (int) (e1 - TA_E0);
-                        *(float *) (img + C::OW + 4 * (4 * wave + k)) = up;
+                        *(float *) (img + C::OE + 4 * (4 * group + k)) = (float) (int) (e1 - TA_E0);
+                        *(float *) (img + C::OW + 4 * (4 * group + k)) = up;
                     }
                 }
             }
             if constexpr (x >= 4) {
                 // V, dim x - 4 of the lane's: keys 16 s + 4 h + 8 y + r are halves y of unit 2 s + h
                 constexpr int B = x - 4;
-                uint8_t * out = img + C::OV + (blk * 4 + 2 * (wave >> 2) + (wave & 1)) * 512 + j * 16 + (wave >> 1 & 1) * 8;
+                uint8_t * out = img + C::OV + (blk * 4 + 2 * (group >> 2) + (group & 1)) * 512 + j * 16 + (group >> 1 & 1) * 8;
                 float f[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) f[k] = byte_f32<B>(cv.w[k]) * cv.d[k];
@@ -341,13 +351,9 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
         };
         // the steps of block X of NBLK
         auto convert_some = [&](auto X, int t, uint32_t alive, uint8_t * img) {
-            constexpr int N = 8 / NBLK;
-            convert(std::integral_constant<int, N * X.value>{}, t, alive, img);
-            if constexpr (N > 1) convert(std::integral_constant<int, N * X.value + 1>{}, t, alive, img);
-            if constexpr (N > 2) {
-                convert(std::integral_constant<int, N * X.value + 2>{}, t, alive, img);
-                convert(std::integral_constant<int, N * X.value + 3>{}, t, alive, img);
-            }
+            constexpr int N = 8 * C::GROUPS / NBLK;
+            auto step = [&](auto S) { convert(std::integral_constant<int, N * decltype(X)::value + S.value>{}, t, alive, img); };
+            for_blocks(step, std::make_integer_sequence<int, N>{});
         };
         auto each_block = [&](auto fn) {
             for_blocks(fn, std::make_integer_sequence<int, NBLK>{});
@@ -584,8 +590,8 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
         if (wrong && tid == 0) atomicOr(a.status, DEVERR_GET_ROWS_INDEX);
         if (length(b) > 0) continue;
         const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int x = tid; x < TA_ROWS * (D / 4); x += TA_THREADS) {
-            const int r = rg * TA_ROWS + x / (D / 4);
+        for (int x = tid; x < C::ROWS * (D / 4); x += C::THREADS) {
+            const int r = rg * C::ROWS + x / (D / 4);
             if (r >= a.R) break;
             const uint32_t t = div_by((uint32_t) r, a.f_rep), h = (uint32_t) (kvh * a.rep + r) - t * (uint32_t) a.rep;
             store4(a.dst + ((((size_t) b * a.T + t) * a.nh + h) * D + 4 * (x % (D / 4))) * es, TYPE, z);
@@ -597,21 +603,26 @@ __global__ __launch_bounds__(TA_THREADS, (ta_cfg<D, TYPE == QWFN_TYPE_BF16 ? 1 :
 #undef half
 }
 
-template <int D>
-int launch(const pa_args & a, int groups, hipStream_t s) {
-    const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * groups)), blk(TA_THREADS);
-    if (a.type == QWFN_TYPE_BF16)     hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_BF16>), grid, blk, 0, s, a);
-    else if (a.type == QWFN_TYPE_F16) hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_F16>), grid, blk, 0, s, a);
-    else                              hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_F32>), grid, blk, 0, s, a);
-    return hip_check(hipGetLastError(), "flash_attn_ext_paged_tree launch");
+template <int D, int WAVES>
+void launch(const pa_args & a, int groups, hipStream_t s) {
+    const dim3 grid((unsigned) ((int64_t) (a.runs + 7) / 8 * 8 * a.nh_kv * groups)), blk(64 * WAVES);
+    if (a.type == QWFN_TYPE_BF16)     hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_BF16, WAVES>), grid, blk, 0, s, a);
+    else if (a.type == QWFN_TYPE_F16) hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_F16, WAVES>), grid, blk, 0, s, a);
+    else                              hipLaunchKernelGGL((k_paged_tree<D, QWFN_TYPE_F32, WAVES>), grid, blk, 0, s, a);
 }
 
 }  // namespace
 
-int tree_rows() { return TA_ROWS; }
-int tree_per_cu(int64_t D) { return D == 256 ? ta_cfg<256, 2>::PER_CU : D == 128 ? ta_cfg<128, 2>::PER_CU : ta_cfg<64, 2>::PER_CU; }
+// 256 rows a workgroup, or two workgroups a CU of up to 128 rows: their tiles are converted twice as often, but fewer waves idle.
+// us, 128 rows a workgroup against 256, D 128, f32, 2 KV heads, 16 requests of 12000 tokens: 96 rows 131 / 147, 128 rows
+// 137 / 151, 192 rows 240 / 187. (D 64 has no such calls, and D 256 no LDS for two.)
+int tree_rows(int64_t D, int64_t R) { return D == 128 && R <= 128 ? 128 : 256; }
 int launch_tree_attn(const pa_args & a, int64_t D, int groups, hipStream_t s) {
-    return D == 256 ? launch<256>(a, groups, s) : D == 128 ? launch<128>(a, groups, s) : launch<64>(a, groups, s);
+    if (D == 256)                         launch<256, 8>(a, groups, s);
+    else if (D == 64)                     launch<64, 8>(a, groups, s);
+    else if (tree_rows(D, a.R) == 128)    launch<128, 4>(a, groups, s);
+    else                                  launch<128, 8>(a, groups, s);
+    return hip_check(hipGetLastError(), "flash_attn_ext_paged_tree launch");
 }
 
 }  // namespace qwfn
