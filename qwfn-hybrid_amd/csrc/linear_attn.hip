@@ -849,6 +849,10 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
 // lo + l n + i (n = the slice's rows / 4), so that a lane's operands are consecutive in memory, and columns 4 m + j of
 // tile j, so that a row of the state is one 16-byte load a lane and 256 bytes a 16 lanes. The state's loads go out first and
 // come in while q, k and the scores are made.
+// Of bf16 inputs (BF) products run on the bf16 cores: the state and the weighted scores as three bf16 terms, 24 bits, against
+// q and v as they are (values that are not finite there become NaN). 48 requests of 32 nodes, 16 / 48 heads of 128: 55 us, 2.7
+// TB/s of the states, three workgroups a CU in three rounds; with F32 instructions, 25 us of them, 80 us; four workgroups a CU
+// (10 registers spilled) 59 us.
 //
 // A v_j that is not finite must not reach nodes that do not see it (0 times infinity): a workgroup that holds one takes its
 // scores times v by plain sums over the masks.
@@ -859,23 +863,34 @@ struct lt_args {
     const int32_t *  n_tree; const uint64_t * masks;
 };
 
-template <int DK, int TT, int CW> struct lt_cfg {
+template <int DK, int TT, int CW, bool BF> struct lt_cfg {
     static constexpr int KS = 4 / CW;                    // slices of the rows
     static constexpr int N = 16 * TT;                    // nodes, padded
     static constexpr int RPL = DK / KS / 4;              // rows of a lane
-    static constexpr int QS = DK + 4, PS = N + 4;        // floats of a row of q and k, of the scores, in LDS
-    static constexpr int JPL = N / 4 / KS > 0 ? N / 4 / KS : 1;            // nodes of a lane in the scores' product
+    static constexpr int QS = BF ? DK / 2 + 4 : DK + 4, PS = N + 4;        // dwords of a row of q and k, of the scores, in LDS
+    static constexpr int JPL = BF ? 4 * ((TT + KS - 1) / KS) : N / 4 / KS > 0 ? N / 4 / KS : 1;     // nodes of a lane in the scores' product
     static constexpr int OQ = 0, OK = N * QS, OP = 2 * N * QS, RED = (KS - 1) * CW * TT * 4 * 64 * 4;
     static constexpr int LDS = OP + N * PS > RED ? OP + N * PS : RED;      // floats
-    static_assert(JPL * 4 * KS == N, "whole nodes a lane");
+    static_assert(BF || JPL * 4 * KS == N, "whole nodes a lane");
+    static_assert(!BF || RPL >= 4, "rows for a matrix instruction");
     static_assert(LDS * 4 + 1536 <= 160 * 1024, "LDS of a CU");
 };
 
 __device__ __forceinline__ v4f mfma_f32(float x, float y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, z, 0, 0, 0); }
 
-template <int DK, int TT, int CW>
+// z + x y, 4 (K 16) or 8 (K 32) bf16 of a lane in each of the terms of y
+template <int DW> __device__ __forceinline__ v4f mfma_rows(const uint32_t * x, const uint32_t (&y)[3][DW], v4f z) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int n = 2; n >= 0; n--)
+        if constexpr (DW == 4) z = mfma_bf16(v4w{x[0], x[1], x[2], x[3]}, v4w{y[n][0], y[n][1], y[n][2], y[n][3]}, z);
+        else z = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, v2w{x[0], x[1]}), __builtin_bit_cast(v4s, v2w{y[n][0], y[n][1]}), z, 0, 0, 0);
+    return z;
+}
+
+template <int DK, int TT, int CW, bool BF>
 __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
-    using F = lt_cfg<DK, TT, CW>;
+    using F = lt_cfg<DK, TT, CW, BF>;
     __shared__ __attribute__((aligned(16))) float lds[F::LDS];
     __shared__ double gl[64], G[64];
     __shared__ float eG[64];
@@ -909,20 +924,29 @@ __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
     }
     // v of the lane's nodes
     float4 V[F::JPL];
-    const int j0 = (ks * 4 + l) * F::JPL;
+    uint2 W[F::JPL];
     const char * vh = a.v + (int64_t) h * a.v_nb1 + (int64_t) c * es;
+    auto node = [&](int i) { return BF ? 16 * (ks + F::KS * (i >> 2)) + 4 * l + (i & 3) : (ks * 4 + l) * F::JPL + i; };
 #pragma unroll
     for (int i = 0; i < F::JPL; i++) {
-        V[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on && j0 + i < nt) V[i] = la_load4(vh + (t0 + j0 + i) * a.v_nb2, a.type);
+        const int j = node(i);
+        if constexpr (BF) {
+            W[i] = make_uint2(0, 0);
+            if (on && j < nt) W[i] = *(const uint2 *) (vh + (t0 + j) * a.v_nb2);
+        } else {
+            V[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (on && j < nt) V[i] = la_load4(vh + (t0 + j) * a.v_nb2, a.type);
+        }
     }
     // q and k
     const char * qh = a.q + (int64_t) (h / a.rep) * a.q_nb1, * kh = a.k + (int64_t) (h / a.rep) * a.k_nb1;
-    for (int u = tid; u < 2 * F::N * (DK / 4); u += LT_THREADS) {
-        const int e4 = u % (DK / 4), t = u / (DK / 4) % F::N, which = u / (DK / 4) / F::N;
+    constexpr int PER = BF ? 8 : 4;                                        // of 16 bytes in LDS
+    for (int u = tid; u < 2 * F::N * (DK / PER); u += LT_THREADS) {
+        const int e = u % (DK / PER), t = u / (DK / PER) % F::N, which = u / (DK / PER) / F::N;
+        const char * from = (which ? kh + (t0 + t) * a.k_nb2 : qh + (t0 + t) * a.q_nb2) + PER * e * es;
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (4 * e4 < a.dk && t < nt) f = la_load4((which ? kh + (t0 + t) * a.k_nb2 : qh + (t0 + t) * a.q_nb2) + 4 * e4 * es, a.type);
-        *(float4 *) &lds[(which ? F::OK : F::OQ) + t * F::QS + 4 * e4] = f;
+        if (PER * e < a.dk && t < nt) f = BF ? *(const float4 *) from : la_load4(from, a.type);
+        *(float4 *) &lds[(which ? F::OK : F::OQ) + t * F::QS + 4 * e] = f;
     }
     // decays
     const uint64_t live = nt < 64 ? (1ull << nt) - 1 : ~0ull;
@@ -942,7 +966,8 @@ __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
     bool fine = true;
 #pragma unroll
     for (int i = 0; i < F::JPL; i++)
-        fine = fine && fabsf(V[i].x) < INFINITY && fabsf(V[i].y) < INFINITY && fabsf(V[i].z) < INFINITY && fabsf(V[i].w) < INFINITY;
+        if constexpr (BF) fine = fine && fabsf(bf16_lo(W[i].x)) < INFINITY && fabsf(bf16_hi(W[i].x)) < INFINITY && fabsf(bf16_lo(W[i].y)) < INFINITY && fabsf(bf16_hi(W[i].y)) < INFINITY;
+        else fine = fine && fabsf(V[i].x) < INFINITY && fabsf(V[i].y) < INFINITY && fabsf(V[i].z) < INFINITY && fabsf(V[i].w) < INFINITY;
     if (!fine) odd = 1;
     __syncthreads();
 
@@ -951,14 +976,19 @@ __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
     for (int tile = w; tile < TT * TT; tile += 4) {
         const int ti = tile / TT, tj = tile % TT;
         v4f s{0.f, 0.f, 0.f, 0.f};
-        const float * qp = &lds[F::OQ + (16 * ti + m) * F::QS + l * SR], * kp = &lds[F::OK + (16 * tj + m) * F::QS + l * SR];
+        const float * qp = &lds[F::OQ + (16 * ti + m) * F::QS], * kp = &lds[F::OK + (16 * tj + m) * F::QS];
+        if constexpr (BF) {
 #pragma unroll
-        for (int i = 0; i < SR; i += 4) {
-            const float4 y = *(const float4 *) (qp + i), z = *(const float4 *) (kp + i);
-            s = mfma_f32(y.x, z.x, s);
-            s = mfma_f32(y.y, z.y, s);
-            s = mfma_f32(y.z, z.z, s);
-            s = mfma_f32(y.w, z.w, s);
+            for (int i = 0; i < DK / 32; i++) s = mfma_bf16(*(const v4w *) (qp + 16 * i + 4 * l), *(const v4w *) (kp + 16 * i + 4 * l), s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < SR; i += 4) {
+                const float4 y = *(const float4 *) (qp + l * SR + i), z = *(const float4 *) (kp + l * SR + i);
+                s = mfma_f32(y.x, z.x, s);
+                s = mfma_f32(y.y, z.y, s);
+                s = mfma_f32(y.z, z.z, s);
+                s = mfma_f32(y.w, z.w, s);
+            }
         }
 #pragma unroll
         for (int r = 0; r < 4; r++) {
@@ -969,18 +999,37 @@ __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
     }
     // the state's part
     v4f O[TT][4] = {};
+    if constexpr (BF) {
+        constexpr int RM = F::RPL >= 8 ? 8 : 4;                            // rows of a lane in a matrix instruction
 #pragma unroll
-    for (int i = 0; i < F::RPL; i += 4) {
+        for (int i = 0; i < F::RPL; i += RM)
 #pragma unroll
-        for (int tt = 0; tt < TT; tt++) {
-            const float4 y = *(const float4 *) &lds[F::OQ + (16 * tt + m) * F::QS + row0 + i];
-            const float q4[4] = {y.x, y.y, y.z, y.w};
+            for (int j = 0; j < 4; j++) {
+                uint32_t y[3][RM / 2];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                O[tt][0] = mfma_f32(q4[k], S[i + k].x, O[tt][0]);
-                O[tt][1] = mfma_f32(q4[k], S[i + k].y, O[tt][1]);
-                O[tt][2] = mfma_f32(q4[k], S[i + k].z, O[tt][2]);
-                O[tt][3] = mfma_f32(q4[k], S[i + k].w, O[tt][3]);
+                for (int k = 0; k < RM / 2; k++) {
+                    uint32_t t[3];
+                    bf16_terms<3>(((const float *) &S[i + 2 * k])[j], ((const float *) &S[i + 2 * k + 1])[j], t);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) y[n][k] = t[n];
+                }
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) O[tt][j] = mfma_rows<RM / 2>((const uint32_t *) &lds[F::OQ + (16 * tt + m) * F::QS + (row0 + i) / 2], y, O[tt][j]);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < F::RPL; i += 4) {
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) {
+                const float4 y = *(const float4 *) &lds[F::OQ + (16 * tt + m) * F::QS + row0 + i];
+                const float q4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    O[tt][0] = mfma_f32(q4[k], S[i + k].x, O[tt][0]);
+                    O[tt][1] = mfma_f32(q4[k], S[i + k].y, O[tt][1]);
+                    O[tt][2] = mfma_f32(q4[k], S[i + k].z, O[tt][2]);
+                    O[tt][3] = mfma_f32(q4[k], S[i + k].w, O[tt][3]);
+                }
             }
         }
     }
@@ -993,16 +1042,47 @@ __global__ __launch_bounds__(LT_THREADS) void k_linear_tree(lt_args x) {
     __syncthreads();
     // the scores' part
     if (!odd) {
+        if constexpr (BF) {
 #pragma unroll
-        for (int i = 0; i < F::JPL; i++)
+            for (int i = 0; i < F::JPL; i += 4) {
+                if (ks + F::KS * (i >> 2) >= TT) continue;                 // (the same for a wave)
 #pragma unroll
-            for (int tt = 0; tt < TT; tt++) {
-                const float p = lds[F::OP + (16 * tt + m) * F::PS + j0 + i];
-                O[tt][0] = mfma_f32(p, V[i].x, O[tt][0]);
-                O[tt][1] = mfma_f32(p, V[i].y, O[tt][1]);
-                O[tt][2] = mfma_f32(p, V[i].z, O[tt][2]);
-                O[tt][3] = mfma_f32(p, V[i].w, O[tt][3]);
+                for (int tt = 0; tt < TT; tt++) {
+                    const float4 p = *(const float4 *) &lds[F::OP + (16 * tt + m) * F::PS + node(i)];
+                    uint32_t y[3][2], t[3];
+                    bf16_terms<3>(p.x, p.y, t);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) y[n][0] = t[n];
+                    bf16_terms<3>(p.z, p.w, t);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) y[n][1] = t[n];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        // column j of the 4 nodes
+                        auto pair = [&](int k) {
+                            const uint32_t u = j < 2 ? W[i + k].x : W[i + k].y, v = j < 2 ? W[i + k + 1].x : W[i + k + 1].y;
+                            return __builtin_amdgcn_perm(v, u, j & 1 ? 0x07060302u : 0x05040100u);
+                        };
+                        typedef short v4s __attribute__((ext_vector_type(4)));
+                        const v4s w4 = __builtin_bit_cast(v4s, v2w{pair(0), pair(2)});
+#pragma unroll
+                        for (int n = 2; n >= 0; n--)
+                            O[tt][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, v2w{y[n][0], y[n][1]}), w4, O[tt][j], 0, 0, 0);
+                    }
+                }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < F::JPL; i++)
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) {
+                    const float p = lds[F::OP + (16 * tt + m) * F::PS + node(0) + i];
+                    O[tt][0] = mfma_f32(p, V[i].x, O[tt][0]);
+                    O[tt][1] = mfma_f32(p, V[i].y, O[tt][1]);
+                    O[tt][2] = mfma_f32(p, V[i].z, O[tt][2]);
+                    O[tt][3] = mfma_f32(p, V[i].w, O[tt][3]);
+                }
+        }
     } else if (ks == 0 && on) {
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
@@ -1155,8 +1235,12 @@ int launch_type(const lc_args & x, const lc_plan & p, hipStream_t s) {
 
 template <int DK, int TT>
 void launch_tree(const lt_args & x, unsigned blocks, bool wide, hipStream_t s) {
-    if (wide) hipLaunchKernelGGL((k_linear_tree<DK, TT, 2>), dim3(blocks), dim3(LT_THREADS), 0, s, x);
-    else      hipLaunchKernelGGL((k_linear_tree<DK, TT, 1>), dim3(blocks), dim3(LT_THREADS), 0, s, x);
+    const dim3 grid(blocks), blk(LT_THREADS);
+    const bool bf = x.a.type == QWFN_TYPE_BF16;
+    if (wide && bf) hipLaunchKernelGGL((k_linear_tree<DK, TT, 2, true>), grid, blk, 0, s, x);
+    else if (wide)  hipLaunchKernelGGL((k_linear_tree<DK, TT, 2, false>), grid, blk, 0, s, x);
+    else if (bf)    hipLaunchKernelGGL((k_linear_tree<DK, TT, 1, true>), grid, blk, 0, s, x);
+    else            hipLaunchKernelGGL((k_linear_tree<DK, TT, 1, false>), grid, blk, 0, s, x);
 }
 template <int DK>
 int launch_tree(const lt_args & x, unsigned blocks, bool wide, hipStream_t s) {

@@ -179,22 +179,33 @@ __global__ __launch_bounds__(SH_THREADS) void k_release_mark(release_args a) {
     report(a.status, bad, DEVERR_PAGES);
 }
 
-// A wave per request: each page that it gives back counts one less, and is free with the last of its holders.
+// A wave per request: each page that it gives back counts one less, and is free with the last of its holders. RD_BATCH pages of a
+// lane are on their way together, for a step is a load and two atomics after each other (512 requests of up to 1024 pages: 14 us
+// one at a time).
+constexpr int RD_BATCH = 8;
+
 __global__ __launch_bounds__(SH_THREADS) void k_release_drop(release_args a) {
     const int lane = threadIdx.x & 63;
     for (int64_t b = (int64_t) blockIdx.x * (SH_THREADS / 64) + (threadIdx.x >> 6); b < a.n_seq; b += (int64_t) gridDim.x * (SH_THREADS / 64)) {
         const pt_req r = a.req[b];
         const int32_t * src = a.table + b * a.t_stride + r.past;
         bool bad = false;
-        for (int32_t c = lane; c < r.have; c += 64) {
-            const int32_t p = src[c];
-            if (!in_pool(p, a.n_pages)) {
-                bad = true;
-                continue;
+        for (int32_t c = lane; c < r.have; c += 64 * RD_BATCH) {
+            int32_t p[RD_BATCH], was[RD_BATCH];
+#pragma unroll
+            for (int i = 0; i < RD_BATCH; i++) p[i] = src[c + 64 * i < r.have ? c + 64 * i : c];
+#pragma unroll
+            for (int i = 0; i < RD_BATCH; i++) {
+                const bool on = c + 64 * i < r.have, ok = on && in_pool(p[i], a.n_pages);
+                bad |= on && !ok;
+                was[i] = 1;
+                if (ok) was[i] = atomicSub(a.shared_out + p[i], 1);
             }
-            const int32_t was = atomicSub(a.shared_out + p, 1);
-            if (was == 0) atomicOr(a.bits + (p >> 5), 1u << (p & 31));
-            bad |= was < 0;
+#pragma unroll
+            for (int i = 0; i < RD_BATCH; i++) {
+                if (was[i] == 0) atomicOr(a.bits + (p[i] >> 5), 1u << (p[i] & 31));
+                bad |= was[i] < 0;
+            }
         }
         report(a.status, bad, DEVERR_PAGES);
     }
@@ -207,6 +218,7 @@ __global__ __launch_bounds__(SH_THREADS) void k_release_push(release_args a) {
     const int tid = threadIdx.x;
     const int64_t w0 = (int64_t) blockIdx.x * SH_THREADS;
     int64_t before = 0;
+#pragma unroll 8
     for (int64_t i = tid; i < w0; i += SH_THREADS) before += __popc(a.bits[i]);
     before = block_scan({before, 0}, &part[0]).x;
     if (tid == SH_THREADS - 1) sum = before;
