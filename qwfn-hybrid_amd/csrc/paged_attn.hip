@@ -650,20 +650,21 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv, bool tree) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    // A tree of many rows takes 256 rows a workgroup (paged_tree.hip), where that is faster than 16. It pays from 65 rows on
-    // (of head size 64: 129), and where each of 512 workgroups of 16 rows would have at least 48 tiles. us, 16 rows against 256,
+    // A tree of many rows takes 128 or 256 rows a workgroup (paged_tree.hip), where that is faster than 16. It pays from 65
+    // rows on, and where each of 512 workgroups of 16 rows would have at least 48 tiles. us, 16 rows against that,
     // f32, 2 KV heads:
     //                                    96 rows        128        256        512       1024
-    //   D 256,  1 request  of  3000      22 / 34    24 / 37    27 / 52    38 / 61    96 / 73
-    //   D 256,  1 request  of 12000      33 / 42    35 / 46    51 / 64    81 / 79   254 / 114
-    //   D 256, 16 requests of  3000     100 / 76    88 / 82   148 / 124  248 / 199  965 / 349
-    //   D 256, 16 requests of 12000    302 / 183  246 / 189  476 / 290  887 / 521  3532 / 978
-    //   D 128, 16 requests of  3000      70 / 57    60 / 61   103 / 81   173 / 130  666 / 225
-    //   D 64,  16 requests of  3000      35 / 45    37 / 46    61 / 60
-    // and of 700 keys 58 / 55 with 1024 rows, 28 / 46 with 512. (64 rows, 16 requests of 12000: 137 / 172.)
+    //   D 256,  1 request  of  3000      22 / 33    24 / 36    27 / 52    38 / 60    94 / 73
+    //   D 256,  1 request  of 12000      33 / 42    35 / 46    51 / 63    81 / 79   255 / 111
+    //   D 256, 16 requests of  3000     100 / 70    88 / 76   148 / 112  248 / 171  975 / 296
+    //   D 256, 16 requests of 12000    299 / 175  246 / 186  475 / 286  887 / 531  3559 / 952
+    //   D 128, 16 requests of  3000      71 / 47    61 / 51   103 / 76   171 / 119  671 / 199
+    //   D 64,  16 requests of  3000      35 / 38    38 / 41    62 / 54   101 / 86   309 / 151
+    //   D 64,  16 requests of 12000      99 / 81    98 / 83   187 / 143  346 / 260 1146 / 495
+    // and of 700 keys 58 / 51 with 1024 rows, 28 / 45 with 512. (64 rows, 16 requests of 12000: 135 / 166.)
     const int64_t tiles = (max_kv + PA_TILE - 1) / PA_TILE * n_seq, narrow = (R + 15) / 16 * nh_kv;
-    p.wide = tree && R > (D == 64 ? PA_NARROW_64 : PA_NARROW_ROWS) && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
-    p.rows = p.wide ? tree_rows(D, R) : 16;
+    p.wide = tree && R > PA_NARROW_ROWS && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
+    p.rows = p.wide ? tree_rows(D) : 16;
     p.groups = (int32_t) ((R + p.rows - 1) / p.rows);
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
     p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>((p.wide ? 256 / p.rows : 2) * PA_CUS / (nh_kv * p.groups), most));

@@ -45,7 +45,7 @@ struct pa_args {
 };
 
 // The attention of a tree with 32 query rows a wave (paged_tree.hip): the rows of a workgroup, workgroups of a CU, and the launch.
-int tree_rows(int64_t D, int64_t R);
+int tree_rows(int64_t D);
 int launch_tree_attn(const pa_args & a, int64_t D, int groups, hipStream_t s);
 
 namespace {
@@ -61,7 +61,7 @@ constexpr int PA_LEAD = 8;             // tiles that a request counts more than 
 constexpr int PA_CUS = 256;            // two workgroups a CU (registers)
 constexpr int PA_MAX_ROWS = 64;        // query rows per KV head
 constexpr int PA_MAX_TREE_ROWS = 1024;
-constexpr int PA_NARROW_ROWS = 64, PA_NARROW_64 = 128, PA_WIDE_ROWS = 512, PA_WIDE_TILES = 48;      // plan_paged
+constexpr int PA_NARROW_ROWS = 64, PA_WIDE_ROWS = 512, PA_WIDE_TILES = 48;      // plan_paged
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_SLACK = 6.f;        // log2 by which M may lie below its request
 constexpr int PA_BIAS = 8;             // P dv < 2^PA_BIAS at M

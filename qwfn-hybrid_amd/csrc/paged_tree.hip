@@ -8,7 +8,7 @@
 //
 // Work: as in k_paged_attn the requests' key tiles of 32 stand in one row, cut into equal runs; a workgroup takes one run for
 // one KV head and 32 query rows a wave, two waves a SIMD. Its waves share a tile: its rows come by LDS DMA two tiles ahead, and
-// each wave converts 4 keys (of 4 waves: 8) for all the rows, between the matrix instructions of the tile before:
+// each wave converts 4 keys (D below 256, 4 waves: 8) for all the rows, between the matrix instructions of the tile before:
 //   K   quants to 16-byte units [block][half][key], the A operands of v_mfma_i32_32x32x32_i8, a whole q8_0 block each
 //   V   to f16 pairs hi + lo of vq dv 2^(22 - e), e the exponent of the key's largest dv (dv < 2^(e - 14)), transposed: a
 //       unit holds 8 keys of one dim, in the order in which S^T leaves them in the registers
@@ -20,12 +20,13 @@
 // Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256). O takes 128
 // registers of D 256, so the queries' scales and five of their blocks lie in LDS.
 //
-// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 267 us with the parts' merge (252 without), 0.39 P operations/s: the
+// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 266 us with the parts' merge (250 without), 0.39 P operations/s: the
 // vector units are busy for 60 % of the cycles, the matrix units for a third. A tile takes a SIMD's two waves 10000 cycles: 3700
 // of vector instructions in the scores, then 3100 of matrix instructions in the product, then 1800 in sending and at the barrier.
 // Slower: one half of the waves a phase behind the other with two barriers a tile, so that a product stands beside scores
 // (292 us), 4 waves of 64 rows with the registers of a whole SIMD (spills), operands of the product read further ahead (spills),
-// the conversion before the scores (291 us).
+// the conversion before the scores (291 us). Of D 128 and 64 two workgroups of 4 waves share a CU, each lane with a key's 4
+// values: 4 requests of 9001 tokens, 24 nodes, 8 KV heads of 128, f16, 79 us; with 8 waves, half of their lanes idle, 112.
 #include "paged_device.h"
 
 #include <type_traits>
@@ -43,7 +44,9 @@ constexpr int TA_E0 = 22;              // a key's dv are stored times 2^(TA_E0 -
 
 template <int D, int NT, int WAVES> struct ta_cfg {
     static constexpr int PER_CU = 8 / WAVES, THREADS = 64 * WAVES, ROWS = 32 * WAVES;      // workgroups a CU, by registers
-    static constexpr int GROUPS = 8 / WAVES;                              // of 4 keys of a tile, a wave
+    // of 4 keys of a tile, a wave, D / 4 lanes each
+    static constexpr int GROUPS = 8 / WAVES;
+    static_assert(GROUPS * D <= 256, "a lane for each");
     static constexpr int NBLK = D / QK, SEG = NBLK * QBLOCK;
     static constexpr int UB = SEG % 16 == 0 ? 16 : 4, UV = SEG / UB;      // DMA units, as in k_paged_attn
     static constexpr int LS = (SEG + 15) / 16 * 16, UPR = LS / UB;
@@ -267,44 +270,45 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
 #pragma unroll
         for (int i = 0; i < 16; i++) ib[i] = PA_IBITS;
 
-        // ---- the wave's keys of a tile into its images, 4 in 8 steps that stand between matrix instructions: a lane 4 values of
-        // each key's K, then of its V (of D 64 and 128 not all lanes)
+        // ---- the wave's keys of a tile into its images, C::GROUPS groups in steps that stand between matrix instructions: a lane 4
+        // values of each of its group's keys' K, then of their V (of D 64 and 128 not always all lanes)
         struct { uint32_t w[4], w2[4], dv[4]; float d[4]; } cv;
-        constexpr bool all = D == 256;
-        auto cv_read = [&](int first) {
-            const int blk = lane >> 3, j = lane & 7;
-            const uint8_t * raw = lds + wave * C::GROUP + first * C::LS + QBLOCK * blk;
-            const uint32_t * wp = (const uint32_t *) (raw + (blk & 1 ? 2 : 0)) + j;
+#define cl (lane & (D / 4 - 1))
+        constexpr bool all = D * C::GROUPS == 256;
+        auto cv_read = [&](int first) {                    // (a scale by the dword that holds it)
+            const int blk = cl >> 3, j = lane & 7, at = QBLOCK * blk + (blk & 1 ? 2 : 0), which = all && D == 256 ? 0 : lane / (D / 4);
+            const uint8_t * raw = lds + wave * C::GROUP + (first + 8 * which) * C::LS + at;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                cv.w[k] = *(const uint32_t *) ((const uint8_t *) wp + k * C::LS);
-                cv.w2[k] = *(const uint32_t *) ((const uint8_t *) (wp + 1) + k * C::LS);
-                cv.dv[k] = *(const uint16_t *) (raw + k * C::LS);
+                cv.w[k] = *(const uint32_t *) (raw + 4 * j + k * C::LS);
+                cv.w2[k] = *(const uint32_t *) (raw + 4 * j + 4 + k * C::LS);
+                cv.dv[k] = *(const uint32_t *) (raw - (blk & 1 ? 4 : 0) + k * C::LS);
             }
         };
         auto cv_align = [&]() {
-            const uint32_t sh8 = lane & 8 ? 0u : 2u;
+            const uint32_t sh8 = lane & 8 ? 0u : 2u, sh16 = lane & 8 ? 16u : 0u;
 #pragma unroll
-            for (int k = 0; k < 4; k++) cv.w[k] = __builtin_amdgcn_alignbyte(cv.w2[k], cv.w[k], sh8);
+            for (int k = 0; k < 4; k++) {
+                cv.w[k] = __builtin_amdgcn_alignbyte(cv.w2[k], cv.w[k], sh8);
+                cv.dv[k] = __builtin_amdgcn_ubfe(cv.dv[k], sh16, 16);
+            }
         };
         auto convert = [&](auto X, int t, uint32_t alive, uint8_t * img) {
-            constexpr int x = X.value & 7, first = X.value & ~7;
-            const int group = wave + WAVES * (X.value >> 3);
-            if (!all && lane >= D / 4) return;
-            const int blk = lane >> 3, j = lane & 7;
-            if constexpr (x == 0) cv_read(first);
+            constexpr int x = X.value;
+            if (!all && lane >= C::GROUPS * (D / 4)) return;
+            const int blk = cl >> 3, j = lane & 7, group = wave + (all && D == 256 ? 0 : WAVES * (lane / (D / 4)));
+            if constexpr (x == 0) cv_read(0);
             if constexpr (x == 1) {
                 // K: word j & 3 of unit (block, half j >> 2, key), units of a plane turned by the plane's number
                 cv_align();
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    *(uint32_t *) (img + (lane >> 2) * 512 + ((4 * group + k + (lane >> 2)) & 31) * 16 + (j & 3) * 4) = cv.w[k];
-                if (j == 0)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) *(uint16_t *) (img + C::OS + (blk * PA_TILE + 4 * group + k) * 2) = (uint16_t) cv.dv[k];
-                cv_read(first + 4);
+                    *(uint32_t *) (img + (cl >> 2) * 512 + ((4 * group + k + (cl >> 2)) & 31) * 16 + (j & 3) * 4) = cv.w[k];
+                if (j == 0) *(uint2 *) (img + C::OS + (blk * PA_TILE + 4 * group) * 2) = make_uint2(cv.dv[0] | cv.dv[1] << 16, cv.dv[2] | cv.dv[3] << 16);
+                cv_read(4);
             }
             if constexpr (x == 2) {
+                cv_align();
                 bool bad = false;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -313,10 +317,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                     cv.dv[k] = on && fine ? cv.dv[k] : 0u;
                 }
                 if (bad) odd[t & 3] = 1;
-                cv_align();
             }
             if constexpr (x == 3) {
-                uint32_t m[2];
+                uint32_t m[2], e[4];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     m[k] = (cv.dv[2 * k] | cv.dv[2 * k + 1] << 16) & 0x7fff7fffu;
@@ -324,15 +327,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                     if constexpr (D >= 128) m[k] = pk_max_lanes<16>(m[k]);
                     if constexpr (D >= 256) m[k] = pk_max_lanes<32>(m[k]);
                 }
+                auto up = [](uint32_t e1) { return __builtin_bit_cast(float, (127 + TA_E0 - e1) << 23); };
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const uint32_t e = (k & 1 ? m[k / 2] >> 26 : m[k / 2] >> 10 & 31u), e1 = e < 1 ? 1u : e;
-                    const float up = __builtin_bit_cast(float, (127 + TA_E0 - e1) << 23);
-                    cv.d[k] = dev::f16_bits_to_f32((uint16_t) cv.dv[k]) * up;
-                    if (lane == k) {
-                        *(float *) (img + C::OE + 4 * (4 * group + k)) = (float) (int) (e1 - TA_E0);
-                        *(float *) (img + C::OW + 4 * (4 * group + k)) = up;
-                    }
+                    e[k] = k & 1 ? m[k / 2] >> 26 : m[k / 2] >> 10 & 31u;
+                    e[k] = e[k] < 1 ? 1u : e[k];
+                    cv.d[k] = dev::f16_bits_to_f32((uint16_t) cv.dv[k]) * up(e[k]);
+                }
+                const uint32_t mine = cl & 2 ? (cl & 1 ? e[3] : e[2]) : (cl & 1 ? e[1] : e[0]);
+                if (cl < 4) {
+                    *(float *) (img + C::OE + 4 * (4 * group + cl)) = (float) ((int) mine - TA_E0);
+                    *(float *) (img + C::OW + 4 * (4 * group + cl)) = up(mine);
                 }
             }
             if constexpr (x >= 4) {
@@ -349,12 +354,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                 if constexpr (NT == 2) *(uint2 *) (out + NBLK * 2048 + B * 128) = lo;
             }
         };
-        // the steps of block X of NBLK
+        // the steps from 1 of block X of NBLK
         auto convert_some = [&](auto X, int t, uint32_t alive, uint8_t * img) {
-            constexpr int N = 8 * C::GROUPS / NBLK;
-            auto step = [&](auto S) { convert(std::integral_constant<int, N * decltype(X)::value + S.value>{}, t, alive, img); };
+            constexpr int N = 8 / NBLK;
+            auto step = [&](auto S) {
+                if constexpr (1 + N * decltype(X)::value + S.value < 8)
+                    convert(std::integral_constant<int, 1 + N * decltype(X)::value + S.value>{}, t, alive, img);
+            };
             for_blocks(step, std::make_integer_sequence<int, N>{});
         };
+        constexpr std::integral_constant<int, 0> step0;
         auto each_block = [&](auto fn) {
             for_blocks(fn, std::make_integer_sequence<int, NBLK>{});
         };
@@ -485,6 +494,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
         // Tile t is multiplied from one image while t + 1 becomes the other and the rows of t + 2 are on their way. A wave converts
         // the keys that it has brought in itself, so one barrier a tile is for the images alone.
         pa_wait<0>();
+        convert(step0, 0, live, lds + C::OI);
         each_block([&](auto X) { convert_some(X, 0, live, lds + C::OI); });
         pa_wait_lds();
         uint32_t next = send(1, page1, at_raw);
@@ -508,10 +518,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                     qk_sums(blk, d);
                     __builtin_amdgcn_sched_barrier(0);
                 });
+                pa_wait<0>();
+                convert(step0, t + 1, next, img1);
                 pv_read(0, 0, img);
                 softmax(t, live, odd[t & 3] != 0, img);
                 __builtin_amdgcn_s_setprio(0);
-                pa_wait<0>();
                 __builtin_amdgcn_sched_barrier(0);
                 // the product, and the next tile's images between
                 each_block([&](auto X) {
@@ -532,6 +543,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                 });
             } else {
                 pa_wait<0>();
+                convert(step0, t + 1, next, img1);
                 each_block([&](auto X) { convert_some(X, t + 1, next, img1); });
             }
             pa_wait_lds();
@@ -601,6 +613,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
 #undef lane
 #undef ln
 #undef half
+#undef cl
 }
 
 template <int D, int WAVES>
@@ -613,15 +626,12 @@ void launch(const pa_args & a, int groups, hipStream_t s) {
 
 }  // namespace
 
-// 256 rows a workgroup, or two workgroups a CU of up to 128 rows: their tiles are converted twice as often, but fewer waves idle.
-// us, 128 rows a workgroup against 256, D 128, f32, 2 KV heads, 16 requests of 12000 tokens: 96 rows 131 / 147, 128 rows
-// 137 / 151, 192 rows 240 / 187. (D 64 has no such calls, and D 256 no LDS for two.)
-int tree_rows(int64_t D, int64_t R) { return D == 128 && R <= 128 ? 128 : 256; }
+// Of D 256 the images and the queries leave no LDS for a second workgroup of a CU.
+int tree_rows(int64_t D) { return D == 256 ? 256 : 128; }
 int launch_tree_attn(const pa_args & a, int64_t D, int groups, hipStream_t s) {
-    if (D == 256)                         launch<256, 8>(a, groups, s);
-    else if (D == 64)                     launch<64, 8>(a, groups, s);
-    else if (tree_rows(D, a.R) == 128)    launch<128, 4>(a, groups, s);
-    else                                  launch<128, 8>(a, groups, s);
+    if (D == 256)      launch<256, 8>(a, groups, s);
+    else if (D == 128) launch<128, 4>(a, groups, s);
+    else               launch<64, 4>(a, groups, s);
     return hip_check(hipGetLastError(), "flash_attn_ext_paged_tree launch");
 }
 

@@ -1,4 +1,4 @@
-"""The attention tests of test_gpu_tree with page tables so wide that the calls take the kernel of 256 query rows a workgroup."""
+"""The attention tests of test_gpu_tree with page tables so wide that the calls take the kernel of 128 or 256 query rows a workgroup."""
 import pytest
 import torch
 
@@ -21,7 +21,7 @@ def wide(monkeypatch):
 @pytest.mark.parametrize("D,kvh,rep,T,page", [
     (256, 2, 8, 9, 7), (256, 1, 3, 22, 1), (256, 2, 8, 16, 32), (256, 2, 8, 17, 100), (256, 1, 8, 32, 16), (256, 2, 8, 33, 32),
     (256, 1, 8, 64, 16), (256, 3, 12, 64, 5), (128, 8, 4, 24, 16), (128, 2, 7, 37, 5), (128, 1, 2, 64, 16), (128, 2, 8, 64, 33),
-    (64, 1, 3, 50, 256), (64, 2, 8, 31, 3), (64, 1, 8, 64, 16)])
+    (64, 1, 3, 50, 256), (64, 2, 8, 31, 3), (64, 3, 5, 17, 9), (64, 1, 8, 64, 16)])
 def test_shapes(gpu, D, kvh, rep, T, page):
     G.test_attention_shapes(gpu, D, kvh, rep, T, page)
 
