@@ -306,8 +306,9 @@ int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_te
  * from n_tree[b] on are not read and give 0. q, k, v, g, dst, the slots and the states as in
  * qwfn_linear_attn (n_tok = n_seq * T; state may be NULL: zeros; a slot of -2 - s leaves the
  * request out, its dst rows are not written). A decay below exp(-693) counts as that. F32
- * products and sums for every type, sums of decays F64; what a node does not see never
- * reaches it, infinite or not. An n_tree outside [0, T] is clipped and sets bit 0 of
+ * products and sums for every type (bf16: the state and the scores as three bf16 terms,
+ * so that an infinity in them gives NaN), sums of decays F64; what a node does not see
+ * never reaches it, infinite or not. An n_tree outside [0, T] is clipped and sets bit 0 of
  * qwfn_device_status, as does a slot outside [-1 - n_slots, n_slots). One launch. */
 int qwfn_linear_attn_tree(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_tensor * v, const float * g,
                           int64_t g_token_stride, const int32_t * n_tree, const uint64_t * masks, int32_t n_seq, int32_t T,
