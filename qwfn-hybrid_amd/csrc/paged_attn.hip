@@ -583,36 +583,42 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
     }
 }
 
-// The same of a tree's many rows with few parts each: D / 4 lanes a row, so that a wave has its row's
-// parts in flight together (PM_ROW of them). 8 requests of 9 to 10 parts, 1024 rows each, D 256: 16 us for 29, 4.7 TB/s.
+// The same of k_paged_tree's parts, which lie as its registers held them: a wave takes 32 rows and, of a block of 32 dims, 4 of each
+// half; of many parts GROUPS waves of a workgroup every GROUPS-th each. PM_ROW parts are in flight together. 8 requests of 9 to 10
+// parts, 1024 rows each, D 256: 19 us; of parts in rows 16 (29 with 16 lanes a row), but their stores cost the main kernel 14 more.
 constexpr int PM_ROW = 12;
 
-template <int D>
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void k_tree_merge(pa_args a) {
-    constexpr int LANES = D / 4;
-    const int64_t unit = (int64_t) blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const uint32_t bk = (uint32_t) (unit / a.R), r = (uint32_t) (unit - (int64_t) bk * a.R);
-    const uint32_t b = div_by(bk, a.f_kv), kvh = bk - b * (uint32_t) a.nh_kv;
+    __shared__ float4 acc[GROUPS][64];
+    __shared__ float2 gl[GROUPS][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = GROUPS > 1 ? wave : 0;
+    const int64_t unit = GROUPS > 1 ? (int64_t) blockIdx.x : (int64_t) blockIdx.x * 4 + wave;
+    const uint32_t tiles = (uint32_t) (a.R + 31) / 32, ut = (uint32_t) (unit / (D / 8)), piece = (uint32_t) (unit - (int64_t) ut * (D / 8));
+    const uint32_t bk = ut / tiles, tile = ut - bk * tiles, b = div_by(bk, a.f_kv), kvh = bk - b * (uint32_t) a.nh_kv;
     if (b >= (uint32_t) a.n_seq) return;
-    const int2 sp = a.span[(int64_t) div_by(r, a.f_group) * a.n_seq + b];
+    const int2 sp = a.span[(int64_t) div_by(32 * tile, a.f_group) * a.n_seq + b];
     if (sp.x == sp.y) return;
-    const int q = threadIdx.x % LANES, n = sp.y - sp.x + 1;
-    const size_t step = (size_t) a.nh_kv * a.R, p0 = ((size_t) (sp.x + (int) b) * a.nh_kv + kvh) * a.R + r;
-    const float * po = a.part_o + p0 * D + 4 * q;
+    const uint32_t row = 32 * tile + (lane & 31), r = row < (uint32_t) a.R ? row : (uint32_t) a.R - 1;
+    const int n = sp.y - sp.x + 1;
+    const size_t p0 = (size_t) (sp.x + (int) b) * a.nh_kv + kvh;
+    const float2 * pm = a.part_ml + p0 * a.R + r;
+    const float * po = a.part_o + (p0 * tiles + tile) * (32 * D) + piece * 256 + lane * 4;
+    const size_t step_m = (size_t) a.nh_kv * a.R, step_o = (size_t) a.nh_kv * tiles * (32 * D);
     float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < n; s0 += PM_ROW) {
+    for (int s0 = grp; s0 < n; s0 += GROUPS * PM_ROW) {
         float2 e[PM_ROW];
         float4 x[PM_ROW];
         float to = M;
 #pragma unroll
         for (int i = 0; i < PM_ROW; i++) {
-            const int s = s0 + i < n ? s0 + i : s0;
-            e[i] = a.part_ml[p0 + s * step];
-            x[i] = *(const float4 *) (po + s * step * D);
+            const int s = s0 + i * GROUPS < n ? s0 + i * GROUPS : s0;
+            e[i] = pm[s * step_m];
+            x[i] = *(const float4 *) (po + s * step_o);
         }
 #pragma unroll
         for (int i = 0; i < PM_ROW; i++) {
-            if (s0 + i >= n) e[i] = make_float2(-INFINITY, 0.f);
+            if (s0 + i * GROUPS >= n) e[i] = make_float2(-INFINITY, 0.f);
             to = fmaxf(to, e[i].x);
         }
         const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to);
@@ -627,11 +633,30 @@ __global__ __launch_bounds__(256) void k_tree_merge(pa_args a) {
         }
         M = to;
     }
+    if constexpr (GROUPS > 1) {
+        acc[grp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+        gl[grp][lane] = make_float2(M, l);
+        __syncthreads();
+        if (grp > 0) return;
+        float to = M;
+#pragma unroll
+        for (int i = 1; i < GROUPS; i++) to = fmaxf(to, gl[i][lane].x);
+        l = o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++) {
+            const float2 e = gl[i][lane];
+            const float4 x = acc[i][lane];
+            const float w = e.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e.x - to);
+            l += w * e.y;
+            if (w != 0.f) { o[0] += w * x.x; o[1] += w * x.y; o[2] += w * x.z; o[3] += w * x.w; }
+        }
+    }
+    if (row >= (uint32_t) a.R) return;
     const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] *= inv;
     const uint32_t t = div_by(r, a.f_rep), h = kvh * (uint32_t) a.rep + r - t * (uint32_t) a.rep;
-    finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 4 * q, o);
+    finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 32 * (piece >> 2) + 16 * (lane >> 5) + 4 * (piece & 3), o);
 }
 
 // ---------------------------------------------------------------- host
@@ -661,7 +686,8 @@ pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_se
     //   D 128, 16 requests of  3000      71 / 47    61 / 51   103 / 76   171 / 119  671 / 199
     //   D 64,  16 requests of  3000      35 / 38    38 / 41    62 / 54   101 / 86   309 / 151
     //   D 64,  16 requests of 12000      99 / 81    98 / 83   187 / 143  346 / 260 1146 / 495
-    // and of 700 keys 58 / 51 with 1024 rows, 28 / 45 with 512. (64 rows, 16 requests of 12000: 135 / 166.)
+    // and of 700 keys 58 / 51 with 1024 rows, 28 / 45 with 512. (64 rows, 16 requests of 12000: 135 / 166.) The lengths are
+    // on the device: the table's width stands for them.
     const int64_t tiles = (max_kv + PA_TILE - 1) / PA_TILE * n_seq, narrow = (R + 15) / 16 * nh_kv;
     p.wide = tree && R > PA_NARROW_ROWS && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
     p.rows = p.wide ? tree_rows(D) : 16;
@@ -669,8 +695,9 @@ pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_se
     const int64_t most = (n_seq * ((max_kv + PA_TILE - 1) / PA_TILE + PA_LEAD) + PA_MIN_TILES - 1) / PA_MIN_TILES;
     p.runs = (int32_t) std::max<int64_t>(1, std::min<int64_t>((p.wide ? 256 / p.rows : 2) * PA_CUS / (nh_kv * p.groups), most));
     const size_t parts = (size_t) (p.runs + n_seq) * nh_kv * R;
+    const size_t rows = (size_t) (p.runs + n_seq) * nh_kv * (p.wide ? (R + 31) / 32 * 32 : R);           // (k_tree_merge: whole tiles)
     p.off_o = round256((size_t) n_seq * (tree ? p.groups : 1) * sizeof(int2));
-    p.off_ml = p.off_o + round256(parts * D * sizeof(float));
+    p.off_ml = p.off_o + round256(rows * D * sizeof(float));
     p.bytes = p.off_ml + round256(parts * sizeof(float2));
     return p;
 }
@@ -720,10 +747,12 @@ int launch_paged(const pa_args & a, const pa_plan & p, hipStream_t s) {
     }
     // the requests' parts: on average runs / n_seq each, with long requests among short ones more
     const int64_t units = (int64_t) a.n_seq * a.nh_kv * a.R * (D / 64);
-    if (a.runs > 16 * (int64_t) a.n_seq)
+    if (TREE && p.wide) {
+        const int64_t pieces = (int64_t) a.n_seq * a.nh_kv * ((a.R + 31) / 32) * (D / 8);
+        if (a.runs > 16 * (int64_t) a.n_seq) hipLaunchKernelGGL((k_tree_merge<D, 4>), dim3((unsigned) pieces), dim3(256), 0, s, a);
+        else                                 hipLaunchKernelGGL((k_tree_merge<D, 1>), dim3((unsigned) ((pieces + 3) / 4)), dim3(256), 0, s, a);
+    } else if (a.runs > 16 * (int64_t) a.n_seq)
         hipLaunchKernelGGL((k_paged_merge<D, 16, TREE>), dim3((unsigned) units), dim3(256), 0, s, a);
-    else if (TREE && p.wide)
-        hipLaunchKernelGGL((k_tree_merge<D>), dim3((unsigned) ((units + 15) / 16)), dim3(256), 0, s, a);
     else
         hipLaunchKernelGGL((k_paged_merge<D, 4, TREE>), dim3((unsigned) ((units + 3) / 4)), dim3(256), 0, s, a);
     return hip_check(hipGetLastError(), "flash_attn_ext_paged launch");

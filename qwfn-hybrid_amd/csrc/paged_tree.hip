@@ -20,13 +20,13 @@
 // Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256). O takes 128
 // registers of D 256, so the queries' scales and five of their blocks lie in LDS.
 //
-// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 266 us with the parts' merge (250 without), 0.39 P operations/s: the
+// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 259 us with the parts' merge (240 without), 0.40 P operations/s: the
 // vector units are busy for 60 % of the cycles, the matrix units for a third. A tile takes a SIMD's two waves 10000 cycles: 3700
 // of vector instructions in the scores, then 3100 of matrix instructions in the product, then 1800 in sending and at the barrier.
 // Slower: one half of the waves a phase behind the other with two barriers a tile, so that a product stands beside scores
 // (292 us), 4 waves of 64 rows with the registers of a whole SIMD (spills), operands of the product read further ahead (spills),
 // the conversion before the scores (291 us). Of D 128 and 64 two workgroups of 4 waves share a CU, each lane with a key's 4
-// values: 4 requests of 9001 tokens, 24 nodes, 8 KV heads of 128, f16, 79 us; with 8 waves, half of their lanes idle, 112.
+// values: 4 requests of 9001 tokens, 24 nodes, 8 KV heads of 128, f16, 76 us; with 8 waves, half of their lanes idle, 112.
 #include "paged_device.h"
 
 #include <type_traits>
@@ -577,13 +577,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                     }
             } else if (to.row < a.R) {
                 if (half == 0) a.part_ml[part] = alive ? make_float2(M, ll) : make_float2(-INFINITY, 0.f);
-                float * po = a.part_o + part * D + 16 * half;
+                // (as the registers lie, k_tree_merge takes them so: a store writes 1 KB in one piece)
+                const int tile = rg * (C::ROWS / 32) + wave;
+                float * po = a.part_o + (((size_t) (g + b) * a.nh_kv + kvh) * ((a.R + 31) / 32) + tile) * (32 * D) + lane * 4;
                 if (alive)
 #pragma unroll
                     for (int blk = 0; blk < NBLK; blk++)
 #pragma unroll
                         for (int x = 0; x < 4; x++)
-                            *(float4 *) (po + QK * blk + 4 * x) = make_float4(O[blk][x], O[blk][4 + x], O[blk][8 + x], O[blk][12 + x]);
+                            *(float4 *) (po + (blk * 4 + x) * 256) = make_float4(O[blk][x], O[blk][4 + x], O[blk][8 + x], O[blk][12 + x]);
             }
         }
         if (run.off == 0 && kvh == 0 && tid == 0) a.span[rg * a.n_seq + b] = make_int2(g, (run.pos + tiles - 1) / run.per);
