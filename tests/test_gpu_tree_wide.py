@@ -71,3 +71,30 @@ def test_strides_and_workspaces(gpu):
 
 def test_captured(gpu):
     G.test_attention_captured(gpu)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams with a workspace each, several in flight: the bits of calls one after another."""
+    G.say("tree attention: two streams")
+    K = gpu
+    cases = [WideCase([900, 40, 1300], 256, 2, 8, 24, 16, n_tree=[24, 3, 20], seed=31), WideCase([1500, 7], 128, 2, 6, 32, 16, seed=32)]
+    want = [c.on_gpu(K) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = []
+    for c, st in zip(cases, streams):
+        nb = (34, c.kd.stride(0), c.D // 32 * 34, c.n_rows * c.kd.stride(0))
+        kv, vv = (K.tensor(x.data_ptr(), K.TYPE_Q8_0, (c.D, c.n_rows, c.kvh, 1), nb) for x in (c.kd, c.vd))
+        q, td, nd, m = c.q.cuda(), G.dev(c.table), G.i32(c.lens), G.words(c.m)
+        nt = None if c.n_tree is None else G.i32(c.n_tree)
+        o = torch.zeros((8,) + tuple(want[len(outs)].shape), device="cuda")
+        qv = K.q_view(q)
+        w = G.ws_of(K.fattn_workspace_size_paged_tree(qv, kv, vv, td, c.page))
+        outs.append((o, (q, td, nd, m, nt, w, kv, vv, qv, c)))
+    torch.cuda.synchronize()
+    for i in range(8):
+        for (o, (q, td, nd, m, nt, w, kv, vv, qv, c)), st in zip(outs, streams):
+            K.flash_attn_ext_paged_tree(qv, kv, vv, td, c.page, nd, m, c.scale, K.out_view(o[i]), n_tree=nt, ws=w, stream=st)
+    torch.cuda.synchronize()
+    for (o, _), x in zip(outs, want):
+        for i in range(8):
+            assert torch.equal(o[i], x)
