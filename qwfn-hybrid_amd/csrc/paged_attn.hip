@@ -679,14 +679,14 @@ pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_se
     // rows on, and where each of 512 workgroups of 16 rows would have at least 48 tiles. us, 16 rows against that,
     // f32, 2 KV heads:
     //                                    96 rows        128        256        512       1024
-    //   D 256,  1 request  of  3000      22 / 33    24 / 36    27 / 52    38 / 60    94 / 73
-    //   D 256,  1 request  of 12000      33 / 42    35 / 46    51 / 63    81 / 79   255 / 111
-    //   D 256, 16 requests of  3000     100 / 70    88 / 76   148 / 112  248 / 171  975 / 296
-    //   D 256, 16 requests of 12000    299 / 175  246 / 186  475 / 286  887 / 531  3559 / 952
-    //   D 128, 16 requests of  3000      71 / 47    61 / 51   103 / 76   171 / 119  671 / 199
-    //   D 64,  16 requests of  3000      35 / 38    38 / 41    62 / 54   101 / 86   309 / 151
-    //   D 64,  16 requests of 12000      99 / 81    98 / 83   187 / 143  346 / 260 1146 / 495
-    // and of 700 keys 58 / 51 with 1024 rows, 28 / 45 with 512. (64 rows, 16 requests of 12000: 135 / 166.) The lengths are
+    //   D 256,  1 request  of  3000      22 / 31    24 / 33    27 / 44    38 / 51    95 / 60
+    //   D 256,  1 request  of 12000      33 / 40    35 / 43    51 / 54    80 / 69   254 / 100
+    //   D 256, 16 requests of  3000     103 / 68    89 / 71   147 / 104  248 / 166  964 / 288
+    //   D 256, 16 requests of 12000    299 / 171  243 / 176  474 / 284  884 / 497  3537 / 898
+    //   D 128, 16 requests of  3000      70 / 45    60 / 48   100 / 68   171 / 111  665 / 197
+    //   D 64,  16 requests of  3000      35 / 38    37 / 40    61 / 53    99 / 86   308 / 153
+    //   D 64,  16 requests of 12000      96 / 80    96 / 82   185 / 142  344 / 262 1135 / 501
+    // and of 700 keys 58 / 46 with 1024 rows, 28 / 41 with 512. (64 rows, 16 requests of 12000: 136 / 162.) The lengths are
     // on the device: the table's width stands for them.
     const int64_t tiles = (max_kv + PA_TILE - 1) / PA_TILE * n_seq, narrow = (R + 15) / 16 * nh_kv;
     p.wide = tree && R > PA_NARROW_ROWS && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
