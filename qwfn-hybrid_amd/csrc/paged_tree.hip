@@ -94,7 +94,6 @@ template <int BIT> __device__ __forceinline__ uint32_t pk_max_lanes(uint32_t x) 
     return pk_max(p, q);
 }
 
-typedef __fp16 v2fp __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk_f16(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)); }
 // x and y as f16: hi cut off with lo the rest, or hi alone, to nearest.
 template <int NT> __device__ __forceinline__ void split2(float x, float y, uint32_t & hi, uint32_t & lo) {
@@ -276,7 +275,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
 #define cl (lane & (D / 4 - 1))
         constexpr bool all = D * C::GROUPS == 256;
         auto cv_read = [&](int first) {                    // (a scale by the dword that holds it)
-            const int blk = cl >> 3, j = lane & 7, at = QBLOCK * blk + (blk & 1 ? 2 : 0), which = all && D == 256 ? 0 : lane / (D / 4);
+            const int blk = cl >> 3, j = lane & 7, at = QBLOCK * blk + (blk & 1 ? 2 : 0), which = C::GROUPS == 1 ? 0 : lane / (D / 4);
             const uint8_t * raw = lds + wave * C::GROUP + (first + 8 * which) * C::LS + at;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -296,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
         auto convert = [&](auto X, int t, uint32_t alive, uint8_t * img) {
             constexpr int x = X.value;
             if (!all && lane >= C::GROUPS * (D / 4)) return;
-            const int blk = cl >> 3, j = lane & 7, group = wave + (all && D == 256 ? 0 : WAVES * (lane / (D / 4)));
+            const int blk = cl >> 3, j = lane & 7, group = wave + (C::GROUPS == 1 ? 0 : WAVES * (lane / (D / 4)));
             if constexpr (x == 0) cv_read(0);
             if constexpr (x == 1) {
                 // K: word j & 3 of unit (block, half j >> 2, key), units of a plane turned by the plane's number
