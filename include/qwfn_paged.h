@@ -113,7 +113,8 @@ int qwfn_paged_trim(const int32_t * n_keep, const int32_t * n_kv, int32_t n_seq,
  *        so does a request of length 0 (a padded batch)
  *   dst  [D, n_head, T, n_seq] contiguous, 16-byte aligned, q's type, not
  *        overlapping q
- *   gate NULL or dst's type and shape: dst = attention * sigmoid(gate); may be dst
+ *   gate NULL or dst's type and shape: dst = attention * sigmoid(gate); may be dst.
+ *        Rows that are 0 stay 0 whatever it holds there
  * D 64, 128 or 256; n_head a multiple of n_head_kv, T * n_head / n_head_kv <= 64;
  * head rows and strides aligned to D / 16 bytes. Arithmetic as
  * qwfn_flash_attn_ext_q8_0: Q requantised to q8_0 with `variant`, exact integer

@@ -475,7 +475,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void k_paged_attn(pa_args a) {
                 if (whole) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) o[k] *= inv;
-                    finish4(a, elem + d0, o);
+                    finish4(a, elem + d0, o, ll);
                 } else {
                     *(float4 *) (a.part_o + part * D + d0) = make_float4(o[0], o[1], o[2], o[3]);
                 }
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(pa_args a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] *= inv;
         const uint32_t t = div_by(r, a.f_rep), h = kvh * (uint32_t) a.rep + r - t * (uint32_t) a.rep;
-        finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 64 * quarter + 4 * q, x);
+        finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 64 * quarter + 4 * q, x, ll);
     }
 }
 
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(pa_args a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] *= inv;
     const uint32_t t = div_by(r, a.f_rep), h = kvh * (uint32_t) a.rep + r - t * (uint32_t) a.rep;
-    finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 32 * (piece >> 2) + 16 * (lane >> 5) + 4 * (piece & 3), o);
+    finish4(a, (((size_t) b * a.T + t) * a.nh + h) * D + 32 * (piece >> 2) + 16 * (lane >> 5) + 4 * (piece & 3), o, l);
 }
 
 // ---------------------------------------------------------------- host

@@ -118,12 +118,13 @@ __device__ __forceinline__ void store4(char * p, int32_t type, const float x[4])
         *(uint2 *) p = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     }
 }
-// TYPE: a.type where it is known (-1: it is not).
+// l: the row's sum of weights. 0 where its query saw nothing (or is no node): x is 0 then and stays 0 whatever the gate holds, NaN
+// in a padded batch. TYPE: a.type where it is known (-1: it is not).
 template <int TYPE = -1>
-__device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[4]) {
+__device__ __forceinline__ void finish4(const pa_args & a, size_t elem, float x[4], float l) {
     const int32_t type = TYPE >= 0 ? TYPE : a.type;
     const size_t es = type == QWFN_TYPE_F32 ? 4 : 2;
-    if (a.gate) {
+    if (a.gate && l != 0.f) {
         float g[4];
         load4(a.gate + elem * es, type, g);
 #pragma unroll

@@ -571,8 +571,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                         float o[4];
 #pragma unroll
                         for (int y = 0; y < 4; y++) o[y] = alive ? O[blk][4 * y + x] * inv : 0.f;
-                        if (alive) finish4<TYPE>(a, elem + QK * blk + 4 * x, o);
-                        else store4(a.dst + (elem + QK * blk + 4 * x) * es, TYPE, o);
+                        finish4<TYPE>(a, elem + QK * blk + 4 * x, o, alive ? ll : 0.f);
                     }
             } else if (to.row < a.R) {
                 if (half == 0) a.part_ml[part] = alive ? make_float2(M, ll) : make_float2(-INFINITY, 0.f);
