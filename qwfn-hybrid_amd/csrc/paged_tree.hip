@@ -15,8 +15,9 @@
 //   S^T = K Q^T: a lane has one query row and 16 keys. The shift of V enters S as e - 22, where it starts, so that
 //       P = 2^(s + e - 22 - M) times the stored V is 2^(s - M) v, and the sum takes P 2^(22 - e). The reference M is the
 //       running maximum of the shifted scores less 8, so P lies below 2^8 (2^14 before M follows), as in k_paged_attn.
-//   O^T = V^T P^T, v_mfma_f32_32x32x16_f16: P, an f16 pair too, is the B operand as it lies; hi hi + hi lo + lo hi, 2^-22. bf16
-//       results take hi hi alone: 2^-11 of a term, an eighth of the result's own rounding.
+//   O^T = V^T P^T, v_mfma_f32_32x32x16_f16: P, an f16 pair too, is the B operand as it lies; hi hi + hi lo + lo hi, 2^-22, for
+//       every type (one f16 each would be 2^-10 off of the sum of p |v|, which bf16's own rounding hides only where the value is
+//       as large as that sum)
 // Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256). O takes 128
 // registers of D 256, so the queries' scales and five of their blocks lie in LDS.
 //
@@ -42,7 +43,7 @@ typedef uint16_t v2us __attribute__((ext_vector_type(2)));
 constexpr int TA_LEAD = 4;             // tiles that a request counts more than it has
 constexpr int TA_E0 = 22;              // a key's dv are stored times 2^(TA_E0 - e), below 2^8
 
-template <int D, int NT, int WAVES> struct ta_cfg {
+template <int D, int WAVES> struct ta_cfg {
     static constexpr int PER_CU = 8 / WAVES, THREADS = 64 * WAVES, ROWS = 32 * WAVES;      // workgroups a CU, by registers
     // of 4 keys of a tile, a wave, D / 4 lanes each
     static constexpr int GROUPS = 8 / WAVES;
@@ -55,7 +56,7 @@ template <int D, int NT, int WAVES> struct ta_cfg {
     static constexpr int UMUL = 65536 / UPR + 1;
     static constexpr int GROUP = GROUPS * 8 * LS, RAW = WAVES * GROUP;
     // an image: K, V, K's scales, the keys' shifts and their inverses
-    static constexpr int OV = NBLK * 1024, OS = OV + NT * NBLK * 2048, OE = OS + NBLK * PA_TILE * 2, OW = OE + PA_TILE * 4, IMG = OW + PA_TILE * 4;
+    static constexpr int OV = NBLK * 1024, OS = OV + 2 * NBLK * 2048, OE = OS + NBLK * PA_TILE * 2, OW = OE + PA_TILE * 4, IMG = OW + PA_TILE * 4;
     static constexpr int OI = RAW, OA = OI + 2 * IMG;
     // and of the queries the scales [wave][block][row] and, of D 256, the later blocks [wave][block][lane], which the registers do not hold
     static constexpr int QREG = NBLK == 8 ? 3 : NBLK, OQ = OA + ROWS * NBLK * 4, LDS = OQ + WAVES * (NBLK - QREG) * 1024;
@@ -95,19 +96,13 @@ template <int BIT> __device__ __forceinline__ uint32_t pk_max_lanes(uint32_t x) 
 }
 
 __device__ __forceinline__ uint32_t pk_f16(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)); }
-// x and y as f16: hi cut off with lo the rest, or hi alone, to nearest.
-template <int NT> __device__ __forceinline__ void split2(float x, float y, uint32_t & hi, uint32_t & lo) {
-    if constexpr (NT == 2) {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        hi = __builtin_bit_cast(uint32_t, h);
-        float x1, y1;                                      // (the compiler takes two instructions each)
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x1) : "v"(hi), "v"(x));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y1) : "v"(hi), "v"(y));
-        lo = pk_f16(x1, y1);
-    } else {
-        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-        hi = __builtin_bit_cast(uint32_t, v2h{(_Float16) x, (_Float16) y});
-    }
+// x and y as f16: hi cut off, lo the rest.
+__device__ __forceinline__ void split2(float x, float y, uint32_t & hi, uint32_t & lo) {
+    hi = pk_f16(x, y);
+    float x1, y1;                                          // (the compiler takes two instructions each)
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x1) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y1) : "v"(hi), "v"(y));
+    lo = pk_f16(x1, y1);
 }
 template <int B> __device__ __forceinline__ float byte_f32(uint32_t w) { return (float) (int8_t) (w >> (8 * B)); }
 
@@ -121,8 +116,7 @@ template <typename F, int... X> __device__ __forceinline__ void for_blocks(F & f
 
 template <int D, int TYPE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
-    constexpr int NT = TYPE == QWFN_TYPE_BF16 ? 1 : 2;
-    using C = ta_cfg<D, NT, WAVES>;
+    using C = ta_cfg<D, WAVES>;
     constexpr int NBLK = C::NBLK;
     __shared__ __attribute__((aligned(16))) uint8_t lds[C::LDS];
     __shared__ int32_t sh[WAVES + 3], odd[4];
@@ -347,10 +341,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) f[k] = byte_f32<B>(cv.w[k]) * cv.d[k];
                 uint2 hi, lo;
-                split2<NT>(f[0], f[1], hi.x, lo.x);
-                split2<NT>(f[2], f[3], hi.y, lo.y);
+                split2(f[0], f[1], hi.x, lo.x);
+                split2(f[2], f[3], hi.y, lo.y);
                 *(uint2 *) (out + B * 128) = hi;
-                if constexpr (NT == 2) *(uint2 *) (out + NBLK * 2048 + B * 128) = lo;
+                *(uint2 *) (out + NBLK * 2048 + B * 128) = lo;
             }
         };
         // the steps from 1 of block X of NBLK
@@ -469,8 +463,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
             for (int st = 0; st < 2; st++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    uint32_t hi, lo = 0;
-                    split2<NT>(p[8 * st + 2 * k], p[8 * st + 2 * k + 1], hi, lo);
+                    uint32_t hi, lo;
+                    split2(p[8 * st + 2 * k], p[8 * st + 2 * k + 1], hi, lo);
                     ph[st][k] = hi;
                     pl[st][k] = lo;
                 }
@@ -478,17 +472,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
         };
 
         // ---- O^T of a row tile, a block a step
-        v4u va[2][NT];                                     // (half a block ahead: a whole one costs 16 registers)
+        v4u va[2][2];                                      // (half a block ahead: a whole one costs 16 registers)
         auto pv_read = [&](int blk, int st, const uint8_t * img) {
 #pragma unroll
-            for (int x = 0; x < NT; x++) va[st][x] = *(const v4u *) (img + C::OV + half * 512 + ln * 16 + x * (NBLK * 2048) + (blk * 4 + 2 * st) * 512);
+            for (int x = 0; x < 2; x++) va[st][x] = *(const v4u *) (img + C::OV + half * 512 + ln * 16 + x * (NBLK * 2048) + (blk * 4 + 2 * st) * 512);
         };
         auto pv_half = [&](int blk, int st) {
             O[blk] = mfma_f16(va[st][0], ph[st], O[blk]);
-            if constexpr (NT == 2) {
-                O[blk] = mfma_f16(va[st][0], pl[st], O[blk]);
-                O[blk] = mfma_f16(va[st][1], ph[st], O[blk]);
-            }
+            O[blk] = mfma_f16(va[st][0], pl[st], O[blk]);
+            O[blk] = mfma_f16(va[st][1], ph[st], O[blk]);
         };
         // Tile t is multiplied from one image while t + 1 becomes the other and the rows of t + 2 are on their way. A wave converts
         // the keys that it has brought in itself, so one barrier a tile is for the images alone.
@@ -532,7 +524,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_paged_tree(pa_args a) {
                     convert_some(X, t + 1, next, img1);
                     if constexpr (blk + 1 < NBLK) pv_read(blk + 1, 0, img);
 #pragma unroll
-                    for (int i = 0; i < (NT == 2 ? 3 : 1); i++) {
+                    for (int i = 0; i < 3; i++) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                         __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
                     }
