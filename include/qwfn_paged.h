@@ -210,10 +210,10 @@ int qwfn_paged_compact(const int32_t * n_kv, int32_t n_seq, int32_t page_size, c
  * s .. s + n - 1 go to d .. d + n - 1. caches: host array of tensors [ne0, n_rows] of one
  * type, shape and row stride, rows contiguous, none over another. moves: device I32
  * [cap][3]; n_moves: device I32 [1], how many of them count, or NULL for all cap. No
- * row that a move writes may be read or written by another. A move with n = 0 is
- * none; one with n outside [0, max_rows] or rows outside the tensor is left out and sets
- * bit 0 of qwfn_device_status, as does an n_moves outside [0, cap] (clipped). One
- * launch for up to 64 tensors. */
+ * row that a move writes may be read or written by another. A move with n = 0 or s = d
+ * is none; one with n outside [0, max_rows], rows outside the tensor or rows that go
+ * over each other (0 < |s - d| < n) is left out and sets bit 0 of qwfn_device_status, as
+ * does an n_moves outside [0, cap] (clipped). One launch for up to 64 tensors. */
 int qwfn_paged_copy(const qwfn_tensor * caches, int32_t n_caches, const int32_t * moves, int32_t cap, const int32_t * n_moves,
                     int32_t max_rows, void * stream);
 

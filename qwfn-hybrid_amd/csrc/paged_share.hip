@@ -364,7 +364,8 @@ struct copy_args {
 };
 
 // A thread per unit of T (16 bytes where rows are whole ones) of a move's rows, blockIdx.y the tensor: every load of a
-// workgroup is in flight before its first store. The units of a move with fewer than max_rows rows stay empty.
+// workgroup is in flight before its first store. The units of a move with fewer than max_rows rows stay empty. They have no
+// order, so a move whose rows go over each other is refused; one onto its own place is none.
 template <typename T>
 __global__ __launch_bounds__(SH_THREADS) void k_paged_copy(copy_args a) {
     bool bad = false;
@@ -379,12 +380,13 @@ __global__ __launch_bounds__(SH_THREADS) void k_paged_copy(copy_args a) {
         if (m >= n) continue;
         const int32_t s = a.moves[3 * m], d = a.moves[3 * m + 1], rows = a.moves[3 * m + 2];
         if (rows == 0) continue;
-        if (rows < 0 || rows > a.max_rows || s < 0 || d < 0 || s + (int64_t) rows > a.n_rows || d + (int64_t) rows > a.n_rows) {
+        if (rows < 0 || rows > a.max_rows || s < 0 || d < 0 || s + (int64_t) rows > a.n_rows || d + (int64_t) rows > a.n_rows ||
+            (s != d && (s < d ? d - s : s - d) < rows)) {
             bad = true;
             continue;
         }
         const uint32_t r = u / (uint32_t) a.upr, c = u - r * (uint32_t) a.upr;
-        if ((int32_t) r < rows)
+        if ((int32_t) r < rows && s != d)
             *(T *) (cache + (size_t) (d + r) * a.nb1 + (size_t) c * sizeof(T)) =
                 *(const T *) (cache + (size_t) (s + r) * a.nb1 + (size_t) c * sizeof(T));
     }
