@@ -805,7 +805,8 @@ int paged_attention(bool tree, const qwfn_tensor * q, const qwfn_tensor * k, con
     if (!is_aligned(table, 4) || !is_aligned(n_kv, 4)) return err(QWFN_EALIGN, ": table and n_kv must be 4-byte aligned");
     if (!is_aligned(n_tree, 4) || !is_aligned(masks, 8)) return err(QWFN_EALIGN, ": n_tree must be 4-byte aligned, masks 8");
     if (ws && !is_aligned(ws, 16)) return err(QWFN_EALIGN, ": ws must be 16-byte aligned");
-    if (ws && ws_bytes < pl.bytes) return err(QWFN_ENOMEM, ": ws smaller than qwfn_fattn_workspace_size_paged");
+    if (ws && ws_bytes < pl.bytes)
+        return err(QWFN_ENOMEM, tree ? ": ws smaller than qwfn_fattn_workspace_size_paged_tree" : ": ws smaller than qwfn_fattn_workspace_size_paged");
     // (a request's queries are read by several workgroups, and one of them may be done before another begins)
     const size_t rows = tensor_extent(dst);
     const span in[] = {{q->data, tensor_extent(q), "q"}, {k->data, view_bytes(*k), "k"}, {v->data, view_bytes(*v), "v"},
