@@ -895,7 +895,7 @@ class CacheList:
         caches = list(caches)
         arr = (Tensor * max(1, len(caches)))()
         for i, c in enumerate(caches):
-            if c.dim() < 2 or not c[0].is_contiguous():
+            if c.dim() < 2 or c.size(0) == 0 or not c[0].is_contiguous():
                 raise ValueError("cache_list: tensors must be [n_rows, ...] with contiguous rows")
             if c.get_device() != caches[0].get_device():
                 raise ValueError("cache_list: tensors must be on one device")
