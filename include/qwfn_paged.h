@@ -221,6 +221,8 @@ int qwfn_paged_copy(const qwfn_tensor * caches, int32_t n_caches, const int32_t 
  *
  * A verify step over a tree: request b has T' = n_tree[b] <= T <= 64 drafted tokens
  * (nodes; n_tree NULL: T, or all where it has fewer), its newest T' tokens in the cache (extend them as usual).
+ * A request that the extend does not serve has none there: give it 0 nodes, as n_tree = n_kv - n_past
+ * does, or its last tokens count as nodes, which qwfn_paged_accept moves and drops.
  * Node t's parent precedes it; masks[b][t] (64-bit words, [n_seq][T]) has the bit of
  * every node that t sees, t itself among them. Per step: qwfn_tree_masks; per
  * attention layer qwfn_flash_attn_ext_q8_0_paged_tree, per recurrent layer

@@ -1027,7 +1027,8 @@ def fattn_workspace_size_paged_tree(qv: Tensor, kv: Tensor, vv: Tensor, table, p
 def flash_attn_ext_paged_tree(qv: Tensor, kv: Tensor, vv: Tensor, table, page_size: int, n_kv, masks, scale: float, ov: Tensor,
                               n_tree=None, gate=None, variant: int = Q8_X86, ws=None, stream=None):
     """flash_attn_ext_paged of the nodes of drafted trees: masks int64 [n_seq, T] (tree_masks), n_tree device int32 [n_seq] or
-    None (T nodes each); a request's nodes are its newest tokens in the cache."""
+    None (T nodes each); a request's nodes are its newest tokens in the cache, so one that the extend did not serve has 0
+    (n_tree = n_kv - n_past)."""
     n_seq, T, dev = qv.ne[3], qv.ne[1], _Torch().device()
     _check_i32("flash_attn_ext_paged_tree", dev, dict(n_kv=(n_kv, n_seq), n_tree=(n_tree, n_seq)), table, n_seq)
     _check_2d("flash_attn_ext_paged_tree", dev, dict(masks=(masks, n_seq, T)))
@@ -1045,7 +1046,8 @@ def flash_attn_ext_paged_tree(qv: Tensor, kv: Tensor, vv: Tensor, table, page_si
 
 def paged_accept(caches, page_size: int, table, n_kv, masks, leaf, n_keep, n_tree=None, cu_path=None, path=None, stream=None):
     """The path to node leaf[b] of each tree moved to the tree's front in every tensor of caches (a cache_list, or tensors):
-    n_keep int32 [n_seq] the tokens then kept, cu_path [n_seq + 1] and path [n_seq * T] the accepted nodes b * T + t."""
+    n_keep int32 [n_seq] the tokens then kept, cu_path [n_seq + 1] and path [n_seq * T] the accepted nodes b * T + t. n_tree as in
+    flash_attn_ext_paged_tree: with None, or too many nodes, tokens of the context are moved and dropped."""
     (n_seq, T), dev = masks.shape, _Torch().device()
     caches = _check_list("paged_accept", caches, dev)
     _check_i32("paged_accept", dev, dict(n_kv=(n_kv, n_seq), leaf=(leaf, n_seq), n_keep=(n_keep, n_seq), n_tree=(n_tree, n_seq),
