@@ -302,7 +302,8 @@ int qwfn_linear_attn(const qwfn_tensor * q, const qwfn_tensor * k, const qwfn_te
  * sum of g over the nodes of masks[b][t] (64-bit words [n_seq][T]; bits from n_tree[b] on
  * count for nothing)
  *   out[t] = scale (exp(G_t) S^T q_t + sum over j in masks[b][t] of exp(G_t - G_j) (q_t . k_j) v_j)
- * which is the recurrence along the path to t where masks are qwfn_tree_masks'. Nodes
+ * which is the recurrence along the path to t where masks are qwfn_tree_masks' (of the plain
+ * decay: qwfn_gated_delta_net, with its delta rule, has no form for a tree). Nodes
  * from n_tree[b] on are not read and give 0. q, k, v, g, dst, the slots and the states as in
  * qwfn_linear_attn (n_tok = n_seq * T; state may be NULL: zeros; a slot of -2 - s leaves the
  * request out, its dst rows are not written). A decay below exp(-693) counts as that. F32

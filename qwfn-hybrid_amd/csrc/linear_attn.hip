@@ -852,7 +852,13 @@ __global__ __launch_bounds__(LA_THREADS) void k_linear_join(lc_args x) {
 // Of bf16 inputs (BF) products run on the bf16 cores: the state and the weighted scores as three bf16 terms, 24 bits, against
 // q and v as they are (values that are not finite there become NaN). 48 requests of 32 nodes, 16 / 48 heads of 128: 55 us, 2.7
 // TB/s of the states, three workgroups a CU in three rounds; with F32 instructions, 25 us of them, 80 us; four workgroups a CU
-// (10 registers spilled) 59 us.
+// (10 registers spilled) 59 us. The same batch, graph-replayed, us (its bytes at a copy's rate, 5.16 TB/s: 34 to 49, of f32 39 to 68):
+//              16 nodes    32    48    64
+//   bf16           41      54    87   158
+//   f16            50      77   143   252
+//   f32            53      79   145   252
+// From 49 nodes on the heads of 128 take 264 to 272 registers (but 236 of bf16 and 64 columns), so one workgroup stands alone on a
+// CU and nothing hides its loads.
 //
 // A v_j that is not finite must not reach nodes that do not see it (0 times infinity): a workgroup that holds one takes its
 // scores times v by plain sums over the masks.

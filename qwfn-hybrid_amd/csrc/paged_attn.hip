@@ -675,9 +675,9 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_seq, int64_t max_kv, bool tree) {
     pa_plan p;
     const int64_t R = T * (nh / nh_kv);
-    // A tree of many rows takes 128 or 256 rows a workgroup (paged_tree.hip), where that is faster than 16. It pays from 65
-    // rows on, and where each of 512 workgroups of 16 rows would have at least 48 tiles. us, 16 rows against that,
-    // f32, 2 KV heads:
+    // A tree of many rows takes 128 or 256 rows a workgroup (paged_tree.hip): from 65 rows on, where each of 512 workgroups of
+    // 16 rows would have at least 48 tiles, and of more than 512 rows always. us, 16 rows against that, f32 (the other types
+    // differ by their queries and results alone), 2 KV heads:
     //                                    96 rows        128        256        512       1024
     //   D 256,  1 request  of  3000      22 / 31    24 / 33    27 / 44    38 / 51    95 / 60
     //   D 256,  1 request  of 12000      33 / 40    35 / 43    51 / 54    80 / 69   254 / 100
@@ -686,8 +686,10 @@ pa_plan plan_paged(int64_t D, int64_t T, int64_t nh, int64_t nh_kv, int64_t n_se
     //   D 128, 16 requests of  3000      70 / 45    60 / 48   100 / 68   171 / 111  665 / 197
     //   D 64,  16 requests of  3000      35 / 38    37 / 40    61 / 53    99 / 86   308 / 153
     //   D 64,  16 requests of 12000      96 / 80    96 / 82   185 / 142  344 / 262 1135 / 501
-    // and of 700 keys 58 / 46 with 1024 rows, 28 / 41 with 512. (64 rows, 16 requests of 12000: 136 / 162.) The lengths are
-    // on the device: the table's width stands for them.
+    // and of 700 keys 58 / 46 with 1024 rows, 28 / 41 with 512. (64 rows, 16 requests of 12000: 136 / 162.) 48 tiles are right for
+    // D 64; of D 128 and 256 calls of 24 to 47 keep 16 rows though the others would take less (16 requests of 3000 with 96 or
+    // 128 rows, one of 12000 with 512). The lengths are on the device: the table's width stands for them, so short
+    // requests in a wide table count as long ones.
     const int64_t tiles = (max_kv + PA_TILE - 1) / PA_TILE * n_seq, narrow = (R + 15) / 16 * nh_kv;
     p.wide = tree && R > PA_NARROW_ROWS && (R > PA_WIDE_ROWS || tiles * narrow >= PA_WIDE_TILES * 2 * PA_CUS);
     p.rows = p.wide ? tree_rows(D) : 16;

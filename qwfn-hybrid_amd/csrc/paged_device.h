@@ -35,7 +35,7 @@ struct pa_args {
     int32_t         runs;              // runs the tiles are cut into, at most
     fast_div        f_runs, f_inner, f_kv, f_rep;      // runs, blocks of a run, KV heads, rep
     float           c;                 // scale * log2(e): scores are in log2 units
-    float *         part_o;            // [run + request][nh_kv][R][D]
+    float *         part_o;            // [run + request][nh_kv][R][D]; k_paged_tree's: [..][nh_kv][tile of 32 rows][as its registers lie]
     float2 *        part_ml;           // [run + request][nh_kv][R]
     int2 *          span;              // [request] (a tree's: [row group][request]): its first and last run
     // trees: nodes of a request (or NULL), what each sees, query rows of a row group

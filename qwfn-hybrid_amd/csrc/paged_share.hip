@@ -211,7 +211,9 @@ __global__ __launch_bounds__(SH_THREADS) void k_release_drop(release_args a) {
     }
 }
 
-// A thread per word of the bitmap; every workgroup counts the bits before its own for itself.
+// A thread per word of the bitmap; every workgroup counts the bits before its own for itself, a launch less than with their sums
+// from one. The counting grows with the pool's square, which shows in pools of tens of millions: 2^24 pages, half of them given back
+// by 64 requests, take 4.7 ms, 2^26 take 23.
 __global__ __launch_bounds__(SH_THREADS) void k_release_push(release_args a) {
     __shared__ pair64 part[2][PT_WAVES];
     __shared__ int64_t sum;

@@ -4,7 +4,7 @@
 //   out = sum_j 2^(s_j - M) v_j / sum_j 2^(s_j - M),   v_j = dv_jb vq_j,   c = scale log2(e)
 //
 // over the tokens before the tree and the nodes in the query's mask. A tree of 64 nodes at 8 heads a KV head has 512 rows:
-// 940 operations a byte of the cache, so the vector and matrix units bound it, not the rows.
+// 960 operations a byte of the cache, so the vector and matrix units bound it, not the rows.
 //
 // Work: as in k_paged_attn the requests' key tiles of 32 stand in one row, cut into equal runs; a workgroup takes one run for
 // one KV head and 32 query rows a wave, two waves a SIMD. Its waves share a tile: its rows come by LDS DMA two tiles ahead, and
@@ -21,9 +21,12 @@
 // Scaling V instead of P dv once a block keeps 20 vector instructions a score out of the loop (8 blocks of D 256). O takes 128
 // registers of D 256, so the queries' scales and five of their blocks lie in LDS.
 //
-// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 259 us with the parts' merge (240 without), 0.40 P operations/s: the
-// vector units are busy for 60 % of the cycles, the matrix units for a third. A tile takes a SIMD's two waves 10000 cycles: 3700
-// of vector instructions in the scores, then 3100 of matrix instructions in the product, then 1800 in sending and at the barrier.
+// 8 requests of 12295 tokens, 64 nodes, 16 heads, f32: 258 us with the parts' merge (about 20) on one card, 274 on another, passes
+// one after another (bursts of ten and kernels under the profiler take up to a tenth more), 0.38 to 0.40 P operations/s: the vector
+// units are busy for 58 % of the cycles, the matrix units for 31 %. A tile takes a wave 9900 cycles on average: 2700 the
+// scores, 800 the softmax, 3800 the product with the next tile's conversion, 900 addresses, 1700 at the barrier (2600 of the
+// waves that come to the scores first, 750 of the others). D 256 spills 6 vector registers.
+// 16 ragged requests, 32 nodes, 16 heads, bf16: 130 us; V and P as one f16 each 115.
 // Slower: one half of the waves a phase behind the other with two barriers a tile, so that a product stands beside scores
 // (292 us), 4 waves of 64 rows with the registers of a whole SIMD (spills), operands of the product read further ahead (spills),
 // the conversion before the scores (291 us). Of D 128 and 64 two workgroups of 4 waves share a CU, each lane with a key's 4
